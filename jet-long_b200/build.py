@@ -15,7 +15,8 @@ CSRC = os.path.join(HERE, "csrc")
 OUT_DIR = os.path.join(HERE, "jetlm", "kernels")
 LIB = os.path.join(OUT_DIR, "libjetlong_b200.so")
 OBJ_DIR = os.path.join(HERE, "build")
-SOURCES = ["capi.cu", "merge.cu", "rotate.cu", "step.cu", "peer.cu", "decode.cu", "prefill_mma.cu", "prefill_tc.cu"]
+SOURCES = ["capi.cu", "merge.cu", "rotate.cu", "step.cu", "peer.cu", "decode.cu", "prefill_mma.cu", "prefill_tc.cu",
+           "tree.cu", "tree_attn.cu", "vocab_head.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr"]
 
@@ -37,7 +38,8 @@ def _stale(target: str, deps: list[str]) -> bool:
 def build(force: bool = False, verbose: bool = False) -> str:
     os.makedirs(OBJ_DIR, exist_ok=True)
     headers = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cuh", ".h"))]
-    headers.append(os.path.join(os.path.dirname(HERE), "include", "jetlong_b200.h"))
+    include = os.path.join(os.path.dirname(HERE), "include")
+    headers += [os.path.join(include, f) for f in os.listdir(include) if f.endswith(".h")]
     nvcc = _nvcc()
     jobs = []
     objs = []

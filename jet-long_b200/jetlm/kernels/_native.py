@@ -1,4 +1,5 @@
-"""ctypes binding of libjetlong_b200.so (the C ABI declared in include/jetlong_b200.h).
+"""ctypes binding of libjetlong_b200.so (the C ABI declared in include/jetlong_b200.h, jetlong_b200_tree.h and
+jetlong_b200_head.h).
 
 There is no fallback: if the shared library is missing, or a call returns a non-zero status, an
 exception is raised.  Build the library with `python jet-long_b200/build.py`.
@@ -160,6 +161,75 @@ EXPORTS = [
     ("jl_decode_append", C.c_int, [C.POINTER(DecodeAppendArgs), C.c_void_p]),
 ]
 
+# ---- include/jetlong_b200_tree.h ----
+
+JL_TREE_MAX_NODES = 256
+
+
+class TreePlanArgs(C.Structure):
+    _fields_ = [("parents", C.c_void_p), ("depth", C.c_void_p), ("mask", C.c_void_p), ("batch", C.c_int32), ("nodes", C.c_int32)]
+
+
+class TreeAppendArgs(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p),
+        *[(f"{t}_stride_{a}", C.c_int64) for t in "qkv" for a in "bsh"],
+        ("q_weight", C.c_void_p), ("k_weight", C.c_void_p), ("q_eps", C.c_float), ("k_eps", C.c_float),
+        ("q_base", C.c_void_p), ("q_group", C.c_void_p), ("k_cache", C.c_void_p), ("v_cache", C.c_void_p),
+        ("k_group_cache", C.c_void_p),
+        *[(f"{t}_stride_{a}", C.c_int64) for t in ("kc", "vc") for a in "bsh"], ("cache_rows", C.c_int64),
+        ("batch", C.c_int32), ("nodes", C.c_int32), ("heads", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32),
+        ("group_size", C.c_int32), ("inv_freq", C.c_void_p), ("lens", C.c_void_p), ("depth", C.c_void_p),
+    ]
+
+
+class TreeAttentionArgs(C.Structure):
+    _fields_ = [
+        ("q_base", C.c_void_p), ("q_group", C.c_void_p), ("k_base", C.c_void_p), ("k_group", C.c_void_p), ("v", C.c_void_p),
+        *[(f"{t}_stride_{a}", C.c_int64) for t in "qkv" for a in "bsh"],
+        ("lens", C.c_void_p), ("depth", C.c_void_p), ("mask", C.c_void_p), ("out", C.c_void_p), ("lse", C.c_void_p),
+        *[(f"o_stride_{a}", C.c_int64) for a in "bsh"],
+        ("batch", C.c_int32), ("nodes", C.c_int32), ("heads", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32),
+        ("rows", C.c_int32), ("w_0", C.c_int64), ("softmax_scale", C.c_float), ("reserved", C.c_int32),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
+TREE_EXPORTS = [
+    ("jl_tree_plan", C.c_int, [C.POINTER(TreePlanArgs), C.c_void_p]),
+    ("jl_tree_append", C.c_int, [C.POINTER(TreeAppendArgs), C.c_void_p]),
+    ("jl_tree_attention_workspace_bytes", C.c_size_t, [C.c_int32] * 5),
+    ("jl_tree_attention", C.c_int, [C.POINTER(TreeAttentionArgs), C.c_void_p]),
+]
+
+
+# ---- include/jetlong_b200_head.h ----
+
+class HeadScoresArgs(C.Structure):
+    _fields_ = [
+        ("hidden", C.c_void_p), ("weight", C.c_void_p), ("hidden_stride", C.c_int64), ("weight_stride", C.c_int64),
+        ("labels", C.c_void_p), ("ignore_index", C.c_int64), ("rows", C.c_int64), ("hidden_size", C.c_int32), ("vocab", C.c_int32),
+        ("nll", C.c_void_p), ("lse", C.c_void_p), ("top", C.c_void_p), ("loss_sum", C.c_void_p), ("loss_count", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
+class HeadGradsArgs(C.Structure):
+    _fields_ = [
+        ("hidden", C.c_void_p), ("weight", C.c_void_p), ("hidden_stride", C.c_int64), ("weight_stride", C.c_int64),
+        ("labels", C.c_void_p), ("ignore_index", C.c_int64), ("rows", C.c_int64), ("hidden_size", C.c_int32), ("vocab", C.c_int32),
+        ("lse", C.c_void_p), ("grad", C.c_void_p), ("grad_stride", C.c_int64), ("grad_count", C.c_void_p),
+        ("d_hidden", C.c_void_p), ("d_weight", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
+HEAD_EXPORTS = [
+    ("jl_head_scores_workspace_bytes", C.c_size_t, [C.c_int64, C.c_int32, C.c_int32]),
+    ("jl_head_scores", C.c_int, [C.POINTER(HeadScoresArgs), C.c_void_p]),
+    ("jl_head_grads_workspace_bytes", C.c_size_t, [C.c_int64, C.c_int32, C.c_int32]),
+    ("jl_head_grads", C.c_int, [C.POINTER(HeadGradsArgs), C.c_void_p]),
+]
+
 _LIB = None
 
 
@@ -181,7 +251,7 @@ def lib() -> C.CDLL:
                 f"{LIB_NAME} not found at {LIB_PATH}: the CUDA extension is required (no CPU or PyTorch "
                 f"fallback exists). Build it with `python jet-long_b200/build.py`.")
         handle = C.CDLL(LIB_PATH)
-        for name, restype, argtypes in EXPORTS:
+        for name, restype, argtypes in EXPORTS + TREE_EXPORTS + HEAD_EXPORTS:
             fn = getattr(handle, name)
             fn.restype = restype
             fn.argtypes = argtypes
