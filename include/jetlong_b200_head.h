@@ -73,6 +73,10 @@ typedef struct {
 size_t jl_head_grads_workspace_bytes(int64_t rows, int32_t hidden_size, int32_t vocab);
 int jl_head_grads(const jl_head_grads_args* args, void* cuda_stream);
 
+/* Diagnostic (synchronises the device): non-zero if a bounded wait (1 s) inside a head kernel has given up on the current
+ * device since the last call; reading a raised status clears it.  The results since the last call are then invalid. */
+int jl_head_status(void);
+
 #ifdef __cplusplus
 }
 #endif

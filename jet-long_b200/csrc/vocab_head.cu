@@ -1,81 +1,385 @@
 // The vocabulary head without logits: softmax statistics of hidden @ weight^T, and the gradients of the cross-entropy
 // loss, formed piece by piece of the vocabulary.
 //
-//   z = h W^T,  lse = log sum exp z,  nll = lse - z_y,  dz = g (exp(z - lse) - onehot(y)),  dh = dz W,  dW = dz^T h
+//   z = h W^T,  lse = log sum exp z,  nll = lse - z_y,  dz = exp(z - lse) - onehot(y),  dh = g dz W,  dW = g dz^T h
 //
-// Scores: one product whose epilogue reduces every 64 x 64 tile of z to (maximum, sum, argmax) per row; a second
-// kernel folds the tiles' partials.  Gradients: for each piece of the vocabulary the product is formed again, its
-// epilogue stores dz of the piece in bf16, and two more products take it to dW (final for the piece) and dh
-// (accumulated in fp32 over the pieces).
-#include "jl_common.cuh"
+// All three products run on one persistent tcgen05 kernel (head_gemm_kernel) whose epilogue is what differs:
+//   scores  z tile -> per row (maximum, sum of exponentials, argmax, logit of the label); a fold kernel joins the tiles
+//   dz      z tile -> exp(z - lse) - onehot in bf16, one piece of the vocabulary at a time
+//   dh      dz W accumulated in fp32 over the pieces (bulk reductions in L2), rounded once at the end
+//   dW      dz^T h, final for the piece
+// The score and dz products read hidden and weight along their rows (K-major); dh reads weight and dW reads dz and
+// hidden across them (MN-major), so nothing is transposed in memory.
+#include <cmath>
+
+#include "tc_common.cuh"
 #include "../../include/jetlong_b200_head.h"
 
 namespace jl {
 
 namespace {
 
-constexpr int kTile = 64, kStep = 16;
+using namespace tc;
 
-// element (r, c) of a row-major or transposed bf16 operand
-struct Operand {
-  const __nv_bfloat16* p;
-  int64_t sr, sc;
-  __device__ float at(int64_t r, int64_t c) const { return __bfloat162float(p[r * sr + c * sc]); }
+__device__ int g_head_status = 0;            // raised when a bounded wait gave up
+
+constexpr int kBK = 64;                      // K step: one 128-byte swizzle row of bf16
+constexpr int kMaxBN = 256;
+constexpr int kABytes = 128 * kBK * 2;       // a CTA's 128 rows of A
+constexpr int kAccCols = 256;                // tensor-memory columns of one accumulator; two of them alternate
+constexpr int kGemmThreads = 256;
+constexpr int kStageBytes = 196608;          // operand ring
+constexpr int kStagingBytes = 2 * 4 * 4096;  // per epilogue warp two buffers of 32 rows x 128 bytes
+constexpr int kMaxStages = 6;
+constexpr int kSms = 148;
+
+enum { kEpiScores = 0, kEpiDz = 1, kEpiF32 = 2, kEpiBf16 = 3 };
+
+struct GradScale {            // scalar factor of both gradients, applied to their fp32 sums
+  const float *grad, *count;
+  int per_row;
+  // dz itself stays p - onehot, whose values next to -1 round to bf16 with little error; scaled by 1 / 4014, say, all of
+  // them would take the same error of 0.3 %.
+  __device__ float get() const {
+    if (per_row) return 1.f;
+    return count == nullptr ? *grad : *count > 0.f ? *grad / *count : 0.f;
+  }
 };
 
-// acc = A[m0 : m0 + 64, 0 : K] B[n0 : n0 + 64, 0 : K]^T of one 64 x 64 tile, 4 x 4 per thread (256 threads)
-__device__ __forceinline__ void tile_product(const Operand& A, const Operand& B, int64_t m0, int64_t n0, int64_t M, int64_t N, int64_t K,
-                                             float (&acc)[4][4]) {
-  __shared__ float sa[kStep][kTile + 1], sb[kStep][kTile + 1];
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  for (int64_t k0 = 0; k0 < K; k0 += kStep) {
-    for (int i = threadIdx.x; i < kTile * kStep; i += 256) {
-      const int r = i / kStep, c = i % kStep;
-      sa[c][r] = m0 + r < M && k0 + c < K ? A.at(m0 + r, k0 + c) : 0.f;
-      sb[c][r] = n0 + r < N && k0 + c < K ? B.at(n0 + r, k0 + c) : 0.f;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < kStep; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(sa[k][ty * 4 + i], sb[k][tx * 4 + j], acc[i][j]);
-    __syncthreads();
+struct GemmParams {
+  int64_t M, N;               // result extents (rows of A, rows of B)
+  int m_tiles, n_tiles, splits, k_blocks, kb_per_split, bn;
+  int group_m;                // > 0: m fastest inside groups of this many m tiles; 0: n fastest
+  int stages;
+  // scores
+  float2* part;               // [row][n tile] (maximum, sum of exponentials relative to it)
+  int* part_arg;              // [row][n tile] or NULL
+  float* picked;              // [row] logit of the label
+  // dz
+  const float* lse;
+  const float* row_grad;      // NULL or one factor per row
+  // both
+  const int64_t* labels;      // may be NULL for scores
+  int64_t ignore, vocab, v0;  // column 0 of the product is vocabulary entry v0
+  // dh: bulk reduction into what is there instead of a store
+  int reduce;
+  GradScale scale;
+};
+
+struct alignas(64) GemmMaps { CUtensorMap a, b, out; };
+
+struct GemmSmem {
+  alignas(1024) uint8_t ring[kStageBytes];
+  alignas(1024) uint8_t staging[kStagingBytes];
+  uint64_t full[kMaxStages], empty[kMaxStages], acc_full[2], acc_free[2];
+  uint32_t tmem_base;
+  int failed;
+};
+constexpr int kGemmSmemBytes = sizeof(GemmSmem) + 1024;
+
+__device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+               ::"r"(smem_u32(dst)), "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, uint32_t leader_bar, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+               ::"r"(smem_u32(dst)), "l"(map), "r"(leader_bar), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, const void* src, int x, int y, int z, bool reduce) {
+  if (reduce)
+    asm volatile("cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3, %4}], [%1];"
+                 ::"l"(map), "r"(smem_u32(src)), "r"(x), "r"(y), "r"(z) : "memory");
+  else
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];"
+                 ::"l"(map), "r"(smem_u32(src)), "r"(x), "r"(y), "r"(z) : "memory");
+}
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
+#define JL_TMEM_LD16(taddr, r)                                                                                             \
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"     \
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), \
+                 "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(taddr))
+
+struct TileCoord { int m, n, split; };
+__device__ __forceinline__ TileCoord tile_coord(const GemmParams& p, int t) {
+  TileCoord c;
+  const int per = p.m_tiles * p.n_tiles;
+  c.split = t / per;
+  int r = t - c.split * per;
+  if (p.group_m > 0) {
+    const int grp = r / (p.group_m * p.n_tiles), m0 = grp * p.group_m, size = min(p.group_m, p.m_tiles - m0);
+    r -= m0 * p.n_tiles;
+    c.n = r / size;
+    c.m = m0 + r - c.n * size;
+  } else {
+    c.m = r / p.n_tiles;
+    c.n = r - c.m * p.n_tiles;
   }
+  return c;
 }
 
-struct Partial {
-  float m, s;
-  int arg;
-  float pad;
-};
+// C tile (128 * kPair rows x bn columns) = A B^T, fp32 accumulation in tensor memory.  kPair = 2: a cluster of two CTAs works
+// on one tile with cta_group::2 MMAs, each CTA loading its own 128 rows of A and half of the rows of B, so every byte of B
+// in shared memory serves 256 rows.  Two accumulators alternate, so the epilogue of a tile runs under the next one's MMAs.
+//   warp 0 TMA producer, warp 1 MMA issuer (rank 0), warp 2 tensor memory, warps 4-7 epilogue (one thread per row)
+template <int kPair, bool kAMn, bool kBMn, int kEpi>
+__global__ void __launch_bounds__(kGemmThreads, 1) head_gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmParams p) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  GemmSmem& sm = *reinterpret_cast<GemmSmem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = kPair == 2 ? static_cast<int>(blockIdx.x & 1) : 0;
+  const int worker = static_cast<int>(blockIdx.x) / kPair, workers = static_cast<int>(gridDim.x) / kPair;
+  const int n_total = p.m_tiles * p.n_tiles * p.splits;
+  const int b_rows = p.bn / kPair;                         // rows of B this CTA loads
+  const int stage_bytes = kABytes + b_rows * kBK * 2;
 
-__global__ void __launch_bounds__(256) scores_kernel(Operand h, Operand w, int64_t N, int V, int K, const int64_t* labels, Partial* part,
-                                                     float* picked, int tiles) {
-  __shared__ float z[kTile][kTile + 1];
-  const int64_t m0 = static_cast<int64_t>(blockIdx.y) * kTile, n0 = static_cast<int64_t>(blockIdx.x) * kTile;
-  float acc[4][4] = {};
-  tile_product(h, w, m0, n0, N, V, K, acc);
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) z[ty * 4 + i][tx * 4 + j] = acc[i][j];
+  if (threadIdx.x == 0) {
+    sm.failed = *reinterpret_cast<volatile int*>(&g_head_status) != 0 ? 1 : 0;
+    for (int i = 0; i < kMaxStages; ++i) { mbar_init(&sm.full[i], 1); mbar_init(&sm.empty[i], 1); }
+    for (int i = 0; i < 2; ++i) { mbar_init(&sm.acc_full[i], 1); mbar_init(&sm.acc_free[i], 4 * kPair); }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 2) {
+    if (kPair == 2) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem_base)), "r"(512u));
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::);
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem_base)), "r"(512u));
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+    }
+  }
+  tc_fence_before();
   __syncthreads();
-  const int64_t row = m0 + threadIdx.x;
-  if (threadIdx.x >= kTile || row >= N) return;
-  const int n = static_cast<int>(min(static_cast<int64_t>(kTile), V - n0));
-  Partial p{z[threadIdx.x][0], 0.f, static_cast<int>(n0), 0.f};
-  for (int j = 1; j < n; ++j)
-    if (z[threadIdx.x][j] > p.m) { p.m = z[threadIdx.x][j]; p.arg = static_cast<int>(n0) + j; }
-  for (int j = 0; j < n; ++j) p.s += expf(z[threadIdx.x][j] - p.m);
-  part[row * tiles + blockIdx.x] = p;
-  if (labels != nullptr && labels[row] >= n0 && labels[row] < n0 + n) picked[row] = z[threadIdx.x][labels[row] - n0];
+  if (kPair == 2) pair::cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem = sm.tmem_base;
+  volatile int* const failed = &sm.failed;       // a wait gave up: nothing more is issued, every later wait returns at once
+
+  if (warp == 0) {
+    // ===================================== TMA producer =====================================
+    if (lane == 0) {
+      int g = 0;
+      for (int t = worker; t < n_total; t += workers) {
+        const TileCoord c = tile_coord(p, t);
+        const int m0 = (c.m * kPair + rank) * 128, n0 = c.n * p.bn + rank * b_rows;
+        const int kb0 = c.split * p.kb_per_split, kb1 = min(kb0 + p.kb_per_split, p.k_blocks);
+        for (int kb = kb0; kb < kb1; ++kb, ++g) {
+          const int s = g % p.stages;
+          mbar_wait(&sm.empty[s], ((g / p.stages) & 1) ^ 1, sm);
+          if (*failed) { t = n_total; break; }
+          if (rank == 0) mbar_expect_tx(&sm.full[s], kPair * stage_bytes);
+          const uint32_t bar = kPair == 2 ? pair::leader_addr(&sm.full[s]) : smem_u32(&sm.full[s]);
+          uint8_t* sa = sm.ring + s * stage_bytes;
+          uint8_t* sb = sa + kABytes;
+          auto load = [&](void* dst, const CUtensorMap* map, int x, int y) {
+            if (kPair == 2) tma_load_2d_pair(dst, map, bar, x, y);
+            else tma_load_2d(dst, map, bar, x, y);
+          };
+          if (kAMn) {
+            load(sa, &maps.a, m0, kb * kBK);
+            load(sa + 8192, &maps.a, m0 + 64, kb * kBK);
+          } else {
+            load(sa, &maps.a, kb * kBK, m0);
+          }
+          if (kBMn) {
+            for (int ch = 0; ch < b_rows / 64; ++ch) load(sb + ch * 8192, &maps.b, n0 + ch * 64, kb * kBK);
+          } else {
+            load(sb, &maps.b, kb * kBK, n0);
+          }
+        }
+      }
+    }
+  } else if (warp == 1 && rank == 0) {
+    // ====================================== MMA issuer ======================================
+    uint32_t leader;
+    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(leader));
+    const uint32_t idesc = instr_desc(128 * kPair, p.bn, kBMn) | (kAMn ? 1u << 15 : 0u);
+    const uint32_t ring = smem_u32(sm.ring);
+    int g = 0, i = 0;
+    for (int t = worker; t < n_total; t += workers, ++i) {
+      const TileCoord c = tile_coord(p, t);
+      const int kb0 = c.split * p.kb_per_split, kb1 = min(kb0 + p.kb_per_split, p.k_blocks);
+      mbar_wait(&sm.acc_free[i & 1], ((i >> 1) & 1) ^ 1, sm);
+      tc_fence_after();
+      const uint32_t acc = tmem + (i & 1) * kAccCols;
+      for (int kb = kb0; kb < kb1; ++kb, ++g) {
+        const int s = g % p.stages;
+        mbar_wait(&sm.full[s], (g / p.stages) & 1, sm);
+        if (*failed) break;
+        tc_fence_after();
+        const uint32_t sa = ring + s * stage_bytes, sb = sa + kABytes;
+        // K-major rows are 128 bytes in 8-row swizzle atoms; MN-major: 64 elements x 8 k-rows per atom, 8 KB per 64 elements
+        const uint64_t ad = kAMn ? smem_desc(sa, 8192, 1024) : smem_desc(sa, 16, 1024);
+        const uint64_t bd = kBMn ? smem_desc(sb, 8192, 1024) : smem_desc(sb, 16, 1024);
+        if (leader) {
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk) {
+            const uint64_t ao = static_cast<uint64_t>((kAMn ? kk * 2048 : kk * 32) >> 4);
+            const uint64_t bo = static_cast<uint64_t>((kBMn ? kk * 2048 : kk * 32) >> 4);
+            if (kPair == 2) pair::mma2_ss(acc, ad + ao, bd + bo, idesc, kb > kb0 || kk > 0);
+            else mma_ss(acc, ad + ao, bd + bo, idesc, kb > kb0 || kk > 0);
+          }
+          if (kPair == 2) pair::commit_both(&sm.empty[s]);
+          else mma_commit(&sm.empty[s]);
+        }
+        __syncwarp();
+      }
+      if (leader) {
+        if (kPair == 2) pair::commit_both(&sm.acc_full[i & 1]);
+        else mma_commit(&sm.acc_full[i & 1]);
+      }
+      __syncwarp();
+    }
+  } else if (warp >= 4) {
+    // ======================================= epilogue =======================================
+    const int quad = warp & 3;
+    const uint32_t lane_base = static_cast<uint32_t>(quad * 32) << 16;
+    uint8_t* const stage = sm.staging + quad * 8192;
+    const uint32_t free_bar[2] = {kPair == 2 ? pair::leader_addr(&sm.acc_free[0]) : smem_u32(&sm.acc_free[0]),
+                                  kPair == 2 ? pair::leader_addr(&sm.acc_free[1]) : smem_u32(&sm.acc_free[1])};
+    const float scale = kEpi == kEpiBf16 ? p.scale.get() : 1.f;
+    int buf = 0;
+    // 32 rows x 128 bytes of results: 16-byte chunk `ch` of this thread's row
+    auto chunk_ptr = [&](int ch) { return reinterpret_cast<uint4*>(stage + buf * 4096 + lane * 128 + ((ch ^ (lane & 7)) << 4)); };
+    auto begin_box = [&]() {
+      if (lane == 0) bulk_wait_read<1>();          // the box before the last one has left this buffer
+      __syncwarp();
+    };
+    auto end_box = [&](int x, int64_t row_w, int z, bool reduce) {
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) {
+        if (row_w < p.M && x < p.N) tma_store_3d(&maps.out, stage + buf * 4096, x, static_cast<int>(row_w), z, reduce);
+        bulk_commit();
+      }
+      buf ^= 1;
+    };
+    int i = 0;
+    for (int t = worker; t < n_total; t += workers, ++i) {
+      const TileCoord c = tile_coord(p, t);
+      const int64_t row_w = (static_cast<int64_t>(c.m) * kPair + rank) * 128 + quad * 32, row = row_w + lane;
+      const int n0 = c.n * p.bn;
+      const uint32_t acc = tmem + (i & 1) * kAccCols + lane_base;
+      mbar_wait(&sm.acc_full[i & 1], (i >> 1) & 1, sm);
+      tc_fence_after();
+
+      if constexpr (kEpi == kEpiScores) {
+        const int valid = static_cast<int>(min(static_cast<int64_t>(p.bn), p.N - n0));
+        float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        for (int c0 = 0; c0 < valid; c0 += 16) {
+          uint32_t z[16];
+          JL_TMEM_LD16(acc + c0, z);
+          tmem_wait_ld();
+          if (c0 + 16 <= valid) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) m4[j & 3] = max3(m4[j & 3], __uint_as_float(z[2 * j]), __uint_as_float(z[2 * j + 1]));
+          } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              if (c0 + j < valid) m4[j & 3] = fmaxf(m4[j & 3], __uint_as_float(z[j]));
+          }
+        }
+        const float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+        const float m_use = m == -INFINITY ? 0.f : m;
+        const int64_t y64 = p.labels != nullptr && row < p.M ? p.labels[row] - p.v0 - n0 : -1;
+        const int y = y64 >= 0 && y64 < valid ? static_cast<int>(y64) : -1;
+        float s4[4] = {0.f, 0.f, 0.f, 0.f}, z_y = 0.f;
+        int arg = 0x7fffffff;
+        for (int c0 = 0; c0 < valid; c0 += 16) {
+          uint32_t z[16];
+          JL_TMEM_LD16(acc + c0, z);
+          tmem_wait_ld();
+          if (__any_sync(0xffffffffu, y >= c0 && y < c0 + 16)) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) z_y = y == c0 + j ? __uint_as_float(z[j]) : z_y;
+          }
+          if (p.part_arg != nullptr) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              if (__uint_as_float(z[j]) == m && c0 + j < valid) arg = min(arg, c0 + j);
+          }
+          // (z - m) first: exact for the logits that count, whatever their size
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const float e = fast_exp2((__uint_as_float(z[j]) - m_use) * kLog2e);
+            if (c0 + j < valid) s4[j & 3] += e;
+          }
+        }
+        tc_fence_before();
+        if (row < p.M) {
+          p.part[row * p.n_tiles + c.n] = make_float2(m, (s4[0] + s4[1]) + (s4[2] + s4[3]));
+          if (p.part_arg != nullptr) p.part_arg[row * p.n_tiles + c.n] = arg == 0x7fffffff ? n0 : n0 + arg;
+          if (y >= 0) p.picked[row] = z_y;
+        }
+      } else {
+        float lse = 0.f, factor = 0.f;
+        int y = -1;
+        if constexpr (kEpi == kEpiDz) {
+          if (row < p.M) {
+            const int64_t label = p.labels[row];
+            lse = p.lse[row];
+            if (label != p.ignore) {
+              factor = p.row_grad != nullptr ? p.row_grad[row] : 1.f;
+              if (label < 0 || label >= p.vocab) factor = __int_as_float(0x7fc00000);
+              const int64_t rel = label - p.v0 - n0;
+              y = rel >= 0 && rel < p.bn ? static_cast<int>(rel) : -1;
+            }
+          }
+        }
+        const bool used = kEpi != kEpiDz || factor != 0.f;
+        constexpr int kCols = kEpi == kEpiF32 ? 32 : 64;             // columns of one 128-byte box; bn is a multiple of 64 here
+        for (int c0 = 0; c0 < p.bn; c0 += kCols) {
+          begin_box();
+          for (int half = 0; half < kCols / 32; ++half) {
+            const int cc = c0 + half * 32;
+            uint32_t z[32];
+            JL_TMEM_LD32(acc + cc, z, 0);
+            tmem_wait_ld();
+            if constexpr (kEpi == kEpiDz) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) {
+                const float pr = fast_exp2((__uint_as_float(z[j]) - lse) * kLog2e) - (y == cc + j ? 1.f : 0.f);
+                z[j] = used ? __float_as_uint(pr * factor) : 0u;      // a row that does not count is zero whatever it holds
+              }
+            }
+            if constexpr (kEpi == kEpiF32) {
+#pragma unroll
+              for (int v = 0; v < 8; ++v) *chunk_ptr(v) = make_uint4(z[4 * v], z[4 * v + 1], z[4 * v + 2], z[4 * v + 3]);
+            } else {
+              auto pk = [&](int j) { return pack_bf16x2(__uint_as_float(z[j]) * scale, __uint_as_float(z[j + 1]) * scale); };
+#pragma unroll
+              for (int v = 0; v < 4; ++v) *chunk_ptr(half * 4 + v) = make_uint4(pk(8 * v), pk(8 * v + 2), pk(8 * v + 4), pk(8 * v + 6));
+            }
+          }
+          end_box(n0 + c0, row_w, kEpi == kEpiF32 ? c.split : 0, kEpi == kEpiF32 && p.reduce);
+        }
+        tc_fence_before();
+      }
+      __syncwarp();
+      if (lane == 0) asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(free_bar[i & 1]) : "memory");
+    }
+    if (lane == 0) bulk_wait_all();
+  }
+
+  __syncthreads();
+  if (*failed) {                                 // copies and MMAs that were under way have long landed after 1 ms
+    const uint64_t t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 1000 * 1000) {}
+  }
+  if (kPair == 2) pair::cluster_sync();          // neither CTA leaves (or frees tensor memory) while the other may still signal it
+  if (warp == 2) {
+    tc_fence_after();
+    if (kPair == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+    else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+  }
+  if (threadIdx.x == 0 && sm.failed) atomicExch(&g_head_status, 1);
 }
 
 // one warp per row folds the tiles' partials
-__global__ void __launch_bounds__(128) scores_fold_kernel(const Partial* part, const float* picked, int tiles, int64_t N, int V,
+__global__ void __launch_bounds__(128) scores_fold_kernel(const float2* part, const int* part_arg, const float* picked, int tiles, int64_t N, int64_t V,
                                                           const int64_t* labels, int64_t ignore, float* nll, float* lse, int64_t* top) {
   const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
@@ -83,10 +387,13 @@ __global__ void __launch_bounds__(128) scores_fold_kernel(const Partial* part, c
   float m = -INFINITY, s = 0.f;
   int arg = 0x7fffffff;
   for (int i = lane; i < tiles; i += 32) {
-    const Partial p = part[row * tiles + i];
-    if (p.m > m || (p.m == m && p.arg < arg)) arg = p.arg;
-    const float mn = fmaxf(m, p.m);
-    s = (m == -INFINITY ? 0.f : s * expf(m - mn)) + p.s * expf(p.m - mn);
+    const float2 p = part[row * tiles + i];
+    if (part_arg != nullptr) {
+      const int a = part_arg[row * tiles + i];
+      if (p.x > m || (p.x == m && a < arg)) arg = a;
+    }
+    const float mn = fmaxf(m, p.x), ref = mn == -INFINITY ? 0.f : mn;
+    s = s * expf(m - ref) + p.y * expf(p.x - ref);
     m = mn;
   }
 #pragma unroll
@@ -94,14 +401,14 @@ __global__ void __launch_bounds__(128) scores_fold_kernel(const Partial* part, c
     const float om = __shfl_xor_sync(0xffffffffu, m, off), os = __shfl_xor_sync(0xffffffffu, s, off);
     const int oa = __shfl_xor_sync(0xffffffffu, arg, off);
     if (om > m || (om == m && oa < arg)) arg = oa;
-    const float mn = fmaxf(m, om);
-    s = (m == -INFINITY ? 0.f : s * expf(m - mn)) + (om == -INFINITY ? 0.f : os * expf(om - mn));
+    const float mn = fmaxf(m, om), ref = mn == -INFINITY ? 0.f : mn;
+    s = s * expf(m - ref) + os * expf(om - ref);
     m = mn;
   }
   if (lane != 0) return;
   const float l = m + logf(s);
   if (lse != nullptr) lse[row] = l;
-  if (top != nullptr) top[row] = arg;
+  if (top != nullptr) top[row] = arg == 0x7fffffff ? 0 : arg;
   if (nll != nullptr) {
     const int64_t y = labels[row];
     nll[row] = y == ignore ? 0.f : (y >= 0 && y < V ? l - picked[row] : __int_as_float(0x7fc00000));
@@ -130,71 +437,162 @@ __global__ void __launch_bounds__(1024) loss_sum_kernel(const float* nll, const 
   if (count != nullptr) *count = c;
 }
 
-struct GradRow {
-  const int64_t* labels;
-  int64_t ignore;
-  const float *lse, *grad, *count;
-  int64_t grad_stride;
-  // One scalar for all rows is applied to the fp32 results: dz itself is then p - onehot, whose large values next to -1
-  // round to bf16 with little error (scaled by 1 / 4014, say, every one of them would take the same error of 0.3 %).
-  __device__ float row_factor(int64_t row) const { return grad_stride != 0 ? grad[row] : 1.f; }
-  __device__ float scale() const {
-    if (grad_stride != 0) return 1.f;
-    return count == nullptr ? *grad : *count > 0.f ? *grad / *count : 0.f;
+// d_hidden = scale * (sum of the K splits' fp32 results), rounded once; 4 values a thread
+__global__ void __launch_bounds__(256) grad_round_kernel(const float* x, int splits, int64_t n, __nv_bfloat16* out, GradScale g) {
+  const int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 4;
+  if (i >= n) return;
+  float4 a = *reinterpret_cast<const float4*>(x + i);
+  for (int s = 1; s < splits; ++s) {
+    const float4 b = *reinterpret_cast<const float4*>(x + s * n + i);
+    a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w;
   }
+  const float c = g.get();
+  *reinterpret_cast<uint2*>(out + i) = make_uint2(pack_bf16x2(a.x * c, a.y * c), pack_bf16x2(a.z * c, a.w * c));
+}
+
+// ---------------------------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------------------------
+
+int64_t cdiv(int64_t x, int64_t y) { return (x + y - 1) / y; }
+size_t up256(size_t x) { return (x + 255) & ~size_t(255); }
+
+// (rows, cols) row-major operand or result as a 2-D (loads) or 3-D (results) map; a box is box_x elements by box_y rows
+int make_map2(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int64_t ld, int box_x, int box_y, bool f32, int64_t planes, bool three) {
+  EncodeTiledFn enc = encode_fn();
+  if (enc == nullptr) return fail(JL_ERR_LAUNCH, "jl_head: cuTensorMapEncodeTiled is not available from the driver");
+  const int es_bytes = f32 ? 4 : 2;
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(planes)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(ld) * es_bytes, static_cast<cuuint64_t>(ld) * es_bytes * static_cast<cuuint64_t>(rows)};
+  const cuuint32_t box[3] = {static_cast<cuuint32_t>(box_x), static_cast<cuuint32_t>(box_y), 1};
+  const cuuint32_t es[3] = {1, 1, 1};
+  const CUresult r = enc(m, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, three ? 3 : 2, const_cast<void*>(base), dims, strides,
+                         box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(JL_ERR_BAD_ARG, "jl_head: tensor map encoding failed (CUresult %d)", static_cast<int>(r));
+  return JL_OK;
+}
+
+struct Matrix {               // row-major bf16
+  const void* p;
+  int64_t rows, cols, ld;
 };
 
-__global__ void __launch_bounds__(256) dz_kernel(Operand h, Operand w, int64_t N, int V, int K, int v0, int piece, GradRow g, __nv_bfloat16* dz, int ld) {
-  const int64_t m0 = static_cast<int64_t>(blockIdx.y) * kTile, n0 = static_cast<int64_t>(blockIdx.x) * kTile;
-  float acc[4][4] = {};
-  w.p += v0 * w.sr;
-  tile_product(h, w, m0, n0, N, piece, K, acc);
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int64_t row = m0 + ty * 4 + i;
-    if (row >= N) continue;
-    const int64_t y = g.labels[row];
-    const bool used = y != g.ignore;
-    float c = g.row_factor(row);
-    if (used && (y < 0 || y >= V)) c = __int_as_float(0x7fc00000);
-    const float l = g.lse[row];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t col = n0 + tx * 4 + j;
-      if (col >= ld) continue;
-      const float p = expf(acc[i][j] - l) - (v0 + col == y ? 1.f : 0.f);
-      dz[row * ld + col] = __float2bfloat16(used && col < piece ? c * p : 0.f);
-    }
+// Result of the product: the output map's base (NULL: none), its row length and type
+struct Result {
+  void* p;
+  int64_t ld;
+  bool f32;
+  int64_t planes;
+};
+
+// Shape of a launch over an M x N result: rows per tile follow from `pair`, the tile's width is the one whose rounds over
+// the GPU's workers cost least (a tile costs its width, plus some columns' worth of hand-over).
+struct Plan { int pair, bn, m_tiles, n_tiles; };
+// `step`: what the width has to be a multiple of (16 columns of each CTA's B; 64 where boxes of 64 columns are loaded or stored).
+Plan plan_tiles(int64_t M, int64_t N, int pair, int step) {
+  Plan best{pair, 0, static_cast<int>(cdiv(M, 128 * pair)), 0};
+  double cost = 1e30;
+  for (int bn = kMaxBN; bn >= step && bn >= 64; bn -= step) {
+    const int64_t tiles = best.m_tiles * cdiv(N, bn);
+    const double rounds = static_cast<double>(cdiv(tiles, kSms / pair)) * (bn + 24);
+    if (rounds < cost * 0.995) { cost = rounds; best.bn = bn; }
   }
+  best.n_tiles = static_cast<int>(cdiv(N, best.bn));
+  return best;
 }
 
-// C = A B^T; fp32 accumulation into acc32 (first: overwrite) or a bf16 result
-__global__ void __launch_bounds__(256) product_kernel(Operand A, Operand B, int64_t M, int64_t N, int64_t K, float* acc32, int first, __nv_bfloat16* out,
-                                                      int64_t ld, GradRow g) {
-  const int64_t m0 = static_cast<int64_t>(blockIdx.x) * kTile, n0 = static_cast<int64_t>(blockIdx.y) * kTile;
-  float acc[4][4] = {};
-  tile_product(A, B, m0, n0, M, N, K, acc);
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t r = m0 + ty * 4 + i, c = n0 + tx * 4 + j;
-      if (r >= M || c >= N) continue;
-      if (out != nullptr) out[r * ld + c] = __float2bfloat16(acc[i][j] * g.scale());
-      else acc32[r * ld + c] = acc[i][j] + (first ? 0.f : acc32[r * ld + c]);
-    }
+template <int kPair, bool kAMn, bool kBMn, int kEpi>
+int launch_gemm(const Matrix& A, const Matrix& B, const Result& out, GemmParams p, const Plan& plan, int64_t K, int splits, cudaStream_t stream) {
+  p.M = kAMn ? A.cols : A.rows;
+  p.N = kBMn ? B.cols : B.rows;
+  p.m_tiles = plan.m_tiles;
+  p.n_tiles = plan.n_tiles;
+  p.bn = plan.bn;
+  p.k_blocks = static_cast<int>(cdiv(K, kBK));
+  p.kb_per_split = static_cast<int>(cdiv(p.k_blocks, splits));
+  p.splits = static_cast<int>(cdiv(p.k_blocks, p.kb_per_split));
+  const int stage = kABytes + plan.bn / kPair * kBK * 2;
+  p.stages = kStageBytes / stage < kMaxStages ? kStageBytes / stage : kMaxStages;
+  GemmMaps maps;
+  int rc = bind_context();
+  if (rc == JL_OK) rc = make_map2(&maps.a, A.p, A.rows, A.cols, A.ld, kBK, kAMn ? kBK : 128, false, 1, false);
+  if (rc == JL_OK) rc = make_map2(&maps.b, B.p, B.rows, B.cols, B.ld, kBK, kBMn ? kBK : plan.bn / kPair, false, 1, false);
+  if (rc == JL_OK && out.p != nullptr) rc = make_map2(&maps.out, out.p, p.M, p.N, out.ld, out.f32 ? 32 : 64, 32, out.f32, out.planes, true);
+  if (rc != JL_OK) return rc;
+  auto kernel = head_gemm_kernel<kPair, kAMn, kBMn, kEpi>;
+  static bool attr_set[64] = {false};
+  int dev = -1;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return fail(JL_ERR_LAUNCH, "jl_head: no current CUDA device");
+  if (!attr_set[dev]) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kGemmSmemBytes) != cudaSuccess)
+      return check_launch("jl_head (shared memory opt-in)");
+    attr_set[dev] = true;
+  }
+  const int64_t tiles = static_cast<int64_t>(p.m_tiles) * p.n_tiles * p.splits;
+  const int workers = static_cast<int>(tiles < kSms / kPair ? tiles : kSms / kPair);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(workers * kPair);
+  cfg.blockDim = dim3(kGemmThreads);
+  cfg.dynamicSmemBytes = kGemmSmemBytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = kPair;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, kernel, maps, p) != cudaSuccess) return check_launch("jl_head");
+  return JL_OK;
 }
 
-__global__ void __launch_bounds__(256) round_kernel(const float* x, __nv_bfloat16* out, int64_t n, GradRow g) {
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (i < n) out[i] = __float2bfloat16(x[i] * g.scale());
+int pair_of(int64_t rows) { return rows > 128 ? 2 : 1; }
+
+// Rows of m tiles whose A panel stays in L2 beside the streamed B: 40 MB of hidden states.
+int group_of(int64_t K, int pair) {
+  const int64_t g = (int64_t(40) << 20) / (K * 2 * 128 * pair);
+  return static_cast<int>(g < 1 ? 1 : g);
 }
 
-constexpr int kPiece = 8192;       // vocabulary rows per piece of the gradient pass
+// The tiles' partials take 12 bytes per row and tile; rows beyond 16384 go through the same workspace in further launches
+// (each reads the weight once more, 0.2 ms beside 14 ms of products at a hidden size of 4096).
+constexpr int64_t kScoreRows = 16384;
+struct ScoresLayout { Plan plan; size_t part, arg, picked, nll, total; };
+ScoresLayout scores_layout(int64_t rows, int32_t vocab) {
+  ScoresLayout l;
+  const int64_t n = rows < 1 ? 1 : rows < kScoreRows ? rows : kScoreRows;
+  l.plan = plan_tiles(n, vocab, pair_of(n), 16 * pair_of(n));
+  const size_t parts = static_cast<size_t>(n) * l.plan.n_tiles;
+  l.part = 0;
+  l.arg = up256(parts * sizeof(float2));
+  l.picked = l.arg + up256(parts * sizeof(int));
+  l.nll = l.picked + up256(n * sizeof(float));
+  l.total = l.nll + up256(static_cast<size_t>(rows) * sizeof(float));
+  return l;
+}
 
-size_t up256(size_t x) { return (x + 255) & ~size_t(255); }
+// Pieces of the vocabulary in the gradient pass: as large as 256 MB of dz allow (fewer, longer launches), balanced, a
+// multiple of 256.  K splits of the dh product: as many as fill the GPU when it has few tiles.
+struct GradsLayout { int64_t piece; Plan dz, dh, dw; int splits; size_t dh32, total; };
+GradsLayout grads_layout(int64_t rows, int32_t hd, int32_t vocab) {
+  GradsLayout l;
+  const int64_t n = rows > 0 ? rows : 1;
+  int64_t most = (int64_t(256) << 20) / (n * 2) / 256 * 256;
+  if (most < 2048) most = 2048;
+  const int64_t pieces = cdiv(vocab, most);
+  l.piece = cdiv(cdiv(vocab, pieces), 256) * 256;
+  l.dz = plan_tiles(n, l.piece < vocab ? l.piece : vocab, pair_of(n), 64);
+  l.dh = plan_tiles(n, hd, pair_of(n), 64 * pair_of(n));
+  l.dw = plan_tiles(l.piece < vocab ? l.piece : vocab, hd, 2, 128);
+  const int64_t tiles = static_cast<int64_t>(l.dh.m_tiles) * l.dh.n_tiles, k_blocks = cdiv(l.piece, kBK);
+  int64_t s = kSms / l.dh.pair / tiles;
+  if (s > k_blocks / 8) s = k_blocks / 8;
+  l.splits = static_cast<int>(s < 1 ? 1 : s);
+  l.splits = static_cast<int>(cdiv(k_blocks, cdiv(k_blocks, l.splits)));
+  l.dh32 = up256(static_cast<size_t>(n) * l.piece * 2);
+  l.total = l.dh32 + up256(static_cast<size_t>(n) * hd * 4 * l.splits);
+  return l;
+}
 
 int validate(const char* op, const void* hidden, const void* weight, int64_t hs, int64_t ws, int64_t rows, int32_t hd, int32_t vocab) {
   if (rows < 0 || hd < 1 || vocab < 1) return fail(JL_ERR_BAD_ARG, "%s: sizes out of range", op);
@@ -208,52 +606,54 @@ int validate(const char* op, const void* hidden, const void* weight, int64_t hs,
   return JL_OK;
 }
 
-}  // namespace
-
-static size_t scores_bytes(int64_t rows, int32_t vocab) {
-  const int64_t tiles = (vocab + kTile - 1) / kTile;
-  return up256(rows * tiles * sizeof(Partial)) + up256(rows * sizeof(float)) * 2;
-}
-
-static size_t grads_bytes(int64_t rows, int32_t hd, int32_t vocab) {
-  const int64_t piece = vocab < kPiece ? (vocab + 7) / 8 * 8 : kPiece;
-  return up256(rows * piece * 2) + up256(rows * static_cast<size_t>(hd) * 4);
-}
-
-static int launch_scores(const jl_head_scores_args* a, cudaStream_t stream) {
+int launch_scores(const jl_head_scores_args* a, cudaStream_t stream) {
   int rc = validate("jl_head_scores", a->hidden, a->weight, a->hidden_stride, a->weight_stride, a->rows, a->hidden_size, a->vocab);
   if (rc != JL_OK) return rc;
   if (a->labels == nullptr && (a->nll != nullptr || a->loss_sum != nullptr || a->loss_count != nullptr))
     return fail(JL_ERR_BAD_ARG, "jl_head_scores: nll and the loss need labels");
-  if (a->workspace == nullptr || a->workspace_bytes < scores_bytes(a->rows, a->vocab))
-    return fail(JL_ERR_WORKSPACE, "jl_head_scores: workspace of %zu bytes needed, %zu given", scores_bytes(a->rows, a->vocab), a->workspace_bytes);
+  const ScoresLayout l = scores_layout(a->rows, a->vocab);
+  if (a->workspace == nullptr || a->workspace_bytes < l.total)
+    return fail(JL_ERR_WORKSPACE, "jl_head_scores: workspace of %zu bytes needed, %zu given", l.total, a->workspace_bytes);
   if (reinterpret_cast<uintptr_t>(a->workspace) & 15) return fail(JL_ERR_BAD_ARG, "jl_head_scores: workspace not 16-byte aligned");
   rc = check_device_arch();
   if (rc != JL_OK) return rc;
-  const int tiles = (a->vocab + kTile - 1) / kTile;
-  Partial* part = static_cast<Partial*>(a->workspace);
-  float* picked = reinterpret_cast<float*>(static_cast<uint8_t*>(a->workspace) + up256(a->rows * static_cast<int64_t>(tiles) * sizeof(Partial)));
-  float* nll = a->nll != nullptr || a->loss_sum == nullptr ? a->nll : reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(picked) + up256(a->rows * sizeof(float)));
-  const Operand h{static_cast<const __nv_bfloat16*>(a->hidden), a->hidden_stride, 1}, w{static_cast<const __nv_bfloat16*>(a->weight), a->weight_stride, 1};
-  if (a->rows > 0) {
-    scores_kernel<<<dim3(tiles, static_cast<unsigned>((a->rows + kTile - 1) / kTile)), 256, 0, stream>>>(h, w, a->rows, a->vocab, a->hidden_size, a->labels, part, picked, tiles);
-    scores_fold_kernel<<<static_cast<unsigned>((a->rows + 3) / 4), 128, 0, stream>>>(part, picked, tiles, a->rows, a->vocab, a->labels, a->ignore_index, nll, a->lse, a->top);
+  uint8_t* ws = static_cast<uint8_t*>(a->workspace);
+  float* nll = a->nll != nullptr || a->loss_sum == nullptr ? a->nll : reinterpret_cast<float*>(ws + l.nll);
+  for (int64_t r0 = 0; r0 < a->rows; r0 += kScoreRows) {
+    const int64_t n = a->rows - r0 < kScoreRows ? a->rows - r0 : kScoreRows;
+    Plan plan = l.plan;
+    plan.m_tiles = static_cast<int>(cdiv(n, 128 * plan.pair));
+    GemmParams p{};
+    p.part = reinterpret_cast<float2*>(ws + l.part);
+    p.part_arg = a->top != nullptr ? reinterpret_cast<int*>(ws + l.arg) : nullptr;
+    p.picked = reinterpret_cast<float*>(ws + l.picked);
+    p.labels = a->labels != nullptr ? a->labels + r0 : nullptr;
+    p.ignore = a->ignore_index; p.vocab = a->vocab;
+    p.group_m = group_of(a->hidden_size, plan.pair);
+    const Matrix h{static_cast<const __nv_bfloat16*>(a->hidden) + r0 * a->hidden_stride, n, a->hidden_size, a->hidden_stride};
+    const Matrix w{a->weight, a->vocab, a->hidden_size, a->weight_stride};
+    rc = plan.pair == 2 ? launch_gemm<2, false, false, kEpiScores>(h, w, Result{}, p, plan, a->hidden_size, 1, stream)
+                        : launch_gemm<1, false, false, kEpiScores>(h, w, Result{}, p, plan, a->hidden_size, 1, stream);
+    if (rc != JL_OK) return rc;
+    scores_fold_kernel<<<static_cast<unsigned>(cdiv(n, 4)), 128, 0, stream>>>(
+        p.part, p.part_arg, p.picked, plan.n_tiles, n, a->vocab, p.labels, a->ignore_index, nll != nullptr ? nll + r0 : nullptr,
+        a->lse != nullptr ? a->lse + r0 : nullptr, a->top != nullptr ? a->top + r0 : nullptr);
   }
   if (a->loss_sum != nullptr || a->loss_count != nullptr)
     loss_sum_kernel<<<1, 1024, 0, stream>>>(nll, a->labels, a->ignore_index, a->rows, a->loss_sum, a->loss_count);
   return check_launch("jl_head_scores");
 }
 
-static int launch_grads(const jl_head_grads_args* a, cudaStream_t stream) {
+int launch_grads(const jl_head_grads_args* a, cudaStream_t stream) {
   int rc = validate("jl_head_grads", a->hidden, a->weight, a->hidden_stride, a->weight_stride, a->rows, a->hidden_size, a->vocab);
   if (rc != JL_OK) return rc;
   if (a->labels == nullptr || a->lse == nullptr || a->grad == nullptr) return fail(JL_ERR_BAD_ARG, "jl_head_grads: NULL pointer");
   if (a->grad_stride != 0 && a->grad_stride != 1) return fail(JL_ERR_BAD_ARG, "jl_head_grads: grad_stride must be 0 or 1");
   if ((reinterpret_cast<uintptr_t>(a->d_hidden) | reinterpret_cast<uintptr_t>(a->d_weight)) & 15)
     return fail(JL_ERR_BAD_ARG, "jl_head_grads: d_hidden and d_weight must be 16-byte aligned");
-  const size_t need = grads_bytes(a->rows, a->hidden_size, a->vocab);
-  if (a->workspace == nullptr || a->workspace_bytes < need)
-    return fail(JL_ERR_WORKSPACE, "jl_head_grads: workspace of %zu bytes needed, %zu given", need, a->workspace_bytes);
+  const GradsLayout l = grads_layout(a->rows, a->hidden_size, a->vocab);
+  if (a->workspace == nullptr || a->workspace_bytes < l.total)
+    return fail(JL_ERR_WORKSPACE, "jl_head_grads: workspace of %zu bytes needed, %zu given", l.total, a->workspace_bytes);
   if (reinterpret_cast<uintptr_t>(a->workspace) & 15) return fail(JL_ERR_BAD_ARG, "jl_head_grads: workspace not 16-byte aligned");
   rc = check_device_arch();
   if (rc != JL_OK) return rc;
@@ -262,34 +662,61 @@ static int launch_grads(const jl_head_grads_args* a, cudaStream_t stream) {
     if (a->d_weight != nullptr && cudaMemsetAsync(a->d_weight, 0, V * H * 2, stream) != cudaSuccess) return check_launch("jl_head_grads");
     return JL_OK;
   }
-  const int ld = static_cast<int>(V < kPiece ? (V + 7) / 8 * 8 : kPiece);
-  __nv_bfloat16* dz = static_cast<__nv_bfloat16*>(a->workspace);
-  float* dh32 = reinterpret_cast<float*>(static_cast<uint8_t*>(a->workspace) + up256(N * static_cast<size_t>(ld) * 2));
-  const Operand h{static_cast<const __nv_bfloat16*>(a->hidden), a->hidden_stride, 1}, w{static_cast<const __nv_bfloat16*>(a->weight), a->weight_stride, 1};
-  const GradRow g{a->labels, a->ignore_index, a->lse, a->grad, a->grad_count, a->grad_stride};
-  auto cdiv = [](int64_t x, int64_t y) { return static_cast<unsigned>((x + y - 1) / y); };
-  for (int64_t v0 = 0; v0 < V; v0 += kPiece) {
-    const int piece = static_cast<int>(V - v0 < kPiece ? V - v0 : kPiece);
-    dz_kernel<<<dim3(cdiv(ld, kTile), cdiv(N, kTile)), 256, 0, stream>>>(h, w, N, a->vocab, a->hidden_size, static_cast<int>(v0), piece, g, dz, ld);
-    if (a->d_hidden != nullptr) {
-      const Operand A{dz, ld, 1}, B{w.p + v0 * w.sr, 1, w.sr};
-      product_kernel<<<dim3(cdiv(N, kTile), cdiv(H, kTile)), 256, 0, stream>>>(A, B, N, H, piece, dh32, v0 == 0, nullptr, H, g);
+  uint8_t* ws = static_cast<uint8_t*>(a->workspace);
+  float* dh32 = reinterpret_cast<float*>(ws + l.dh32);
+  GemmParams base{};
+  base.labels = a->labels; base.ignore = a->ignore_index; base.vocab = V;
+  base.lse = a->lse;
+  base.row_grad = a->grad_stride != 0 ? a->grad : nullptr;
+  base.scale = GradScale{a->grad, a->grad_count, a->grad_stride != 0};
+  const Matrix h{a->hidden, N, H, a->hidden_stride};
+  int splits = 1;
+  for (int64_t v0 = 0; v0 < V; v0 += l.piece) {
+    const int64_t piece = V - v0 < l.piece ? V - v0 : l.piece;
+    const Matrix w{static_cast<const __nv_bfloat16*>(a->weight) + v0 * a->weight_stride, piece, H, a->weight_stride};
+    const Matrix dz{ws, N, piece, l.piece};
+    const Result dz_out{ws, l.piece, false, 1};
+    GemmParams p = base;
+    p.v0 = v0;
+    p.group_m = group_of(H, l.dz.pair);
+    Plan plan = l.dz;
+    plan.n_tiles = static_cast<int>(cdiv(piece, plan.bn));
+    rc = plan.pair == 2 ? launch_gemm<2, false, false, kEpiDz>(h, w, dz_out, p, plan, H, 1, stream)
+                        : launch_gemm<1, false, false, kEpiDz>(h, w, dz_out, p, plan, H, 1, stream);
+    if (rc == JL_OK && a->d_hidden != nullptr) {
+      p = base;
+      p.reduce = v0 > 0;
+      p.group_m = 1 << 20;
+      const Result out{dh32, H, true, l.splits};
+      const int64_t kb = cdiv(piece, kBK);
+      // a short last piece has fewer K splits than the others: the planes it does not reach keep their sums
+      const int s = static_cast<int>(kb < l.splits ? kb : l.splits);
+      rc = l.dh.pair == 2 ? launch_gemm<2, false, true, kEpiF32>(dz, w, out, p, l.dh, piece, s, stream)
+                          : launch_gemm<1, false, true, kEpiF32>(dz, w, out, p, l.dh, piece, s, stream);
+      if (v0 == 0) splits = static_cast<int>(cdiv(kb, cdiv(kb, s)));
     }
-    if (a->d_weight != nullptr) {
-      const Operand A{dz, 1, ld}, B{h.p, 1, h.sr};
-      product_kernel<<<dim3(cdiv(piece, kTile), cdiv(H, kTile)), 256, 0, stream>>>(A, B, piece, H, N, nullptr, 0, static_cast<__nv_bfloat16*>(a->d_weight) + v0 * H, H, g);
+    if (rc == JL_OK && a->d_weight != nullptr) {
+      p = base;
+      p.group_m = 0;
+      plan = l.dw;
+      plan.m_tiles = static_cast<int>(cdiv(piece, 256));
+      rc = launch_gemm<2, true, true, kEpiBf16>(dz, h, Result{static_cast<__nv_bfloat16*>(a->d_weight) + v0 * H, H, false, 1}, p, plan, N, 1, stream);
     }
+    if (rc != JL_OK) return rc;
   }
-  if (a->d_hidden != nullptr) round_kernel<<<cdiv(N * H, 256), 256, 0, stream>>>(dh32, static_cast<__nv_bfloat16*>(a->d_hidden), N * H, g);
+  if (a->d_hidden != nullptr)
+    grad_round_kernel<<<static_cast<unsigned>(cdiv(N * H, 1024)), 256, 0, stream>>>(dh32, splits, N * H, static_cast<__nv_bfloat16*>(a->d_hidden), base.scale);
   return check_launch("jl_head_grads");
 }
+
+}  // namespace
 
 }  // namespace jl
 
 extern "C" {
 
 size_t jl_head_scores_workspace_bytes(int64_t rows, int32_t hidden_size, int32_t vocab) {
-  return rows < 0 || hidden_size < 1 || vocab < 1 ? 0 : jl::scores_bytes(rows, vocab) + 256;
+  return rows < 0 || hidden_size < 1 || vocab < 1 ? 0 : jl::scores_layout(rows, vocab).total + 256;
 }
 
 int jl_head_scores(const jl_head_scores_args* args, void* cuda_stream) {
@@ -298,12 +725,20 @@ int jl_head_scores(const jl_head_scores_args* args, void* cuda_stream) {
 }
 
 size_t jl_head_grads_workspace_bytes(int64_t rows, int32_t hidden_size, int32_t vocab) {
-  return rows < 0 || hidden_size < 1 || vocab < 1 ? 0 : jl::grads_bytes(rows, hidden_size, vocab) + 256;
+  return rows < 0 || hidden_size < 1 || vocab < 1 ? 0 : jl::grads_layout(rows, hidden_size, vocab).total + 256;
 }
 
 int jl_head_grads(const jl_head_grads_args* args, void* cuda_stream) {
   if (args == nullptr) return jl::fail(JL_ERR_BAD_ARG, "jl_head_grads: args is NULL");
   return jl::launch_grads(args, static_cast<cudaStream_t>(cuda_stream));
+}
+
+int jl_head_status(void) {
+  int v = 0;
+  if (cudaMemcpyFromSymbol(&v, jl::g_head_status, sizeof(int)) != cudaSuccess) return -1;
+  const int zero = 0;
+  if (v != 0) cudaMemcpyToSymbol(jl::g_head_status, &zero, sizeof(int));
+  return v;
 }
 
 }  // extern "C"

@@ -228,6 +228,7 @@ HEAD_EXPORTS = [
     ("jl_head_scores", C.c_int, [C.POINTER(HeadScoresArgs), C.c_void_p]),
     ("jl_head_grads_workspace_bytes", C.c_size_t, [C.c_int64, C.c_int32, C.c_int32]),
     ("jl_head_grads", C.c_int, [C.POINTER(HeadGradsArgs), C.c_void_p]),
+    ("jl_head_status", C.c_int, []),
 ]
 
 _LIB = None
