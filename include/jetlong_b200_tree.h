@@ -105,6 +105,10 @@ typedef struct {
 size_t jl_tree_attention_workspace_bytes(int32_t batch, int32_t nodes, int32_t heads, int32_t kv_heads, int32_t rows);
 int jl_tree_attention(const jl_tree_attention_args* args, void* cuda_stream);
 
+/* Diagnostic (synchronises the device): non-zero if a bounded wait (1 s) inside jl_tree_attention has given up on the
+ * current device since the last call; reading a raised status clears it.  The results since the last call are then invalid. */
+int jl_tree_status(void);
+
 #ifdef __cplusplus
 }
 #endif

@@ -168,6 +168,7 @@ int launch_tree_append(const jl_tree_append_args* a, cudaStream_t stream) {
 }  // namespace
 
 int launch_tree_attention(const jl_tree_attention_args* a, cudaStream_t stream);
+int tree_status();
 size_t tree_attention_workspace_bytes(int32_t batch, int32_t nodes, int32_t heads, int32_t kv_heads, int32_t rows);
 
 static int validate_tree_attention(const jl_tree_attention_args* a) {
@@ -192,6 +193,9 @@ static int validate_tree_attention(const jl_tree_attention_args* a) {
                         a->v_stride_b, a->v_stride_s, a->v_stride_h, a->o_stride_b, a->o_stride_s, a->o_stride_h};
   for (int64_t x : st)
     if (x % 8 != 0) return fail(JL_ERR_BAD_ARG, "jl_tree_attention: strides must be multiples of 8 elements (16 bytes)");
+  const int64_t size[] = {a->batch, a->nodes, a->heads, a->batch, a->rows, a->kv_heads, a->batch, a->rows, a->kv_heads, a->batch, a->nodes, a->heads};
+  for (int i = 0; i < 12; ++i)
+    if (size[i] > 1 && st[i] <= 0) return fail(JL_ERR_UNSUPPORTED, "jl_tree_attention: a dimension larger than 1 needs a positive stride");
   return JL_OK;
 }
 
@@ -222,5 +226,7 @@ int jl_tree_attention(const jl_tree_attention_args* args, void* cuda_stream) {
   if (rc != JL_OK) return rc;
   return jl::launch_tree_attention(args, static_cast<cudaStream_t>(cuda_stream));
 }
+
+int jl_tree_status(void) { return jl::tree_status(); }
 
 }  // extern "C"

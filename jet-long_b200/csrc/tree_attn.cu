@@ -1,80 +1,696 @@
-// Attention of a tree of drafted tokens over the bifocal cache.
+// Attention of a tree of drafted tokens over the bifocal cache, on the Blackwell tensor path.
 //
-// One block per (node, head, sample): its warps take the keys in turn, one key per step with 4 dimensions a lane, and
-// keep a running (maximum, sum, output) in fp32; the warps' states are merged through shared memory.
-#include "jl_common.cuh"
+// The rows of one product are the (node, query head) pairs that share a key head: row r of a 128-row tile is node
+// r / rep, head r % rep of the key head's group (rep = heads / kv_heads), so one pass over the cache serves every drafted
+// token.  A tree of up to 128 rows per key head takes ONE row tile, whose two softmax warpgroups work on alternate key
+// tiles of the same rows (two running states, joined at the end); a larger tree takes TWO row tiles per CTA, and further
+// CTAs that walk the same keys at the same time for its further rows.
+//
+// Work is a line of VISITS: for every (sample, key head) the key tiles of the far class, then those of the near class (a
+// tile crossed by the boundary is visited in both with complementary masks).  The line is cut into equal parts, one per
+// SM, wherever that falls, so a batch of any lengths fills the GPU evenly; a part is made of SEGMENTS of one (sample, key
+// head) each, and every segment leaves one normalised fp32 partial (O, LSE) per row that tree_combine_kernel joins.
+// Nothing on the host depends on the lengths, which are read on the device.
+//
+//   warp 0      TMA producer of K (ring of 3) and V (ring of 2), running ahead over class and segment borders
+//   warp 1      MMA issuer: S_t = Q K^T two items ahead of O_t += P V
+//   warp 2      tensor memory; zeroes the value rows behind the last node, which may hold anything (0 * NaN is NaN)
+//   warp 3      TMA producer of the query tiles of the current class
+//   warps 4-11  softmax: one thread per row, 128 scores in registers, P back to tensor memory over S
+#include "tc_common.cuh"
 #include "../../include/jetlong_b200_tree.h"
 
 namespace jl {
 
 namespace {
 
-constexpr int kWarps = 8;
+using namespace tc;
 
-__global__ void __launch_bounds__(kWarps * 32) tree_attention_kernel(const jl_tree_attention_args a) {
-  const int t = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int kvh = h / (a.heads / a.kv_heads);
-  const int T = a.nodes, words = (T + 63) / 64;
-  const int len = min(max(a.lens[b], 0), a.rows - T);
-  const int64_t node = static_cast<int64_t>(b) * T + t;
-  const int d = a.depth[node];
-  auto row4 = [&](const void* base, int64_t off) {
-    const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(base) + off + 4 * lane);
-    const float2 x = unpack_bf16x2(u.x), y = unpack_bf16x2(u.y);
-    return make_float4(x.x, x.y, y.x, y.y);
-  };
-  const int64_t q_off = b * a.q_stride_b + t * a.q_stride_s + h * a.q_stride_h;
-  const float4 qb = row4(a.q_base, q_off), qg = a.q_group != nullptr ? row4(a.q_group, q_off) : qb;
-  float m = -INFINITY, l = 0.f;
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  const int n = d < 0 ? 0 : len + T;
-  for (int j = warp; j < n; j += kWarps) {
-    int pk = j;
-    if (j >= len) {
-      const int u = j - len;
-      if (!((a.mask[node * words + (u >> 6)] >> (u & 63)) & 1)) continue;
-      pk = len + a.depth[static_cast<int64_t>(b) * T + u];
+__device__ int g_tree_status = 0;            // raised when a bounded wait gave up
+
+constexpr int kTileN = 128;                  // keys per visit
+constexpr int kKStages = 3, kVStages = 2;
+constexpr int kTileBytes = 128 * 256;        // 128 rows x 128 bf16
+constexpr int kHalfBytes = 128 * 128;        // one 64-column half (a TMA box)
+constexpr int kThreads = 384;
+constexpr int kRegsLow = 72, kRegsHigh = 216;     // 128 x 72 + 256 x 216 = the launch total 384 x 168
+constexpr int kSms = 148;
+constexpr unsigned kPolyMask = 0x11;         // of every 8 score pairs these two take the FMA-pipe exponential
+
+struct TreeParams {
+  int batch, nodes, words, rep, kv_heads, rows;
+  int npt;                     // nodes per row tile
+  int rpt;                     // rows per row tile that can be in use
+  int two_tiles;               // two row tiles per CTA instead of two states of one
+  int mbs, workers;            // CTAs per part of the line, parts
+  int two_classes, nodes_far;  // nodes_far: w_0 is so small that drafted keys can be in the far class
+  int64_t w_0;
+  float scale_log2;
+  const int32_t *lens, *depth;
+  const uint64_t* mask;
+  float *part_o, *part_lse;    // [slot][state or tile][rpt] rows
+  __nv_bfloat16* out;
+  float* lse;
+  int64_t os_b, os_s, os_h;
+};
+
+struct TreeMaps { CUtensorMap q[2], k[2], v; };       // [0] near (base), [1] far (regrouped)
+
+struct TreeSmem {
+  alignas(1024) uint8_t q[2][kTileBytes];    // two row tiles, or two class operands of one
+  alignas(1024) uint8_t k[kKStages][kTileBytes];
+  alignas(1024) uint8_t v[kVStages][kTileBytes];
+  uint64_t q_full[2], q_free[2], k_full[kKStages], k_empty[kKStages], v_full[kVStages], v_empty[kVStages];
+  uint64_t s_full[2], p_half[2][2], v_clean[kVStages], all_done;
+  int64_t lo, hi;                            // this CTA's part of the line
+  int start_b, start_kvh, start_v;
+  uint32_t tmem_base;
+  int failed;
+};
+
+// The visits of one (sample, key head): far key tiles [0, far), then near key tiles near0 ..
+struct Visits { int len, far, near0, n; };
+__device__ __forceinline__ Visits visits_of(const TreeParams& p, int b) {
+  Visits v;
+  v.len = min(max(p.lens[b], 0), p.rows - p.nodes);
+  const int64_t end = v.len + p.nodes;
+  v.far = v.near0 = 0;
+  if (p.two_classes) {
+    int64_t hi = p.nodes_far ? end : v.len + p.nodes - 1 - p.w_0;              // keys below this can be far for some node
+    hi = hi < 0 ? 0 : (hi > end ? end : hi);
+    v.far = static_cast<int>((hi + kTileN - 1) / kTileN);
+    const int64_t lo = v.len - p.w_0;                                          // keys from this on can be near
+    v.near0 = static_cast<int>((lo < 0 ? 0 : lo) / kTileN);
+  }
+  v.n = v.far + static_cast<int>((end + kTileN - 1) / kTileN) - v.near0;
+  return v;
+}
+
+// Parts that the line is cut into: one per worker, but none empty.
+__device__ __forceinline__ int64_t parts_of(const TreeParams& p, int64_t total) { return min(static_cast<int64_t>(p.workers), total); }
+
+struct Segment {
+  int b, kvh, v0, v1;          // visits [v0, v1)
+  Visits vis;
+  __device__ __forceinline__ int key_tile(int v) const { return v < vis.far ? v : vis.near0 + v - vis.far; }
+  __device__ __forceinline__ bool tail(int v) const { return (key_tile(v) + 1) * kTileN > vis.len; }     // holds rows that are not committed
+};
+
+struct Walk {
+  int b, kvh, v;
+  int64_t left;
+  __device__ __forceinline__ explicit Walk(const TreeSmem& sm) : b(sm.start_b), kvh(sm.start_kvh), v(sm.start_v), left(sm.hi - sm.lo) {}
+  __device__ __forceinline__ bool next(const TreeParams& p, Segment& s) {
+    if (left <= 0) return false;
+    s.b = b;
+    s.kvh = kvh;
+    s.vis = visits_of(p, b);
+    s.v0 = v;
+    s.v1 = static_cast<int>(min(static_cast<int64_t>(s.vis.n), v + left));
+    left -= s.v1 - s.v0;
+    v = 0;
+    if (++kvh == p.kv_heads) { kvh = 0; ++b; }
+    return true;
+  }
+};
+
+// Products in issue order.  Two row tiles: (visit, 0), (visit, 1); one: (visit, alternating state).  Consecutive items never
+// share a state, whatever segment they belong to.
+struct Item { int t, cls, visit, use; bool first_use, last_use, q_first, q_last, o_first, tail; };
+struct Items {
+  Walk w;
+  Segment seg;
+  int v, t, visit, use;
+  bool open;
+  __device__ __forceinline__ explicit Items(const TreeSmem& sm) : w(sm), v(0), t(0), visit(-1), use(-1), open(false) {}
+  __device__ __forceinline__ bool next(const TreeParams& p, Item& it) {
+    if (open && p.two_tiles && t == 0) {
+      t = 1;                                           // the second row tile of the same visit
+    } else {
+      if (!open || v + 1 == seg.v1) {
+        if (!w.next(p, seg)) return false;
+        open = true;
+        v = seg.v0;
+      } else {
+        ++v;
+      }
+      ++visit;
+      t = p.two_tiles ? 0 : visit & 1;
     }
-    const bool far = a.q_group != nullptr && len + d - pk > a.w_0;
-    const float4 k = row4(far ? a.k_group : a.k_base, b * a.k_stride_b + j * a.k_stride_s + kvh * a.k_stride_h);
-    const float4 q = far ? qg : qb;
-    float s = q.x * k.x + q.y * k.y + q.z * k.z + q.w * k.w;
+    const bool class_start = v == seg.v0 || v == seg.vis.far, class_end = v + 1 == seg.v1 || v + 1 == seg.vis.far;
+    it.first_use = !p.two_tiles || t == 0;
+    it.last_use = !p.two_tiles || t == 1;
+    it.q_first = class_start && it.first_use;
+    it.q_last = class_end && it.last_use;
+    if (it.q_first) ++use;
+    it.t = t;
+    it.cls = v < seg.vis.far;
+    it.visit = visit;
+    it.use = use;
+    it.o_first = v - seg.v0 < (p.two_tiles ? 1 : 2);
+    it.tail = seg.tail(v);
+    return true;
+  }
+};
+
+__global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __grid_constant__ TreeMaps maps, const TreeParams p) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  TreeSmem& sm = *reinterpret_cast<TreeSmem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int mb = static_cast<int>(blockIdx.x) % p.mbs, worker = static_cast<int>(blockIdx.x) / p.mbs;
+  const int q_slots = p.two_tiles ? 1 : 2;
+
+  if (warp == 0) {
+    // ---- this CTA's part of the line of visits: total and start, 32 samples at a time ----
+    int64_t total = 0;
+    for (int b0 = 0; b0 < p.batch; b0 += 32) total += b0 + lane < p.batch ? visits_of(p, b0 + lane).n : 0;
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-    s *= a.softmax_scale;
-    const float4 v = row4(a.v, b * a.v_stride_b + j * a.v_stride_s + kvh * a.v_stride_h);
-    const float mn = fmaxf(m, s), f = expf(m - mn), e = expf(s - mn);
-    m = mn;
-    l = l * f + e;
-    o.x = o.x * f + e * v.x; o.y = o.y * f + e * v.y; o.z = o.z * f + e * v.z; o.w = o.w * f + e * v.w;
+    for (int off = 16; off > 0; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
+    total *= p.kv_heads;
+    const int64_t parts = parts_of(p, total), lo = min(static_cast<int64_t>(worker), parts) * total / parts;
+    const int64_t hi = min(static_cast<int64_t>(worker) + 1, parts) * total / parts;
+    int64_t base = 0;
+    for (int b0 = 0; b0 < p.batch; b0 += 32) {
+      const int64_t mine = b0 + lane < p.batch ? static_cast<int64_t>(visits_of(p, b0 + lane).n) * p.kv_heads : 0;
+      int64_t before = mine;                           // inclusive prefix sum over the 32 samples
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const int64_t o = __shfl_up_sync(0xffffffffu, before, off);
+        if (lane >= off) before += o;
+      }
+      const int64_t from = base + before - mine;
+      if (mine > 0 && lo >= from && lo < from + mine) {
+        const int n = static_cast<int>(mine / p.kv_heads);
+        sm.start_b = b0 + lane;
+        sm.start_kvh = static_cast<int>((lo - from) / n);
+        sm.start_v = static_cast<int>((lo - from) % n);
+      }
+      base += __shfl_sync(0xffffffffu, before, 31);
+    }
+    if (lane == 0) { sm.lo = lo; sm.hi = hi; }
   }
-  __shared__ float sm[kWarps], sl[kWarps], so[kWarps][kHeadDim];
-  *reinterpret_cast<float4*>(&so[warp][4 * lane]) = o;
-  if (lane == 0) { sm[warp] = m; sl[warp] = l; }
+  if (threadIdx.x == 32) {
+    sm.failed = *reinterpret_cast<volatile int*>(&g_tree_status) != 0 ? 1 : 0;
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sm.q_full[i], 1);
+      mbar_init(&sm.q_free[i], 1);
+      mbar_init(&sm.s_full[i], 1);
+      mbar_init(&sm.p_half[i][0], 128);
+      mbar_init(&sm.p_half[i][1], 128);
+    }
+    for (int i = 0; i < kKStages; ++i) { mbar_init(&sm.k_full[i], 1); mbar_init(&sm.k_empty[i], 1); }
+    for (int i = 0; i < kVStages; ++i) { mbar_init(&sm.v_full[i], 1); mbar_init(&sm.v_empty[i], 1); mbar_init(&sm.v_clean[i], 32); }
+    mbar_init(&sm.all_done, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 2) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem_base)), "r"(512u));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+  }
+  tc_fence_before();
   __syncthreads();
-  if (threadIdx.x >= kHeadDim) return;
-  float M = -INFINITY, L = 0.f, acc = 0.f;
-  for (int w = 0; w < kWarps; ++w) M = fmaxf(M, sm[w]);
-  for (int w = 0; w < kWarps && M != -INFINITY; ++w) {
-    const float f = expf(sm[w] - M);
-    L += sl[w] * f;
-    acc += so[w][threadIdx.x] * f;
+  tc_fence_after();
+  const uint32_t tmem = sm.tmem_base;
+  volatile int* const failed = &sm.failed;       // a wait gave up: no more copies are issued, every later wait returns at once
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsLow));
+    if (warp == 0) {
+      // ================================ TMA producer of K and V ================================
+      if (lane == 0) {
+        Walk w(sm);
+        Segment seg;
+        int g = 0;
+        while (w.next(p, seg)) {
+          for (int v = seg.v0; v < seg.v1; ++v, ++g) {
+            const CUtensorMap* km = &maps.k[v < seg.vis.far ? 1 : 0];
+            const int row = seg.key_tile(v) * kTileN, ks = g % kKStages, vs = g % kVStages;
+            mbar_wait(&sm.k_empty[ks], ((g / kKStages) & 1) ^ 1, sm);
+            if (*failed) break;
+            mbar_expect_tx(&sm.k_full[ks], kTileBytes);
+            for (int h = 0; h < 2; ++h) tma_load_4d(sm.k[ks] + h * kHalfBytes, km, &sm.k_full[ks], h * 64, seg.kvh, row, seg.b);
+            mbar_wait(&sm.v_empty[vs], ((g / kVStages) & 1) ^ 1, sm);
+            if (*failed) break;
+            mbar_expect_tx(&sm.v_full[vs], kTileBytes);
+            for (int h = 0; h < 2; ++h) tma_load_4d(sm.v[vs] + h * kHalfBytes, &maps.v, &sm.v_full[vs], h * 64, seg.kvh, row, seg.b);
+          }
+        }
+      }
+    } else if (warp == 3) {
+      // ================================ TMA producer of the queries ================================
+      if (lane == 0) {
+        Walk w(sm);
+        Segment seg;
+        int u = 0;
+        const uint32_t half = static_cast<uint32_t>(p.npt) * p.rep * 128;
+        while (w.next(p, seg)) {
+          for (int cls = 1; cls >= 0; --cls) {
+            const bool any = cls == 1 ? seg.v0 < seg.vis.far : seg.v1 > seg.vis.far;
+            if (!any) continue;
+            const int slot = u % q_slots;
+            mbar_wait(&sm.q_free[slot], ((u / q_slots) & 1) ^ 1, sm);
+            if (*failed) break;
+            mbar_expect_tx(&sm.q_full[slot], (p.two_tiles ? 4 : 2) * half);
+            for (int t = 0; t < (p.two_tiles ? 2 : 1); ++t)
+              for (int h = 0; h < 2; ++h)
+                tma_load_4d(sm.q[slot + t] + h * kHalfBytes, &maps.q[cls], &sm.q_full[slot], h * 64, seg.kvh * p.rep, (mb * 2 + t) * p.npt, seg.b);
+            ++u;
+          }
+        }
+      }
+    } else if (warp == 1) {
+      // ====================================== MMA issuer ======================================
+      uint32_t leader;
+      asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(leader));
+      const uint32_t idesc_qk = instr_desc(128, kTileN, 0), idesc_pv = instr_desc(128, kHeadDim, 1);
+      const uint64_t q_desc = smem_desc(smem_u32(sm.q[0]), 16, 1024), k_desc = smem_desc(smem_u32(sm.k[0]), 16, 1024);
+      const uint64_t v_desc = smem_desc(smem_u32(sm.v[0]), kHalfBytes, 1024);
+      Items ahead(sm), now(sm);
+      Item it;
+      auto issue_qk = [&]() {                          // the next item's scores, if there is one
+        Item n;
+        if (!ahead.next(p, n)) return;
+        const int ks = n.visit % kKStages, slot = n.use % q_slots;
+        if (n.q_first) mbar_wait(&sm.q_full[slot], (n.use / q_slots) & 1, sm);
+        if (n.first_use) mbar_wait(&sm.k_full[ks], (n.visit / kKStages) & 1, sm);
+        tc_fence_after();
+        const uint64_t qd = q_desc + static_cast<uint64_t>(((p.two_tiles ? n.t : slot) * kTileBytes) >> 4);
+        const uint64_t kd = k_desc + static_cast<uint64_t>((ks * kTileBytes) >> 4);
+        if (leader) {
+#pragma unroll
+          for (int kk = 0; kk < 8; ++kk) {
+            const uint64_t off = static_cast<uint64_t>(((kk >> 2) * kHalfBytes + (kk & 3) * 32) >> 4);
+            mma_ss(tmem + n.t * 128, qd + off, kd + off, idesc_qk, kk > 0);
+          }
+          mma_commit(&sm.s_full[n.t]);
+          if (n.last_use) mma_commit(&sm.k_empty[ks]);
+          if (n.q_last) mma_commit(&sm.q_free[slot]);
+        }
+        __syncwarp();
+      };
+      issue_qk();
+      issue_qk();
+      int done[2] = {0, 0}, cleaned[kVStages] = {0, 0};
+      while (now.next(p, it)) {
+        const int vs = it.visit % kVStages;
+        const uint64_t vd = v_desc + static_cast<uint64_t>((vs * kTileBytes) >> 4);
+        const int parity = (it.t ? done[1] : done[0]) & 1;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          mbar_wait(&sm.p_half[it.t][h], parity, sm);
+          if (h == 0 && it.first_use) {
+            mbar_wait(&sm.v_full[vs], (it.visit / kVStages) & 1, sm);
+            if (it.tail) {
+              mbar_wait(&sm.v_clean[vs], (vs ? cleaned[1] : cleaned[0]) & 1, sm);
+              if (vs) ++cleaned[1]; else ++cleaned[0];
+            }
+          }
+          tc_fence_after();
+          if (leader) {
+#pragma unroll
+            for (int kk = 4 * h; kk < 4 * h + 4; ++kk)
+              mma_ts(tmem + 256 + it.t * 128, tmem + it.t * 128 + kk * 8, vd + static_cast<uint64_t>((kk * 2048) >> 4), idesc_pv,
+                     (!it.o_first || kk > 0) ? 1u : 0u);
+            if (h == 1 && it.last_use) mma_commit(&sm.v_empty[vs]);
+          }
+          __syncwarp();
+        }
+        if (it.t) ++done[1]; else ++done[0];
+        issue_qk();
+      }
+      if (leader) mma_commit(&sm.all_done);
+      __syncwarp();
+    } else {
+      // ============================ value rows that belong to nobody ============================
+      Walk w(sm);
+      Segment seg;
+      int g = 0;
+      while (w.next(p, seg)) {
+        for (int v = seg.v0; v < seg.v1; ++v, ++g) {
+          if (!seg.tail(v)) continue;
+          const int vs = g % kVStages;
+          mbar_wait(&sm.v_full[vs], (g / kVStages) & 1, sm);
+          for (int r0 = 0; r0 < kTileN; r0 += 32) {
+            const int u = seg.key_tile(v) * kTileN + r0 + lane - seg.vis.len;      // node index
+            const bool keep = u < 0 || (u < p.nodes && p.depth[static_cast<int64_t>(seg.b) * p.nodes + u] >= 0);
+            for (uint32_t dead = __ballot_sync(0xffffffffu, !keep); dead != 0u; dead &= dead - 1)
+              if (lane < 16)
+                *reinterpret_cast<uint4*>(sm.v[vs] + (lane >> 3) * kHalfBytes + (r0 + __ffs(dead) - 1) * 128 + (lane & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          mbar_arrive(&sm.v_clean[vs]);
+        }
+      }
+    }
+  } else {
+    // ===================================== softmax =====================================
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsHigh));
+    const int t = (warp - 4) >> 2, quad = warp & 3;
+    const int r = quad * 32 + lane;
+    const int node = p.two_tiles ? (mb * 2 + t) * p.npt + r / p.rep : r / p.rep;
+    const bool row_used = r < p.npt * p.rep && node < p.nodes;
+    const uint32_t lane_base = static_cast<uint32_t>(quad * 32) << 16;
+    const uint32_t t_s = tmem + lane_base + t * 128;        // my row of scores; the bf16 P overlays its first 64 columns
+    const uint32_t t_o = tmem + lane_base + 256 + t * 128;  // my row of the output accumulator
+    const uint64_t scale2 = pack2(p.scale_log2, p.scale_log2);
+
+    float m_ref = -INFINITY, l_sum = 0.f;
+    auto exp_block = [&](const uint32_t (&s)[128], int e0, uint64_t negm2, uint32_t col, uint64_t (&acc2)[4]) {
+      uint32_t pk[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int e = e0 + 2 * i;
+        const uint64_t x = fma2(pack2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), scale2, negm2);
+        const uint64_t pp = ((kPolyMask >> (i & 7)) & 1u) ? exp2_pair_fma(x) : exp2_pair_sfu(x);
+        acc2[i & 3] = add2(acc2[i & 3], pp);
+        float p0, p1;
+        unpack2(pp, p0, p1);
+        pk[i] = pack_bf16x2(p0, p1);
+      }
+      JL_TMEM_ST16(t_s + col, pk, 0);
+    };
+    auto max_block = [&](const uint32_t (&s)[128], int e0, float (&m4)[4]) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) m4[i & 3] = max3(m4[i & 3], __uint_as_float(s[e0 + 2 * i]), __uint_as_float(s[e0 + 2 * i + 1]));
+    };
+    auto publish = [&](int half) {
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(&sm.p_half[t][half]);
+    };
+    // the partial of a finished segment: O / l in fp32 and the LSE in the log2 domain
+    auto leave_partial = [&](const Segment& s, int d, bool any) {
+      const int64_t slot = static_cast<int64_t>(mb) * (p.workers + p.batch * p.kv_heads) + worker + s.b * p.kv_heads + s.kvh;
+      const int64_t prow = (slot * 2 + t) * p.rpt + r;
+      const bool seen = any && d >= 0 && m_ref != -INFINITY;          // masked scores add ~1e-38 each to l_sum, never to m_ref
+      const float inv = seen ? 1.f / l_sum : 0.f;
+      if (any) {
+#pragma unroll
+        for (int ch = 0; ch < 4; ++ch) {
+          uint32_t o[32];
+          JL_TMEM_LD32(t_o + ch * 32, o, 0);
+          tmem_wait_ld();
+          if (row_used && seen) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              *reinterpret_cast<float4*>(p.part_o + prow * kHeadDim + ch * 32 + 4 * i) =
+                  make_float4(__uint_as_float(o[4 * i]) * inv, __uint_as_float(o[4 * i + 1]) * inv, __uint_as_float(o[4 * i + 2]) * inv,
+                              __uint_as_float(o[4 * i + 3]) * inv);
+          }
+        }
+      }
+      if (row_used) p.part_lse[prow] = seen ? m_ref + log2f(l_sum) : -INFINITY;
+      m_ref = -INFINITY;
+      l_sum = 0.f;
+    };
+
+    Walk w(sm);
+    Segment seg, prev;
+    int prev_d = -1, n_done = 0, g = 0;
+    bool have_prev = false;
+    while (w.next(p, seg)) {
+      const int step = p.two_tiles ? 1 : 2, first = seg.v0 + (p.two_tiles ? 0 : (g ^ t) & 1);
+      g += seg.v1 - seg.v0;
+      const int64_t nrow = static_cast<int64_t>(seg.b) * p.nodes + (row_used ? node : 0);
+      const int d = row_used ? p.depth[nrow] : -1;
+      const int len = seg.vis.len;
+      if (first >= seg.v1) {                           // this state has no visit in the segment
+        if (have_prev) {
+          // O of the previous segment is complete once everything issued so far has retired: it is drained at the next wait
+          // for scores, so the empty partial must not disturb its state
+          const float m_keep = m_ref, l_keep = l_sum;
+          leave_partial(seg, -1, false);
+          m_ref = m_keep; l_sum = l_keep;
+        } else {
+          leave_partial(seg, -1, false);
+        }
+        continue;
+      }
+      for (int v = first; v < seg.v1; v += step, ++n_done) {
+        const bool far = v < seg.vis.far;
+        const int tp0 = seg.key_tile(v) * kTileN;
+        // every key of the tile is committed and of this class for nodes of any depth
+        bool uniform = tp0 + kTileN <= len;
+        if (p.two_classes) uniform &= far ? tp0 + kTileN <= len - p.w_0 : tp0 >= len + p.nodes - 1 - p.w_0;
+
+        mbar_wait(&sm.s_full[t], n_done & 1, sm);
+        tc_fence_after();
+        if (v == first && have_prev) leave_partial(prev, prev_d, true);
+        const bool o_live = v != first;                // O holds something of this segment
+        uint32_t s[128];
+        uint64_t acc2[4] = {0ull, 0ull, 0ull, 0ull};
+        float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        if (uniform) {
+          JL_TMEM_LD32(t_s + 0, s, 0);
+#pragma unroll
+          for (int ch = 0; ch < 4; ++ch) {
+            tmem_wait_ld();
+            if (ch + 1 < 4) JL_TMEM_LD32(t_s + (ch + 1) * 32, s, (ch + 1) * 32);
+            max_block(s, ch * 32, m4);
+          }
+        } else {
+#pragma unroll
+          for (int ch = 0; ch < 4; ++ch) JL_TMEM_LD32(t_s + ch * 32, s, ch * 32);
+          // committed keys of this class: positions [lo, hi); drafted keys: bits of the node's mask, by their own depth
+          const int64_t edge = static_cast<int64_t>(len) + d - p.w_0;          // pk < edge: far
+          int64_t lo = p.two_classes && !far ? edge : 0, hi = p.two_classes && far && edge < len ? edge : len;
+          lo -= tp0;
+          hi -= tp0;
+          const int c_lo = lo < 0 ? 0 : (lo > 128 ? 128 : static_cast<int>(lo)), c_hi = hi < 0 ? 0 : (hi > 128 ? 128 : static_cast<int>(hi));
+          uint32_t keep[4];
+          const uint32_t* words = reinterpret_cast<const uint32_t*>(p.mask + nrow * p.words);
+#pragma unroll
+          for (int wd = 0; wd < 4; ++wd) {
+            const int a = max(c_lo - wd * 32, 0), z = min(c_hi - wd * 32, 32);
+            keep[wd] = z > a ? (0xffffffffu >> (32 - (z - a))) << a : 0u;
+            const int u0 = tp0 + wd * 32 - len;        // first node of this word's columns (negative: columns before the nodes)
+            if (d >= 0 && u0 > -32 && u0 < p.nodes && (!far || p.nodes_far)) {
+              const int i0 = u0 >> 5, sh = u0 & 31;
+              const uint32_t w0 = i0 >= 0 ? __ldg(words + i0) : 0u, w1 = i0 + 1 < 2 * p.words ? __ldg(words + i0 + 1) : 0u;
+              uint32_t bits = __funnelshift_r(w0, w1, sh);
+              const int left = p.nodes - u0;
+              if (left < 32) bits &= 0xffffffffu >> (32 - left);
+              if (p.nodes_far) {
+                uint32_t todo = bits;
+                while (todo != 0u) {
+                  const int j = __ffs(todo) - 1;
+                  todo &= todo - 1;
+                  const int du = p.depth[static_cast<int64_t>(seg.b) * p.nodes + u0 + j];
+                  if ((d - du > p.w_0) != far) bits &= ~(1u << j);
+                }
+              }
+              keep[wd] |= bits;
+            }
+            if (d < 0) keep[wd] = 0u;
+          }
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 128; ++i)
+            if (!((keep[i >> 5] >> (i & 31)) & 1u)) s[i] = 0xff800000u;        // -inf
+#pragma unroll
+          for (int ch = 0; ch < 4; ++ch) max_block(s, ch * 32, m4);
+        }
+        const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * p.scale_log2;
+        // lazy rescale: only when some row of the warp outgrew its reference maximum by 2^8
+        if (__any_sync(0xffffffffu, mx > m_ref + 8.f)) {
+          const float m_new = fmaxf(m_ref, mx);
+          const float alpha = m_new == -INFINITY ? 1.f : fast_exp2(m_ref - m_new);
+          l_sum *= alpha;
+          if (o_live) {
+            // O is quiescent: these scores ready implies P V of the state's previous item retired, and the next one waits for our P
+#pragma unroll
+            for (int ch = 0; ch < 4; ++ch) {
+              uint32_t o[32];
+              JL_TMEM_LD32(t_o + ch * 32, o, 0);
+              tmem_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+              JL_TMEM_ST32(t_o + ch * 32, o, 0);
+            }
+          }
+          m_ref = m_new;
+        }
+        const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
+        const uint64_t negm2 = pack2(-m_use, -m_use);
+        exp_block(s, 0, negm2, 0, acc2);
+        exp_block(s, 32, negm2, 16, acc2);
+        publish(0);
+        exp_block(s, 64, negm2, 32, acc2);
+        exp_block(s, 96, negm2, 48, acc2);
+        publish(1);
+        float a0, a1;
+        unpack2(add2(add2(acc2[0], acc2[1]), add2(acc2[2], acc2[3])), a0, a1);
+        l_sum += a0 + a1;
+      }
+      prev = seg;
+      prev_d = d;
+      have_prev = true;
+    }
+    if (have_prev) {
+      mbar_wait(&sm.all_done, 0, sm);
+      tc_fence_after();
+      leave_partial(prev, prev_d, true);
+    }
   }
-  static_cast<__nv_bfloat16*>(a.out)[b * a.o_stride_b + t * a.o_stride_s + h * a.o_stride_h + threadIdx.x] =
-      __float2bfloat16(L > 0.f ? acc / L : 0.f);
-  if (threadIdx.x == 0 && a.lse != nullptr)
-    a.lse[(static_cast<int64_t>(b) * a.heads + h) * T + t] = L > 0.f ? M + logf(L) : -INFINITY;
+
+  tc_fence_before();
+  __syncthreads();
+  if (*failed) {                                 // copies and MMAs that were under way have long landed after 1 ms
+    const uint64_t t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 1000 * 1000) {}
+  }
+  if (warp == 2) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+  }
+  if (threadIdx.x == 0 && sm.failed) atomicExch(&g_tree_status, 1);
+}
+
+// One warp per (sample, node, head) joins the partials of the segments that cover the (sample, key head).
+__global__ void __launch_bounds__(128) tree_combine_kernel(const TreeParams p) {
+  const int lane = threadIdx.x & 31;
+  const int heads = p.kv_heads * p.rep;
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+  if (item >= static_cast<int64_t>(p.batch) * p.nodes * heads) return;
+  const int b = static_cast<int>(item / (static_cast<int64_t>(p.nodes) * heads));
+  const int rest = static_cast<int>(item - static_cast<int64_t>(b) * p.nodes * heads);
+  const int node = rest / heads, h = rest - node * heads, kvh = h / p.rep;
+  int64_t total = 0, before = 0;
+  for (int i = lane; i < p.batch; i += 32) {
+    const int n = visits_of(p, i).n;
+    total += n;
+    before += i < b ? n : 0;
+  }
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) {
+    total += __shfl_xor_sync(0xffffffffu, total, off);
+    before += __shfl_xor_sync(0xffffffffu, before, off);
+  }
+  total *= p.kv_heads;
+  const int n_b = visits_of(p, b).n;
+  const int64_t lo = before * p.kv_heads + static_cast<int64_t>(kvh) * n_b, hi = lo + n_b - 1;     // first and last visit
+  const int64_t parts = parts_of(p, total);
+  // the part that holds visit x of the line: the largest i with i * total / parts <= x
+  const int i0 = static_cast<int>(((lo + 1) * parts + total - 1) / total) - 1, i1 = static_cast<int>(((hi + 1) * parts + total - 1) / total) - 1;
+  const int tile = node / p.npt, mb = p.two_tiles ? tile >> 1 : 0;
+  const int r = (node - tile * p.npt) * p.rep + h - kvh * p.rep;
+  const int states = p.two_tiles ? 1 : 2, t0 = p.two_tiles ? tile & 1 : 0;
+  const int64_t slot0 = static_cast<int64_t>(mb) * (p.workers + p.batch * p.kv_heads) + b * p.kv_heads + kvh;
+  const int n_parts = (i1 - i0 + 1) * states;
+  auto part_row = [&](int k) { return ((slot0 + i0 + k / states) * 2 + t0 + k % states) * p.rpt + r; };
+  float m = -INFINITY;
+  for (int k = lane; k < n_parts; k += 32) m = fmaxf(m, p.part_lse[part_row(k)]);
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+  float sum = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int k = 0; k < n_parts && m != -INFINITY; ++k) {
+    const int64_t row = part_row(k);
+    const float l = p.part_lse[row];
+    if (l == -INFINITY) continue;                // such a partial has no output row
+    const float wgt = exp2f(l - m);
+    const float4 x = *reinterpret_cast<const float4*>(p.part_o + row * kHeadDim + 4 * lane);
+    sum += wgt;
+    acc.x = fmaf(wgt, x.x, acc.x); acc.y = fmaf(wgt, x.y, acc.y); acc.z = fmaf(wgt, x.z, acc.z); acc.w = fmaf(wgt, x.w, acc.w);
+  }
+  const float inv = sum > 0.f ? 1.f / sum : 0.f;
+  *reinterpret_cast<uint2*>(p.out + b * p.os_b + node * p.os_s + h * p.os_h + 4 * lane) =
+      make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+  if (p.lse != nullptr && lane == 0) p.lse[(static_cast<int64_t>(b) * heads + h) * p.nodes + node] = sum > 0.f ? (m + log2f(sum)) * kLn2 : -INFINITY;
+}
+
+struct Layout { int npt, rpt, two_tiles, mbs, workers; size_t lse, total; };
+Layout layout_of(int32_t batch, int32_t nodes, int32_t heads, int32_t kv_heads) {
+  Layout l;
+  const int rep = heads / kv_heads;
+  l.npt = 128 / rep;
+  const int tiles = (nodes + l.npt - 1) / l.npt;
+  l.two_tiles = tiles > 1;
+  l.mbs = (tiles + 1) / 2;
+  l.rpt = (l.two_tiles ? l.npt : nodes) * rep;
+  l.workers = kSms / l.mbs;
+  if (l.workers < 1) l.workers = 1;
+  const size_t rows = static_cast<size_t>(l.mbs) * (l.workers + static_cast<size_t>(batch) * kv_heads) * 2 * l.rpt;
+  l.lse = rows * kHeadDim * sizeof(float);
+  l.total = l.lse + rows * sizeof(float);
+  return l;
+}
+
+// (B, S, Hx, 128) bf16 view -> 4-D map (d, h, s, b), box 64 x box_h x box_s x 1, 128-byte swizzle, zero fill past the end
+int make_map4(CUtensorMap* m, const void* base, int batch, int seq, int heads, int64_t sb, int64_t ss, int64_t sh, int box_h, int box_s) {
+  EncodeTiledFn enc = encode_fn();
+  if (enc == nullptr) return fail(JL_ERR_LAUNCH, "jl_tree_attention: cuTensorMapEncodeTiled is not available from the driver");
+  const int64_t dflt = 128;                      // size-1 dimensions may arrive with stride 0; the encoder wants positive multiples of 16 bytes
+  const cuuint64_t dims[4] = {128, static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(seq), static_cast<cuuint64_t>(batch)};
+  const cuuint64_t strides[3] = {static_cast<cuuint64_t>((heads > 1 && sh > 0 ? sh : dflt) * 2), static_cast<cuuint64_t>((seq > 1 && ss > 0 ? ss : dflt) * 2),
+                                 static_cast<cuuint64_t>((batch > 1 && sb > 0 ? sb : dflt) * 2)};
+  const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(box_h), static_cast<cuuint32_t>(box_s), 1};
+  const cuuint32_t es[4] = {1, 1, 1, 1};
+  const CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(JL_ERR_BAD_ARG, "jl_tree_attention: tensor map encoding failed (CUresult %d)", static_cast<int>(r));
+  return JL_OK;
 }
 
 }  // namespace
 
-size_t tree_attention_workspace_bytes(int32_t, int32_t, int32_t, int32_t, int32_t) { return 16; }
+size_t tree_attention_workspace_bytes(int32_t batch, int32_t nodes, int32_t heads, int32_t kv_heads, int32_t) {
+  if (batch < 1 || nodes < 1 || kv_heads < 1 || heads < kv_heads || heads / kv_heads > 128) return 0;
+  return layout_of(batch, nodes, heads, kv_heads).total;
+}
 
 int launch_tree_attention(const jl_tree_attention_args* a, cudaStream_t stream) {
-  if (a->batch > 65535 || a->heads > 65535) return fail(JL_ERR_UNSUPPORTED, "jl_tree_attention: batch and heads must be at most 65535");
-  tree_attention_kernel<<<dim3(a->nodes, a->heads, a->batch), kWarps * 32, 0, stream>>>(*a);
-  return check_launch("jl_tree_attention");
+  const Layout l = layout_of(a->batch, a->nodes, a->heads, a->kv_heads);
+  if (a->workspace == nullptr || a->workspace_bytes < l.total)
+    return fail(JL_ERR_WORKSPACE, "jl_tree_attention: workspace of %zu bytes needed, %zu given", l.total, a->workspace_bytes);
+  if (reinterpret_cast<uintptr_t>(a->workspace) & 15) return fail(JL_ERR_BAD_ARG, "jl_tree_attention: workspace not 16-byte aligned");
+  TreeParams p{};
+  p.batch = a->batch; p.nodes = a->nodes; p.words = (a->nodes + 63) / 64; p.kv_heads = a->kv_heads; p.rep = a->heads / a->kv_heads; p.rows = a->rows;
+  p.npt = l.npt; p.rpt = l.rpt; p.two_tiles = l.two_tiles; p.mbs = l.mbs; p.workers = l.workers;
+  p.two_classes = a->q_group != nullptr;
+  p.w_0 = a->w_0 < (int64_t(1) << 32) ? a->w_0 : (int64_t(1) << 32);           // no cache reaches further
+  p.nodes_far = p.two_classes && p.w_0 < a->nodes - 1;
+  p.scale_log2 = a->softmax_scale * kLog2e;
+  p.lens = a->lens; p.depth = a->depth; p.mask = a->mask;
+  p.part_o = static_cast<float*>(a->workspace);
+  p.part_lse = reinterpret_cast<float*>(static_cast<uint8_t*>(a->workspace) + l.lse);
+  p.out = static_cast<__nv_bfloat16*>(a->out);
+  p.lse = a->lse;
+  p.os_b = a->o_stride_b; p.os_s = a->o_stride_s; p.os_h = a->o_stride_h;
+  TreeMaps maps;
+  int rc = bind_context();
+  for (int c = 0; c < 2 && rc == JL_OK; ++c) {
+    const bool far = c == 1 && p.two_classes;
+    rc = make_map4(&maps.q[c], far ? a->q_group : a->q_base, a->batch, a->nodes, a->heads, a->q_stride_b, a->q_stride_s, a->q_stride_h, p.rep, p.npt);
+    if (rc == JL_OK)
+      rc = make_map4(&maps.k[c], far ? a->k_group : a->k_base, a->batch, a->rows, a->kv_heads, a->k_stride_b, a->k_stride_s, a->k_stride_h, 1, kTileN);
+  }
+  if (rc == JL_OK) rc = make_map4(&maps.v, a->v, a->batch, a->rows, a->kv_heads, a->v_stride_b, a->v_stride_s, a->v_stride_h, 1, kTileN);
+  if (rc != JL_OK) return rc;
+  constexpr int kSmemBytes = sizeof(TreeSmem) + 1024;
+  static bool attr_set[64] = {false};
+  int dev = -1;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return fail(JL_ERR_LAUNCH, "jl_tree_attention: no current CUDA device");
+  if (!attr_set[dev]) {
+    if (cudaFuncSetAttribute(tree_attention_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes) != cudaSuccess)
+      return check_launch("jl_tree_attention (shared memory opt-in)");
+    attr_set[dev] = true;
+  }
+  const int64_t items = static_cast<int64_t>(a->batch) * a->nodes * a->heads;
+  if ((items + 3) / 4 > 0x7fffffff) return fail(JL_ERR_UNSUPPORTED, "jl_tree_attention: too many rows for one launch");
+  tree_attention_kernel<<<p.mbs * p.workers, kThreads, kSmemBytes, stream>>>(maps, p);
+  rc = check_launch("jl_tree_attention");
+  if (rc != JL_OK) return rc;
+  tree_combine_kernel<<<static_cast<unsigned>((items + 3) / 4), 128, 0, stream>>>(p);
+  return check_launch("jl_tree_attention (combine)");
+}
+
+int tree_status() {
+  int v = 0;
+  if (cudaMemcpyFromSymbol(&v, g_tree_status, sizeof(int)) != cudaSuccess) return -1;
+  const int zero = 0;
+  if (v != 0) cudaMemcpyToSymbol(g_tree_status, &zero, sizeof(int));
+  return v;
 }
 
 }  // namespace jl

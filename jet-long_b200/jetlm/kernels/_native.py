@@ -200,6 +200,7 @@ TREE_EXPORTS = [
     ("jl_tree_append", C.c_int, [C.POINTER(TreeAppendArgs), C.c_void_p]),
     ("jl_tree_attention_workspace_bytes", C.c_size_t, [C.c_int32] * 5),
     ("jl_tree_attention", C.c_int, [C.POINTER(TreeAttentionArgs), C.c_void_p]),
+    ("jl_tree_status", C.c_int, []),
 ]
 
 

@@ -152,6 +152,9 @@ def tree_attention(q_base: torch.Tensor, q_group: torch.Tensor, key_rows: torch.
     if key_group_rows is not None and (key_group_rows.shape != key_rows.shape
                                        or [_st(key_group_rows, i) for i in range(3)] != [_st(key_rows, i) for i in range(3)]):
         raise ValueError(f"{op}: key_group_rows must match key_rows in shape and strides")
+    for name, t in tensors:
+        if any(t.shape[i] > 1 and t.stride(i) <= 0 for i in range(3)):
+            raise ValueError(f"{op}: {name} must not be a broadcast view; call {name}.contiguous()")
     if Hk < 1 or H % Hk != 0:
         raise ValueError(f"{op}: query heads must be divisible by kv heads")
     if int(w_0) < 0:

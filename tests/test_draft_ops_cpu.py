@@ -59,6 +59,9 @@ def test_c_entries_refuse_before_they_touch_a_device():
         a = n.TreeAttentionArgs()
         a.q_base = a.k_base = a.v = a.out = a.lens = a.depth = a.mask = 1024
         a.batch, a.nodes, a.heads, a.kv_heads, a.head_dim, a.rows, a.w_0 = 1, 4, 4, 2, 128, 64, 16
+        for t in "qkvo":
+            setattr(a, f"{t}_stride_s", 512)
+            setattr(a, f"{t}_stride_h", 128)
         for k, v in kw.items():
             setattr(a, k, v)
         return lib.jl_tree_attention(C.byref(a), None)
@@ -67,7 +70,7 @@ def test_c_entries_refuse_before_they_touch_a_device():
     for want, kw in [(no, dict(head_dim=64)), (bad, dict(kv_heads=3)), (bad, dict(nodes=0)), (bad, dict(nodes=257)), (bad, dict(rows=3)),
                      (bad, dict(w_0=-1)), (bad, dict(q_group=1024)), (bad, dict(k_group=1024)), (bad, dict(v=None)), (bad, dict(mask=None)),
                      (bad, dict(q_base=1032)), (bad, dict(k_stride_s=129)), (bad, dict(o_stride_h=4)), (bad, dict(batch=-1)),
-                     (no, dict(heads=258, kv_heads=2))]:
+                     (no, dict(heads=258, kv_heads=2)), (no, dict(k_stride_s=0)), (no, dict(q_stride_h=-128)), (no, dict(batch=2))]:
         assert attention(**kw) == want, kw
     assert attention(batch=0) == n.JL_OK
 
