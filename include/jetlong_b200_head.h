@@ -19,8 +19,8 @@ extern "C" {
  * A label outside [0, vocab) that is not ignore_index gives nll = NaN; nothing is read out of range.
  * hidden (rows, hidden) and weight (vocab, hidden) bf16 with row strides that are multiples of 8, innermost dimension
  * contiguous, 16-byte aligned; hidden size a multiple of 8.  labels (rows,) int64, may be NULL with nll NULL.
- * nll, lse, top, loss_sum, loss_count may each be NULL.  loss_sum = sum of nll, loss_count = number of rows whose
- * label is not ignore_index (both fp32 scalars, summed in a fixed order).
+ * nll, lse, top, loss_sum, loss_count, loss_mean may each be NULL.  loss_sum = sum of nll, loss_count = number of rows
+ * whose label is not ignore_index, loss_mean = their quotient (fp32 scalars, summed in a fixed order).
  * workspace: jl_head_scores_workspace_bytes, 16-byte aligned, not initialised by the caller.
  * ------------------------------------------------------------------------------------------- */
 typedef struct {
@@ -36,6 +36,7 @@ typedef struct {
   int64_t* top;
   float* loss_sum;
   float* loss_count;
+  float* loss_mean;
   void* workspace;
   size_t workspace_bytes;
 } jl_head_scores_args;

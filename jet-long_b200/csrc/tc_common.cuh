@@ -161,6 +161,12 @@ __device__ __forceinline__ uint64_t exp2_pair_sfu(uint64_t x) {
 }
 
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// Waits for the loads before it with the loaded registers as operands, so that no use of them can be moved ahead of the wait
+// (a plain wait orders memory, not the registers of an earlier asm statement).
+#define JL_P16(r, o) "+r"(r[o + 0]), "+r"(r[o + 1]), "+r"(r[o + 2]), "+r"(r[o + 3]), "+r"(r[o + 4]), "+r"(r[o + 5]), "+r"(r[o + 6]), "+r"(r[o + 7]), \
+  "+r"(r[o + 8]), "+r"(r[o + 9]), "+r"(r[o + 10]), "+r"(r[o + 11]), "+r"(r[o + 12]), "+r"(r[o + 13]), "+r"(r[o + 14]), "+r"(r[o + 15])
+#define JL_TMEM_WAIT_LD16(r, o) asm volatile("tcgen05.wait::ld.sync.aligned;" : JL_P16(r, o) : : "memory")
+#define JL_TMEM_WAIT_LD32(r, o) asm volatile("tcgen05.wait::ld.sync.aligned;" : JL_P16(r, o), JL_P16(r, o + 16) : : "memory")
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // ---- cta_group::2: the two CTAs of a cluster pair; rank 0 issues the MMAs ----
@@ -202,7 +208,27 @@ __device__ __forceinline__ void commit_both(uint64_t* bar) {
 
 }  // namespace pair
 
+// Programmatic dependent launch: the kernel before lets its successor start early, the successor waits for its results.
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_prerequisites() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 }  // namespace tc
+
+// Launch whose blocks may become resident before the stream's previous kernel has ended; they call wait_prerequisites().
+template <class... Params, class... Args>
+cudaError_t launch_dependent(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, const Args&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                                   const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,

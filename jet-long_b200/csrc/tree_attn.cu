@@ -12,9 +12,10 @@
 // head) each, and every segment leaves one normalised fp32 partial (O, LSE) per row that tree_combine_kernel joins.
 // Nothing on the host depends on the lengths, which are read on the device.
 //
-//   warp 0      TMA producer of K (ring of 3) and V (ring of 2), running ahead over class and segment borders
-//   warp 1      MMA issuer: S_t = Q K^T two items ahead of O_t += P V
-//   warp 2      tensor memory; zeroes the value rows behind the last node, which may hold anything (0 * NaN is NaN)
+//   warp 0      TMA producer of K and V tiles (one ring of 5, in the order of their use), running ahead over all borders
+//   warp 1      MMA issuer: S_t = Q K^T two items ahead of O_t += P V; in tiles that reach past the committed rows it first
+//               zeroes the value rows that belong to no node, which may hold anything (0 * NaN is NaN)
+//   warp 2      tensor memory
 //   warp 3      TMA producer of the query tiles of the current class
 //   warps 4-11  softmax: one thread per row, 128 scores in registers, P back to tensor memory over S
 #include "tc_common.cuh"
@@ -29,7 +30,7 @@ using namespace tc;
 __device__ int g_tree_status = 0;            // raised when a bounded wait gave up
 
 constexpr int kTileN = 128;                  // keys per visit
-constexpr int kKStages = 3, kVStages = 2;
+constexpr int kStages = 5;                   // tiles in the ring: K of visit g is its tile 2 g, V is tile 2 g + 1
 constexpr int kTileBytes = 128 * 256;        // 128 rows x 128 bf16
 constexpr int kHalfBytes = 128 * 128;        // one 64-column half (a TMA box)
 constexpr int kThreads = 384;
@@ -58,10 +59,9 @@ struct TreeMaps { CUtensorMap q[2], k[2], v; };       // [0] near (base), [1] fa
 
 struct TreeSmem {
   alignas(1024) uint8_t q[2][kTileBytes];    // two row tiles, or two class operands of one
-  alignas(1024) uint8_t k[kKStages][kTileBytes];
-  alignas(1024) uint8_t v[kVStages][kTileBytes];
-  uint64_t q_full[2], q_free[2], k_full[kKStages], k_empty[kKStages], v_full[kVStages], v_empty[kVStages];
-  uint64_t s_full[2], p_half[2][2], v_clean[kVStages], all_done;
+  alignas(1024) uint8_t kv[kStages][kTileBytes];
+  uint64_t q_full[2], q_free[2], full[kStages], empty[kStages];
+  uint64_t s_full[2], p_half[2][2], o_full[2];
   int64_t lo, hi;                            // this CTA's part of the line
   int start_b, start_kvh, start_v;
   uint32_t tmem_base;
@@ -116,7 +116,7 @@ struct Walk {
 
 // Products in issue order.  Two row tiles: (visit, 0), (visit, 1); one: (visit, alternating state).  Consecutive items never
 // share a state, whatever segment they belong to.
-struct Item { int t, cls, visit, use; bool first_use, last_use, q_first, q_last, o_first, tail; };
+struct Item { int t, visit, use, b, u0; bool first_use, last_use, q_first, q_last, o_first, o_last, tail; };     // u0: node index of the tile's first row
 struct Items {
   Walk w;
   Segment seg;
@@ -144,11 +144,13 @@ struct Items {
     it.q_last = class_end && it.last_use;
     if (it.q_first) ++use;
     it.t = t;
-    it.cls = v < seg.vis.far;
     it.visit = visit;
     it.use = use;
     it.o_first = v - seg.v0 < (p.two_tiles ? 1 : 2);
+    it.o_last = v + (p.two_tiles ? 1 : 2) >= seg.v1;
     it.tail = seg.tail(v);
+    it.b = seg.b;
+    it.u0 = seg.key_tile(v) * kTileN - seg.vis.len;
     return true;
   }
 };
@@ -158,6 +160,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
   TreeSmem& sm = *reinterpret_cast<TreeSmem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int mb = static_cast<int>(blockIdx.x) % p.mbs, worker = static_cast<int>(blockIdx.x) / p.mbs;
+  launch_dependents();                           // the combine kernel may take its place and wait there for our end
   const int q_slots = p.two_tiles ? 1 : 2;
 
   if (warp == 0) {
@@ -198,9 +201,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
       mbar_init(&sm.p_half[i][0], 128);
       mbar_init(&sm.p_half[i][1], 128);
     }
-    for (int i = 0; i < kKStages; ++i) { mbar_init(&sm.k_full[i], 1); mbar_init(&sm.k_empty[i], 1); }
-    for (int i = 0; i < kVStages; ++i) { mbar_init(&sm.v_full[i], 1); mbar_init(&sm.v_empty[i], 1); mbar_init(&sm.v_clean[i], 32); }
-    mbar_init(&sm.all_done, 1);
+    for (int i = 0; i < kStages; ++i) { mbar_init(&sm.full[i], 1); mbar_init(&sm.empty[i], 1); }
+    for (int i = 0; i < 2; ++i) mbar_init(&sm.o_full[i], 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 2) {
@@ -223,16 +225,15 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
         int g = 0;
         while (w.next(p, seg)) {
           for (int v = seg.v0; v < seg.v1; ++v, ++g) {
-            const CUtensorMap* km = &maps.k[v < seg.vis.far ? 1 : 0];
-            const int row = seg.key_tile(v) * kTileN, ks = g % kKStages, vs = g % kVStages;
-            mbar_wait(&sm.k_empty[ks], ((g / kKStages) & 1) ^ 1, sm);
-            if (*failed) break;
-            mbar_expect_tx(&sm.k_full[ks], kTileBytes);
-            for (int h = 0; h < 2; ++h) tma_load_4d(sm.k[ks] + h * kHalfBytes, km, &sm.k_full[ks], h * 64, seg.kvh, row, seg.b);
-            mbar_wait(&sm.v_empty[vs], ((g / kVStages) & 1) ^ 1, sm);
-            if (*failed) break;
-            mbar_expect_tx(&sm.v_full[vs], kTileBytes);
-            for (int h = 0; h < 2; ++h) tma_load_4d(sm.v[vs] + h * kHalfBytes, &maps.v, &sm.v_full[vs], h * 64, seg.kvh, row, seg.b);
+            const int row = seg.key_tile(v) * kTileN;
+            for (int kv = 0; kv < 2; ++kv) {
+              const CUtensorMap* map = kv == 1 ? &maps.v : &maps.k[v < seg.vis.far ? 1 : 0];
+              const int i = 2 * g + kv, st = i % kStages;
+              mbar_wait(&sm.empty[st], ((i / kStages) & 1) ^ 1, sm);
+              if (*failed) break;
+              mbar_expect_tx(&sm.full[st], kTileBytes);
+              for (int h = 0; h < 2; ++h) tma_load_4d(sm.kv[st] + h * kHalfBytes, map, &sm.full[st], h * 64, seg.kvh, row, seg.b);
+            }
           }
         }
       }
@@ -263,16 +264,16 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
       uint32_t leader;
       asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(leader));
       const uint32_t idesc_qk = instr_desc(128, kTileN, 0), idesc_pv = instr_desc(128, kHeadDim, 1);
-      const uint64_t q_desc = smem_desc(smem_u32(sm.q[0]), 16, 1024), k_desc = smem_desc(smem_u32(sm.k[0]), 16, 1024);
-      const uint64_t v_desc = smem_desc(smem_u32(sm.v[0]), kHalfBytes, 1024);
+      const uint64_t q_desc = smem_desc(smem_u32(sm.q[0]), 16, 1024), k_desc = smem_desc(smem_u32(sm.kv[0]), 16, 1024);
+      const uint64_t v_desc = smem_desc(smem_u32(sm.kv[0]), kHalfBytes, 1024);
       Items ahead(sm), now(sm);
       Item it;
       auto issue_qk = [&]() {                          // the next item's scores, if there is one
         Item n;
         if (!ahead.next(p, n)) return;
-        const int ks = n.visit % kKStages, slot = n.use % q_slots;
+        const int ks = 2 * n.visit % kStages, slot = n.use % q_slots;
         if (n.q_first) mbar_wait(&sm.q_full[slot], (n.use / q_slots) & 1, sm);
-        if (n.first_use) mbar_wait(&sm.k_full[ks], (n.visit / kKStages) & 1, sm);
+        if (n.first_use) mbar_wait(&sm.full[ks], (2 * n.visit / kStages) & 1, sm);
         tc_fence_after();
         const uint64_t qd = q_desc + static_cast<uint64_t>(((p.two_tiles ? n.t : slot) * kTileBytes) >> 4);
         const uint64_t kd = k_desc + static_cast<uint64_t>((ks * kTileBytes) >> 4);
@@ -283,26 +284,34 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
             mma_ss(tmem + n.t * 128, qd + off, kd + off, idesc_qk, kk > 0);
           }
           mma_commit(&sm.s_full[n.t]);
-          if (n.last_use) mma_commit(&sm.k_empty[ks]);
+          if (n.last_use) mma_commit(&sm.empty[ks]);
           if (n.q_last) mma_commit(&sm.q_free[slot]);
         }
         __syncwarp();
       };
       issue_qk();
       issue_qk();
-      int done[2] = {0, 0}, cleaned[kVStages] = {0, 0};
+      int done[2] = {0, 0};
       while (now.next(p, it)) {
-        const int vs = it.visit % kVStages;
+        const int vs = (2 * it.visit + 1) % kStages;
         const uint64_t vd = v_desc + static_cast<uint64_t>((vs * kTileBytes) >> 4);
         const int parity = (it.t ? done[1] : done[0]) & 1;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           mbar_wait(&sm.p_half[it.t][h], parity, sm);
           if (h == 0 && it.first_use) {
-            mbar_wait(&sm.v_full[vs], (it.visit / kVStages) & 1, sm);
+            mbar_wait(&sm.full[vs], ((2 * it.visit + 1) / kStages) & 1, sm);
             if (it.tail) {
-              mbar_wait(&sm.v_clean[vs], (vs ? cleaned[1] : cleaned[0]) & 1, sm);
-              if (vs) ++cleaned[1]; else ++cleaned[0];
+              for (int r0 = 0; r0 < kTileN; r0 += 32) {
+                const int u = it.u0 + r0 + lane;
+                const bool keep = u < 0 || (u < p.nodes && p.depth[static_cast<int64_t>(it.b) * p.nodes + u] >= 0);
+                for (uint32_t dead = __ballot_sync(0xffffffffu, !keep); dead != 0u; dead &= dead - 1)
+                  if (lane < 16)
+                    *reinterpret_cast<uint4*>(sm.kv[vs] + (lane >> 3) * kHalfBytes + (r0 + __ffs(dead) - 1) * 128 + (lane & 7) * 16) =
+                        make_uint4(0u, 0u, 0u, 0u);
+              }
+              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+              __syncwarp();
             }
           }
           tc_fence_after();
@@ -311,35 +320,13 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
             for (int kk = 4 * h; kk < 4 * h + 4; ++kk)
               mma_ts(tmem + 256 + it.t * 128, tmem + it.t * 128 + kk * 8, vd + static_cast<uint64_t>((kk * 2048) >> 4), idesc_pv,
                      (!it.o_first || kk > 0) ? 1u : 0u);
-            if (h == 1 && it.last_use) mma_commit(&sm.v_empty[vs]);
+            if (h == 1 && it.last_use) mma_commit(&sm.empty[vs]);
+            if (h == 1 && it.o_last) mma_commit(&sm.o_full[it.t]);
           }
           __syncwarp();
         }
         if (it.t) ++done[1]; else ++done[0];
         issue_qk();
-      }
-      if (leader) mma_commit(&sm.all_done);
-      __syncwarp();
-    } else {
-      // ============================ value rows that belong to nobody ============================
-      Walk w(sm);
-      Segment seg;
-      int g = 0;
-      while (w.next(p, seg)) {
-        for (int v = seg.v0; v < seg.v1; ++v, ++g) {
-          if (!seg.tail(v)) continue;
-          const int vs = g % kVStages;
-          mbar_wait(&sm.v_full[vs], (g / kVStages) & 1, sm);
-          for (int r0 = 0; r0 < kTileN; r0 += 32) {
-            const int u = seg.key_tile(v) * kTileN + r0 + lane - seg.vis.len;      // node index
-            const bool keep = u < 0 || (u < p.nodes && p.depth[static_cast<int64_t>(seg.b) * p.nodes + u] >= 0);
-            for (uint32_t dead = __ballot_sync(0xffffffffu, !keep); dead != 0u; dead &= dead - 1)
-              if (lane < 16)
-                *reinterpret_cast<uint4*>(sm.v[vs] + (lane >> 3) * kHalfBytes + (r0 + __ffs(dead) - 1) * 128 + (lane & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
-          }
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          mbar_arrive(&sm.v_clean[vs]);
-        }
       }
     }
   } else {
@@ -378,52 +365,44 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
       tc_fence_before();
       mbar_arrive(&sm.p_half[t][half]);
     };
-    // the partial of a finished segment: O / l in fp32 and the LSE in the log2 domain
+    // the segment's partial: O / l in fp32 (zero where the row saw nothing) and the LSE in the log2 domain
     auto leave_partial = [&](const Segment& s, int d, bool any) {
       const int64_t slot = static_cast<int64_t>(mb) * (p.workers + p.batch * p.kv_heads) + worker + s.b * p.kv_heads + s.kvh;
       const int64_t prow = (slot * 2 + t) * p.rpt + r;
       const bool seen = any && d >= 0 && m_ref != -INFINITY;          // masked scores add ~1e-38 each to l_sum, never to m_ref
       const float inv = seen ? 1.f / l_sum : 0.f;
-      if (any) {
 #pragma unroll
-        for (int ch = 0; ch < 4; ++ch) {
-          uint32_t o[32];
+      for (int ch = 0; ch < 4; ++ch) {
+        uint32_t o[32];
+        if (any) {
           JL_TMEM_LD32(t_o + ch * 32, o, 0);
-          tmem_wait_ld();
-          if (row_used && seen) {
+          JL_TMEM_WAIT_LD32(o, 0);
+        }
+        if (row_used) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-              *reinterpret_cast<float4*>(p.part_o + prow * kHeadDim + ch * 32 + 4 * i) =
-                  make_float4(__uint_as_float(o[4 * i]) * inv, __uint_as_float(o[4 * i + 1]) * inv, __uint_as_float(o[4 * i + 2]) * inv,
-                              __uint_as_float(o[4 * i + 3]) * inv);
-          }
+          for (int i = 0; i < 8; ++i)
+            *reinterpret_cast<float4*>(p.part_o + prow * kHeadDim + ch * 32 + 4 * i) =
+                seen ? make_float4(__uint_as_float(o[4 * i]) * inv, __uint_as_float(o[4 * i + 1]) * inv, __uint_as_float(o[4 * i + 2]) * inv,
+                                   __uint_as_float(o[4 * i + 3]) * inv)
+                     : make_float4(0.f, 0.f, 0.f, 0.f);
         }
       }
       if (row_used) p.part_lse[prow] = seen ? m_ref + log2f(l_sum) : -INFINITY;
-      m_ref = -INFINITY;
-      l_sum = 0.f;
     };
 
     Walk w(sm);
-    Segment seg, prev;
-    int prev_d = -1, n_done = 0, g = 0;
-    bool have_prev = false;
+    Segment seg;
+    int n_done = 0, n_segs = 0, g = 0;
     while (w.next(p, seg)) {
       const int step = p.two_tiles ? 1 : 2, first = seg.v0 + (p.two_tiles ? 0 : (g ^ t) & 1);
       g += seg.v1 - seg.v0;
       const int64_t nrow = static_cast<int64_t>(seg.b) * p.nodes + (row_used ? node : 0);
       const int d = row_used ? p.depth[nrow] : -1;
       const int len = seg.vis.len;
+      m_ref = -INFINITY;
+      l_sum = 0.f;
       if (first >= seg.v1) {                           // this state has no visit in the segment
-        if (have_prev) {
-          // O of the previous segment is complete once everything issued so far has retired: it is drained at the next wait
-          // for scores, so the empty partial must not disturb its state
-          const float m_keep = m_ref, l_keep = l_sum;
-          leave_partial(seg, -1, false);
-          m_ref = m_keep; l_sum = l_keep;
-        } else {
-          leave_partial(seg, -1, false);
-        }
+        leave_partial(seg, -1, false);
         continue;
       }
       for (int v = first; v < seg.v1; v += step, ++n_done) {
@@ -435,7 +414,6 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
 
         mbar_wait(&sm.s_full[t], n_done & 1, sm);
         tc_fence_after();
-        if (v == first && have_prev) leave_partial(prev, prev_d, true);
         const bool o_live = v != first;                // O holds something of this segment
         uint32_t s[128];
         uint64_t acc2[4] = {0ull, 0ull, 0ull, 0ull};
@@ -444,13 +422,11 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
           JL_TMEM_LD32(t_s + 0, s, 0);
 #pragma unroll
           for (int ch = 0; ch < 4; ++ch) {
-            tmem_wait_ld();
+            JL_TMEM_WAIT_LD32(s, ch * 32);
             if (ch + 1 < 4) JL_TMEM_LD32(t_s + (ch + 1) * 32, s, (ch + 1) * 32);
             max_block(s, ch * 32, m4);
           }
         } else {
-#pragma unroll
-          for (int ch = 0; ch < 4; ++ch) JL_TMEM_LD32(t_s + ch * 32, s, ch * 32);
           // committed keys of this class: positions [lo, hi); drafted keys: bits of the node's mask, by their own depth
           const int64_t edge = static_cast<int64_t>(len) + d - p.w_0;          // pk < edge: far
           int64_t lo = p.two_classes && !far ? edge : 0, hi = p.two_classes && far && edge < len ? edge : len;
@@ -483,7 +459,10 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
             }
             if (d < 0) keep[wd] = 0u;
           }
-          tmem_wait_ld();
+#pragma unroll
+          for (int ch = 0; ch < 4; ++ch) JL_TMEM_LD32(t_s + ch * 32, s, ch * 32);
+#pragma unroll
+          for (int ch = 0; ch < 4; ++ch) JL_TMEM_WAIT_LD32(s, ch * 32);
 #pragma unroll
           for (int i = 0; i < 128; ++i)
             if (!((keep[i >> 5] >> (i & 31)) & 1u)) s[i] = 0xff800000u;        // -inf
@@ -502,7 +481,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
             for (int ch = 0; ch < 4; ++ch) {
               uint32_t o[32];
               JL_TMEM_LD32(t_o + ch * 32, o, 0);
-              tmem_wait_ld();
+              JL_TMEM_WAIT_LD32(o, 0);
 #pragma unroll
               for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
               JL_TMEM_ST32(t_o + ch * 32, o, 0);
@@ -522,14 +501,10 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
         unpack2(add2(add2(acc2[0], acc2[1]), add2(acc2[2], acc2[3])), a0, a1);
         l_sum += a0 + a1;
       }
-      prev = seg;
-      prev_d = d;
-      have_prev = true;
-    }
-    if (have_prev) {
-      mbar_wait(&sm.all_done, 0, sm);
+      mbar_wait(&sm.o_full[t], n_segs++ & 1, sm);
       tc_fence_after();
-      leave_partial(prev, prev_d, true);
+      leave_partial(seg, d, true);
+      tc_fence_before();                               // the next segment's P V follows our next P
     }
   }
 
@@ -574,24 +549,42 @@ __global__ void __launch_bounds__(128) tree_combine_kernel(const TreeParams p) {
   const int i0 = static_cast<int>(((lo + 1) * parts + total - 1) / total) - 1, i1 = static_cast<int>(((hi + 1) * parts + total - 1) / total) - 1;
   const int tile = node / p.npt, mb = p.two_tiles ? tile >> 1 : 0;
   const int r = (node - tile * p.npt) * p.rep + h - kvh * p.rep;
-  const int states = p.two_tiles ? 1 : 2, t0 = p.two_tiles ? tile & 1 : 0;
-  const int64_t slot0 = static_cast<int64_t>(mb) * (p.workers + p.batch * p.kv_heads) + b * p.kv_heads + kvh;
-  const int n_parts = (i1 - i0 + 1) * states;
-  auto part_row = [&](int k) { return ((slot0 + i0 + k / states) * 2 + t0 + k % states) * p.rpt + r; };
-  float m = -INFINITY;
-  for (int k = lane; k < n_parts; k += 32) m = fmaxf(m, p.part_lse[part_row(k)]);
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
-  float sum = 0.f;
+  const int shift = p.two_tiles ? 0 : 1, t0 = p.two_tiles ? tile & 1 : 0;      // two states per slot, or one of the slot's tiles
+  const int64_t slot0 = static_cast<int64_t>(mb) * (p.workers + p.batch * p.kv_heads) + b * p.kv_heads + kvh + i0;
+  const int n_parts = (i1 - i0 + 1) << shift;
+  auto part_row = [&](int k) { return ((slot0 + (k >> shift)) * 2 + t0 + (shift ? k & 1 : 0)) * p.rpt + r; };
+  wait_prerequisites();
+  // rounds of 32 partials: lane i holds the weight of partial k0 + i, 8 output rows are in flight at a time; the running
+  // maximum moves once a round
+  float m = -INFINITY, sum = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int k = 0; k < n_parts && m != -INFINITY; ++k) {
-    const int64_t row = part_row(k);
-    const float l = p.part_lse[row];
-    if (l == -INFINITY) continue;                // such a partial has no output row
-    const float wgt = exp2f(l - m);
-    const float4 x = *reinterpret_cast<const float4*>(p.part_o + row * kHeadDim + 4 * lane);
-    sum += wgt;
-    acc.x = fmaf(wgt, x.x, acc.x); acc.y = fmaf(wgt, x.y, acc.y); acc.z = fmaf(wgt, x.z, acc.z); acc.w = fmaf(wgt, x.w, acc.w);
+  for (int k0 = 0; k0 < n_parts; k0 += 32) {
+    const int n = min(32, n_parts - k0);
+    float l = lane < n ? p.part_lse[part_row(k0 + lane)] : -INFINITY, mr = l;
+    float4 x[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      x[j] = j < n ? *reinterpret_cast<const float4*>(p.part_o + part_row(k0 + j) * kHeadDim + 4 * lane) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) mr = fmaxf(mr, __shfl_xor_sync(0xffffffffu, mr, off));
+    const float mn = fmaxf(m, mr), ref = mn == -INFINITY ? 0.f : mn;
+    const float f = exp2f(m - ref), wgt = exp2f(l - ref);
+    m = mn;
+    sum *= f; acc.x *= f; acc.y *= f; acc.z *= f; acc.w *= f;
+    for (int j0 = 0; j0 < n; j0 += 8) {
+      float4 nx[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        nx[j] = j0 + 8 + j < n ? *reinterpret_cast<const float4*>(p.part_o + part_row(k0 + j0 + 8 + j) * kHeadDim + 4 * lane)
+                               : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float w = __shfl_sync(0xffffffffu, wgt, (j0 + j) & 31);          // 0 past the last partial
+        sum += w;
+        acc.x = fmaf(w, x[j].x, acc.x); acc.y = fmaf(w, x[j].y, acc.y); acc.z = fmaf(w, x[j].z, acc.z); acc.w = fmaf(w, x[j].w, acc.w);
+        x[j] = nx[j];
+      }
+    }
   }
   const float inv = sum > 0.f ? 1.f / sum : 0.f;
   *reinterpret_cast<uint2*>(p.out + b * p.os_b + node * p.os_s + h * p.os_h + 4 * lane) =
@@ -681,8 +674,9 @@ int launch_tree_attention(const jl_tree_attention_args* a, cudaStream_t stream) 
   tree_attention_kernel<<<p.mbs * p.workers, kThreads, kSmemBytes, stream>>>(maps, p);
   rc = check_launch("jl_tree_attention");
   if (rc != JL_OK) return rc;
-  tree_combine_kernel<<<static_cast<unsigned>((items + 3) / 4), 128, 0, stream>>>(p);
-  return check_launch("jl_tree_attention (combine)");
+  if (launch_dependent(tree_combine_kernel, dim3(static_cast<unsigned>((items + 3) / 4)), dim3(128), 0, stream, p) != cudaSuccess)
+    return check_launch("jl_tree_attention (combine)");
+  return JL_OK;
 }
 
 int tree_status() {

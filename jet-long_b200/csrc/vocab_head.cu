@@ -155,6 +155,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) head_gemm_kernel(const __grid
   __syncthreads();
   if (kPair == 2) pair::cluster_sync();
   tc_fence_after();
+  launch_dependents();
   const uint32_t tmem = sm.tmem_base;
   volatile int* const failed = &sm.failed;       // a wait gave up: nothing more is issued, every later wait returns at once
 
@@ -272,7 +273,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) head_gemm_kernel(const __grid
         for (int c0 = 0; c0 < valid; c0 += 16) {
           uint32_t z[16];
           JL_TMEM_LD16(acc + c0, z);
-          tmem_wait_ld();
+          JL_TMEM_WAIT_LD16(z, 0);
           if (c0 + 16 <= valid) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) m4[j & 3] = max3(m4[j & 3], __uint_as_float(z[2 * j]), __uint_as_float(z[2 * j + 1]));
@@ -291,7 +292,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) head_gemm_kernel(const __grid
         for (int c0 = 0; c0 < valid; c0 += 16) {
           uint32_t z[16];
           JL_TMEM_LD16(acc + c0, z);
-          tmem_wait_ld();
+          JL_TMEM_WAIT_LD16(z, 0);
           if (__any_sync(0xffffffffu, y >= c0 && y < c0 + 16)) {
 #pragma unroll
             for (int j = 0; j < 16; ++j) z_y = y == c0 + j ? __uint_as_float(z[j]) : z_y;
@@ -337,7 +338,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) head_gemm_kernel(const __grid
             const int cc = c0 + half * 32;
             uint32_t z[32];
             JL_TMEM_LD32(acc + cc, z, 0);
-            tmem_wait_ld();
+            JL_TMEM_WAIT_LD32(z, 0);
             if constexpr (kEpi == kEpiDz) {
 #pragma unroll
               for (int j = 0; j < 32; ++j) {
@@ -378,34 +379,51 @@ __global__ void __launch_bounds__(kGemmThreads, 1) head_gemm_kernel(const __grid
   if (threadIdx.x == 0 && sm.failed) atomicExch(&g_head_status, 1);
 }
 
-// one warp per row folds the tiles' partials
-__global__ void __launch_bounds__(128) scores_fold_kernel(const float2* part, const int* part_arg, const float* picked, int tiles, int64_t N, int64_t V,
+// (maximum, sum of exponentials relative to it, lowest index of the maximum) of two disjoint sets of logits
+__device__ __forceinline__ void join_scores(float& m, float& s, int& arg, float om, float os, int oa) {
+  if (om > m || (om == m && oa < arg)) arg = oa;
+  const float mn = fmaxf(m, om), ref = mn == -INFINITY ? 0.f : mn;
+  s = s * fast_exp2((m - ref) * kLog2e) + os * fast_exp2((om - ref) * kLog2e);
+  m = mn;
+}
+
+// Folds the tiles' partials of a row; kWarps warps share a row (8 when there are few rows: 731 partials of one row took
+// one warp 14 us).  Every lane reads 4 partials at a time.
+template <int kWarps>
+__global__ void __launch_bounds__(256) scores_fold_kernel(const float2* part, const int* part_arg, const float* picked, int tiles, int64_t N, int64_t V,
                                                           const int64_t* labels, int64_t ignore, float* nll, float* lse, int64_t* top) {
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (row >= N) return;
+  __shared__ float sm[8], ss[8];
+  __shared__ int sa[8];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (8 / kWarps) + warp / kWarps;
+  launch_dependents();
+  wait_prerequisites();
   float m = -INFINITY, s = 0.f;
   int arg = 0x7fffffff;
-  for (int i = lane; i < tiles; i += 32) {
-    const float2 p = part[row * tiles + i];
-    if (part_arg != nullptr) {
-      const int a = part_arg[row * tiles + i];
-      if (p.x > m || (p.x == m && a < arg)) arg = a;
+  if (row < N) {
+    for (int i0 = (warp % kWarps) * 32 + lane; i0 < tiles; i0 += 4 * 32 * kWarps) {
+      float2 p[4];
+      int a[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int i = i0 + j * 32 * kWarps;
+        p[j] = i < tiles ? part[row * tiles + i] : make_float2(-INFINITY, 0.f);
+        a[j] = i < tiles && part_arg != nullptr ? part_arg[row * tiles + i] : 0x7fffffff;
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) join_scores(m, s, arg, p[j].x, p[j].y, a[j]);
     }
-    const float mn = fmaxf(m, p.x), ref = mn == -INFINITY ? 0.f : mn;
-    s = s * expf(m - ref) + p.y * expf(p.x - ref);
-    m = mn;
   }
 #pragma unroll
-  for (int off = 16; off > 0; off >>= 1) {
-    const float om = __shfl_xor_sync(0xffffffffu, m, off), os = __shfl_xor_sync(0xffffffffu, s, off);
-    const int oa = __shfl_xor_sync(0xffffffffu, arg, off);
-    if (om > m || (om == m && oa < arg)) arg = oa;
-    const float mn = fmaxf(m, om), ref = mn == -INFINITY ? 0.f : mn;
-    s = s * expf(m - ref) + os * expf(om - ref);
-    m = mn;
+  for (int off = 16; off > 0; off >>= 1)
+    join_scores(m, s, arg, __shfl_xor_sync(0xffffffffu, m, off), __shfl_xor_sync(0xffffffffu, s, off), __shfl_xor_sync(0xffffffffu, arg, off));
+  if (kWarps > 1) {
+    if (lane == 0) { sm[warp] = m; ss[warp] = s; sa[warp] = arg; }
+    __syncthreads();
+    if (warp != 0) return;
+    for (int i = 1; i < kWarps; ++i) join_scores(m, s, arg, sm[i], ss[i], sa[i]);
   }
-  if (lane != 0) return;
+  if (lane != 0 || row >= N) return;
   const float l = m + logf(s);
   if (lse != nullptr) lse[row] = l;
   if (top != nullptr) top[row] = arg == 0x7fffffff ? 0 : arg;
@@ -415,14 +433,14 @@ __global__ void __launch_bounds__(128) scores_fold_kernel(const float2* part, co
   }
 }
 
-// sum of nll and number of counted rows, in a fixed order (one block)
-__global__ void __launch_bounds__(1024) loss_sum_kernel(const float* nll, const int64_t* labels, int64_t ignore, int64_t N, float* sum, float* count) {
+// sum of nll, number of counted rows and their quotient, in a fixed order (one block)
+__global__ void __launch_bounds__(1024) loss_sum_kernel(const float* nll, const int64_t* labels, int64_t ignore, int64_t N, float* sum, float* count,
+                                                        float* mean) {
   __shared__ float ss[32], sc[32];
   float s = 0.f, c = 0.f;
-  for (int64_t i = threadIdx.x; i < N; i += 1024) {
-    if (nll != nullptr) s += nll[i];
-    c += labels[i] != ignore ? 1.f : 0.f;
-  }
+  for (int64_t i = threadIdx.x; i < N; i += 1024) c += labels[i] != ignore ? 1.f : 0.f;
+  wait_prerequisites();
+  for (int64_t i = threadIdx.x; i < N; i += 1024) s += nll[i];
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) {
     s += __shfl_xor_sync(0xffffffffu, s, off);
@@ -435,6 +453,7 @@ __global__ void __launch_bounds__(1024) loss_sum_kernel(const float* nll, const 
   for (int i = 0; i < 32; ++i) { s += ss[i]; c += sc[i]; }
   if (sum != nullptr) *sum = s;
   if (count != nullptr) *count = c;
+  if (mean != nullptr) *mean = s / c;
 }
 
 // d_hidden = scale * (sum of the K splits' fp32 results), rounded once; 4 values a thread
@@ -609,7 +628,8 @@ int validate(const char* op, const void* hidden, const void* weight, int64_t hs,
 int launch_scores(const jl_head_scores_args* a, cudaStream_t stream) {
   int rc = validate("jl_head_scores", a->hidden, a->weight, a->hidden_stride, a->weight_stride, a->rows, a->hidden_size, a->vocab);
   if (rc != JL_OK) return rc;
-  if (a->labels == nullptr && (a->nll != nullptr || a->loss_sum != nullptr || a->loss_count != nullptr))
+  const bool want_loss = a->loss_sum != nullptr || a->loss_count != nullptr || a->loss_mean != nullptr;
+  if (a->labels == nullptr && (a->nll != nullptr || want_loss))
     return fail(JL_ERR_BAD_ARG, "jl_head_scores: nll and the loss need labels");
   const ScoresLayout l = scores_layout(a->rows, a->vocab);
   if (a->workspace == nullptr || a->workspace_bytes < l.total)
@@ -618,7 +638,7 @@ int launch_scores(const jl_head_scores_args* a, cudaStream_t stream) {
   rc = check_device_arch();
   if (rc != JL_OK) return rc;
   uint8_t* ws = static_cast<uint8_t*>(a->workspace);
-  float* nll = a->nll != nullptr || a->loss_sum == nullptr ? a->nll : reinterpret_cast<float*>(ws + l.nll);
+  float* nll = a->nll != nullptr || !want_loss ? a->nll : reinterpret_cast<float*>(ws + l.nll);
   for (int64_t r0 = 0; r0 < a->rows; r0 += kScoreRows) {
     const int64_t n = a->rows - r0 < kScoreRows ? a->rows - r0 : kScoreRows;
     Plan plan = l.plan;
@@ -635,13 +655,17 @@ int launch_scores(const jl_head_scores_args* a, cudaStream_t stream) {
     rc = plan.pair == 2 ? launch_gemm<2, false, false, kEpiScores>(h, w, Result{}, p, plan, a->hidden_size, 1, stream)
                         : launch_gemm<1, false, false, kEpiScores>(h, w, Result{}, p, plan, a->hidden_size, 1, stream);
     if (rc != JL_OK) return rc;
-    scores_fold_kernel<<<static_cast<unsigned>(cdiv(n, 4)), 128, 0, stream>>>(
-        p.part, p.part_arg, p.picked, plan.n_tiles, n, a->vocab, p.labels, a->ignore_index, nll != nullptr ? nll + r0 : nullptr,
-        a->lse != nullptr ? a->lse + r0 : nullptr, a->top != nullptr ? a->top + r0 : nullptr);
+    const bool few = n < 4 * kSms;
+    if (launch_dependent(few ? scores_fold_kernel<8> : scores_fold_kernel<1>, dim3(static_cast<unsigned>(few ? n : cdiv(n, 8))), dim3(256), 0, stream,
+                         static_cast<const float2*>(p.part), static_cast<const int*>(p.part_arg), static_cast<const float*>(p.picked), plan.n_tiles, n,
+                         static_cast<int64_t>(a->vocab), p.labels, a->ignore_index, nll != nullptr ? nll + r0 : nullptr,
+                         a->lse != nullptr ? a->lse + r0 : nullptr, a->top != nullptr ? a->top + r0 : nullptr) != cudaSuccess)
+      return check_launch("jl_head_scores (fold)");
   }
-  if (a->loss_sum != nullptr || a->loss_count != nullptr)
-    loss_sum_kernel<<<1, 1024, 0, stream>>>(nll, a->labels, a->ignore_index, a->rows, a->loss_sum, a->loss_count);
-  return check_launch("jl_head_scores");
+  if (want_loss && launch_dependent(loss_sum_kernel, dim3(1), dim3(1024), 0, stream, static_cast<const float*>(nll), a->labels, a->ignore_index, a->rows,
+                                    a->loss_sum, a->loss_count, a->loss_mean) != cudaSuccess)
+    return check_launch("jl_head_scores (loss)");
+  return JL_OK;
 }
 
 int launch_grads(const jl_head_grads_args* a, cudaStream_t stream) {

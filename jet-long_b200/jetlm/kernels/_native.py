@@ -211,6 +211,7 @@ class HeadScoresArgs(C.Structure):
         ("hidden", C.c_void_p), ("weight", C.c_void_p), ("hidden_stride", C.c_int64), ("weight_stride", C.c_int64),
         ("labels", C.c_void_p), ("ignore_index", C.c_int64), ("rows", C.c_int64), ("hidden_size", C.c_int32), ("vocab", C.c_int32),
         ("nll", C.c_void_p), ("lse", C.c_void_p), ("top", C.c_void_p), ("loss_sum", C.c_void_p), ("loss_count", C.c_void_p),
+        ("loss_mean", C.c_void_p),
         ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
     ]
 

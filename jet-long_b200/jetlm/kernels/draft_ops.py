@@ -21,7 +21,42 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _native as N
-from .jetlong_ops import _SUPPORTED_DTYPES, _call, _check_view, _require_arch, _require_contiguous, _st, _stream
+from .jetlong_ops import _SUPPORTED_DTYPES, _check_view, _require_arch, _require_contiguous, _st
+
+# Checked call layouts: what a call's shapes, strides, types and devices were found to allow, with the argument structure
+# filled in except for its pointers.  A decode loop makes the same call for every layer and step, and the checks took longer
+# than the kernels (attention: 78 us a call, 34 with the layouts kept).
+_LAYOUTS: dict = {}
+
+
+def _keep_layout(key, value):
+    if len(_LAYOUTS) >= 1024:
+        _LAYOUTS.clear()
+    _LAYOUTS[key] = value
+    return value
+
+
+def _sig(t: Optional[torch.Tensor]):
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
+
+
+def _aligned(op: str, pointers: dict, to: int = 16) -> None:
+    bits = 0
+    for p in pointers.values():
+        bits |= p
+    if bits % to:
+        raise ValueError(f"{op}: {next(n for n, p in pointers.items() if p % to)} must be {to}-byte aligned")
+
+
+def _run(op: str, fn, args, index: int) -> None:
+    """One C call on the current stream of the tensors' device."""
+    if torch.cuda.current_device() == index:
+        status = fn(C.byref(args), torch.cuda.current_stream().cuda_stream)
+    else:
+        with torch.cuda.device(index):
+            status = fn(C.byref(args), torch.cuda.current_stream().cuda_stream)
+    if status != N.JL_OK:
+        N.check(op, status)
 
 
 class DraftTree(NamedTuple):
@@ -71,10 +106,8 @@ def draft_tree(parents: torch.Tensor) -> DraftTree:
     parents = parents.contiguous()
     depth = torch.empty(B, T, dtype=torch.int32, device=dev)
     mask = torch.empty(B, T, (T + 63) // 64, dtype=torch.int64, device=dev)
-    a = N.TreePlanArgs(parents.data_ptr(), depth.data_ptr(), mask.data_ptr(), B, T)
     if B > 0:
-        with torch.cuda.device(dev):
-            _call("jl_tree_plan", lambda: N.lib().jl_tree_plan(C.byref(a), _stream()))
+        _run("jl_tree_plan", N.lib().jl_tree_plan, N.TreePlanArgs(parents.data_ptr(), depth.data_ptr(), mask.data_ptr(), B, T), dev.index)
     return DraftTree(depth, mask)
 
 
@@ -87,6 +120,32 @@ def tree_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_weight: tor
     key_group_rows (shape and strides of key_rows) receives the regrouped keys.  Absent nodes get zero queries and write
     nothing.  Returns (q_base, q_group), each (B,T,H,D); q_group is q_base when group_size == 1."""
     op = "tree_append"
+    key = (op, _sig(q), _sig(k), _sig(v), _sig(q_weight), _sig(k_weight), _sig(inv_freq), _sig(key_rows), _sig(value_rows),
+           _sig(key_group_rows), _sig(tree.depth), _sig(tree.mask), _sig(lens), q_eps, k_eps, group_size)
+    template = _LAYOUTS.get(key)
+    if template is None:
+        template = _keep_layout(key, _append_layout(op, q, k, v, q_weight, k_weight, inv_freq, key_rows, value_rows, tree, lens,
+                                                    q_eps, k_eps, group_size, key_group_rows))
+    if inv_freq.device != q.device or inv_freq.dtype != torch.float32 or not inv_freq.is_contiguous():
+        inv_freq = inv_freq.to(device=q.device, dtype=torch.float32).contiguous()
+    q_base = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    q_group = torch.empty(q.shape, dtype=q.dtype, device=q.device) if group_size > 1 else None
+    a = N.TreeAppendArgs.from_buffer_copy(template)
+    ptrs = dict(q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), key_rows=key_rows.data_ptr(), value_rows=value_rows.data_ptr(),
+                q_weight=q_weight.data_ptr(), k_weight=k_weight.data_ptr())
+    a.q, a.k, a.v, a.k_cache, a.v_cache, a.q_weight, a.k_weight = ptrs.values()
+    a.q_base = q_base.data_ptr()
+    if q_group is not None:
+        a.q_group = q_group.data_ptr()
+    if key_group_rows is not None:
+        a.k_group_cache = ptrs["key_group_rows"] = key_group_rows.data_ptr()
+    a.inv_freq, a.lens, a.depth = inv_freq.data_ptr(), lens.data_ptr(), tree.depth.data_ptr()
+    _aligned(op, ptrs)
+    _run("jl_tree_append", N.lib().jl_tree_append, a, q.device.index)
+    return q_base, (q_group if q_group is not None else q_base)
+
+
+def _append_layout(op, q, k, v, q_weight, k_weight, inv_freq, key_rows, value_rows, tree, lens, q_eps, k_eps, group_size, key_group_rows):
     for name, t in (("q", q), ("k", k), ("v", v), ("key_rows", key_rows), ("value_rows", value_rows)):
         _check_view(op, name, t)
         if t.dtype not in _SUPPORTED_DTYPES:
@@ -108,22 +167,14 @@ def tree_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_weight: tor
     if key_group_rows is not None and (key_group_rows.shape != key_rows.shape or key_group_rows.dtype != key_rows.dtype
                                        or [_st(key_group_rows, i) for i in range(3)] != [_st(key_rows, i) for i in range(3)]):
         raise ValueError(f"{op}: key_group_rows must match key_rows in shape, strides and dtype")
-    dev = _require_cuda(op, q, k, v, q_weight, k_weight, key_rows, value_rows, key_group_rows, tree.depth, tree.mask, lens)
-    _require_arch(op, dev)
-    inv_freq = inv_freq.to(device=dev, dtype=torch.float32).contiguous()
-    q_base = torch.empty(B, T, H, D, dtype=q.dtype, device=dev)
-    q_group = torch.empty(B, T, H, D, dtype=q.dtype, device=dev) if group_size > 1 else None
-    a = N.TreeAppendArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                         *(_st(t, i) for t in (q, k, v) for i in range(3)),
-                         q_weight.data_ptr(), k_weight.data_ptr(), float(q_eps), float(k_eps),
-                         q_base.data_ptr(), q_group.data_ptr() if q_group is not None else None,
-                         key_rows.data_ptr(), value_rows.data_ptr(),
-                         key_group_rows.data_ptr() if key_group_rows is not None else None,
-                         *(_st(t, i) for t in (key_rows, value_rows) for i in range(3)), int(key_rows.shape[1]),
-                         B, T, H, Hk, D, int(group_size), inv_freq.data_ptr(), lens.data_ptr(), tree.depth.data_ptr())
-    with torch.cuda.device(dev):
-        _call("jl_tree_append", lambda: N.lib().jl_tree_append(C.byref(a), _stream()))
-    return q_base, (q_group if q_group is not None else q_base)
+    _require_arch(op, _require_cuda(op, q, k, v, q_weight, k_weight, key_rows, value_rows, key_group_rows, tree.depth, tree.mask, lens))
+    a = N.TreeAppendArgs()
+    for name, t in (("q", q), ("k", k), ("v", v), ("kc", key_rows), ("vc", value_rows)):
+        for i, axis in enumerate("bsh"):
+            setattr(a, f"{name}_stride_{axis}", _st(t, i))
+    a.q_eps, a.k_eps, a.cache_rows, a.group_size = float(q_eps), float(k_eps), int(key_rows.shape[1]), int(group_size)
+    a.batch, a.nodes, a.heads, a.kv_heads, a.head_dim = B, T, H, Hk, D
+    return a
 
 
 def tree_attention(q_base: torch.Tensor, q_group: torch.Tensor, key_rows: torch.Tensor, value_rows: torch.Tensor,
@@ -136,6 +187,36 @@ def tree_attention(q_base: torch.Tensor, q_group: torch.Tensor, key_rows: torch.
     (group size 1) every pair is scored q_base . key_rows.  Nothing depends on lens on the host, so the launches can sit
     in a CUDA graph.  Returns (out (B,T,H,D), lse (B,H,T) fp32) or out; a row that sees no key is zero with lse -inf."""
     op = "tree_attention"
+    key = (op, _sig(q_base), _sig(q_group), _sig(key_rows), _sig(value_rows), _sig(key_group_rows), _sig(tree.depth), _sig(tree.mask),
+           _sig(lens), _sig(out), w_0, softmax_scale)
+    plan = _LAYOUTS.get(key)
+    if plan is None:
+        plan = _keep_layout(key, _attention_layout(op, q_base, q_group, key_rows, value_rows, tree, lens, w_0, key_group_rows,
+                                                   softmax_scale, out))
+    template, ws_bytes = plan
+    dev = q_base.device
+    if out is None:
+        out = torch.empty(q_base.shape, dtype=q_base.dtype, device=dev)
+    # split partials: this call's own memory from the stream-ordered allocator, so concurrent calls and captured graphs
+    # never share it
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    a = N.TreeAttentionArgs.from_buffer_copy(template)
+    ptrs = dict(q_base=q_base.data_ptr(), key_rows=key_rows.data_ptr(), value_rows=value_rows.data_ptr(), out=out.data_ptr())
+    a.q_base, a.k_base, a.v, a.out = ptrs.values()
+    if key_group_rows is not None:
+        a.q_group = ptrs["q_group"] = q_group.data_ptr()
+        a.k_group = ptrs["key_group_rows"] = key_group_rows.data_ptr()
+    _aligned(op, ptrs)
+    a.lens, a.depth, a.mask, a.workspace = lens.data_ptr(), tree.depth.data_ptr(), tree.mask.data_ptr(), ws.data_ptr()
+    lse = None
+    if return_lse:
+        lse = torch.empty(a.batch, a.heads, a.nodes, dtype=torch.float32, device=dev)
+        a.lse = lse.data_ptr()
+    _run("jl_tree_attention", N.lib().jl_tree_attention, a, dev.index)
+    return (out, lse) if return_lse else out
+
+
+def _attention_layout(op, q_base, q_group, key_rows, value_rows, tree, lens, w_0, key_group_rows, softmax_scale, out):
     tensors = [("q_base", q_base), ("q_group", q_group), ("key_rows", key_rows), ("value_rows", value_rows)]
     if key_group_rows is not None:
         tensors.append(("key_group_rows", key_group_rows))
@@ -162,31 +243,22 @@ def tree_attention(q_base: torch.Tensor, q_group: torch.Tensor, key_rows: torch.
     _require_tree(op, tree, lens, B, T)
     if rows < T:
         raise ValueError(f"{op}: the cache ({rows} rows) does not hold the {T} nodes")
-    dev = _require_cuda(op, *(t for _, t in tensors), tree.depth, tree.mask, lens, out)
-    _require_arch(op, dev)
-    if out is None:
-        out = torch.empty(B, T, H, D, dtype=q_base.dtype, device=dev)
-    else:
+    if out is not None:
         if tuple(out.shape) != (B, T, H, D) or out.dtype != q_base.dtype:
             raise ValueError(f"{op}: out must be {q_base.dtype} with shape {(B, T, H, D)}")
         _check_view(op, "out", out)
-    lse = torch.empty(B, H, T, dtype=torch.float32, device=dev) if return_lse else None
-    lib = N.lib()
-    # split partials: this call's own memory from the stream-ordered allocator, so concurrent calls and captured graphs
-    # never share it
-    ws = torch.empty(max(16, lib.jl_tree_attention_workspace_bytes(B, T, H, Hk, rows)), dtype=torch.uint8, device=dev)
-    two = key_group_rows is not None
-    a = N.TreeAttentionArgs(q_base.data_ptr(), q_group.data_ptr() if two else None, key_rows.data_ptr(),
-                            key_group_rows.data_ptr() if two else None, value_rows.data_ptr(),
-                            *(_st(t, i) for t in (q_base, key_rows, value_rows) for i in range(3)),
-                            lens.data_ptr(), tree.depth.data_ptr(), tree.mask.data_ptr(), out.data_ptr(),
-                            lse.data_ptr() if lse is not None else None, *(_st(out, i) for i in range(3)),
-                            B, T, H, Hk, D, rows, int(w_0),
-                            float(softmax_scale) if softmax_scale is not None else 1.0 / math.sqrt(D), 0,
-                            ws.data_ptr(), ws.numel())
-    with torch.cuda.device(dev):
-        _call("jl_tree_attention", lambda: lib.jl_tree_attention(C.byref(a), _stream()))
-    return (out, lse) if return_lse else out
+    _require_arch(op, _require_cuda(op, *(t for _, t in tensors), tree.depth, tree.mask, lens, out))
+    o_st = [_st(out, i) for i in range(3)] if out is not None else [T * H * D, H * D, D]
+    ws_bytes = max(16, N.lib().jl_tree_attention_workspace_bytes(B, T, H, Hk, rows))
+    a = N.TreeAttentionArgs()
+    for name, st in (("q", [_st(q_base, i) for i in range(3)]), ("k", [_st(key_rows, i) for i in range(3)]),
+                     ("v", [_st(value_rows, i) for i in range(3)]), ("o", o_st)):
+        for axis, x in zip("bsh", st):
+            setattr(a, f"{name}_stride_{axis}", x)
+    a.batch, a.nodes, a.heads, a.kv_heads, a.head_dim, a.rows, a.w_0 = B, T, H, Hk, D, rows, int(w_0)
+    a.softmax_scale = float(softmax_scale) if softmax_scale is not None else 1.0 / math.sqrt(D)
+    a.workspace_bytes = ws_bytes
+    return a, ws_bytes
 
 
 def keep_path(buffer: torch.Tensor, path: torch.Tensor, start: int) -> None:

@@ -9,13 +9,13 @@ Kernels run on the current torch CUDA stream; there is no PyTorch fallback.
 """
 from __future__ import annotations
 
-import ctypes as C
 from typing import NamedTuple, Optional
 
 import torch
 
 from . import _native as N
-from .jetlong_ops import _SUPPORTED_DTYPES, _call, _require_arch, _stream
+from .draft_ops import _LAYOUTS, _keep_layout, _run, _sig
+from .jetlong_ops import _SUPPORTED_DTYPES, _require_arch
 
 
 class TokenScores(NamedTuple):
@@ -27,7 +27,22 @@ class TokenScores(NamedTuple):
 
 
 def _rows(op: str, hidden: torch.Tensor, weight: torch.Tensor, labels: Optional[torch.Tensor]):
-    """(hidden as (rows, H), weight, labels as (rows,)) with the checks the kernels rely on."""
+    """(hidden as (rows, H), labels as (rows,)) with the checks the kernels rely on; the layout checks are made once per layout."""
+    key = (op, _sig(hidden), _sig(weight), None if labels is None else (labels.shape, labels.dtype, labels.device))
+    if key not in _LAYOUTS:
+        _check_rows(op, hidden, weight, labels)
+        _keep_layout(key, True)
+    h = hidden if hidden.dim() == 2 else hidden.reshape(-1, hidden.shape[-1])          # a copy only where the leading dimensions do not collapse
+    for name, t in (("hidden", h), ("weight", weight)):
+        if t.shape[0] > 0 and (t.stride(1) != 1 or (t.shape[0] > 1 and (t.stride(0) % 8 or t.stride(0) < t.shape[1])) or t.data_ptr() % 16):
+            raise ValueError(f"{op}: {name} rows must be contiguous, 16-byte aligned and a multiple of 8 elements apart; "
+                             f"call {name}.contiguous()")
+    if labels is not None and (labels.dim() != 1 or not labels.is_contiguous()):
+        labels = labels.reshape(-1).contiguous()
+    return h, labels
+
+
+def _check_rows(op, hidden, weight, labels):
     if hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1]:
         raise ValueError(f"{op}: expects hidden (..., H) and weight (V, H), got {tuple(hidden.shape)} and {tuple(weight.shape)}")
     if hidden.dtype not in _SUPPORTED_DTYPES or weight.dtype != hidden.dtype:
@@ -36,38 +51,41 @@ def _rows(op: str, hidden: torch.Tensor, weight: torch.Tensor, labels: Optional[
         raise ValueError(f"{op}: hidden and weight must be on one CUDA device")
     if weight.shape[0] < 1 or weight.shape[1] < 8 or weight.shape[1] % 8:
         raise ValueError(f"{op}: the hidden size must be a multiple of 8 and the vocabulary not empty, got {tuple(weight.shape)}")
-    if labels is not None:
-        if labels.shape != hidden.shape[:-1] or labels.dtype != torch.int64 or labels.device != hidden.device:
-            raise ValueError(f"{op}: labels must be int64 with shape {tuple(hidden.shape[:-1])} on {hidden.device}")
-        labels = labels.reshape(-1).contiguous()
+    if labels is not None and (labels.shape != hidden.shape[:-1] or labels.dtype != torch.int64 or labels.device != hidden.device):
+        raise ValueError(f"{op}: labels must be int64 with shape {tuple(hidden.shape[:-1])} on {hidden.device}")
     _require_arch(op, hidden.device)
-    h = hidden.reshape(-1, hidden.shape[-1])          # a copy only where the leading dimensions do not collapse
-    for name, t in (("hidden", h), ("weight", weight)):
-        if t.shape[0] > 0 and (t.stride(1) != 1 or (t.shape[0] > 1 and (t.stride(0) % 8 or t.stride(0) < t.shape[1])) or t.data_ptr() % 16):
-            raise ValueError(f"{op}: {name} rows must be contiguous, 16-byte aligned and a multiple of 8 elements apart; "
-                             f"call {name}.contiguous()")
-    return h, weight, labels
 
 
 def _row_stride(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
-def _scores(op, h, w, labels, ignore_index, *, nll, lse, top, loss):
-    """One jl_head_scores call on (rows, H) operands; returns (nll, lse, top, loss_sum, loss_count), None where not asked for."""
-    n, dev = h.shape[0], h.device
-    f32 = lambda *s: torch.empty(*s, dtype=torch.float32, device=dev)      # noqa: E731
-    out = (f32(n) if nll else None, f32(n) if lse else None, torch.empty(n, dtype=torch.int64, device=dev) if top else None,
-           f32(()) if loss else None, f32(()) if loss else None)
+def _scores(h, w, labels, ignore_index, *, nll, top, reduction=None):
+    """One jl_head_scores call on (rows, H) operands; returns (nll, lse, top, loss, loss_count), None where not asked for."""
+    n, dev, a = h.shape[0], h.device, N.HeadScoresArgs()
+    per_row = torch.empty(2 if nll else 1, n, dtype=torch.float32, device=dev)
+    best = torch.empty(n, dtype=torch.int64, device=dev) if top else None
+    scalars = torch.empty(2, dtype=torch.float32, device=dev) if reduction is not None else None
     lib = N.lib()
     ws = torch.empty(lib.jl_head_scores_workspace_bytes(n, w.shape[1], w.shape[0]), dtype=torch.uint8, device=dev)
-    ptr = lambda t: t.data_ptr() if t is not None else None                # noqa: E731
-    a = N.HeadScoresArgs(h.data_ptr() if n else w.data_ptr(), w.data_ptr(), _row_stride(h), _row_stride(w),
-                         ptr(labels) if n or labels is None else w.data_ptr(), int(ignore_index),
-                         n, w.shape[1], w.shape[0], *(ptr(t) for t in out), ws.data_ptr(), ws.numel())
-    with torch.cuda.device(dev):
-        _call("jl_head_scores", lambda: lib.jl_head_scores(C.byref(a), _stream()))
-    return out
+    a.weight, a.hidden_stride, a.weight_stride, a.ignore_index = w.data_ptr(), _row_stride(h), _row_stride(w), int(ignore_index)
+    a.hidden, a.rows, a.hidden_size, a.vocab = h.data_ptr() or a.weight, n, w.shape[1], w.shape[0]
+    if labels is not None:
+        a.labels = labels.data_ptr() or a.weight                # no rows: never read
+    a.lse = per_row.data_ptr()
+    if nll:
+        a.nll = a.lse + 4 * n if n else a.weight
+    if top:
+        a.top = best.data_ptr()
+    if reduction is not None:
+        a.loss_count = scalars.data_ptr() + 4
+        if reduction == "mean":
+            a.loss_mean = scalars.data_ptr()
+        else:
+            a.loss_sum = scalars.data_ptr()
+    a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+    _run("jl_head_scores", lib.jl_head_scores, a, dev.index)
+    return (per_row[1] if nll else None, per_row[0], best, *((scalars[0], scalars[1]) if scalars is not None else (None, None)))
 
 
 def token_scores(hidden: torch.Tensor, weight: torch.Tensor, labels: Optional[torch.Tensor] = None, *, ignore_index: int = -100,
@@ -76,43 +94,46 @@ def token_scores(hidden: torch.Tensor, weight: torch.Tensor, labels: Optional[to
     the most likely token of every row (the lowest index of equal ones) — in fp32, with no logits in memory.
     hidden (..., H) and weight (V, H) bf16, labels (...) int64.  A label that is neither ignore_index nor in [0, V) gives
     NaN.  Not differentiable: linear_cross_entropy is."""
-    op = "token_scores"
-    with torch.no_grad():
-        h, w, lab = _rows(op, hidden.detach(), weight.detach(), labels)
-        nll, lse, best, _, _ = _scores(op, h, w, lab, ignore_index, nll=labels is not None, lse=True, top=top, loss=False)
-    shape = hidden.shape[:-1]
-    return TokenScores(nll.view(shape) if nll is not None else None, lse.view(shape), best.view(shape) if best is not None else None)
+    h, lab = _rows("token_scores", hidden.detach(), weight, labels)
+    nll, lse, best, _, _ = _scores(h, weight, lab, ignore_index, nll=labels is not None, top=top)
+    if hidden.dim() != 2:
+        shape = hidden.shape[:-1]
+        nll, lse, best = (t.view(shape) if t is not None else None for t in (nll, lse, best))
+    return TokenScores(nll, lse, best)
 
 
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, labels, ignore_index, reduction):
-        h, w, lab = _rows("linear_cross_entropy", hidden, weight, labels)
-        nll, lse, _, total, count = _scores("linear_cross_entropy", h, w, lab, ignore_index, nll=reduction == "none", lse=True,
-                                            top=False, loss=reduction != "none")
-        ctx.save_for_backward(hidden, weight, lab, lse, count if reduction == "mean" else None)
-        ctx.ignore_index, ctx.per_row = int(ignore_index), reduction == "none"
-        return nll.view(labels.shape) if ctx.per_row else total / count if reduction == "mean" else total
+        h, lab = _rows("linear_cross_entropy", hidden, weight, labels)
+        per_row = reduction == "none"
+        nll, lse, _, loss, count = _scores(h, weight, lab, ignore_index, nll=per_row, top=False, reduction=None if per_row else reduction)
+        ctx.save_for_backward(h, weight, lab, lse, count if reduction == "mean" else None)
+        ctx.ignore_index, ctx.per_row, ctx.shape = int(ignore_index), per_row, hidden.shape
+        return nll.view(labels.shape) if per_row else loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        hidden, weight, lab, lse, count = ctx.saved_tensors
-        h, w, _ = _rows("linear_cross_entropy", hidden, weight, None)
-        n, dev = h.shape[0], h.device
+        h, w, lab, lse, count = ctx.saved_tensors
+        n, dev, a, lib = h.shape[0], h.device, N.HeadGradsArgs(), N.lib()
         d_h = torch.empty(h.shape, dtype=h.dtype, device=dev) if ctx.needs_input_grad[0] else None
         d_w = torch.empty(w.shape, dtype=w.dtype, device=dev) if ctx.needs_input_grad[1] else None
-        grad = grad.to(torch.float32).reshape(-1).contiguous()
-        lib = N.lib()
+        if grad.dtype != torch.float32 or (ctx.per_row and (grad.dim() != 1 or not grad.is_contiguous())):
+            grad = grad.to(torch.float32).reshape(-1).contiguous()
         ws = torch.empty(lib.jl_head_grads_workspace_bytes(n, w.shape[1], w.shape[0]), dtype=torch.uint8, device=dev)
-        some = lambda t: t.data_ptr() if t.numel() else w.data_ptr()       # noqa: E731  (no rows: never read)
-        a = N.HeadGradsArgs(some(h), w.data_ptr(), _row_stride(h), _row_stride(w), some(lab), ctx.ignore_index, n, w.shape[1], w.shape[0],
-                            some(lse), some(grad), 1 if ctx.per_row else 0, count.data_ptr() if count is not None else None,
-                            d_h.data_ptr() if d_h is not None and n else None, d_w.data_ptr() if d_w is not None else None,
-                            ws.data_ptr(), ws.numel())
-        with torch.cuda.device(dev):
-            _call("jl_head_grads", lambda: lib.jl_head_grads(C.byref(a), _stream()))
-        return d_h.view(hidden.shape) if d_h is not None else None, d_w, None, None, None
+        a.weight, a.hidden_stride, a.weight_stride, a.ignore_index = w.data_ptr(), _row_stride(h), _row_stride(w), ctx.ignore_index
+        a.hidden, a.labels, a.lse, a.grad = (t.data_ptr() or a.weight for t in (h, lab, lse, grad))      # no rows: never read
+        a.rows, a.hidden_size, a.vocab, a.grad_stride = n, w.shape[1], w.shape[0], 1 if ctx.per_row else 0
+        if count is not None:
+            a.grad_count = count.data_ptr()
+        if d_h is not None and n:
+            a.d_hidden = d_h.data_ptr()
+        if d_w is not None:
+            a.d_weight = d_w.data_ptr()
+        a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+        _run("jl_head_grads", lib.jl_head_grads, a, dev.index)
+        return d_h.view(ctx.shape) if d_h is not None else None, d_w, None, None, None
 
 
 def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, *, ignore_index: int = -100,
