@@ -12,12 +12,13 @@
 // head) each, and every segment leaves one normalised fp32 partial (O, LSE) per row that tree_combine_kernel joins.
 // Nothing on the host depends on the lengths, which are read on the device.
 //
-//   warp 0      TMA producer of K and V tiles (one ring of 5, in the order of their use), running ahead over all borders
-//   warp 1      MMA issuer: S_t = Q K^T two items ahead of O_t += P V; in tiles that reach past the committed rows it first
-//               zeroes the value rows that belong to no node, which may hold anything (0 * NaN is NaN)
-//   warp 2      tensor memory
+//   warp 0      TMA producer of K and V tiles (one ring of 5, in the order of their use), running ahead over all borders; it
+//               also leaves one word per visit that tells the issuers what is particular about it
+//   warp 1      issues S_t = Q K^T;  warp 2 issues O_t += P V (and owns tensor memory).  Two issuers, because the issue of an MMA
+//               blocks while two or three are queued: with one, the waits for one tile's operands stood between the products of
+//               the other (2000 clocks per 128 x 128 x 256 product pair instead of 1450)
 //   warp 3      TMA producer of the query tiles of the current class
-//   warps 4-11  softmax: one thread per row, 128 scores in registers, P back to tensor memory over S
+//   warps 4-11  softmax: one thread per row, P back to tensor memory over S
 #include "tc_common.cuh"
 #include "../../include/jetlong_b200_tree.h"
 
@@ -44,12 +45,13 @@ struct TreeParams {
   int rpt;                     // rows per row tile that can be in use
   int two_tiles;               // two row tiles per CTA instead of two states of one
   int mbs, workers;            // CTAs per part of the line, parts
+  int unrolled;                // enough visits per part to pay for the unrolled softmax's instruction fetches
   int two_classes, nodes_far;  // nodes_far: w_0 is so small that drafted keys can be in the far class
   int64_t w_0;
   float scale_log2;
   const int32_t *lens, *depth;
   const uint64_t* mask;
-  float *part_o, *part_lse;    // [slot][state or tile][rpt] rows
+  float *part_o, *part_lse;    // [slot][state or tile] of [32 column groups][rpt rows][4] and [rpt rows]
   __nv_bfloat16* out;
   float* lse;
   int64_t os_b, os_s, os_h;
@@ -57,11 +59,16 @@ struct TreeParams {
 
 struct TreeMaps { CUtensorMap q[2], k[2], v; };       // [0] near (base), [1] far (regrouped)
 
+// What is particular about a visit.
+enum : int { kQFirst = 1, kQLast = 2, kOFirst = 4, kTail = 8 };
+constexpr int kVisitRing = 8;                // the producer is at most 3 visits ahead of the last consumer
+
 struct TreeSmem {
   alignas(1024) uint8_t q[2][kTileBytes];    // two row tiles, or two class operands of one
   alignas(1024) uint8_t kv[kStages][kTileBytes];
   uint64_t q_full[2], q_free[2], full[kStages], empty[kStages];
-  uint64_t s_full[2], p_half[2][2], o_full[2];
+  uint64_t s_full[2], p_half[2][2], pv_done[2];
+  alignas(16) int4 visit[kVisitRing];        // flags, sample, node index of the key tile's first row
   int64_t lo, hi;                            // this CTA's part of the line
   int start_b, start_kvh, start_v;
   uint32_t tmem_base;
@@ -114,44 +121,14 @@ struct Walk {
   }
 };
 
-// Products in issue order.  Two row tiles: (visit, 0), (visit, 1); one: (visit, alternating state).  Consecutive items never
-// share a state, whatever segment they belong to.
-struct Item { int t, visit, use, b, u0; bool first_use, last_use, q_first, q_last, o_first, o_last, tail; };     // u0: node index of the tile's first row
-struct Items {
-  Walk w;
-  Segment seg;
-  int v, t, visit, use;
-  bool open;
-  __device__ __forceinline__ explicit Items(const TreeSmem& sm) : w(sm), v(0), t(0), visit(-1), use(-1), open(false) {}
-  __device__ __forceinline__ bool next(const TreeParams& p, Item& it) {
-    if (open && p.two_tiles && t == 0) {
-      t = 1;                                           // the second row tile of the same visit
-    } else {
-      if (!open || v + 1 == seg.v1) {
-        if (!w.next(p, seg)) return false;
-        open = true;
-        v = seg.v0;
-      } else {
-        ++v;
-      }
-      ++visit;
-      t = p.two_tiles ? 0 : visit & 1;
-    }
-    const bool class_start = v == seg.v0 || v == seg.vis.far, class_end = v + 1 == seg.v1 || v + 1 == seg.vis.far;
-    it.first_use = !p.two_tiles || t == 0;
-    it.last_use = !p.two_tiles || t == 1;
-    it.q_first = class_start && it.first_use;
-    it.q_last = class_end && it.last_use;
-    if (it.q_first) ++use;
-    it.t = t;
-    it.visit = visit;
-    it.use = use;
-    it.o_first = v - seg.v0 < (p.two_tiles ? 1 : 2);
-    it.o_last = v + (p.two_tiles ? 1 : 2) >= seg.v1;
-    it.tail = seg.tail(v);
-    it.b = seg.b;
-    it.u0 = seg.key_tile(v) * kTileN - seg.vis.len;
-    return true;
+// Ring slot of the next K or V tile and the parity of its use
+struct RingPos {
+  int slot;
+  uint32_t parity;
+  __device__ __forceinline__ explicit RingPos(int first) : slot(first), parity(0) {}
+  __device__ __forceinline__ void next() {       // two tiles per visit
+    slot += 2;
+    if (slot >= kStages) { slot -= kStages; parity ^= 1; }
   }
 };
 
@@ -161,6 +138,10 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int mb = static_cast<int>(blockIdx.x) % p.mbs, worker = static_cast<int>(blockIdx.x) / p.mbs;
   launch_dependents();                           // the combine kernel may take its place and wait there for our end
+  if (threadIdx.x >= 64 && threadIdx.x < 69) {   // the tensor maps: q[0], q[1], k[0], k[1], v
+    const CUtensorMap* m = reinterpret_cast<const CUtensorMap*>(&maps) + (threadIdx.x - 64);
+    asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
+  }
   const int q_slots = p.two_tiles ? 1 : 2;
 
   if (warp == 0) {
@@ -202,7 +183,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
       mbar_init(&sm.p_half[i][1], 128);
     }
     for (int i = 0; i < kStages; ++i) { mbar_init(&sm.full[i], 1); mbar_init(&sm.empty[i], 1); }
-    for (int i = 0; i < 2; ++i) mbar_init(&sm.o_full[i], 1);
+    for (int i = 0; i < 2; ++i) mbar_init(&sm.pv_done[i], 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 2) {
@@ -223,16 +204,23 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
         Walk w(sm);
         Segment seg;
         int g = 0;
-        while (w.next(p, seg)) {
+        RingPos pos[2] = {RingPos(0), RingPos(1)};
+        const int step = p.two_tiles ? 1 : 2;
+        while (w.next(p, seg) && !*failed) {
           for (int v = seg.v0; v < seg.v1; ++v, ++g) {
             const int row = seg.key_tile(v) * kTileN;
+            const int flags = (v == seg.v0 || v == seg.vis.far ? kQFirst : 0) | (v + 1 == seg.v1 || v + 1 == seg.vis.far ? kQLast : 0) |
+                              (v - seg.v0 < step ? kOFirst : 0) | (seg.tail(v) ? kTail : 0);
+#pragma unroll
             for (int kv = 0; kv < 2; ++kv) {
               const CUtensorMap* map = kv == 1 ? &maps.v : &maps.k[v < seg.vis.far ? 1 : 0];
-              const int i = 2 * g + kv, st = i % kStages;
-              mbar_wait(&sm.empty[st], ((i / kStages) & 1) ^ 1, sm);
+              const int st = pos[kv].slot;
+              mbar_wait(&sm.empty[st], pos[kv].parity ^ 1, sm);
               if (*failed) break;
+              if (kv == 0) sm.visit[g % kVisitRing] = make_int4(flags, seg.b, row - seg.vis.len, 0);      // published by the arrivals below
               mbar_expect_tx(&sm.full[st], kTileBytes);
               for (int h = 0; h < 2; ++h) tma_load_4d(sm.kv[st] + h * kHalfBytes, map, &sm.full[st], h * 64, seg.kvh, row, seg.b);
+              pos[kv].next();
             }
           }
         }
@@ -259,74 +247,95 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
           }
         }
       }
-    } else if (warp == 1) {
-      // ====================================== MMA issuer ======================================
+    } else {
+      // ==================================== MMA issuers ====================================
+      // The whole warp walks the visits, so that ring indices, parities and descriptors are warp-uniform; one elected lane issues.
       uint32_t leader;
       asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(leader));
-      const uint32_t idesc_qk = instr_desc(128, kTileN, 0), idesc_pv = instr_desc(128, kHeadDim, 1);
-      const uint64_t q_desc = smem_desc(smem_u32(sm.q[0]), 16, 1024), k_desc = smem_desc(smem_u32(sm.kv[0]), 16, 1024);
-      const uint64_t v_desc = smem_desc(smem_u32(sm.kv[0]), kHalfBytes, 1024);
-      Items ahead(sm), now(sm);
-      Item it;
-      auto issue_qk = [&]() {                          // the next item's scores, if there is one
-        Item n;
-        if (!ahead.next(p, n)) return;
-        const int ks = 2 * n.visit % kStages, slot = n.use % q_slots;
-        if (n.q_first) mbar_wait(&sm.q_full[slot], (n.use / q_slots) & 1, sm);
-        if (n.first_use) mbar_wait(&sm.full[ks], (2 * n.visit / kStages) & 1, sm);
-        tc_fence_after();
-        const uint64_t qd = q_desc + static_cast<uint64_t>(((p.two_tiles ? n.t : slot) * kTileBytes) >> 4);
-        const uint64_t kd = k_desc + static_cast<uint64_t>((ks * kTileBytes) >> 4);
-        if (leader) {
-#pragma unroll
-          for (int kk = 0; kk < 8; ++kk) {
-            const uint64_t off = static_cast<uint64_t>(((kk >> 2) * kHalfBytes + (kk & 3) * 32) >> 4);
-            mma_ss(tmem + n.t * 128, qd + off, kd + off, idesc_qk, kk > 0);
+      const int n = static_cast<int>(sm.hi - sm.lo), tiles = p.two_tiles ? 2 : 1;
+      RingPos pos(warp - 1);                           // K tiles are the ring's even tiles, V tiles the odd ones
+      uint32_t parity = 0u;                            // bit t: parity of state t's next barrier phase
+      if (warp == 1) {
+        const uint32_t idesc = instr_desc(128, kTileN, 0);
+        const uint64_t q_desc = smem_desc(smem_u32(sm.q[0]), 16, 1024), k_desc = smem_desc(smem_u32(sm.kv[0]), 16, 1024);
+        int use = -1;                                  // query operands taken so far
+        for (int g = 0; g < n; ++g, pos.next()) {
+          mbar_wait(&sm.full[pos.slot], pos.parity, sm);
+          const int flags = *reinterpret_cast<volatile int*>(&sm.visit[g % kVisitRing].x);
+          if (__any_sync(0xffffffffu, flags & kQFirst)) {
+            ++use;
+            mbar_wait(&sm.q_full[p.two_tiles ? 0 : use & 1], (p.two_tiles ? use : use >> 1) & 1, sm);
           }
-          mma_commit(&sm.s_full[n.t]);
-          if (n.last_use) mma_commit(&sm.empty[ks]);
-          if (n.q_last) mma_commit(&sm.q_free[slot]);
-        }
-        __syncwarp();
-      };
-      issue_qk();
-      issue_qk();
-      int done[2] = {0, 0};
-      while (now.next(p, it)) {
-        const int vs = (2 * it.visit + 1) % kStages;
-        const uint64_t vd = v_desc + static_cast<uint64_t>((vs * kTileBytes) >> 4);
-        const int parity = (it.t ? done[1] : done[0]) & 1;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          mbar_wait(&sm.p_half[it.t][h], parity, sm);
-          if (h == 0 && it.first_use) {
-            mbar_wait(&sm.full[vs], ((2 * it.visit + 1) / kStages) & 1, sm);
-            if (it.tail) {
-              for (int r0 = 0; r0 < kTileN; r0 += 32) {
-                const int u = it.u0 + r0 + lane;
-                const bool keep = u < 0 || (u < p.nodes && p.depth[static_cast<int64_t>(it.b) * p.nodes + u] >= 0);
-                for (uint32_t dead = __ballot_sync(0xffffffffu, !keep); dead != 0u; dead &= dead - 1)
-                  if (lane < 16)
-                    *reinterpret_cast<uint4*>(sm.kv[vs] + (lane >> 3) * kHalfBytes + (r0 + __ffs(dead) - 1) * 128 + (lane & 7) * 16) =
-                        make_uint4(0u, 0u, 0u, 0u);
-              }
-              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-              __syncwarp();
+          if (*failed) break;
+          const uint64_t kd = k_desc + static_cast<uint64_t>((pos.slot * kTileBytes) >> 4);
+          for (int i = 0; i < tiles; ++i) {
+            const int t = p.two_tiles ? i : g & 1;
+            // the scores go where the probabilities of the state's previous item are: P V has to be done with them
+            if (g >= (p.two_tiles ? 1 : 2)) {
+              mbar_wait(&sm.pv_done[t], (parity >> t) & 1u, sm);
+              parity ^= 1u << t;
             }
-          }
-          tc_fence_after();
-          if (leader) {
+            tc_fence_after();
+            const uint64_t qd = q_desc + static_cast<uint64_t>(((p.two_tiles ? i : use & 1) * kTileBytes) >> 4);
+            if (leader) {
 #pragma unroll
-            for (int kk = 4 * h; kk < 4 * h + 4; ++kk)
-              mma_ts(tmem + 256 + it.t * 128, tmem + it.t * 128 + kk * 8, vd + static_cast<uint64_t>((kk * 2048) >> 4), idesc_pv,
-                     (!it.o_first || kk > 0) ? 1u : 0u);
-            if (h == 1 && it.last_use) mma_commit(&sm.empty[vs]);
-            if (h == 1 && it.o_last) mma_commit(&sm.o_full[it.t]);
+              for (int kk = 0; kk < 8; ++kk) {
+                const uint64_t off = static_cast<uint64_t>(((kk >> 2) * kHalfBytes + (kk & 3) * 32) >> 4);
+                mma_ss(tmem + t * 128, qd + off, kd + off, idesc, kk > 0);
+              }
+              mma_commit(&sm.s_full[t]);
+            }
+            __syncwarp();
+          }
+          if (leader) {
+            mma_commit(&sm.empty[pos.slot]);
+            if (flags & kQLast) mma_commit(&sm.q_free[p.two_tiles ? 0 : use & 1]);
           }
           __syncwarp();
         }
-        if (it.t) ++done[1]; else ++done[0];
-        issue_qk();
+      } else {
+        const uint32_t idesc = instr_desc(128, kHeadDim, 1);
+        const uint64_t v_desc = smem_desc(smem_u32(sm.kv[0]), kHalfBytes, 1024);
+        for (int g = 0; g < n; ++g, pos.next()) {
+          mbar_wait(&sm.full[pos.slot], pos.parity, sm);
+          if (*failed) break;
+          const int4 visit = make_int4(*reinterpret_cast<volatile int*>(&sm.visit[g % kVisitRing].x), *reinterpret_cast<volatile int*>(&sm.visit[g % kVisitRing].y),
+                                       *reinterpret_cast<volatile int*>(&sm.visit[g % kVisitRing].z), 0);
+          if (__any_sync(0xffffffffu, visit.x & kTail)) {
+            // value rows that belong to no node may hold anything, and 0 * NaN is NaN
+            for (int r0 = 0; r0 < kTileN; r0 += 32) {
+              const int u = visit.z + r0 + lane;
+              const bool keep = u < 0 || (u < p.nodes && p.depth[static_cast<int64_t>(visit.y) * p.nodes + u] >= 0);
+              for (uint32_t dead = __ballot_sync(0xffffffffu, !keep); dead != 0u; dead &= dead - 1)
+                if (lane < 16)
+                  *reinterpret_cast<uint4*>(sm.kv[pos.slot] + (lane >> 3) * kHalfBytes + (r0 + __ffs(dead) - 1) * 128 + (lane & 7) * 16) =
+                      make_uint4(0u, 0u, 0u, 0u);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+          }
+          const uint64_t vd = v_desc + static_cast<uint64_t>((pos.slot * kTileBytes) >> 4);
+          for (int i = 0; i < tiles; ++i) {
+            const int t = p.two_tiles ? i : g & 1;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              mbar_wait(&sm.p_half[t][h], (parity >> t) & 1u, sm);
+              tc_fence_after();
+              if (leader) {
+#pragma unroll
+                for (int kk = 4 * h; kk < 4 * h + 4; ++kk)
+                  mma_ts(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, vd + static_cast<uint64_t>((kk * 2048) >> 4), idesc,
+                         (!(visit.x & kOFirst) || kk > 0) ? 1u : 0u);
+              }
+              __syncwarp();
+            }
+            parity ^= 1u << t;
+            if (leader) mma_commit(&sm.pv_done[t]);
+            __syncwarp();
+          }
+          if (leader) mma_commit(&sm.empty[pos.slot]);
+          __syncwarp();
+        }
       }
     }
   } else {
@@ -340,59 +349,36 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
     const uint32_t t_s = tmem + lane_base + t * 128;        // my row of scores; the bf16 P overlays its first 64 columns
     const uint32_t t_o = tmem + lane_base + 256 + t * 128;  // my row of the output accumulator
     const uint64_t scale2 = pack2(p.scale_log2, p.scale_log2);
-
     float m_ref = -INFINITY, l_sum = 0.f;
-    auto exp_block = [&](const uint32_t (&s)[128], int e0, uint64_t negm2, uint32_t col, uint64_t (&acc2)[4]) {
-      uint32_t pk[16];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int e = e0 + 2 * i;
-        const uint64_t x = fma2(pack2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), scale2, negm2);
-        const uint64_t pp = ((kPolyMask >> (i & 7)) & 1u) ? exp2_pair_fma(x) : exp2_pair_sfu(x);
-        acc2[i & 3] = add2(acc2[i & 3], pp);
-        float p0, p1;
-        unpack2(pp, p0, p1);
-        pk[i] = pack_bf16x2(p0, p1);
-      }
-      JL_TMEM_ST16(t_s + col, pk, 0);
-    };
-    auto max_block = [&](const uint32_t (&s)[128], int e0, float (&m4)[4]) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) m4[i & 3] = max3(m4[i & 3], __uint_as_float(s[e0 + 2 * i]), __uint_as_float(s[e0 + 2 * i + 1]));
-    };
-    auto publish = [&](int half) {
-      tmem_wait_st();
-      tc_fence_before();
-      mbar_arrive(&sm.p_half[t][half]);
-    };
+
     // the segment's partial: O / l in fp32 (zero where the row saw nothing) and the LSE in the log2 domain
     auto leave_partial = [&](const Segment& s, int d, bool any) {
       const int64_t slot = static_cast<int64_t>(mb) * (p.workers + p.batch * p.kv_heads) + worker + s.b * p.kv_heads + s.kvh;
-      const int64_t prow = (slot * 2 + t) * p.rpt + r;
+      const int64_t prow = (slot * 2 + t) * p.rpt;
       const bool seen = any && d >= 0 && m_ref != -INFINITY;          // masked scores add ~1e-38 each to l_sum, never to m_ref
       const float inv = seen ? 1.f / l_sum : 0.f;
-#pragma unroll
+#pragma unroll 1
       for (int ch = 0; ch < 4; ++ch) {
         uint32_t o[32];
         if (any) {
           JL_TMEM_LD32(t_o + ch * 32, o, 0);
           JL_TMEM_WAIT_LD32(o, 0);
         }
-        if (row_used) {
+        if (row_used) {        // [4 columns][row]: 32 rows of a warp are 512 contiguous bytes (a row at a time cost 7000 clocks)
+          float4* dst = reinterpret_cast<float4*>(p.part_o + prow * kHeadDim) + r;
 #pragma unroll
           for (int i = 0; i < 8; ++i)
-            *reinterpret_cast<float4*>(p.part_o + prow * kHeadDim + ch * 32 + 4 * i) =
-                seen ? make_float4(__uint_as_float(o[4 * i]) * inv, __uint_as_float(o[4 * i + 1]) * inv, __uint_as_float(o[4 * i + 2]) * inv,
-                                   __uint_as_float(o[4 * i + 3]) * inv)
-                     : make_float4(0.f, 0.f, 0.f, 0.f);
+            dst[(ch * 8 + i) * p.rpt] = seen ? make_float4(__uint_as_float(o[4 * i]) * inv, __uint_as_float(o[4 * i + 1]) * inv,
+                                                           __uint_as_float(o[4 * i + 2]) * inv, __uint_as_float(o[4 * i + 3]) * inv)
+                                             : make_float4(0.f, 0.f, 0.f, 0.f);
         }
       }
-      if (row_used) p.part_lse[prow] = seen ? m_ref + log2f(l_sum) : -INFINITY;
+      if (row_used) p.part_lse[prow + r] = seen ? m_ref + log2f(l_sum) : -INFINITY;
     };
 
     Walk w(sm);
     Segment seg;
-    int n_done = 0, n_segs = 0, g = 0;
+    int n_done = 0, g = 0;
     while (w.next(p, seg)) {
       const int step = p.two_tiles ? 1 : 2, first = seg.v0 + (p.two_tiles ? 0 : (g ^ t) & 1);
       g += seg.v1 - seg.v0;
@@ -411,97 +397,136 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
         // every key of the tile is committed and of this class for nodes of any depth
         bool uniform = tp0 + kTileN <= len;
         if (p.two_classes) uniform &= far ? tp0 + kTileN <= len - p.w_0 : tp0 >= len + p.nodes - 1 - p.w_0;
-
+        // otherwise: committed keys of this class at columns [c_lo, c_hi), drafted keys by the bits of the node's mask and their depth
+        int c_lo = 0, c_hi = 0;
+        if (!uniform) {
+          const int64_t edge = static_cast<int64_t>(len) + d - p.w_0;          // pk < edge: far
+          const int64_t lo = (p.two_classes && !far ? edge : 0) - tp0, hi = (p.two_classes && far && edge < len ? edge : len) - tp0;
+          c_lo = lo < 0 ? 0 : (lo > 128 ? 128 : static_cast<int>(lo));
+          c_hi = d < 0 || hi < 0 ? 0 : (hi > 128 ? 128 : static_cast<int>(hi));
+        }
         mbar_wait(&sm.s_full[t], n_done & 1, sm);
         tc_fence_after();
-        const bool o_live = v != first;                // O holds something of this segment
-        uint32_t s[128];
+        auto raise_reference = [&](float mx) {
+          // lazy rescale: only when some row of the warp outgrew its reference maximum by 2^8
+          if (__any_sync(0xffffffffu, mx > m_ref + 8.f)) {
+            const float m_new = fmaxf(m_ref, mx);
+            const float alpha = m_new == -INFINITY ? 1.f : fast_exp2(m_ref - m_new);
+            l_sum *= alpha;
+            if (v > first) {                           // O holds something of this segment
+              // O is quiescent: these scores ready implies P V of the state's previous item retired, and the next one waits for our P
+#pragma unroll 1
+              for (int oc = 0; oc < 4; ++oc) {
+                uint32_t o[32];
+                JL_TMEM_LD32(t_o + oc * 32, o, 0);
+                JL_TMEM_WAIT_LD32(o, 0);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                JL_TMEM_ST32(t_o + oc * 32, o, 0);
+              }
+            }
+            m_ref = m_new;
+          }
+        };
+        auto exp_block = [&](const uint32_t* s, uint64_t negm2, uint32_t col, uint64_t (&acc2)[4]) {      // 32 scores -> 16 packed pairs
+          uint32_t pk[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const uint64_t x = fma2(pack2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), scale2, negm2);
+            const uint64_t pp = ((kPolyMask >> (i & 7)) & 1u) ? exp2_pair_fma(x) : exp2_pair_sfu(x);
+            acc2[i & 3] = add2(acc2[i & 3], pp);
+            float p0, p1;
+            unpack2(pp, p0, p1);
+            pk[i] = pack_bf16x2(p0, p1);
+          }
+          JL_TMEM_ST16(t_s + col, pk, 0);
+        };
+        auto publish = [&](int half) {
+          tmem_wait_st();
+          tc_fence_before();
+          mbar_arrive(&sm.p_half[t][half]);
+        };
         uint64_t acc2[4] = {0ull, 0ull, 0ull, 0ull};
-        float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        if (uniform) {
+        if (uniform && p.unrolled) {
+          // all 128 scores in registers: half the loads, and the halves of P published 1300 clocks earlier than by the loop below
+          uint32_t s[128];
+          float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
           JL_TMEM_LD32(t_s + 0, s, 0);
 #pragma unroll
           for (int ch = 0; ch < 4; ++ch) {
             JL_TMEM_WAIT_LD32(s, ch * 32);
             if (ch + 1 < 4) JL_TMEM_LD32(t_s + (ch + 1) * 32, s, (ch + 1) * 32);
-            max_block(s, ch * 32, m4);
-          }
-        } else {
-          // committed keys of this class: positions [lo, hi); drafted keys: bits of the node's mask, by their own depth
-          const int64_t edge = static_cast<int64_t>(len) + d - p.w_0;          // pk < edge: far
-          int64_t lo = p.two_classes && !far ? edge : 0, hi = p.two_classes && far && edge < len ? edge : len;
-          lo -= tp0;
-          hi -= tp0;
-          const int c_lo = lo < 0 ? 0 : (lo > 128 ? 128 : static_cast<int>(lo)), c_hi = hi < 0 ? 0 : (hi > 128 ? 128 : static_cast<int>(hi));
-          uint32_t keep[4];
-          const uint32_t* words = reinterpret_cast<const uint32_t*>(p.mask + nrow * p.words);
 #pragma unroll
-          for (int wd = 0; wd < 4; ++wd) {
-            const int a = max(c_lo - wd * 32, 0), z = min(c_hi - wd * 32, 32);
-            keep[wd] = z > a ? (0xffffffffu >> (32 - (z - a))) << a : 0u;
-            const int u0 = tp0 + wd * 32 - len;        // first node of this word's columns (negative: columns before the nodes)
+            for (int i = 0; i < 16; ++i) m4[i & 3] = max3(m4[i & 3], __uint_as_float(s[ch * 32 + 2 * i]), __uint_as_float(s[ch * 32 + 2 * i + 1]));
+          }
+          raise_reference(fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * p.scale_log2);
+          const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
+          const uint64_t negm2 = pack2(-m_use, -m_use);
+          exp_block(s, negm2, 0, acc2);
+          exp_block(s + 32, negm2, 16, acc2);
+          publish(0);
+          exp_block(s + 64, negm2, 32, acc2);
+          exp_block(s + 96, negm2, 48, acc2);
+          publish(1);
+          float a0, a1;
+          unpack2(add2(add2(acc2[0], acc2[1]), add2(acc2[2], acc2[3])), a0, a1);
+          l_sum += a0 + a1;
+          continue;
+        }
+        // Two passes over the row's scores, 32 columns at a time: maximum, then probabilities (written over scores that have
+        // been read).  The loop is kept rolled on purpose: the stream of keys evicts the kernel's code from L2, so its first
+        // pass runs at the rate of instruction fetches from HBM; unrolled over 128 columns that took 9 us of a 100 us launch.
+        float mx = -INFINITY;
+        uint64_t negm2 = 0ull;
+#pragma unroll 1
+        for (int step32 = 0; step32 < 8; ++step32) {
+          const int ch = step32 & 3;
+          uint32_t s[32];
+          JL_TMEM_LD32(t_s + ch * 32, s, 0);
+          JL_TMEM_WAIT_LD32(s, 0);
+          if (!uniform) {
+            const int a = max(c_lo - ch * 32, 0), z = min(c_hi - ch * 32, 32);
+            uint32_t keep = z > a ? (0xffffffffu >> (32 - (z - a))) << a : 0u;
+            const int u0 = tp0 + ch * 32 - len;        // first node of these columns (negative: columns before the nodes)
             if (d >= 0 && u0 > -32 && u0 < p.nodes && (!far || p.nodes_far)) {
+              const uint32_t* words = reinterpret_cast<const uint32_t*>(p.mask + nrow * p.words);
               const int i0 = u0 >> 5, sh = u0 & 31;
               const uint32_t w0 = i0 >= 0 ? __ldg(words + i0) : 0u, w1 = i0 + 1 < 2 * p.words ? __ldg(words + i0 + 1) : 0u;
               uint32_t bits = __funnelshift_r(w0, w1, sh);
               const int left = p.nodes - u0;
               if (left < 32) bits &= 0xffffffffu >> (32 - left);
               if (p.nodes_far) {
-                uint32_t todo = bits;
-                while (todo != 0u) {
+                for (uint32_t todo = bits; todo != 0u; todo &= todo - 1) {
                   const int j = __ffs(todo) - 1;
-                  todo &= todo - 1;
-                  const int du = p.depth[static_cast<int64_t>(seg.b) * p.nodes + u0 + j];
-                  if ((d - du > p.w_0) != far) bits &= ~(1u << j);
+                  if ((d - p.depth[static_cast<int64_t>(seg.b) * p.nodes + u0 + j] > p.w_0) != far) bits &= ~(1u << j);
                 }
               }
-              keep[wd] |= bits;
+              keep |= bits;
             }
-            if (d < 0) keep[wd] = 0u;
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (!((keep >> i) & 1u)) s[i] = 0xff800000u;        // -inf
           }
+          if (step32 < 4) {
+            float m2[2] = {mx, -INFINITY};
 #pragma unroll
-          for (int ch = 0; ch < 4; ++ch) JL_TMEM_LD32(t_s + ch * 32, s, ch * 32);
-#pragma unroll
-          for (int ch = 0; ch < 4; ++ch) JL_TMEM_WAIT_LD32(s, ch * 32);
-#pragma unroll
-          for (int i = 0; i < 128; ++i)
-            if (!((keep[i >> 5] >> (i & 31)) & 1u)) s[i] = 0xff800000u;        // -inf
-#pragma unroll
-          for (int ch = 0; ch < 4; ++ch) max_block(s, ch * 32, m4);
-        }
-        const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * p.scale_log2;
-        // lazy rescale: only when some row of the warp outgrew its reference maximum by 2^8
-        if (__any_sync(0xffffffffu, mx > m_ref + 8.f)) {
-          const float m_new = fmaxf(m_ref, mx);
-          const float alpha = m_new == -INFINITY ? 1.f : fast_exp2(m_ref - m_new);
-          l_sum *= alpha;
-          if (o_live) {
-            // O is quiescent: these scores ready implies P V of the state's previous item retired, and the next one waits for our P
-#pragma unroll
-            for (int ch = 0; ch < 4; ++ch) {
-              uint32_t o[32];
-              JL_TMEM_LD32(t_o + ch * 32, o, 0);
-              JL_TMEM_WAIT_LD32(o, 0);
-#pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-              JL_TMEM_ST32(t_o + ch * 32, o, 0);
-            }
+            for (int i = 0; i < 16; ++i) m2[i & 1] = max3(m2[i & 1], __uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]));
+            mx = fmaxf(m2[0], m2[1]);
+            if (step32 < 3) continue;
+            mx *= p.scale_log2;
+            raise_reference(mx);
+            const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
+            negm2 = pack2(-m_use, -m_use);
+            continue;
           }
-          m_ref = m_new;
+          exp_block(s, negm2, ch * 16, acc2);
+          if (ch & 1) publish(ch >> 1);                // keys 0..63 are published with their own barrier, then keys 64..127
         }
-        const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
-        const uint64_t negm2 = pack2(-m_use, -m_use);
-        exp_block(s, 0, negm2, 0, acc2);
-        exp_block(s, 32, negm2, 16, acc2);
-        publish(0);
-        exp_block(s, 64, negm2, 32, acc2);
-        exp_block(s, 96, negm2, 48, acc2);
-        publish(1);
         float a0, a1;
         unpack2(add2(add2(acc2[0], acc2[1]), add2(acc2[2], acc2[3])), a0, a1);
         l_sum += a0 + a1;
       }
-      mbar_wait(&sm.o_full[t], n_segs++ & 1, sm);
+      mbar_wait(&sm.pv_done[t], (n_done - 1) & 1, sm);
       tc_fence_after();
       leave_partial(seg, d, true);
       tc_fence_before();                               // the next segment's P V follows our next P
@@ -521,15 +546,12 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
   if (threadIdx.x == 0 && sm.failed) atomicExch(&g_tree_status, 1);
 }
 
-// One warp per (sample, node, head) joins the partials of the segments that cover the (sample, key head).
+// Joins the partials of the segments that cover a (sample, key head).  One thread per (row, 4 columns), rows fastest, so that
+// partials are read as they were written.  grid x: blocks of 128 threads over a tile's 32 * rpt such items, y: row tile of the
+// (sample, key head), z: (sample, key head).
 __global__ void __launch_bounds__(128) tree_combine_kernel(const TreeParams p) {
   const int lane = threadIdx.x & 31;
-  const int heads = p.kv_heads * p.rep;
-  const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  if (item >= static_cast<int64_t>(p.batch) * p.nodes * heads) return;
-  const int b = static_cast<int>(item / (static_cast<int64_t>(p.nodes) * heads));
-  const int rest = static_cast<int>(item - static_cast<int64_t>(b) * p.nodes * heads);
-  const int node = rest / heads, h = rest - node * heads, kvh = h / p.rep;
+  const int heads = p.kv_heads * p.rep, b = static_cast<int>(blockIdx.z) / p.kv_heads, kvh = static_cast<int>(blockIdx.z) % p.kv_heads;
   int64_t total = 0, before = 0;
   for (int i = lane; i < p.batch; i += 32) {
     const int n = visits_of(p, i).n;
@@ -547,49 +569,46 @@ __global__ void __launch_bounds__(128) tree_combine_kernel(const TreeParams p) {
   const int64_t parts = parts_of(p, total);
   // the part that holds visit x of the line: the largest i with i * total / parts <= x
   const int i0 = static_cast<int>(((lo + 1) * parts + total - 1) / total) - 1, i1 = static_cast<int>(((hi + 1) * parts + total - 1) / total) - 1;
-  const int tile = node / p.npt, mb = p.two_tiles ? tile >> 1 : 0;
-  const int r = (node - tile * p.npt) * p.rep + h - kvh * p.rep;
-  const int shift = p.two_tiles ? 0 : 1, t0 = p.two_tiles ? tile & 1 : 0;      // two states per slot, or one of the slot's tiles
+  const int item = blockIdx.x * 128 + threadIdx.x, c = item / p.rpt, r = item - c * p.rpt;
+  const int tile = blockIdx.y, mb = p.two_tiles ? tile >> 1 : 0;
+  const int nd = tile * p.npt + r / p.rep, h = kvh * p.rep + r % p.rep;
+  if (c >= 32 || nd >= p.nodes) return;
   const int64_t slot0 = static_cast<int64_t>(mb) * (p.workers + p.batch * p.kv_heads) + b * p.kv_heads + kvh + i0;
-  const int n_parts = (i1 - i0 + 1) << shift;
-  auto part_row = [&](int k) { return ((slot0 + (k >> shift)) * 2 + t0 + (shift ? k & 1 : 0)) * p.rpt + r; };
+  // two states per slot, or one of the slot's two tiles
+  const int n_parts = (i1 - i0 + 1) * (p.two_tiles ? 1 : 2), stride = p.two_tiles ? 2 : 1;
+  const int64_t first = slot0 * 2 + (p.two_tiles ? tile & 1 : 0);
+  const float* lse = p.part_lse + first * p.rpt + r;
+  const float4* o = reinterpret_cast<const float4*>(p.part_o) + first * p.rpt * 32 + item;
+  const int64_t lse_step = static_cast<int64_t>(stride) * p.rpt, o_step = lse_step * 32;
   wait_prerequisites();
-  // rounds of 32 partials: lane i holds the weight of partial k0 + i, 8 output rows are in flight at a time; the running
-  // maximum moves once a round
   float m = -INFINITY, sum = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int k0 = 0; k0 < n_parts; k0 += 32) {
-    const int n = min(32, n_parts - k0);
-    float l = lane < n ? p.part_lse[part_row(k0 + lane)] : -INFINITY, mr = l;
+  for (int k0 = 0; k0 < n_parts; k0 += 8) {                // 8 partials in flight; the running maximum moves once a round
+    float l[8];
     float4 x[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      x[j] = j < n ? *reinterpret_cast<const float4*>(p.part_o + part_row(k0 + j) * kHeadDim + 4 * lane) : make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int j = 0; j < 8; ++j) {
+      const bool in = k0 + j < n_parts;
+      l[j] = in ? lse[(k0 + j) * lse_step] : -INFINITY;
+      x[j] = in ? o[(k0 + j) * o_step] : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    float mn = m;
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) mr = fmaxf(mr, __shfl_xor_sync(0xffffffffu, mr, off));
-    const float mn = fmaxf(m, mr), ref = mn == -INFINITY ? 0.f : mn;
-    const float f = exp2f(m - ref), wgt = exp2f(l - ref);
+    for (int j = 0; j < 8; ++j) mn = fmaxf(mn, l[j]);
+    const float ref = mn == -INFINITY ? 0.f : mn, f = fast_exp2(m - ref);
     m = mn;
     sum *= f; acc.x *= f; acc.y *= f; acc.z *= f; acc.w *= f;
-    for (int j0 = 0; j0 < n; j0 += 8) {
-      float4 nx[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        nx[j] = j0 + 8 + j < n ? *reinterpret_cast<const float4*>(p.part_o + part_row(k0 + j0 + 8 + j) * kHeadDim + 4 * lane)
-                               : make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float w = __shfl_sync(0xffffffffu, wgt, (j0 + j) & 31);          // 0 past the last partial
-        sum += w;
-        acc.x = fmaf(w, x[j].x, acc.x); acc.y = fmaf(w, x[j].y, acc.y); acc.z = fmaf(w, x[j].z, acc.z); acc.w = fmaf(w, x[j].w, acc.w);
-        x[j] = nx[j];
-      }
+    for (int j = 0; j < 8; ++j) {
+      const float w = fast_exp2(l[j] - ref);
+      sum += w;
+      acc.x = fmaf(w, x[j].x, acc.x); acc.y = fmaf(w, x[j].y, acc.y); acc.z = fmaf(w, x[j].z, acc.z); acc.w = fmaf(w, x[j].w, acc.w);
     }
   }
   const float inv = sum > 0.f ? 1.f / sum : 0.f;
-  *reinterpret_cast<uint2*>(p.out + b * p.os_b + node * p.os_s + h * p.os_h + 4 * lane) =
+  *reinterpret_cast<uint2*>(p.out + b * p.os_b + nd * p.os_s + h * p.os_h + 4 * c) =
       make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
-  if (p.lse != nullptr && lane == 0) p.lse[(static_cast<int64_t>(b) * heads + h) * p.nodes + node] = sum > 0.f ? (m + log2f(sum)) * kLn2 : -INFINITY;
+  if (p.lse != nullptr && c == 0) p.lse[(static_cast<int64_t>(b) * heads + h) * p.nodes + nd] = sum > 0.f ? (m + log2f(sum)) * kLn2 : -INFINITY;
 }
 
 struct Layout { int npt, rpt, two_tiles, mbs, workers; size_t lse, total; };
@@ -643,6 +662,8 @@ int launch_tree_attention(const jl_tree_attention_args* a, cudaStream_t stream) 
   p.two_classes = a->q_group != nullptr;
   p.w_0 = a->w_0 < (int64_t(1) << 32) ? a->w_0 : (int64_t(1) << 32);           // no cache reaches further
   p.nodes_far = p.two_classes && p.w_0 < a->nodes - 1;
+  // Two row tiles keep the softmax threads busy, and the unrolled form saves 1300 clocks a visit; its instructions, cold, cost 8 us.
+  p.unrolled = l.two_tiles && static_cast<int64_t>(a->batch) * a->kv_heads * (a->rows / kTileN) >= 16ll * l.workers;
   p.scale_log2 = a->softmax_scale * kLog2e;
   p.lens = a->lens; p.depth = a->depth; p.mask = a->mask;
   p.part_o = static_cast<float*>(a->workspace);
@@ -669,12 +690,13 @@ int launch_tree_attention(const jl_tree_attention_args* a, cudaStream_t stream) 
       return check_launch("jl_tree_attention (shared memory opt-in)");
     attr_set[dev] = true;
   }
-  const int64_t items = static_cast<int64_t>(a->batch) * a->nodes * a->heads;
-  if ((items + 3) / 4 > 0x7fffffff) return fail(JL_ERR_UNSUPPORTED, "jl_tree_attention: too many rows for one launch");
+  const int row_tiles = (a->nodes + l.npt - 1) / l.npt;
+  if (static_cast<int64_t>(a->batch) * a->kv_heads > 65535)
+    return fail(JL_ERR_UNSUPPORTED, "jl_tree_attention: batch * kv_heads must be at most 65535");
   tree_attention_kernel<<<p.mbs * p.workers, kThreads, kSmemBytes, stream>>>(maps, p);
   rc = check_launch("jl_tree_attention");
   if (rc != JL_OK) return rc;
-  if (launch_dependent(tree_combine_kernel, dim3(static_cast<unsigned>((items + 3) / 4)), dim3(128), 0, stream, p) != cudaSuccess)
+  if (launch_dependent(tree_combine_kernel, dim3((32 * l.rpt + 127) / 128, row_tiles, a->batch * a->kv_heads), dim3(128), 0, stream, p) != cudaSuccess)
     return check_launch("jl_tree_attention (combine)");
   return JL_OK;
 }
