@@ -11,6 +11,7 @@
 // The score and dz products read hidden and weight along their rows (K-major); dh reads weight and dW reads dz and
 // hidden across them (MN-major), so nothing is transposed in memory.
 #include <cmath>
+#include <type_traits>
 
 #include "tc_common.cuh"
 #include "../../include/jetlong_b200_head.h"
@@ -28,9 +29,13 @@ constexpr int kMaxBN = 256;
 constexpr int kABytes = 128 * kBK * 2;       // a CTA's 128 rows of A
 constexpr int kAccCols = 256;                // tensor-memory columns of one accumulator; two of them alternate
 constexpr int kGemmThreads = 256;
-constexpr int kStageBytes = 196608;          // operand ring
-constexpr int kStagingBytes = 2 * 4 * 4096;  // per epilogue warp two buffers of 32 rows x 128 bytes
+constexpr int kRingBytes = 196608;           // operand ring
 constexpr int kMaxStages = 6;
+template <int kPair>
+struct Ring {                                // a stage: 128 rows of A and this CTA's rows of B, 64 deep
+  static constexpr int kStageBytes = kABytes + kMaxBN / kPair * kBK * 2, kStages = kRingBytes / kStageBytes;
+};
+constexpr int kStagingBytes = 2 * 4 * 4096;  // per epilogue warp two buffers of 32 rows x 128 bytes
 constexpr int kSms = 148;
 
 enum { kEpiScores = 0, kEpiDz = 1, kEpiF32 = 2, kEpiBf16 = 3 };
@@ -50,7 +55,7 @@ struct GemmParams {
   int64_t M, N;               // result extents (rows of A, rows of B)
   int m_tiles, n_tiles, splits, k_blocks, kb_per_split, bn;
   int group_m;                // > 0: m fastest inside groups of this many m tiles; 0: n fastest
-  int stages;
+  int behind, alone_rounds;   // see TileWalk
   // scores
   float2* part;               // [row][n tile] (maximum, sum of exponentials relative to it)
   int* part_arg;              // [row][n tile] or NULL
@@ -69,7 +74,7 @@ struct GemmParams {
 struct alignas(64) GemmMaps { CUtensorMap a, b, out; };
 
 struct GemmSmem {
-  alignas(1024) uint8_t ring[kStageBytes];
+  alignas(1024) uint8_t ring[kRingBytes];
   alignas(1024) uint8_t staging[kStagingBytes];
   uint64_t full[kMaxStages], empty[kMaxStages], acc_full[2], acc_free[2];
   uint32_t tmem_base;
@@ -84,6 +89,16 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, u
 __device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, uint32_t leader_bar, int x, int y) {
   asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
                ::"r"(smem_u32(dst)), "l"(map), "r"(leader_bar), "r"(x), "r"(y) : "memory");
+}
+// 64 columns of a matrix that lies in blocks of 64 columns: rows from y on of block z
+template <int kPair>
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, uint32_t bar, int y, int z) {
+  if (kPair == 2)
+    asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+                 ::"r"(smem_u32(dst)), "l"(map), "r"(bar), "r"(0), "r"(y), "r"(z) : "memory");
+  else
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+                 ::"r"(smem_u32(dst)), "l"(map), "r"(bar), "r"(0), "r"(y), "r"(z) : "memory");
 }
 __device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, const void* src, int x, int y, int z, bool reduce) {
   if (reduce)
@@ -121,20 +136,265 @@ __device__ __forceinline__ TileCoord tile_coord(const GemmParams& p, int t) {
   return c;
 }
 
-// C tile (128 * kPair rows x bn columns) = A B^T, fp32 accumulation in tensor memory.  kPair = 2: a cluster of two CTAs works
-// on one tile with cta_group::2 MMAs, each CTA loading its own 128 rows of A and half of the rows of B, so every byte of B
-// in shared memory serves 256 rows.  Two accumulators alternate, so the epilogue of a tile runs under the next one's MMAs.
+// Persistent walk of a worker over the tiles of one product.  The first `behind` workers of a launch carry one tile more of the
+// product before this one: the others do `alone_rounds` rounds without them, so that all end together.
+struct TileWalk {
+  int worker, workers, behind, alone, rounds;
+  int n, round;
+  __device__ __forceinline__ TileWalk(const GemmParams& p, int w, int ws)
+      : worker(w), workers(ws), behind(p.behind), alone(p.alone_rounds), n(p.m_tiles * p.n_tiles * p.splits), round(w < p.behind ? p.alone_rounds : 0) {}
+  __device__ __forceinline__ bool next(int& tile) {
+    tile = round < alone ? round * (workers - behind) + worker - behind : alone * (workers - behind) + (round - alone) * workers + worker;
+    ++round;
+    return tile < n;
+  }
+};
+
+// The ring and the accumulators go on from one product of a launch to the next.
+struct PipeState { int g, i; };       // stages used, tiles done
+
+// Operand kinds of a product C = A B^T: which of A and B are read across their rows (MN-major), and what becomes of C.
+template <int kPair_, bool kAMn_, bool kBMn_, int kEpi_>
+struct Product {
+  static constexpr int kPair = kPair_, kEpi = kEpi_;
+  static constexpr bool kAMn = kAMn_, kBMn = kBMn_;
+  static constexpr bool kABlocked = kEpi_ == kEpiF32 || kEpi_ == kEpiBf16;     // A is dz
+};
+
+template <class P>
+__device__ __forceinline__ void produce(const GemmMaps& maps, const GemmParams& p, GemmSmem& sm, int rank, int worker, int workers, PipeState& st) {
+  constexpr int kPair = P::kPair, kStages = Ring<kPair>::kStages, kStageBytes = Ring<kPair>::kStageBytes;
+  const int b_rows = p.bn / kPair, stage_bytes = kABytes + b_rows * kBK * 2;
+  TileWalk walk(p, worker, workers);
+  for (int t; walk.next(t);) {
+    const TileCoord c = tile_coord(p, t);
+    const int m0 = (c.m * kPair + rank) * 128, n0 = c.n * p.bn + rank * b_rows;
+    const int kb0 = c.split * p.kb_per_split, kb1 = min(kb0 + p.kb_per_split, p.k_blocks);
+    for (int kb = kb0; kb < kb1; ++kb, ++st.g) {
+      const int s = st.g % kStages;
+      mbar_wait(&sm.empty[s], ((st.g / kStages) & 1) ^ 1, sm);
+      if (*reinterpret_cast<volatile int*>(&sm.failed)) return;
+      if (rank == 0) mbar_expect_tx(&sm.full[s], kPair * stage_bytes);
+      const uint32_t bar = kPair == 2 ? pair::leader_addr(&sm.full[s]) : smem_u32(&sm.full[s]);
+      uint8_t* sa = sm.ring + s * kStageBytes;
+      uint8_t* sb = sa + kABytes;
+      auto load = [&](void* dst, const CUtensorMap* map, int x, int y) {
+        if (kPair == 2) tma_load_2d_pair(dst, map, bar, x, y);
+        else tma_load_2d(dst, map, bar, x, y);
+      };
+      auto load_a = [&](void* dst, int x, int y) {           // dz lies in blocks of 64 columns: (column in the block, row, block)
+        if (P::kABlocked) tma_load_3d<kPair>(dst, &maps.a, bar, y, x >> 6);
+        else load(dst, &maps.a, x, y);
+      };
+      if (P::kAMn) {
+        load_a(sa, m0, kb * kBK);
+        load_a(sa + 8192, m0 + 64, kb * kBK);
+      } else {
+        load_a(sa, kb * kBK, m0);
+      }
+      if (P::kBMn) {
+        for (int ch = 0; ch < b_rows / 64; ++ch) load(sb + ch * 8192, &maps.b, n0 + ch * 64, kb * kBK);
+      } else {
+        load(sb, &maps.b, kb * kBK, n0);
+      }
+    }
+  }
+}
+
+template <class P>
+__device__ __forceinline__ void issue(const GemmParams& p, GemmSmem& sm, uint32_t tmem, uint32_t leader, int worker, int workers, PipeState& st) {
+  constexpr int kPair = P::kPair, kStages = Ring<kPair>::kStages, kStageBytes = Ring<kPair>::kStageBytes;
+  const uint32_t idesc = instr_desc(128 * kPair, p.bn, P::kBMn) | (P::kAMn ? 1u << 15 : 0u);
+  const uint32_t ring = smem_u32(sm.ring);
+  TileWalk walk(p, worker, workers);
+  for (int t; walk.next(t); ++st.i) {
+    const TileCoord c = tile_coord(p, t);
+    const int kb0 = c.split * p.kb_per_split, kb1 = min(kb0 + p.kb_per_split, p.k_blocks);
+    mbar_wait(&sm.acc_free[st.i & 1], ((st.i >> 1) & 1) ^ 1, sm);
+    tc_fence_after();
+    const uint32_t acc = tmem + (st.i & 1) * kAccCols;
+    for (int kb = kb0; kb < kb1; ++kb, ++st.g) {
+      const int s = st.g % kStages;
+      mbar_wait(&sm.full[s], (st.g / kStages) & 1, sm);
+      if (*reinterpret_cast<volatile int*>(&sm.failed)) return;
+      tc_fence_after();
+      const uint32_t sa = ring + s * kStageBytes, sb = sa + kABytes;
+      // K-major rows are 128 bytes in 8-row swizzle atoms; MN-major: 64 elements x 8 k-rows per atom, 8 KB per 64 elements
+      const uint64_t ad = P::kAMn ? smem_desc(sa, 8192, 1024) : smem_desc(sa, 16, 1024);
+      const uint64_t bd = P::kBMn ? smem_desc(sb, 8192, 1024) : smem_desc(sb, 16, 1024);
+      if (leader) {
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+          const uint64_t ao = static_cast<uint64_t>((P::kAMn ? kk * 2048 : kk * 32) >> 4);
+          const uint64_t bo = static_cast<uint64_t>((P::kBMn ? kk * 2048 : kk * 32) >> 4);
+          if (kPair == 2) pair::mma2_ss(acc, ad + ao, bd + bo, idesc, kb > kb0 || kk > 0);
+          else mma_ss(acc, ad + ao, bd + bo, idesc, kb > kb0 || kk > 0);
+        }
+        if (kPair == 2) pair::commit_both(&sm.empty[s]);
+        else mma_commit(&sm.empty[s]);
+      }
+      __syncwarp();
+    }
+    if (leader) {
+      if (kPair == 2) pair::commit_both(&sm.acc_full[st.i & 1]);
+      else mma_commit(&sm.acc_full[st.i & 1]);
+    }
+    __syncwarp();
+  }
+}
+
+template <class P>
+__device__ __forceinline__ void finish(const GemmMaps& maps, const GemmParams& p, GemmSmem& sm, uint32_t tmem, int quad, int lane, int rank, int worker,
+                                       int workers, PipeState& st, int& buf) {
+  constexpr int kPair = P::kPair, kEpi = P::kEpi;
+  const uint32_t lane_base = static_cast<uint32_t>(quad * 32) << 16;
+  uint8_t* const stage = sm.staging + quad * 8192;
+  const uint32_t free_bar[2] = {kPair == 2 ? pair::leader_addr(&sm.acc_free[0]) : smem_u32(&sm.acc_free[0]),
+                                kPair == 2 ? pair::leader_addr(&sm.acc_free[1]) : smem_u32(&sm.acc_free[1])};
+  const float scale = kEpi == kEpiBf16 ? p.scale.get() : 1.f;
+  // 32 rows x 128 bytes of results: 16-byte chunk `ch` of this thread's row
+  auto chunk_ptr = [&](int ch) { return reinterpret_cast<uint4*>(stage + buf * 4096 + lane * 128 + ((ch ^ (lane & 7)) << 4)); };
+  auto begin_box = [&]() {
+    if (lane == 0) bulk_wait_read<1>();          // the box before the last one has left this buffer
+    __syncwarp();
+  };
+  auto end_box = [&](int x, int64_t row_w, int z, bool reduce) {
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+    if (lane == 0) {
+      if (row_w < p.M && x < p.N) {
+        if (kEpi == kEpiDz) tma_store_3d(&maps.out, stage + buf * 4096, 0, static_cast<int>(row_w), x >> 6, false);      // blocks of 64 columns
+        else tma_store_3d(&maps.out, stage + buf * 4096, x, static_cast<int>(row_w), z, reduce);
+      }
+      bulk_commit();
+    }
+    buf ^= 1;
+  };
+  TileWalk walk(p, worker, workers);
+  for (int t; walk.next(t); ++st.i) {
+    const TileCoord c = tile_coord(p, t);
+    const int64_t row_w = (static_cast<int64_t>(c.m) * kPair + rank) * 128 + quad * 32, row = row_w + lane;
+    const int n0 = c.n * p.bn;
+    const uint32_t acc = tmem + (st.i & 1) * kAccCols + lane_base;
+    mbar_wait(&sm.acc_full[st.i & 1], (st.i >> 1) & 1, sm);
+    tc_fence_after();
+
+    if constexpr (kEpi == kEpiScores) {
+      const int valid = static_cast<int>(min(static_cast<int64_t>(p.bn), p.N - n0));
+      float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      for (int c0 = 0; c0 < valid; c0 += 16) {
+        uint32_t z[16];
+        JL_TMEM_LD16(acc + c0, z);
+        JL_TMEM_WAIT_LD16(z, 0);
+        if (c0 + 16 <= valid) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) m4[j & 3] = max3(m4[j & 3], __uint_as_float(z[2 * j]), __uint_as_float(z[2 * j + 1]));
+        } else {
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            if (c0 + j < valid) m4[j & 3] = fmaxf(m4[j & 3], __uint_as_float(z[j]));
+        }
+      }
+      const float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+      const float m_use = m == -INFINITY ? 0.f : m;
+      const int64_t y64 = p.labels != nullptr && row < p.M ? p.labels[row] - p.v0 - n0 : -1;
+      const int y = y64 >= 0 && y64 < valid ? static_cast<int>(y64) : -1;
+      float s4[4] = {0.f, 0.f, 0.f, 0.f}, z_y = 0.f;
+      int arg = 0x7fffffff;
+      for (int c0 = 0; c0 < valid; c0 += 16) {
+        uint32_t z[16];
+        JL_TMEM_LD16(acc + c0, z);
+        JL_TMEM_WAIT_LD16(z, 0);
+        if (__any_sync(0xffffffffu, y >= c0 && y < c0 + 16)) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) z_y = y == c0 + j ? __uint_as_float(z[j]) : z_y;
+        }
+        if (p.part_arg != nullptr) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            if (__uint_as_float(z[j]) == m && c0 + j < valid) arg = min(arg, c0 + j);
+        }
+        // (z - m) first: exact for the logits that count, whatever their size
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const float e = fast_exp2((__uint_as_float(z[j]) - m_use) * kLog2e);
+          if (c0 + j < valid) s4[j & 3] += e;
+        }
+      }
+      tc_fence_before();
+      if (row < p.M) {
+        p.part[row * p.n_tiles + c.n] = make_float2(m, (s4[0] + s4[1]) + (s4[2] + s4[3]));
+        if (p.part_arg != nullptr) p.part_arg[row * p.n_tiles + c.n] = arg == 0x7fffffff ? n0 : n0 + arg;
+        if (y >= 0) p.picked[row] = z_y;
+      }
+    } else {
+      float lse = 0.f, factor = 0.f;
+      int y = -1;
+      if constexpr (kEpi == kEpiDz) {
+        if (row < p.M) {
+          const int64_t label = p.labels[row];
+          lse = p.lse[row];
+          if (label != p.ignore) {
+            factor = p.row_grad != nullptr ? p.row_grad[row] : 1.f;
+            if (label < 0 || label >= p.vocab) factor = __int_as_float(0x7fc00000);
+            const int64_t rel = label - p.v0 - n0;
+            y = rel >= 0 && rel < p.bn ? static_cast<int>(rel) : -1;
+          }
+        }
+      }
+      const bool used = kEpi != kEpiDz || factor != 0.f;
+      constexpr int kCols = kEpi == kEpiF32 ? 32 : 64;             // columns of one 128-byte box; bn is a multiple of 64 here
+      for (int c0 = 0; c0 < p.bn; c0 += kCols) {
+        begin_box();
+        for (int half = 0; half < kCols / 32; ++half) {
+          const int cc = c0 + half * 32;
+          uint32_t z[32];
+          JL_TMEM_LD32(acc + cc, z, 0);
+          JL_TMEM_WAIT_LD32(z, 0);
+          if constexpr (kEpi == kEpiDz) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              const float pr = fast_exp2((__uint_as_float(z[j]) - lse) * kLog2e) - (y == cc + j ? 1.f : 0.f);
+              z[j] = used ? __float_as_uint(pr * factor) : 0u;      // a row that does not count is zero whatever it holds
+            }
+            if (n0 + cc + 32 > p.N) {                              // the piece's last block of 64 columns is stored whole
+#pragma unroll
+              for (int j = 0; j < 32; ++j) z[j] = n0 + cc + j < p.N ? z[j] : 0u;
+            }
+          }
+          if constexpr (kEpi == kEpiF32) {
+#pragma unroll
+            for (int v = 0; v < 8; ++v) *chunk_ptr(v) = make_uint4(z[4 * v], z[4 * v + 1], z[4 * v + 2], z[4 * v + 3]);
+          } else {
+            auto pk = [&](int j) { return pack_bf16x2(__uint_as_float(z[j]) * scale, __uint_as_float(z[j + 1]) * scale); };
+#pragma unroll
+            for (int v = 0; v < 4; ++v) *chunk_ptr(half * 4 + v) = make_uint4(pk(8 * v), pk(8 * v + 2), pk(8 * v + 4), pk(8 * v + 6));
+          }
+        }
+        end_box(n0 + c0, row_w, kEpi == kEpiF32 ? c.split : 0, kEpi == kEpiF32 && p.reduce);
+      }
+      tc_fence_before();
+    }
+    __syncwarp();
+    if (lane == 0) asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(free_bar[st.i & 1]) : "memory");
+  }
+}
+
+// C tiles (128 * kPair rows x bn columns), fp32 accumulation in tensor memory, of one product or of two that need nothing of each
+// other, the second filling the SMs that the first leaves.  kPair = 2: a cluster of two CTAs works on one tile with cta_group::2
+// MMAs, each CTA loading its own 128 rows of A and half of the rows of B, so every byte of B in shared memory serves 256 rows.
+// Two accumulators alternate, so the epilogue of a tile runs under the next one's MMAs.
 //   warp 0 TMA producer, warp 1 MMA issuer (rank 0), warp 2 tensor memory, warps 4-7 epilogue (one thread per row)
-template <int kPair, bool kAMn, bool kBMn, int kEpi>
-__global__ void __launch_bounds__(kGemmThreads, 1) head_gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmParams p) {
+template <class P0, class P1>
+__global__ void __launch_bounds__(kGemmThreads, 1) head_gemm_kernel(const __grid_constant__ GemmMaps maps0, const GemmParams p0,
+                                                                    const __grid_constant__ GemmMaps maps1, const GemmParams p1) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   GemmSmem& sm = *reinterpret_cast<GemmSmem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  constexpr int kPair = P0::kPair;
+  constexpr bool kTwo = !std::is_same<P1, void>::value;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = kPair == 2 ? static_cast<int>(blockIdx.x & 1) : 0;
   const int worker = static_cast<int>(blockIdx.x) / kPair, workers = static_cast<int>(gridDim.x) / kPair;
-  const int n_total = p.m_tiles * p.n_tiles * p.splits;
-  const int b_rows = p.bn / kPair;                         // rows of B this CTA loads
-  const int stage_bytes = kABytes + b_rows * kBK * 2;
 
   if (threadIdx.x == 0) {
     sm.failed = *reinterpret_cast<volatile int*>(&g_head_status) != 0 ? 1 : 0;
@@ -157,216 +417,27 @@ __global__ void __launch_bounds__(kGemmThreads, 1) head_gemm_kernel(const __grid
   tc_fence_after();
   launch_dependents();
   const uint32_t tmem = sm.tmem_base;
-  volatile int* const failed = &sm.failed;       // a wait gave up: nothing more is issued, every later wait returns at once
 
+  PipeState st{0, 0};
   if (warp == 0) {
-    // ===================================== TMA producer =====================================
     if (lane == 0) {
-      int g = 0;
-      for (int t = worker; t < n_total; t += workers) {
-        const TileCoord c = tile_coord(p, t);
-        const int m0 = (c.m * kPair + rank) * 128, n0 = c.n * p.bn + rank * b_rows;
-        const int kb0 = c.split * p.kb_per_split, kb1 = min(kb0 + p.kb_per_split, p.k_blocks);
-        for (int kb = kb0; kb < kb1; ++kb, ++g) {
-          const int s = g % p.stages;
-          mbar_wait(&sm.empty[s], ((g / p.stages) & 1) ^ 1, sm);
-          if (*failed) { t = n_total; break; }
-          if (rank == 0) mbar_expect_tx(&sm.full[s], kPair * stage_bytes);
-          const uint32_t bar = kPair == 2 ? pair::leader_addr(&sm.full[s]) : smem_u32(&sm.full[s]);
-          uint8_t* sa = sm.ring + s * stage_bytes;
-          uint8_t* sb = sa + kABytes;
-          auto load = [&](void* dst, const CUtensorMap* map, int x, int y) {
-            if (kPair == 2) tma_load_2d_pair(dst, map, bar, x, y);
-            else tma_load_2d(dst, map, bar, x, y);
-          };
-          if (kAMn) {
-            load(sa, &maps.a, m0, kb * kBK);
-            load(sa + 8192, &maps.a, m0 + 64, kb * kBK);
-          } else {
-            load(sa, &maps.a, kb * kBK, m0);
-          }
-          if (kBMn) {
-            for (int ch = 0; ch < b_rows / 64; ++ch) load(sb + ch * 8192, &maps.b, n0 + ch * 64, kb * kBK);
-          } else {
-            load(sb, &maps.b, kb * kBK, n0);
-          }
-        }
-      }
+      produce<P0>(maps0, p0, sm, rank, worker, workers, st);
+      if constexpr (kTwo) produce<P1>(maps1, p1, sm, rank, worker, workers, st);
     }
   } else if (warp == 1 && rank == 0) {
-    // ====================================== MMA issuer ======================================
     uint32_t leader;
     asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(leader));
-    const uint32_t idesc = instr_desc(128 * kPair, p.bn, kBMn) | (kAMn ? 1u << 15 : 0u);
-    const uint32_t ring = smem_u32(sm.ring);
-    int g = 0, i = 0;
-    for (int t = worker; t < n_total; t += workers, ++i) {
-      const TileCoord c = tile_coord(p, t);
-      const int kb0 = c.split * p.kb_per_split, kb1 = min(kb0 + p.kb_per_split, p.k_blocks);
-      mbar_wait(&sm.acc_free[i & 1], ((i >> 1) & 1) ^ 1, sm);
-      tc_fence_after();
-      const uint32_t acc = tmem + (i & 1) * kAccCols;
-      for (int kb = kb0; kb < kb1; ++kb, ++g) {
-        const int s = g % p.stages;
-        mbar_wait(&sm.full[s], (g / p.stages) & 1, sm);
-        if (*failed) break;
-        tc_fence_after();
-        const uint32_t sa = ring + s * stage_bytes, sb = sa + kABytes;
-        // K-major rows are 128 bytes in 8-row swizzle atoms; MN-major: 64 elements x 8 k-rows per atom, 8 KB per 64 elements
-        const uint64_t ad = kAMn ? smem_desc(sa, 8192, 1024) : smem_desc(sa, 16, 1024);
-        const uint64_t bd = kBMn ? smem_desc(sb, 8192, 1024) : smem_desc(sb, 16, 1024);
-        if (leader) {
-#pragma unroll
-          for (int kk = 0; kk < 4; ++kk) {
-            const uint64_t ao = static_cast<uint64_t>((kAMn ? kk * 2048 : kk * 32) >> 4);
-            const uint64_t bo = static_cast<uint64_t>((kBMn ? kk * 2048 : kk * 32) >> 4);
-            if (kPair == 2) pair::mma2_ss(acc, ad + ao, bd + bo, idesc, kb > kb0 || kk > 0);
-            else mma_ss(acc, ad + ao, bd + bo, idesc, kb > kb0 || kk > 0);
-          }
-          if (kPair == 2) pair::commit_both(&sm.empty[s]);
-          else mma_commit(&sm.empty[s]);
-        }
-        __syncwarp();
-      }
-      if (leader) {
-        if (kPair == 2) pair::commit_both(&sm.acc_full[i & 1]);
-        else mma_commit(&sm.acc_full[i & 1]);
-      }
-      __syncwarp();
-    }
+    issue<P0>(p0, sm, tmem, leader, worker, workers, st);
+    if constexpr (kTwo) issue<P1>(p1, sm, tmem, leader, worker, workers, st);
   } else if (warp >= 4) {
-    // ======================================= epilogue =======================================
-    const int quad = warp & 3;
-    const uint32_t lane_base = static_cast<uint32_t>(quad * 32) << 16;
-    uint8_t* const stage = sm.staging + quad * 8192;
-    const uint32_t free_bar[2] = {kPair == 2 ? pair::leader_addr(&sm.acc_free[0]) : smem_u32(&sm.acc_free[0]),
-                                  kPair == 2 ? pair::leader_addr(&sm.acc_free[1]) : smem_u32(&sm.acc_free[1])};
-    const float scale = kEpi == kEpiBf16 ? p.scale.get() : 1.f;
     int buf = 0;
-    // 32 rows x 128 bytes of results: 16-byte chunk `ch` of this thread's row
-    auto chunk_ptr = [&](int ch) { return reinterpret_cast<uint4*>(stage + buf * 4096 + lane * 128 + ((ch ^ (lane & 7)) << 4)); };
-    auto begin_box = [&]() {
-      if (lane == 0) bulk_wait_read<1>();          // the box before the last one has left this buffer
-      __syncwarp();
-    };
-    auto end_box = [&](int x, int64_t row_w, int z, bool reduce) {
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) {
-        if (row_w < p.M && x < p.N) tma_store_3d(&maps.out, stage + buf * 4096, x, static_cast<int>(row_w), z, reduce);
-        bulk_commit();
-      }
-      buf ^= 1;
-    };
-    int i = 0;
-    for (int t = worker; t < n_total; t += workers, ++i) {
-      const TileCoord c = tile_coord(p, t);
-      const int64_t row_w = (static_cast<int64_t>(c.m) * kPair + rank) * 128 + quad * 32, row = row_w + lane;
-      const int n0 = c.n * p.bn;
-      const uint32_t acc = tmem + (i & 1) * kAccCols + lane_base;
-      mbar_wait(&sm.acc_full[i & 1], (i >> 1) & 1, sm);
-      tc_fence_after();
-
-      if constexpr (kEpi == kEpiScores) {
-        const int valid = static_cast<int>(min(static_cast<int64_t>(p.bn), p.N - n0));
-        float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        for (int c0 = 0; c0 < valid; c0 += 16) {
-          uint32_t z[16];
-          JL_TMEM_LD16(acc + c0, z);
-          JL_TMEM_WAIT_LD16(z, 0);
-          if (c0 + 16 <= valid) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) m4[j & 3] = max3(m4[j & 3], __uint_as_float(z[2 * j]), __uint_as_float(z[2 * j + 1]));
-          } else {
-#pragma unroll
-            for (int j = 0; j < 16; ++j)
-              if (c0 + j < valid) m4[j & 3] = fmaxf(m4[j & 3], __uint_as_float(z[j]));
-          }
-        }
-        const float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-        const float m_use = m == -INFINITY ? 0.f : m;
-        const int64_t y64 = p.labels != nullptr && row < p.M ? p.labels[row] - p.v0 - n0 : -1;
-        const int y = y64 >= 0 && y64 < valid ? static_cast<int>(y64) : -1;
-        float s4[4] = {0.f, 0.f, 0.f, 0.f}, z_y = 0.f;
-        int arg = 0x7fffffff;
-        for (int c0 = 0; c0 < valid; c0 += 16) {
-          uint32_t z[16];
-          JL_TMEM_LD16(acc + c0, z);
-          JL_TMEM_WAIT_LD16(z, 0);
-          if (__any_sync(0xffffffffu, y >= c0 && y < c0 + 16)) {
-#pragma unroll
-            for (int j = 0; j < 16; ++j) z_y = y == c0 + j ? __uint_as_float(z[j]) : z_y;
-          }
-          if (p.part_arg != nullptr) {
-#pragma unroll
-            for (int j = 0; j < 16; ++j)
-              if (__uint_as_float(z[j]) == m && c0 + j < valid) arg = min(arg, c0 + j);
-          }
-          // (z - m) first: exact for the logits that count, whatever their size
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const float e = fast_exp2((__uint_as_float(z[j]) - m_use) * kLog2e);
-            if (c0 + j < valid) s4[j & 3] += e;
-          }
-        }
-        tc_fence_before();
-        if (row < p.M) {
-          p.part[row * p.n_tiles + c.n] = make_float2(m, (s4[0] + s4[1]) + (s4[2] + s4[3]));
-          if (p.part_arg != nullptr) p.part_arg[row * p.n_tiles + c.n] = arg == 0x7fffffff ? n0 : n0 + arg;
-          if (y >= 0) p.picked[row] = z_y;
-        }
-      } else {
-        float lse = 0.f, factor = 0.f;
-        int y = -1;
-        if constexpr (kEpi == kEpiDz) {
-          if (row < p.M) {
-            const int64_t label = p.labels[row];
-            lse = p.lse[row];
-            if (label != p.ignore) {
-              factor = p.row_grad != nullptr ? p.row_grad[row] : 1.f;
-              if (label < 0 || label >= p.vocab) factor = __int_as_float(0x7fc00000);
-              const int64_t rel = label - p.v0 - n0;
-              y = rel >= 0 && rel < p.bn ? static_cast<int>(rel) : -1;
-            }
-          }
-        }
-        const bool used = kEpi != kEpiDz || factor != 0.f;
-        constexpr int kCols = kEpi == kEpiF32 ? 32 : 64;             // columns of one 128-byte box; bn is a multiple of 64 here
-        for (int c0 = 0; c0 < p.bn; c0 += kCols) {
-          begin_box();
-          for (int half = 0; half < kCols / 32; ++half) {
-            const int cc = c0 + half * 32;
-            uint32_t z[32];
-            JL_TMEM_LD32(acc + cc, z, 0);
-            JL_TMEM_WAIT_LD32(z, 0);
-            if constexpr (kEpi == kEpiDz) {
-#pragma unroll
-              for (int j = 0; j < 32; ++j) {
-                const float pr = fast_exp2((__uint_as_float(z[j]) - lse) * kLog2e) - (y == cc + j ? 1.f : 0.f);
-                z[j] = used ? __float_as_uint(pr * factor) : 0u;      // a row that does not count is zero whatever it holds
-              }
-            }
-            if constexpr (kEpi == kEpiF32) {
-#pragma unroll
-              for (int v = 0; v < 8; ++v) *chunk_ptr(v) = make_uint4(z[4 * v], z[4 * v + 1], z[4 * v + 2], z[4 * v + 3]);
-            } else {
-              auto pk = [&](int j) { return pack_bf16x2(__uint_as_float(z[j]) * scale, __uint_as_float(z[j + 1]) * scale); };
-#pragma unroll
-              for (int v = 0; v < 4; ++v) *chunk_ptr(half * 4 + v) = make_uint4(pk(8 * v), pk(8 * v + 2), pk(8 * v + 4), pk(8 * v + 6));
-            }
-          }
-          end_box(n0 + c0, row_w, kEpi == kEpiF32 ? c.split : 0, kEpi == kEpiF32 && p.reduce);
-        }
-        tc_fence_before();
-      }
-      __syncwarp();
-      if (lane == 0) asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(free_bar[i & 1]) : "memory");
-    }
+    finish<P0>(maps0, p0, sm, tmem, warp & 3, lane, rank, worker, workers, st, buf);
+    if constexpr (kTwo) finish<P1>(maps1, p1, sm, tmem, warp & 3, lane, rank, worker, workers, st, buf);
     if (lane == 0) bulk_wait_all();
   }
 
   __syncthreads();
-  if (*failed) {                                 // copies and MMAs that were under way have long landed after 1 ms
+  if (*reinterpret_cast<volatile int*>(&sm.failed)) {      // a wait gave up: copies and MMAs under way have long landed after 1 ms
     const uint64_t t0 = globaltimer_ns();
     while (globaltimer_ns() - t0 < 1000 * 1000) {}
   }
@@ -492,12 +563,12 @@ int make_map2(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int6
   return JL_OK;
 }
 
-struct Matrix {               // row-major bf16
+struct Matrix {               // bf16, row-major with rows `ld` apart, or (ld 0) in blocks of 64 columns, each block row-major
   const void* p;
   int64_t rows, cols, ld;
 };
 
-// Result of the product: the output map's base (NULL: none), its row length and type
+// Result of the product: base (NULL: none), row length (0: blocks of 64 columns) and type
 struct Result {
   void* p;
   int64_t ld;
@@ -505,10 +576,10 @@ struct Result {
   int64_t planes;
 };
 
-// Shape of a launch over an M x N result: rows per tile follow from `pair`, the tile's width is the one whose rounds over
-// the GPU's workers cost least (a tile costs its width, plus some columns' worth of hand-over).
-struct Plan { int pair, bn, m_tiles, n_tiles; };
+// Tiles of a launch over an M x N result: rows per tile follow from `pair`, the width is the one whose rounds over the GPU's
+// workers cost least (a tile costs its width, plus some columns' worth of hand-over).
 // `step`: what the width has to be a multiple of (16 columns of each CTA's B; 64 where boxes of 64 columns are loaded or stored).
+struct Plan { int pair, bn, m_tiles, n_tiles; };
 Plan plan_tiles(int64_t M, int64_t N, int pair, int step) {
   Plan best{pair, 0, static_cast<int>(cdiv(M, 128 * pair)), 0};
   double cost = 1e30;
@@ -521,25 +592,56 @@ Plan plan_tiles(int64_t M, int64_t N, int pair, int step) {
   return best;
 }
 
-template <int kPair, bool kAMn, bool kBMn, int kEpi>
-int launch_gemm(const Matrix& A, const Matrix& B, const Result& out, GemmParams p, const Plan& plan, int64_t K, int splits, cudaStream_t stream) {
-  p.M = kAMn ? A.cols : A.rows;
-  p.N = kBMn ? B.cols : B.rows;
+// The dh product has few tiles and a long K: width and K splits together, least bytes of operands per worker.
+Plan plan_split(int64_t M, int64_t N, int pair, int64_t k_blocks, int& splits) {
+  Plan best{pair, 0, static_cast<int>(cdiv(M, 128 * pair)), 0};
+  double cost = 1e30;
+  const int workers = kSms / pair;
+  splits = 1;
+  for (int bn = kMaxBN; bn >= 64 * pair; bn -= 64 * pair) {
+    const int64_t tiles = best.m_tiles * cdiv(N, bn);
+    int64_t s = workers / tiles;
+    if (s > k_blocks / 8) s = k_blocks / 8;
+    if (s < 1) s = 1;
+    const int64_t depth = cdiv(k_blocks, s);
+    const double c = static_cast<double>(cdiv(tiles * s, workers)) * depth * (128 * pair + bn);
+    if (c < cost * 0.995) { cost = c; best.bn = bn; splits = static_cast<int>(cdiv(k_blocks, depth)); }
+  }
+  best.n_tiles = static_cast<int>(cdiv(N, best.bn));
+  return best;
+}
+
+struct Gemm { GemmMaps maps; GemmParams p; };
+
+template <class P>
+int prepare(Gemm& g, const Matrix& A, const Matrix& B, const Result& out, const Plan& plan, int64_t K, int splits) {
+  GemmParams& p = g.p;
+  p.M = P::kAMn ? A.cols : A.rows;
+  p.N = P::kBMn ? B.cols : B.rows;
   p.m_tiles = plan.m_tiles;
   p.n_tiles = plan.n_tiles;
   p.bn = plan.bn;
   p.k_blocks = static_cast<int>(cdiv(K, kBK));
   p.kb_per_split = static_cast<int>(cdiv(p.k_blocks, splits));
   p.splits = static_cast<int>(cdiv(p.k_blocks, p.kb_per_split));
-  const int stage = kABytes + plan.bn / kPair * kBK * 2;
-  p.stages = kStageBytes / stage < kMaxStages ? kStageBytes / stage : kMaxStages;
-  GemmMaps maps;
+  p.behind = p.alone_rounds = 0;
   int rc = bind_context();
-  if (rc == JL_OK) rc = make_map2(&maps.a, A.p, A.rows, A.cols, A.ld, kBK, kAMn ? kBK : 128, false, 1, false);
-  if (rc == JL_OK) rc = make_map2(&maps.b, B.p, B.rows, B.cols, B.ld, kBK, kBMn ? kBK : plan.bn / kPair, false, 1, false);
-  if (rc == JL_OK && out.p != nullptr) rc = make_map2(&maps.out, out.p, p.M, p.N, out.ld, out.f32 ? 32 : 64, 32, out.f32, out.planes, true);
-  if (rc != JL_OK) return rc;
-  auto kernel = head_gemm_kernel<kPair, kAMn, kBMn, kEpi>;
+  const int a_rows = P::kAMn ? kBK : 128;
+  if (rc == JL_OK) rc = A.ld == 0 ? make_map2(&g.maps.a, A.p, A.rows, 64, 64, 64, a_rows, false, cdiv(A.cols, 64), true)
+                                  : make_map2(&g.maps.a, A.p, A.rows, A.cols, A.ld, kBK, a_rows, false, 1, false);
+  if (rc == JL_OK) rc = make_map2(&g.maps.b, B.p, B.rows, B.cols, B.ld, kBK, P::kBMn ? kBK : plan.bn / P::kPair, false, 1, false);
+  if (rc == JL_OK && out.p != nullptr)
+    rc = out.ld == 0 ? make_map2(&g.maps.out, out.p, p.M, 64, 64, 64, 32, false, cdiv(p.N, 64), true)
+                     : make_map2(&g.maps.out, out.p, p.M, p.N, out.ld, out.f32 ? 32 : 64, 32, out.f32, out.planes, true);
+  return rc;
+}
+
+int64_t tiles_of(const GemmParams& p) { return static_cast<int64_t>(p.m_tiles) * p.n_tiles * p.splits; }
+
+template <class P0, class P1>
+int launch(const Gemm& g0, const Gemm& g1, cudaStream_t stream) {
+  constexpr int kPair = P0::kPair;
+  auto kernel = head_gemm_kernel<P0, P1>;
   static bool attr_set[64] = {false};
   int dev = -1;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return fail(JL_ERR_LAUNCH, "jl_head: no current CUDA device");
@@ -548,7 +650,7 @@ int launch_gemm(const Matrix& A, const Matrix& B, const Result& out, GemmParams 
       return check_launch("jl_head (shared memory opt-in)");
     attr_set[dev] = true;
   }
-  const int64_t tiles = static_cast<int64_t>(p.m_tiles) * p.n_tiles * p.splits;
+  const int64_t tiles = std::is_same<P1, void>::value ? tiles_of(g0.p) : kSms;
   const int workers = static_cast<int>(tiles < kSms / kPair ? tiles : kSms / kPair);
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(workers * kPair);
@@ -561,8 +663,34 @@ int launch_gemm(const Matrix& A, const Matrix& B, const Result& out, GemmParams 
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, kernel, maps, p) != cudaSuccess) return check_launch("jl_head");
+  if (cudaLaunchKernelEx(&cfg, kernel, g0.maps, g0.p, g1.maps, g1.p) != cudaSuccess) return check_launch("jl_head");
   return JL_OK;
+}
+
+template <class P>
+int launch_one(const Gemm& g, cudaStream_t stream) { return launch<P, void>(g, g, stream); }
+
+using Scores1 = Product<1, false, false, kEpiScores>;
+using Scores2 = Product<2, false, false, kEpiScores>;
+using Dz1 = Product<1, false, false, kEpiDz>;
+using Dz2 = Product<2, false, false, kEpiDz>;
+using Dh1 = Product<1, false, true, kEpiF32>;
+using Dh2 = Product<2, false, true, kEpiF32>;
+using Dw2 = Product<2, true, true, kEpiBf16>;
+
+// Cost of a tile in K blocks: its own, and about three for a short tile's hand-over.
+int64_t tile_cost(const GemmParams& p) { return p.kb_per_split + 3; }
+
+// Shares of the second product of a launch, so that the workers that carry one tile more of the first end with the others.
+void balance(const Gemm& first, Gemm& second) {
+  const int64_t W = kSms / 2, n0 = tiles_of(first.p), n1 = tiles_of(second.p), c0 = tile_cost(first.p), c1 = tile_cost(second.p);
+  const int64_t l = n0 / W, rem = n0 % W;
+  int64_t late = ((n0 * c0 + n1 * c1) / W - (l + 1) * c0) / c1;            // rounds of the workers with l + 1 tiles
+  if (late < 0) late = 0;
+  int64_t rounds = cdiv(n1 - rem * late, W - rem);
+  if (rounds < late) rounds = late = cdiv(n1, W);
+  second.p.behind = static_cast<int>(rem);
+  second.p.alone_rounds = static_cast<int>(rounds - late);
 }
 
 int pair_of(int64_t rows) { return rows > 128 ? 2 : 1; }
@@ -591,7 +719,7 @@ ScoresLayout scores_layout(int64_t rows, int32_t vocab) {
 }
 
 // Pieces of the vocabulary in the gradient pass: as large as 256 MB of dz allow (fewer, longer launches), balanced, a
-// multiple of 256.  K splits of the dh product: as many as fill the GPU when it has few tiles.
+// multiple of 256.
 struct GradsLayout { int64_t piece; Plan dz, dh, dw; int splits; size_t dh32, total; };
 GradsLayout grads_layout(int64_t rows, int32_t hd, int32_t vocab) {
   GradsLayout l;
@@ -601,13 +729,8 @@ GradsLayout grads_layout(int64_t rows, int32_t hd, int32_t vocab) {
   const int64_t pieces = cdiv(vocab, most);
   l.piece = cdiv(cdiv(vocab, pieces), 256) * 256;
   l.dz = plan_tiles(n, l.piece < vocab ? l.piece : vocab, pair_of(n), 64);
-  l.dh = plan_tiles(n, hd, pair_of(n), 64 * pair_of(n));
   l.dw = plan_tiles(l.piece < vocab ? l.piece : vocab, hd, 2, 128);
-  const int64_t tiles = static_cast<int64_t>(l.dh.m_tiles) * l.dh.n_tiles, k_blocks = cdiv(l.piece, kBK);
-  int64_t s = kSms / l.dh.pair / tiles;
-  if (s > k_blocks / 8) s = k_blocks / 8;
-  l.splits = static_cast<int>(s < 1 ? 1 : s);
-  l.splits = static_cast<int>(cdiv(k_blocks, cdiv(k_blocks, l.splits)));
+  l.dh = plan_split(n, hd, pair_of(n), cdiv(l.piece, kBK), l.splits);
   l.dh32 = up256(static_cast<size_t>(n) * l.piece * 2);
   l.total = l.dh32 + up256(static_cast<size_t>(n) * hd * 4 * l.splits);
   return l;
@@ -643,7 +766,8 @@ int launch_scores(const jl_head_scores_args* a, cudaStream_t stream) {
     const int64_t n = a->rows - r0 < kScoreRows ? a->rows - r0 : kScoreRows;
     Plan plan = l.plan;
     plan.m_tiles = static_cast<int>(cdiv(n, 128 * plan.pair));
-    GemmParams p{};
+    Gemm g{};
+    GemmParams& p = g.p;
     p.part = reinterpret_cast<float2*>(ws + l.part);
     p.part_arg = a->top != nullptr ? reinterpret_cast<int*>(ws + l.arg) : nullptr;
     p.picked = reinterpret_cast<float*>(ws + l.picked);
@@ -652,8 +776,13 @@ int launch_scores(const jl_head_scores_args* a, cudaStream_t stream) {
     p.group_m = group_of(a->hidden_size, plan.pair);
     const Matrix h{static_cast<const __nv_bfloat16*>(a->hidden) + r0 * a->hidden_stride, n, a->hidden_size, a->hidden_stride};
     const Matrix w{a->weight, a->vocab, a->hidden_size, a->weight_stride};
-    rc = plan.pair == 2 ? launch_gemm<2, false, false, kEpiScores>(h, w, Result{}, p, plan, a->hidden_size, 1, stream)
-                        : launch_gemm<1, false, false, kEpiScores>(h, w, Result{}, p, plan, a->hidden_size, 1, stream);
+    if (plan.pair == 2) {
+      rc = prepare<Scores2>(g, h, w, Result{}, plan, a->hidden_size, 1);
+      if (rc == JL_OK) rc = launch_one<Scores2>(g, stream);
+    } else {
+      rc = prepare<Scores1>(g, h, w, Result{}, plan, a->hidden_size, 1);
+      if (rc == JL_OK) rc = launch_one<Scores1>(g, stream);
+    }
     if (rc != JL_OK) return rc;
     const bool few = n < 4 * kSms;
     if (launch_dependent(few ? scores_fold_kernel<8> : scores_fold_kernel<1>, dim3(static_cast<unsigned>(few ? n : cdiv(n, 8))), dim3(256), 0, stream,
@@ -698,33 +827,43 @@ int launch_grads(const jl_head_grads_args* a, cudaStream_t stream) {
   for (int64_t v0 = 0; v0 < V; v0 += l.piece) {
     const int64_t piece = V - v0 < l.piece ? V - v0 : l.piece;
     const Matrix w{static_cast<const __nv_bfloat16*>(a->weight) + v0 * a->weight_stride, piece, H, a->weight_stride};
-    const Matrix dz{ws, N, piece, l.piece};
-    const Result dz_out{ws, l.piece, false, 1};
-    GemmParams p = base;
-    p.v0 = v0;
-    p.group_m = group_of(H, l.dz.pair);
+    const Matrix dz{ws, N, piece, 0};
+    Gemm z{GemmMaps{}, base}, dh{GemmMaps{}, base}, dw{GemmMaps{}, base};
+    z.p.v0 = v0;
+    z.p.group_m = group_of(H, l.dz.pair);
     Plan plan = l.dz;
     plan.n_tiles = static_cast<int>(cdiv(piece, plan.bn));
-    rc = plan.pair == 2 ? launch_gemm<2, false, false, kEpiDz>(h, w, dz_out, p, plan, H, 1, stream)
-                        : launch_gemm<1, false, false, kEpiDz>(h, w, dz_out, p, plan, H, 1, stream);
+    const Result z_out{ws, 0, false, 1};
+    if (plan.pair == 2) {
+      rc = prepare<Dz2>(z, h, w, z_out, plan, H, 1);
+      if (rc == JL_OK) rc = launch_one<Dz2>(z, stream);
+    } else {
+      rc = prepare<Dz1>(z, h, w, z_out, plan, H, 1);
+      if (rc == JL_OK) rc = launch_one<Dz1>(z, stream);
+    }
     if (rc == JL_OK && a->d_hidden != nullptr) {
-      p = base;
-      p.reduce = v0 > 0;
-      p.group_m = 1 << 20;
-      const Result out{dh32, H, true, l.splits};
+      dh.p.reduce = v0 > 0;
+      dh.p.group_m = 1 << 20;
       const int64_t kb = cdiv(piece, kBK);
       // a short last piece has fewer K splits than the others: the planes it does not reach keep their sums
       const int s = static_cast<int>(kb < l.splits ? kb : l.splits);
-      rc = l.dh.pair == 2 ? launch_gemm<2, false, true, kEpiF32>(dz, w, out, p, l.dh, piece, s, stream)
-                          : launch_gemm<1, false, true, kEpiF32>(dz, w, out, p, l.dh, piece, s, stream);
-      if (v0 == 0) splits = static_cast<int>(cdiv(kb, cdiv(kb, s)));
+      const Result out{dh32, H, true, l.splits};
+      rc = l.dh.pair == 2 ? prepare<Dh2>(dh, dz, w, out, l.dh, piece, s) : prepare<Dh1>(dh, dz, w, out, l.dh, piece, s);
+      if (v0 == 0) splits = dh.p.splits;
     }
     if (rc == JL_OK && a->d_weight != nullptr) {
-      p = base;
-      p.group_m = 0;
       plan = l.dw;
       plan.m_tiles = static_cast<int>(cdiv(piece, 256));
-      rc = launch_gemm<2, true, true, kEpiBf16>(dz, h, Result{static_cast<__nv_bfloat16*>(a->d_weight) + v0 * H, H, false, 1}, p, plan, N, 1, stream);
+      dw.p.group_m = 0;
+      rc = prepare<Dw2>(dw, dz, h, Result{static_cast<__nv_bfloat16*>(a->d_weight) + v0 * H, H, false, 1}, plan, N, 1);
+    }
+    if (rc == JL_OK && a->d_hidden != nullptr && a->d_weight != nullptr && l.dh.pair == 2) {
+      // dh has few, long tiles (160 on 74 pairs for 4096 rows x 2560: 72 % of three rounds); dW's many short ones fill in
+      balance(dh, dw);
+      rc = launch<Dh2, Dw2>(dh, dw, stream);
+    } else {
+      if (rc == JL_OK && a->d_hidden != nullptr) rc = l.dh.pair == 2 ? launch_one<Dh2>(dh, stream) : launch_one<Dh1>(dh, stream);
+      if (rc == JL_OK && a->d_weight != nullptr) rc = launch_one<Dw2>(dw, stream);
     }
     if (rc != JL_OK) return rc;
   }
