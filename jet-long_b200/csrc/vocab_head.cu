@@ -28,14 +28,12 @@ constexpr int kBK = 64;                      // K step: one 128-byte swizzle row
 constexpr int kMaxBN = 256;
 constexpr int kABytes = 128 * kBK * 2;       // a CTA's 128 rows of A
 constexpr int kAccCols = 256;                // tensor-memory columns of one accumulator; two of them alternate
-constexpr int kGemmThreads = 256;
-constexpr int kRingBytes = 196608;           // operand ring
-constexpr int kMaxStages = 6;
-template <int kPair>
-struct Ring {                                // a stage: 128 rows of A and this CTA's rows of B, 64 deep
-  static constexpr int kStageBytes = kABytes + kMaxBN / kPair * kBK * 2, kStages = kRingBytes / kStageBytes;
-};
-constexpr int kStagingBytes = 2 * 4 * 4096;  // per epilogue warp two buffers of 32 rows x 128 bytes
+constexpr int kEpiWarps = 8;                 // two per quarter of the accumulator's rows, each with half of the columns
+constexpr int kGemmThreads = 128 + 32 * kEpiWarps;
+constexpr int kRegsLow = 72, kRegsHigh = 216;     // 128 x 72 + 256 x 216 = the launch total 384 x 168
+constexpr int kRingBytes = 196608;           // operand ring: as many stages of A and B rows, 64 deep, as fit
+constexpr int kMaxStages = 8;
+constexpr int kStagingBytes = kEpiWarps * 4096;      // per epilogue warp a box of 32 rows x 128 bytes
 constexpr int kSms = 148;
 
 enum { kEpiScores = 0, kEpiDz = 1, kEpiF32 = 2, kEpiBf16 = 3 };
@@ -56,9 +54,10 @@ struct GemmParams {
   int m_tiles, n_tiles, splits, k_blocks, kb_per_split, bn;
   int group_m;                // > 0: m fastest inside groups of this many m tiles; 0: n fastest
   int behind, alone_rounds;   // see TileWalk
+  int a_bytes, stage_bytes, stages;      // of the operand ring, per CTA
   // scores
-  float2* part;               // [row][n tile] (maximum, sum of exponentials relative to it)
-  int* part_arg;              // [row][n tile] or NULL
+  float2* part;               // [row][n tile][half] (maximum, sum of exponentials relative to it)
+  int* part_arg;              // [row][n tile][half] or NULL
   float* picked;              // [row] logit of the label
   // dz
   const float* lse;
@@ -151,7 +150,13 @@ struct TileWalk {
 };
 
 // The ring and the accumulators go on from one product of a launch to the next.
-struct PipeState { int g, i; };       // stages used, tiles done
+struct PipeState {
+  int slot, i;                        // next stage, tiles done
+  uint32_t parity;
+  __device__ __forceinline__ void next(int stages) {
+    if (++slot == stages) { slot = 0; parity ^= 1u; }
+  }
+};
 
 // Operand kinds of a product C = A B^T: which of A and B are read across their rows (MN-major), and what becomes of C.
 template <int kPair_, bool kAMn_, bool kBMn_, int kEpi_>
@@ -159,25 +164,31 @@ struct Product {
   static constexpr int kPair = kPair_, kEpi = kEpi_;
   static constexpr bool kAMn = kAMn_, kBMn = kBMn_;
   static constexpr bool kABlocked = kEpi_ == kEpiF32 || kEpi_ == kEpiBf16;     // A is dz
+  // K blocks that an accumulator takes before it is handed over.  The tensor cores cut every sum off instead of rounding it: over
+  // the 256 steps of K = 4096 a logit lost 2^-24 of its size 256 times, up to 1e-5 in all, and so did the losses.  Scores
+  // therefore take K in parts that are added in fp32 registers.  Error of the loss / time of 8191 rows x 4096 with parts of 256,
+  // 512, 1024 and all of K: 2e-7 / 8.0 ms, 3.5e-7 / 7.5, 8e-7 / 7.25, 4e-6 / 7.1; a few rows are bound by the weight's bytes and
+  // take the shortest parts at no cost.  Results that are rounded to bf16 need none of this.
+  static constexpr int kPart = kEpi_ != kEpiScores ? 1 << 30 : kPair_ == 1 ? 4 : 8;
 };
 
 template <class P>
 __device__ __forceinline__ void produce(const GemmMaps& maps, const GemmParams& p, GemmSmem& sm, int rank, int worker, int workers, PipeState& st) {
-  constexpr int kPair = P::kPair, kStages = Ring<kPair>::kStages, kStageBytes = Ring<kPair>::kStageBytes;
-  const int b_rows = p.bn / kPair, stage_bytes = kABytes + b_rows * kBK * 2;
+  constexpr int kPair = P::kPair;
+  const int b_rows = p.bn / kPair, tx_bytes = p.a_bytes + b_rows * kBK * 2;
   TileWalk walk(p, worker, workers);
   for (int t; walk.next(t);) {
     const TileCoord c = tile_coord(p, t);
     const int m0 = (c.m * kPair + rank) * 128, n0 = c.n * p.bn + rank * b_rows;
     const int kb0 = c.split * p.kb_per_split, kb1 = min(kb0 + p.kb_per_split, p.k_blocks);
-    for (int kb = kb0; kb < kb1; ++kb, ++st.g) {
-      const int s = st.g % kStages;
-      mbar_wait(&sm.empty[s], ((st.g / kStages) & 1) ^ 1, sm);
+    for (int kb = kb0; kb < kb1; ++kb, st.next(p.stages)) {
+      const int s = st.slot;
+      mbar_wait(&sm.empty[s], st.parity ^ 1u, sm);
       if (*reinterpret_cast<volatile int*>(&sm.failed)) return;
-      if (rank == 0) mbar_expect_tx(&sm.full[s], kPair * stage_bytes);
+      if (rank == 0) mbar_expect_tx(&sm.full[s], kPair * tx_bytes);
       const uint32_t bar = kPair == 2 ? pair::leader_addr(&sm.full[s]) : smem_u32(&sm.full[s]);
-      uint8_t* sa = sm.ring + s * kStageBytes;
-      uint8_t* sb = sa + kABytes;
+      uint8_t* sa = sm.ring + s * p.stage_bytes;
+      uint8_t* sb = sa + p.a_bytes;
       auto load = [&](void* dst, const CUtensorMap* map, int x, int y) {
         if (kPair == 2) tma_load_2d_pair(dst, map, bar, x, y);
         else tma_load_2d(dst, map, bar, x, y);
@@ -203,22 +214,26 @@ __device__ __forceinline__ void produce(const GemmMaps& maps, const GemmParams& 
 
 template <class P>
 __device__ __forceinline__ void issue(const GemmParams& p, GemmSmem& sm, uint32_t tmem, uint32_t leader, int worker, int workers, PipeState& st) {
-  constexpr int kPair = P::kPair, kStages = Ring<kPair>::kStages, kStageBytes = Ring<kPair>::kStageBytes;
+  constexpr int kPair = P::kPair;
   const uint32_t idesc = instr_desc(128 * kPair, p.bn, P::kBMn) | (P::kAMn ? 1u << 15 : 0u);
   const uint32_t ring = smem_u32(sm.ring);
   TileWalk walk(p, worker, workers);
-  for (int t; walk.next(t); ++st.i) {
+  for (int t; walk.next(t);) {
     const TileCoord c = tile_coord(p, t);
     const int kb0 = c.split * p.kb_per_split, kb1 = min(kb0 + p.kb_per_split, p.k_blocks);
-    mbar_wait(&sm.acc_free[st.i & 1], ((st.i >> 1) & 1) ^ 1, sm);
-    tc_fence_after();
-    const uint32_t acc = tmem + (st.i & 1) * kAccCols;
-    for (int kb = kb0; kb < kb1; ++kb, ++st.g) {
-      const int s = st.g % kStages;
-      mbar_wait(&sm.full[s], (st.g / kStages) & 1, sm);
+    uint32_t acc = 0;
+    for (int kb = kb0; kb < kb1; ++kb, st.next(p.stages)) {
+      const bool first = kb == kb0 || (P::kEpi == kEpiScores && (kb - kb0) % P::kPart == 0);
+      const bool last = kb + 1 == kb1 || (P::kEpi == kEpiScores && (kb + 1 - kb0) % P::kPart == 0);
+      if (first) {
+        mbar_wait(&sm.acc_free[st.i & 1], ((st.i >> 1) & 1) ^ 1, sm);
+        acc = tmem + (st.i & 1) * kAccCols;
+      }
+      const int s = st.slot;
+      mbar_wait(&sm.full[s], st.parity, sm);
       if (*reinterpret_cast<volatile int*>(&sm.failed)) return;
       tc_fence_after();
-      const uint32_t sa = ring + s * kStageBytes, sb = sa + kABytes;
+      const uint32_t sa = ring + s * p.stage_bytes, sb = sa + p.a_bytes;
       // K-major rows are 128 bytes in 8-row swizzle atoms; MN-major: 64 elements x 8 k-rows per atom, 8 KB per 64 elements
       const uint64_t ad = P::kAMn ? smem_desc(sa, 8192, 1024) : smem_desc(sa, 16, 1024);
       const uint64_t bd = P::kBMn ? smem_desc(sb, 8192, 1024) : smem_desc(sb, 16, 1024);
@@ -227,35 +242,36 @@ __device__ __forceinline__ void issue(const GemmParams& p, GemmSmem& sm, uint32_
         for (int kk = 0; kk < 4; ++kk) {
           const uint64_t ao = static_cast<uint64_t>((P::kAMn ? kk * 2048 : kk * 32) >> 4);
           const uint64_t bo = static_cast<uint64_t>((P::kBMn ? kk * 2048 : kk * 32) >> 4);
-          if (kPair == 2) pair::mma2_ss(acc, ad + ao, bd + bo, idesc, kb > kb0 || kk > 0);
-          else mma_ss(acc, ad + ao, bd + bo, idesc, kb > kb0 || kk > 0);
+          if (kPair == 2) pair::mma2_ss(acc, ad + ao, bd + bo, idesc, !first || kk > 0);
+          else mma_ss(acc, ad + ao, bd + bo, idesc, !first || kk > 0);
         }
         if (kPair == 2) pair::commit_both(&sm.empty[s]);
         else mma_commit(&sm.empty[s]);
+        if (last) {
+          if (kPair == 2) pair::commit_both(&sm.acc_full[st.i & 1]);
+          else mma_commit(&sm.acc_full[st.i & 1]);
+        }
       }
       __syncwarp();
+      if (last) ++st.i;
     }
-    if (leader) {
-      if (kPair == 2) pair::commit_both(&sm.acc_full[st.i & 1]);
-      else mma_commit(&sm.acc_full[st.i & 1]);
-    }
-    __syncwarp();
   }
 }
 
 template <class P>
-__device__ __forceinline__ void finish(const GemmMaps& maps, const GemmParams& p, GemmSmem& sm, uint32_t tmem, int quad, int lane, int rank, int worker,
-                                       int workers, PipeState& st, int& buf) {
+__device__ __forceinline__ void finish(const GemmMaps& maps, const GemmParams& p, GemmSmem& sm, uint32_t tmem, int ew, int lane, int rank, int worker,
+                                       int workers, PipeState& st) {
   constexpr int kPair = P::kPair, kEpi = P::kEpi;
+  const int quad = ew & 3, half = ew >> 2;         // rows quad * 32 .. of the accumulator, first or second half of its columns
   const uint32_t lane_base = static_cast<uint32_t>(quad * 32) << 16;
-  uint8_t* const stage = sm.staging + quad * 8192;
+  uint8_t* const stage = sm.staging + ew * 4096;
   const uint32_t free_bar[2] = {kPair == 2 ? pair::leader_addr(&sm.acc_free[0]) : smem_u32(&sm.acc_free[0]),
                                 kPair == 2 ? pair::leader_addr(&sm.acc_free[1]) : smem_u32(&sm.acc_free[1])};
   const float scale = kEpi == kEpiBf16 ? p.scale.get() : 1.f;
   // 32 rows x 128 bytes of results: 16-byte chunk `ch` of this thread's row
-  auto chunk_ptr = [&](int ch) { return reinterpret_cast<uint4*>(stage + buf * 4096 + lane * 128 + ((ch ^ (lane & 7)) << 4)); };
+  auto chunk_ptr = [&](int ch) { return reinterpret_cast<uint4*>(stage + lane * 128 + ((ch ^ (lane & 7)) << 4)); };
   auto begin_box = [&]() {
-    if (lane == 0) bulk_wait_read<1>();          // the box before the last one has left this buffer
+    if (lane == 0) bulk_wait_read<0>();          // the box before has left the buffer
     __syncwarp();
   };
   auto end_box = [&](int x, int64_t row_w, int z, bool reduce) {
@@ -263,71 +279,81 @@ __device__ __forceinline__ void finish(const GemmMaps& maps, const GemmParams& p
     __syncwarp();
     if (lane == 0) {
       if (row_w < p.M && x < p.N) {
-        if (kEpi == kEpiDz) tma_store_3d(&maps.out, stage + buf * 4096, 0, static_cast<int>(row_w), x >> 6, false);      // blocks of 64 columns
-        else tma_store_3d(&maps.out, stage + buf * 4096, x, static_cast<int>(row_w), z, reduce);
+        if (kEpi == kEpiDz) tma_store_3d(&maps.out, stage, 0, static_cast<int>(row_w), x >> 6, false);      // blocks of 64 columns
+        else tma_store_3d(&maps.out, stage, x, static_cast<int>(row_w), z, reduce);
       }
       bulk_commit();
     }
-    buf ^= 1;
+  };
+  auto hand_back = [&]() {                         // this warp has read the accumulator
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(free_bar[st.i & 1]) : "memory");
+    ++st.i;
   };
   TileWalk walk(p, worker, workers);
-  for (int t; walk.next(t); ++st.i) {
+  for (int t; walk.next(t);) {
     const TileCoord c = tile_coord(p, t);
     const int64_t row_w = (static_cast<int64_t>(c.m) * kPair + rank) * 128 + quad * 32, row = row_w + lane;
     const int n0 = c.n * p.bn;
-    const uint32_t acc = tmem + (st.i & 1) * kAccCols + lane_base;
-    mbar_wait(&sm.acc_full[st.i & 1], (st.i >> 1) & 1, sm);
-    tc_fence_after();
 
     if constexpr (kEpi == kEpiScores) {
-      const int valid = static_cast<int>(min(static_cast<int64_t>(p.bn), p.N - n0));
-      float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-      for (int c0 = 0; c0 < valid; c0 += 16) {
-        uint32_t z[16];
-        JL_TMEM_LD16(acc + c0, z);
-        JL_TMEM_WAIT_LD16(z, 0);
-        if (c0 + 16 <= valid) {
+      // columns [c_lo, c_lo + width) of the tile, up to 128 of them in registers, summed over the parts of K
+      const int c_lo = half == 0 ? 0 : (p.bn / 2 + 15) / 16 * 16, width = half == 0 ? (p.bn / 2 + 15) / 16 * 16 : p.bn - c_lo;
+      float z[128];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) m4[j & 3] = max3(m4[j & 3], __uint_as_float(z[2 * j]), __uint_as_float(z[2 * j + 1]));
-        } else {
+      for (int j = 0; j < 128; ++j) z[j] = 0.f;
+      for (int part = 0; part * P::kPart < p.k_blocks; ++part) {
+        const uint32_t acc = tmem + (st.i & 1) * kAccCols + lane_base + c_lo;
+        mbar_wait(&sm.acc_full[st.i & 1], (st.i >> 1) & 1, sm);
+        tc_fence_after();
 #pragma unroll
-          for (int j = 0; j < 16; ++j)
-            if (c0 + j < valid) m4[j & 3] = fmaxf(m4[j & 3], __uint_as_float(z[j]));
+        for (int ch = 0; ch < 8; ++ch) {
+          if (ch * 16 < width) {
+            uint32_t x[16];
+            JL_TMEM_LD16(acc + ch * 16, x);
+            JL_TMEM_WAIT_LD16(x, 0);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) z[ch * 16 + j] += __uint_as_float(x[j]);
+          }
         }
+        hand_back();
+      }
+      const int64_t rest = p.N - n0 - c_lo;
+      const int valid = static_cast<int>(rest < 0 ? 0 : rest < width ? rest : width);
+      float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int j = 0; j < 128; ++j) {
+        if (j >= valid) z[j] = -INFINITY;
+        m4[j & 3] = fmaxf(m4[j & 3], z[j]);
       }
       const float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
       const float m_use = m == -INFINITY ? 0.f : m;
-      const int64_t y64 = p.labels != nullptr && row < p.M ? p.labels[row] - p.v0 - n0 : -1;
+      const int64_t y64 = p.labels != nullptr && row < p.M ? p.labels[row] - p.v0 - n0 - c_lo : -1;
       const int y = y64 >= 0 && y64 < valid ? static_cast<int>(y64) : -1;
       float s4[4] = {0.f, 0.f, 0.f, 0.f}, z_y = 0.f;
       int arg = 0x7fffffff;
-      for (int c0 = 0; c0 < valid; c0 += 16) {
-        uint32_t z[16];
-        JL_TMEM_LD16(acc + c0, z);
-        JL_TMEM_WAIT_LD16(z, 0);
-        if (__any_sync(0xffffffffu, y >= c0 && y < c0 + 16)) {
+      if (__any_sync(0xffffffffu, y >= 0)) {
 #pragma unroll
-          for (int j = 0; j < 16; ++j) z_y = y == c0 + j ? __uint_as_float(z[j]) : z_y;
-        }
-        if (p.part_arg != nullptr) {
-#pragma unroll
-          for (int j = 0; j < 16; ++j)
-            if (__uint_as_float(z[j]) == m && c0 + j < valid) arg = min(arg, c0 + j);
-        }
-        // (z - m) first: exact for the logits that count, whatever their size
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const float e = fast_exp2((__uint_as_float(z[j]) - m_use) * kLog2e);
-          if (c0 + j < valid) s4[j & 3] += e;
-        }
+        for (int j = 0; j < 128; ++j) z_y = y == j ? z[j] : z_y;
       }
-      tc_fence_before();
+      if (p.part_arg != nullptr) {
+#pragma unroll
+        for (int j = 127; j >= 0; --j) arg = z[j] == m && j < valid ? j : arg;
+      }
+      // (z - m) first: exact for the logits that count, whatever their size
+#pragma unroll
+      for (int j = 0; j < 128; ++j) s4[j & 3] += fast_exp2((z[j] - m_use) * kLog2e);
       if (row < p.M) {
-        p.part[row * p.n_tiles + c.n] = make_float2(m, (s4[0] + s4[1]) + (s4[2] + s4[3]));
-        if (p.part_arg != nullptr) p.part_arg[row * p.n_tiles + c.n] = arg == 0x7fffffff ? n0 : n0 + arg;
+        const int64_t at = (row * p.n_tiles + c.n) * 2 + half;
+        p.part[at] = make_float2(m, (s4[0] + s4[1]) + (s4[2] + s4[3]));
+        if (p.part_arg != nullptr) p.part_arg[at] = arg == 0x7fffffff ? arg : n0 + c_lo + arg;
         if (y >= 0) p.picked[row] = z_y;
       }
     } else {
+      const uint32_t acc = tmem + (st.i & 1) * kAccCols + lane_base;
+      mbar_wait(&sm.acc_full[st.i & 1], (st.i >> 1) & 1, sm);
+      tc_fence_after();
       float lse = 0.f, factor = 0.f;
       int y = -1;
       if constexpr (kEpi == kEpiDz) {
@@ -344,10 +370,10 @@ __device__ __forceinline__ void finish(const GemmMaps& maps, const GemmParams& p
       }
       const bool used = kEpi != kEpiDz || factor != 0.f;
       constexpr int kCols = kEpi == kEpiF32 ? 32 : 64;             // columns of one 128-byte box; bn is a multiple of 64 here
-      for (int c0 = 0; c0 < p.bn; c0 += kCols) {
+      for (int c0 = half * kCols; c0 < p.bn; c0 += 2 * kCols) {      // the two warps of a row quarter take the boxes in turn
         begin_box();
-        for (int half = 0; half < kCols / 32; ++half) {
-          const int cc = c0 + half * 32;
+        for (int hc = 0; hc < kCols / 32; ++hc) {
+          const int cc = c0 + hc * 32;
           uint32_t z[32];
           JL_TMEM_LD32(acc + cc, z, 0);
           JL_TMEM_WAIT_LD32(z, 0);
@@ -368,15 +394,13 @@ __device__ __forceinline__ void finish(const GemmMaps& maps, const GemmParams& p
           } else {
             auto pk = [&](int j) { return pack_bf16x2(__uint_as_float(z[j]) * scale, __uint_as_float(z[j + 1]) * scale); };
 #pragma unroll
-            for (int v = 0; v < 4; ++v) *chunk_ptr(half * 4 + v) = make_uint4(pk(8 * v), pk(8 * v + 2), pk(8 * v + 4), pk(8 * v + 6));
+            for (int v = 0; v < 4; ++v) *chunk_ptr(hc * 4 + v) = make_uint4(pk(8 * v), pk(8 * v + 2), pk(8 * v + 4), pk(8 * v + 6));
           }
         }
         end_box(n0 + c0, row_w, kEpi == kEpiF32 ? c.split : 0, kEpi == kEpiF32 && p.reduce);
       }
-      tc_fence_before();
+      hand_back();
     }
-    __syncwarp();
-    if (lane == 0) asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(free_bar[st.i & 1]) : "memory");
   }
 }
 
@@ -384,7 +408,7 @@ __device__ __forceinline__ void finish(const GemmMaps& maps, const GemmParams& p
 // other, the second filling the SMs that the first leaves.  kPair = 2: a cluster of two CTAs works on one tile with cta_group::2
 // MMAs, each CTA loading its own 128 rows of A and half of the rows of B, so every byte of B in shared memory serves 256 rows.
 // Two accumulators alternate, so the epilogue of a tile runs under the next one's MMAs.
-//   warp 0 TMA producer, warp 1 MMA issuer (rank 0), warp 2 tensor memory, warps 4-7 epilogue (one thread per row)
+//   warp 0 TMA producer, warp 1 MMA issuer (rank 0), warp 2 tensor memory, warps 4-11 epilogue (one thread per row and half)
 template <class P0, class P1>
 __global__ void __launch_bounds__(kGemmThreads, 1) head_gemm_kernel(const __grid_constant__ GemmMaps maps0, const GemmParams p0,
                                                                     const __grid_constant__ GemmMaps maps1, const GemmParams p1) {
@@ -399,7 +423,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) head_gemm_kernel(const __grid
   if (threadIdx.x == 0) {
     sm.failed = *reinterpret_cast<volatile int*>(&g_head_status) != 0 ? 1 : 0;
     for (int i = 0; i < kMaxStages; ++i) { mbar_init(&sm.full[i], 1); mbar_init(&sm.empty[i], 1); }
-    for (int i = 0; i < 2; ++i) { mbar_init(&sm.acc_full[i], 1); mbar_init(&sm.acc_free[i], 4 * kPair); }
+    for (int i = 0; i < 2; ++i) { mbar_init(&sm.acc_full[i], 1); mbar_init(&sm.acc_free[i], kEpiWarps * kPair); }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 2) {
@@ -418,21 +442,25 @@ __global__ void __launch_bounds__(kGemmThreads, 1) head_gemm_kernel(const __grid
   launch_dependents();
   const uint32_t tmem = sm.tmem_base;
 
-  PipeState st{0, 0};
-  if (warp == 0) {
-    if (lane == 0) {
-      produce<P0>(maps0, p0, sm, rank, worker, workers, st);
-      if constexpr (kTwo) produce<P1>(maps1, p1, sm, rank, worker, workers, st);
+  PipeState st{0, 0, 0u};
+  // the control warps give registers back, the epilogue warps (128 logits of a row each) take them
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsLow));
+    if (warp == 0) {
+      if (lane == 0) {
+        produce<P0>(maps0, p0, sm, rank, worker, workers, st);
+        if constexpr (kTwo) produce<P1>(maps1, p1, sm, rank, worker, workers, st);
+      }
+    } else if (warp == 1 && rank == 0) {
+      uint32_t leader;
+      asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(leader));
+      issue<P0>(p0, sm, tmem, leader, worker, workers, st);
+      if constexpr (kTwo) issue<P1>(p1, sm, tmem, leader, worker, workers, st);
     }
-  } else if (warp == 1 && rank == 0) {
-    uint32_t leader;
-    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(leader));
-    issue<P0>(p0, sm, tmem, leader, worker, workers, st);
-    if constexpr (kTwo) issue<P1>(p1, sm, tmem, leader, worker, workers, st);
-  } else if (warp >= 4) {
-    int buf = 0;
-    finish<P0>(maps0, p0, sm, tmem, warp & 3, lane, rank, worker, workers, st, buf);
-    if constexpr (kTwo) finish<P1>(maps1, p1, sm, tmem, warp & 3, lane, rank, worker, workers, st, buf);
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsHigh));
+    finish<P0>(maps0, p0, sm, tmem, warp - 4, lane, rank, worker, workers, st);
+    if constexpr (kTwo) finish<P1>(maps1, p1, sm, tmem, warp - 4, lane, rank, worker, workers, st);
     if (lane == 0) bulk_wait_all();
   }
 
@@ -500,7 +528,8 @@ __global__ void __launch_bounds__(256) scores_fold_kernel(const float2* part, co
   if (top != nullptr) top[row] = arg == 0x7fffffff ? 0 : arg;
   if (nll != nullptr) {
     const int64_t y = labels[row];
-    nll[row] = y == ignore ? 0.f : (y >= 0 && y < V ? l - picked[row] : __int_as_float(0x7fc00000));
+    // (m - z_y) + log s, not lse - z_y: a small loss keeps its digits
+    nll[row] = y == ignore ? 0.f : (y >= 0 && y < V ? (m - picked[row]) + logf(s) : __int_as_float(0x7fc00000));
   }
 }
 
@@ -626,7 +655,13 @@ int prepare(Gemm& g, const Matrix& A, const Matrix& B, const Result& out, const 
   p.splits = static_cast<int>(cdiv(p.k_blocks, p.kb_per_split));
   p.behind = p.alone_rounds = 0;
   int rc = bind_context();
-  const int a_rows = P::kAMn ? kBK : 128;
+  // a single CTA's one row tile may be short: only its rows are loaded (what the others hold reaches no result)
+  const int a_rows = P::kAMn ? kBK : P::kPair == 1 && p.M < 128 ? static_cast<int>(cdiv(p.M, 8)) * 8 : 128;
+  p.a_bytes = P::kAMn ? kABytes : a_rows * kBK * 2;
+  // pairs have one geometry, so that two products can share a launch; a single CTA's ring is as deep as its tiles allow (reads of
+  // A rows past a short tile stay inside the ring and the staging behind it)
+  p.stage_bytes = P::kPair == 2 ? kABytes + kMaxBN / 2 * kBK * 2 : p.a_bytes + plan.bn * kBK * 2;
+  p.stages = kRingBytes / p.stage_bytes < kMaxStages ? kRingBytes / p.stage_bytes : kMaxStages;
   if (rc == JL_OK) rc = A.ld == 0 ? make_map2(&g.maps.a, A.p, A.rows, 64, 64, 64, a_rows, false, cdiv(A.cols, 64), true)
                                   : make_map2(&g.maps.a, A.p, A.rows, A.cols, A.ld, kBK, a_rows, false, 1, false);
   if (rc == JL_OK) rc = make_map2(&g.maps.b, B.p, B.rows, B.cols, B.ld, kBK, P::kBMn ? kBK : plan.bn / P::kPair, false, 1, false);
@@ -701,7 +736,7 @@ int group_of(int64_t K, int pair) {
   return static_cast<int>(g < 1 ? 1 : g);
 }
 
-// The tiles' partials take 12 bytes per row and tile; rows beyond 16384 go through the same workspace in further launches
+// The tiles' partials take 24 bytes per row and tile; rows beyond 16384 go through the same workspace in further launches
 // (each reads the weight once more, 0.2 ms beside 14 ms of products at a hidden size of 4096).
 constexpr int64_t kScoreRows = 16384;
 struct ScoresLayout { Plan plan; size_t part, arg, picked, nll, total; };
@@ -709,7 +744,7 @@ ScoresLayout scores_layout(int64_t rows, int32_t vocab) {
   ScoresLayout l;
   const int64_t n = rows < 1 ? 1 : rows < kScoreRows ? rows : kScoreRows;
   l.plan = plan_tiles(n, vocab, pair_of(n), 16 * pair_of(n));
-  const size_t parts = static_cast<size_t>(n) * l.plan.n_tiles;
+  const size_t parts = static_cast<size_t>(n) * l.plan.n_tiles * 2;
   l.part = 0;
   l.arg = up256(parts * sizeof(float2));
   l.picked = l.arg + up256(parts * sizeof(int));
@@ -786,7 +821,7 @@ int launch_scores(const jl_head_scores_args* a, cudaStream_t stream) {
     if (rc != JL_OK) return rc;
     const bool few = n < 4 * kSms;
     if (launch_dependent(few ? scores_fold_kernel<8> : scores_fold_kernel<1>, dim3(static_cast<unsigned>(few ? n : cdiv(n, 8))), dim3(256), 0, stream,
-                         static_cast<const float2*>(p.part), static_cast<const int*>(p.part_arg), static_cast<const float*>(p.picked), plan.n_tiles, n,
+                         static_cast<const float2*>(p.part), static_cast<const int*>(p.part_arg), static_cast<const float*>(p.picked), plan.n_tiles * 2, n,
                          static_cast<int64_t>(a->vocab), p.labels, a->ignore_index, nll != nullptr ? nll + r0 : nullptr,
                          a->lse != nullptr ? a->lse + r0 : nullptr, a->top != nullptr ? a->top + r0 : nullptr) != cudaSuccess)
       return check_launch("jl_head_scores (fold)");
