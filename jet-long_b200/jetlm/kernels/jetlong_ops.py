@@ -79,9 +79,11 @@ def register_peer_exchange(exchange) -> None:
 
 def kernel_status() -> dict:
     """What the kernels' bounded waits reported since the last call (synchronises the current device; reading a
-    raised prefill status clears it): {"prefill_wait_timeouts": 0 / 1, "peer_exchange_failed": bool}."""
+    raised kernel status clears it): {"prefill_wait_timeouts": 0 / 1, "peer_exchange_failed": bool,
+    "tree_wait_timeouts": 0 / 1, "head_wait_timeouts": 0 / 1}."""
     failed = any(bool(ex.status.item()) for ex in list(_PEER_EXCHANGES))
-    return dict(prefill_wait_timeouts=int(N.lib().jl_prefill_status()), peer_exchange_failed=failed)
+    return dict(prefill_wait_timeouts=int(N.lib().jl_prefill_status()), peer_exchange_failed=failed,
+                tree_wait_timeouts=int(N.lib().jl_tree_status()), head_wait_timeouts=int(N.lib().jl_head_status()))
 
 
 def clear_peer_status() -> None:
@@ -91,10 +93,10 @@ def clear_peer_status() -> None:
 
 
 def check_status() -> None:
-    """Raise if a bounded wait inside jl_prefill or jl_peer_merge gave up: the results produced since the
-    last check are then invalid.  Call at a point that synchronises anyway (end of a step, before logits leave)."""
+    """Raise if a bounded wait inside jl_prefill, jl_tree_attention, the head kernels or jl_peer_merge gave up: the results
+    produced since the last check are then invalid.  Call at a point that synchronises anyway (end of a step, before logits leave)."""
     st = kernel_status()
-    if st["prefill_wait_timeouts"] or st["peer_exchange_failed"]:
+    if any(st.values()):
         raise RuntimeError(f"a bounded wait inside the attention kernels gave up ({st}); results since the last "
                            f"check are invalid")
 

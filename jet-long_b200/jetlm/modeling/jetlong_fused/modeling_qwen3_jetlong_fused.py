@@ -62,6 +62,15 @@ class BifocalPlan:
     replicated: bool = False     # sharded cache, but every rank runs all tokens of this call (decode)
     step: object = None          # ops.StepState: positions and cache rows come from device memory (graph replay)
     pads: Optional[list] = None  # left-padded batch: number of leading pad rows of every sample's cache
+    tree: object = None          # TreeStep: the call's tokens are a drafted tree behind the cache
+
+
+@dataclass
+class TreeStep:
+    """A tree of drafted tokens behind the committed rows of a BifocalKVCache (one sample)."""
+    tree: object                 # draft_ops.DraftTree
+    lens: torch.Tensor           # (1,) int32, committed tokens, on the device
+    far_rows: Optional[int]      # rows whose regrouped keys have to be formed for this call; None: the cache keeps them
 
 
 class Qwen3JetLongFusedRotaryEmbedding(Qwen3RotaryEmbedding):
@@ -197,6 +206,9 @@ class Qwen3JetLongFusedAttention(nn.Module):
                                                      exchange_slot=(self.layer_idx, self.config.num_hidden_layers))
             return self.o_proj(attn.reshape(*out_shape, -1)), None
 
+        if plan.tree is not None:
+            return self._drafted_tree(q, k, v, plan, group, inv_freq, past_key_values, out_shape, ops)
+
         if plan.token_shard is not None:
             return self._token_sharded(q, k, v, plan, group, inv_freq, past_key_values, out_shape, backend, ops)
 
@@ -261,6 +273,23 @@ class Qwen3JetLongFusedAttention(nn.Module):
             attn = backend.fused_jetlong_decode_cache(
                 q_base, q_group, k_all.transpose(1, 2), v_all.transpose(1, 2), boundary=boundary, inv_freq=inv_freq,
                 group_size=group, softmax_scale=self.scaling, has_any_pad=plan.has_any_pad, training=self.training)
+        return self.o_proj(attn.reshape(*out_shape, -1)), None
+
+    def _drafted_tree(self, q, k, v, plan, group, inv_freq, cache, out_shape, ops):
+        """The tokens of the call are a tree of drafts (TreeStep): their keys and values go into the cache rows behind the
+        committed ones without being committed, every node attends the committed rows and its own path."""
+        from jetlm.kernels import draft_ops
+        st, slot = plan.tree, cache.layers[self.layer_idx]
+        kg = None
+        if group > 1:
+            kg = slot.group_keys if st.far_rows is None else cache.group_scratch(slot.capacity)
+            if st.far_rows:
+                ops.rope_regroup(slot.keys[:, : st.far_rows], inv_freq, group_size=group, out=kg[:, : st.far_rows])
+        q_base, q_group = draft_ops.tree_append(q, k, v, self.q_norm.weight, self.k_norm.weight, inv_freq, slot.keys, slot.values,
+                                                st.tree, st.lens, q_eps=self.q_norm.variance_epsilon,
+                                                k_eps=self.k_norm.variance_epsilon, group_size=group, key_group_rows=kg)
+        attn = draft_ops.tree_attention(q_base, q_group, slot.keys, slot.values, st.tree, st.lens, w_0=self.jetlong_w_0,
+                                        key_group_rows=kg, softmax_scale=self.scaling, return_lse=False)
         return self.o_proj(attn.reshape(*out_shape, -1)), None
 
     def _extended_left_padded(self, q, k, v, plan, group, inv_freq, past_key_values, slot, seen, out_shape, backend, ops):
@@ -511,6 +540,18 @@ class Qwen3JetLongFusedModel(Qwen3PreTrainedModel):
                            position_ids=None, past_key_values=cache, use_cache=True)
         return self.norm(hidden)
 
+    def tree_step(self, tokens, cache, step: TreeStep, group: int):
+        """Final hidden states (1, T, hidden) of a tree of drafted tokens (1, T) behind the committed rows of `cache`
+        (a BifocalKVCache), with group size `group`.  Writes the nodes' rows, commits nothing."""
+        inv_freq = self.rotary_emb.inv_freq.to(device=tokens.device, dtype=torch.float32)
+        plan = BifocalPlan(int(group), -1, -1, False, tree=step)
+        position_embeddings = (None, None, int(group), inv_freq, None, plan)
+        hidden = self.embed_tokens(tokens)
+        for layer in self.layers[: self.config.num_hidden_layers]:
+            hidden = layer(hidden, attention_mask=None, position_embeddings=position_embeddings,
+                           position_ids=None, past_key_values=cache, use_cache=True)
+        return self.norm(hidden)
+
     def _forward_token_sharded(self, input_ids, past_key_values, use_cache, shard, **kwargs) -> BaseModelOutputWithPast:
         """Sequence-parallel forward; `input_ids` is the whole (B, S) call on every rank.
         S a multiple of world * block (a prefill chunk): this rank embeds, projects and stores only its
@@ -552,6 +593,9 @@ class Qwen3JetLongFusedForCausalLM(Qwen3PreTrainedModel, GenerationMixin):
     _tied_weights_keys = {"lm_head.weight": "model.embed_tokens.weight"}
     _tp_plan = {"lm_head": "colwise_gather_output"}
     _pp_plan = {"lm_head": (["hidden_states"], ["logits"])}
+    # True: forward(labels=...) takes the loss straight from the hidden states and the lm_head weight (head_ops), without
+    # forming the logits, and returns logits=None.  Needs bf16 on a B200.
+    fused_loss = False
 
     def __init__(self, config):
         super().__init__(config)
@@ -588,6 +632,10 @@ class Qwen3JetLongFusedForCausalLM(Qwen3PreTrainedModel, GenerationMixin):
             cache_position=cache_position, **kwargs)
         hidden = outputs.last_hidden_state
         keep = slice(-logits_to_keep, None) if isinstance(logits_to_keep, int) else logits_to_keep
+        if labels is not None and self.fused_loss:
+            return CausalLMOutputWithPast(loss=self._fused_loss(hidden[:, keep, :], labels, **kwargs), logits=None,
+                                          past_key_values=outputs.past_key_values, hidden_states=outputs.hidden_states,
+                                          attentions=outputs.attentions)
         logits = self.lm_head(hidden[:, keep, :])
         loss = None
         if labels is not None:
@@ -595,6 +643,116 @@ class Qwen3JetLongFusedForCausalLM(Qwen3PreTrainedModel, GenerationMixin):
         return CausalLMOutputWithPast(loss=loss, logits=logits, past_key_values=outputs.past_key_values,
                                       hidden_states=outputs.hidden_states, attentions=outputs.attentions)
 
+
+    def _fused_loss(self, hidden, labels, num_items_in_batch=None, ignore_index: int = -100, shift_labels=None, **kwargs):
+        """transformers' causal-LM loss (labels shifted by one, mean over the counted ones or sum / num_items_in_batch)."""
+        from jetlm.kernels import head_ops
+        if shift_labels is None:
+            shift_labels = nn.functional.pad(labels, (0, 1), value=ignore_index)[..., 1:]
+        loss = head_ops.linear_cross_entropy(hidden, self.lm_head.weight, shift_labels.to(hidden.device), ignore_index=ignore_index,
+                                             reduction="mean" if num_items_in_batch is None else "sum")
+        return loss if num_items_in_batch is None else loss / num_items_in_batch
+
+    @torch.no_grad()
+    def score_tokens(self, input_ids, chunk_tokens: int = 32768, past_key_values=None):
+        """Negative log-likelihood (B, S - 1) in fp32 of every token given the ones before it: chunked prefill into a
+        preallocated BifocalKVCache, losses straight from the hidden states — no logits of the prompt are formed (39.8 GB at
+        131072 tokens).  G is recomputed per call, as in generate_long."""
+        from jetlm.kernels import cute_jetlong_backend as backend
+        from jetlm.kernels import head_ops
+        from jetlm.kernels.kv_cache import BifocalKVCache
+        if getattr(self.model, "token_sharded", False) and backend.sequence_shard() is not None:
+            raise RuntimeError("score_tokens runs on one GPU: turn token sharding off")
+        bsz, n = input_ids.shape
+        if past_key_values is None:
+            past_key_values = BifocalKVCache(self.config, n, batch=bsz, device=input_ids.device, dtype=self.lm_head.weight.dtype)
+        out = torch.empty(bsz, max(n - 1, 0), dtype=torch.float32, device=input_ids.device)
+        for lo in range(0, n - 1, chunk_tokens):
+            hi = min(lo + chunk_tokens, n - 1)                    # the last token predicts nothing
+            hidden = self.model(input_ids=input_ids[:, lo:hi], past_key_values=past_key_values, use_cache=True).last_hidden_state
+            out[:, lo:hi] = head_ops.token_scores(hidden, self.lm_head.weight, input_ids[:, lo + 1: hi + 1]).nll
+        return out
+
+    @torch.no_grad()
+    def generate_drafted(self, input_ids, max_new_tokens: int, draft, chunk_tokens: int = 32768, past_key_values=None):
+        """Greedy continuation of one long prompt in which every step verifies a TREE of drafted tokens in one pass over the
+        cache (draft_ops) and keeps the path that greedy decoding takes.
+
+        draft(ids): called with the list of all tokens so far, returns (tokens, parents), two lists of up to 255 drafted
+        tokens and the index of each one's parent among them, -1 for a continuation of `ids` (parents before children; empty
+        lists: plain decoding).  The result does not depend on what is drafted, up to the rounding of differently shaped
+        products; only the number of steps does.  Drafts deeper than the current group size reaches are left for the next step.
+        Returns (1, max_new_tokens) token ids; self.drafted_steps holds the number of steps taken."""
+        from jetlm.kernels import cute_jetlong_backend as backend
+        from jetlm.kernels import draft_ops, head_ops
+        from jetlm.kernels import jetlong_ops as ops
+        from jetlm.kernels.kv_cache import BifocalKVCache
+        if getattr(self.model, "token_sharded", False) and backend.sequence_shard() is not None:
+            raise RuntimeError("generate_drafted runs on one GPU: turn token sharding off")
+        if input_ids.shape[0] != 1:
+            raise ValueError("generate_drafted takes one prompt at a time")
+        dev, n_prompt = input_ids.device, input_ids.shape[1]
+        cache = past_key_values
+        if cache is None:
+            cache = BifocalKVCache(self.config, n_prompt + max_new_tokens + 256, batch=1, device=dev, dtype=self.lm_head.weight.dtype,
+                                   regrouped_far_keys=True)
+        w, w_0 = self.model.rotary_emb.jetlong_w, self.model.rotary_emb.jetlong_w_0
+        hidden = None
+        for lo in range(0, n_prompt, chunk_tokens):
+            hidden = self.model(input_ids=input_ids[:, lo: lo + chunk_tokens], past_key_values=cache, use_cache=True).last_hidden_state
+        weight = self.lm_head.weight
+        out = [int(head_ops.token_scores(hidden[:, -1], weight, top=True).top)]
+        ids, inv_freq, regrouped, steps = input_ids[0].tolist(), self.model.rotary_emb.inv_freq, None, 0
+        while len(out) < max_new_tokens:
+            seen = cache.get_seq_length()
+            group = max(1, math.ceil((seen + 1) / w))
+            # node 0 is the last token, whose key is not in the cache yet; the drafts hang below it
+            drafted, links = draft(ids + out)
+            tokens, parents, depth, place = [out[-1]], [-1], [0], []
+            deepest = min(group * w - seen, max_new_tokens - len(out)) - 1
+            room = min(256, cache.layers[0].capacity - seen)
+            if room < 1:
+                raise RuntimeError(f"KV cache capacity exceeded: {seen + 1} rows > {cache.layers[0].capacity}")
+            for i, (tok, up) in enumerate(zip(drafted, links)):
+                if not -1 <= up < i:
+                    raise ValueError(f"draft: the parent of token {i} must be -1 or an earlier token, got {up}")
+                at = 0 if up < 0 else place[up]
+                if at is None or depth[at] + 1 > deepest or len(tokens) >= room:
+                    place.append(None)
+                    continue
+                place.append(len(tokens))
+                tokens.append(int(tok))
+                parents.append(at)
+                depth.append(depth[at] + 1)
+            far_rows = None
+            if group > 1 and cache.layers[0].group_keys is None:
+                far_rows = max(0, min(seen, seen + max(depth) - w_0))
+            elif group > 1 and regrouped != group:               # rows appended from here on carry their own regrouped copies
+                for layer in cache.layers:
+                    ops.rope_regroup(layer.keys[:, :seen], inv_freq, group_size=group, out=layer.group_keys[:, :seen])
+                regrouped = group
+            step = TreeStep(draft_ops.draft_tree(torch.tensor([parents], dtype=torch.int32, device=dev)),
+                            torch.tensor([seen], dtype=torch.int32, device=dev), far_rows)
+            hidden = self.model.tree_step(torch.tensor([tokens], dtype=torch.long, device=dev), cache, step, group)
+            best = head_ops.token_scores(hidden[0], weight, top=True).top.tolist()
+            steps += 1
+            path = [0]
+            while True:
+                out.append(best[path[-1]])
+                nxt = next((i for i in range(path[-1] + 1, len(tokens)) if parents[i] == path[-1] and tokens[i] == out[-1]), None)
+                if nxt is None or len(out) >= max_new_tokens:
+                    break
+                path.append(nxt)
+            if path != list(range(len(path))):
+                rows = torch.tensor(path, dtype=torch.long, device=dev)
+                for layer in cache.layers:
+                    for buf in (layer.keys, layer.values, layer.group_keys):
+                        if buf is not None:
+                            draft_ops.keep_path(buf, rows, seen)
+            for layer in cache.layers:
+                layer.commit(len(path))
+        self.drafted_steps = steps
+        return torch.tensor([out[:max_new_tokens]], dtype=torch.long, device=dev)
 
     @torch.no_grad()
     def generate_long(self, input_ids, max_new_tokens: int, chunk_tokens: int = 32768, past_key_values=None,
