@@ -1,6 +1,6 @@
 // A tree of drafted tokens on the bifocal cache: ancestor masks from parent links, the fused "norm -> RoPE -> cache
 // write" of the drafted nodes, and the C entry points of the three tree operators.
-#include "jl_common.cuh"
+#include "tc_common.cuh"
 #include "../../include/jetlong_b200_tree.h"
 
 namespace jl {
@@ -13,6 +13,8 @@ __global__ void __launch_bounds__(JL_TREE_MAX_NODES) tree_plan_kernel(const int3
   __shared__ int par[JL_TREE_MAX_NODES];
   const int b = blockIdx.x, t = threadIdx.x;
   const int64_t base = static_cast<int64_t>(b) * nodes;
+  tc::launch_dependents();
+  tc::wait_prerequisites();
   if (t < nodes) par[t] = parents[base + t];
   __syncthreads();
   if (t >= nodes) return;
@@ -49,6 +51,8 @@ struct AppendParams {
 
 // One warp per (node, head) row of 128 values: query heads, then key heads, then value heads of the node.
 __global__ void __launch_bounds__(128) tree_append_kernel(const AppendParams p) {
+  tc::launch_dependents();
+  tc::wait_prerequisites();
   const int lane = threadIdx.x & 31;
   const int per_node = p.heads + 2 * p.kv_heads;
   const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
@@ -115,8 +119,9 @@ int launch_tree_plan(const jl_tree_plan_args* a, cudaStream_t stream) {
   if (a->batch == 0) return JL_OK;
   const int rc = check_device_arch();
   if (rc != JL_OK) return rc;
-  tree_plan_kernel<<<a->batch, (a->nodes + 31) / 32 * 32, 0, stream>>>(a->parents, a->depth, a->mask, a->nodes);
-  return check_launch("jl_tree_plan");
+  if (launch_dependent(tree_plan_kernel, dim3(a->batch), dim3((a->nodes + 31) / 32 * 32), 0, stream, a->parents, a->depth, a->mask, a->nodes) != cudaSuccess)
+    return check_launch("jl_tree_plan");
+  return JL_OK;
 }
 
 int launch_tree_append(const jl_tree_append_args* a, cudaStream_t stream) {
@@ -161,8 +166,8 @@ int launch_tree_append(const jl_tree_append_args* a, cudaStream_t stream) {
   p.inv_freq = a->inv_freq; p.lens = a->lens; p.depth = a->depth;
   const int64_t blocks = (static_cast<int64_t>(a->batch) * a->nodes * (a->heads + 2 * a->kv_heads) + 3) / 4;
   if (blocks > 0x7fffffff) return fail(JL_ERR_UNSUPPORTED, "jl_tree_append: too many rows for one launch");
-  tree_append_kernel<<<static_cast<unsigned>(blocks), 128, 0, stream>>>(p);
-  return check_launch("jl_tree_append");
+  if (launch_dependent(tree_append_kernel, dim3(static_cast<unsigned>(blocks)), dim3(128), 0, stream, p) != cudaSuccess) return check_launch("jl_tree_append");
+  return JL_OK;
 }
 
 }  // namespace

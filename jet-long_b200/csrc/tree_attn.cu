@@ -143,6 +143,24 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
   }
   const int q_slots = p.two_tiles ? 1 : 2;
 
+  if (threadIdx.x == 32) {
+    sm.failed = *reinterpret_cast<volatile int*>(&g_tree_status) != 0 ? 1 : 0;
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sm.q_full[i], 1);
+      mbar_init(&sm.q_free[i], 1);
+      mbar_init(&sm.s_full[i], 1);
+      mbar_init(&sm.p_half[i][0], 128);
+      mbar_init(&sm.p_half[i][1], 128);
+    }
+    for (int i = 0; i < kStages; ++i) { mbar_init(&sm.full[i], 1); mbar_init(&sm.empty[i], 1); }
+    for (int i = 0; i < 2; ++i) mbar_init(&sm.pv_done[i], 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 2) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem_base)), "r"(512u));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+  }
+  wait_prerequisites();                          // nothing before this reads what an earlier kernel wrote
   if (warp == 0) {
     // ---- this CTA's part of the line of visits: total and start, 32 samples at a time ----
     int64_t total = 0;
@@ -171,23 +189,6 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
       base += __shfl_sync(0xffffffffu, before, 31);
     }
     if (lane == 0) { sm.lo = lo; sm.hi = hi; }
-  }
-  if (threadIdx.x == 32) {
-    sm.failed = *reinterpret_cast<volatile int*>(&g_tree_status) != 0 ? 1 : 0;
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&sm.q_full[i], 1);
-      mbar_init(&sm.q_free[i], 1);
-      mbar_init(&sm.s_full[i], 1);
-      mbar_init(&sm.p_half[i][0], 128);
-      mbar_init(&sm.p_half[i][1], 128);
-    }
-    for (int i = 0; i < kStages; ++i) { mbar_init(&sm.full[i], 1); mbar_init(&sm.empty[i], 1); }
-    for (int i = 0; i < 2; ++i) mbar_init(&sm.pv_done[i], 1);
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
-  if (warp == 2) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem_base)), "r"(512u));
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
   }
   tc_fence_before();
   __syncthreads();
@@ -302,13 +303,15 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                                        *reinterpret_cast<volatile int*>(&sm.visit[g % kVisitRing].z), 0);
           if (__any_sync(0xffffffffu, visit.x & kTail)) {
             // value rows that belong to no node may hold anything, and 0 * NaN is NaN
+#pragma unroll 1
             for (int r0 = 0; r0 < kTileN; r0 += 32) {
               const int u = visit.z + r0 + lane;
               const bool keep = u < 0 || (u < p.nodes && p.depth[static_cast<int64_t>(visit.y) * p.nodes + u] >= 0);
-              for (uint32_t dead = __ballot_sync(0xffffffffu, !keep); dead != 0u; dead &= dead - 1)
-                if (lane < 16)
-                  *reinterpret_cast<uint4*>(sm.kv[pos.slot] + (lane >> 3) * kHalfBytes + (r0 + __ffs(dead) - 1) * 128 + (lane & 7) * 16) =
-                      make_uint4(0u, 0u, 0u, 0u);
+              const uint32_t dead = __ballot_sync(0xffffffffu, !keep);
+              if (dead == 0u) continue;
+              uint8_t* const base = sm.kv[pos.slot] + ((lane >> 3) & 1) * kHalfBytes + (lane & 7) * 16;      // 16 lanes a row, two rows at a time
+              for (int r = lane >> 4; r < 32; r += 2)
+                if ((dead >> r) & 1u) *reinterpret_cast<uint4*>(base + (r0 + r) * 128) = make_uint4(0u, 0u, 0u, 0u);
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
@@ -692,9 +695,8 @@ int launch_tree_attention(const jl_tree_attention_args* a, cudaStream_t stream) 
   const int row_tiles = (a->nodes + l.npt - 1) / l.npt;
   if (static_cast<int64_t>(a->batch) * a->kv_heads > 65535)
     return fail(JL_ERR_UNSUPPORTED, "jl_tree_attention: batch * kv_heads must be at most 65535");
-  tree_attention_kernel<<<p.mbs * p.workers, kThreads, kSmemBytes, stream>>>(maps, p);
-  rc = check_launch("jl_tree_attention");
-  if (rc != JL_OK) return rc;
+  if (launch_dependent(tree_attention_kernel, dim3(p.mbs * p.workers), dim3(kThreads), kSmemBytes, stream, maps, p) != cudaSuccess)
+    return check_launch("jl_tree_attention");
   if (launch_dependent(tree_combine_kernel, dim3((32 * l.rpt + 127) / 128, row_tiles, a->batch * a->kv_heads), dim3(128), 0, stream, p) != cudaSuccess)
     return check_launch("jl_tree_attention (combine)");
   return JL_OK;

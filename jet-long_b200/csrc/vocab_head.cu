@@ -440,6 +440,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) head_gemm_kernel(const __grid
   if (kPair == 2) pair::cluster_sync();
   tc_fence_after();
   launch_dependents();
+  wait_prerequisites();                          // nothing before this reads what an earlier kernel wrote
   const uint32_t tmem = sm.tmem_base;
 
   PipeState st{0, 0, 0u};
@@ -559,6 +560,7 @@ __global__ void __launch_bounds__(1024) loss_sum_kernel(const float* nll, const 
 // d_hidden = scale * (sum of the K splits' fp32 results), rounded once; 4 values a thread
 __global__ void __launch_bounds__(256) grad_round_kernel(const float* x, int splits, int64_t n, __nv_bfloat16* out, GradScale g) {
   const int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 4;
+  wait_prerequisites();
   if (i >= n) return;
   float4 a = *reinterpret_cast<const float4*>(x + i);
   for (int s = 1; s < splits; ++s) {
@@ -692,12 +694,14 @@ int launch(const Gemm& g0, const Gemm& g1, cudaStream_t stream) {
   cfg.blockDim = dim3(kGemmThreads);
   cfg.dynamicSmemBytes = kGemmSmemBytes;
   cfg.stream = stream;
-  cudaLaunchAttribute at[1];
+  cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim.x = kPair;
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   if (cudaLaunchKernelEx(&cfg, kernel, g0.maps, g0.p, g1.maps, g1.p) != cudaSuccess) return check_launch("jl_head");
   return JL_OK;
 }
@@ -902,9 +906,11 @@ int launch_grads(const jl_head_grads_args* a, cudaStream_t stream) {
     }
     if (rc != JL_OK) return rc;
   }
-  if (a->d_hidden != nullptr)
-    grad_round_kernel<<<static_cast<unsigned>(cdiv(N * H, 1024)), 256, 0, stream>>>(dh32, splits, N * H, static_cast<__nv_bfloat16*>(a->d_hidden), base.scale);
-  return check_launch("jl_head_grads");
+  if (a->d_hidden != nullptr &&
+      launch_dependent(grad_round_kernel, dim3(static_cast<unsigned>(cdiv(N * H, 1024))), dim3(256), 0, stream, static_cast<const float*>(dh32), splits, N * H,
+                       static_cast<__nv_bfloat16*>(a->d_hidden), base.scale) != cudaSuccess)
+    return check_launch("jl_head_grads (rounding)");
+  return JL_OK;
 }
 
 }  // namespace
