@@ -270,6 +270,9 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
           const uint64_t kd = k_desc + static_cast<uint64_t>((pos.slot * kTileBytes) >> 4);
           for (int i = 0; i < tiles; ++i) {
             const int t = p.two_tiles ? i : g & 1;
+            // The second tile starts when the first one's probabilities are out: half a visit apart, one tile's softmax runs under the
+            // other's products, and they stay apart (64 nodes over 131072 keys: 142 -> 137 us).
+            if (p.two_tiles && g == 0 && i == 1) mbar_wait(&sm.p_half[0][1], 0u, sm);
             // the scores go where the probabilities of the state's previous item are: P V has to be done with them
             if (g >= (p.two_tiles ? 1 : 2)) {
               mbar_wait(&sm.pv_done[t], (parity >> t) & 1u, sm);
@@ -450,7 +453,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
         };
         uint64_t acc2[4] = {0ull, 0ull, 0ull, 0ull};
         if (uniform && p.unrolled) {
-          // all 128 scores in registers: half the loads, and the halves of P published 1300 clocks earlier than by the loop below
+          // all 128 scores in registers: half the loads, and P published 1300 clocks earlier than by the loop below
           uint32_t s[128];
           float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
           JL_TMEM_LD32(t_s + 0, s, 0);
@@ -664,8 +667,9 @@ int launch_tree_attention(const jl_tree_attention_args* a, cudaStream_t stream) 
   p.two_classes = a->q_group != nullptr;
   p.w_0 = a->w_0 < (int64_t(1) << 32) ? a->w_0 : (int64_t(1) << 32);           // no cache reaches further
   p.nodes_far = p.two_classes && p.w_0 < a->nodes - 1;
-  // Two row tiles keep the softmax threads busy, and the unrolled form saves 1300 clocks a visit; its instructions, cold, cost 8 us.
-  p.unrolled = l.two_tiles && static_cast<int64_t>(a->batch) * a->kv_heads * (a->rows / kTileN) >= 16ll * l.workers;
+  // The unrolled softmax saves 1300 clocks a visit, and its instructions, cold, cost 8 us once: 16 nodes over 131072 keys 106.5 us
+  // rolled and 102.8 unrolled, 64 nodes 171 and 142; the two are equal at 8 visits a part.
+  p.unrolled = static_cast<int64_t>(a->batch) * a->kv_heads * (a->rows / kTileN) >= 16ll * l.workers;
   p.scale_log2 = a->softmax_scale * kLog2e;
   p.lens = a->lens; p.depth = a->depth; p.mask = a->mask;
   p.part_o = static_cast<float*>(a->workspace);
