@@ -131,6 +131,7 @@ def tree_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_weight: tor
     key_group_rows (shape and strides of key_rows) receives the regrouped keys.  Absent nodes get zero queries and write
     nothing.  Returns (q_base, q_group), each (B,T,H,D); q_group is q_base when group_size == 1."""
     op = "tree_append"
+    q_eps, k_eps, group_size = float(q_eps), float(k_eps), int(group_size)
     key = (op, _sig(q), _sig(k), _sig(v), _sig(q_weight), _sig(k_weight), _sig(inv_freq), _sig(key_rows), _sig(value_rows),
            _sig(key_group_rows), _sig(tree.depth), _sig(tree.mask), _sig(lens), q_eps, k_eps, group_size)
     template = _LAYOUTS.get(key)
@@ -198,6 +199,7 @@ def tree_attention(q_base: torch.Tensor, q_group: torch.Tensor, key_rows: torch.
     (group size 1) every pair is scored q_base . key_rows.  Nothing depends on lens on the host, so the launches can sit
     in a CUDA graph.  Returns (out (B,T,H,D), lse (B,H,T) fp32) or out; a row that sees no key is zero with lse -inf."""
     op = "tree_attention"
+    w_0, softmax_scale = int(w_0), None if softmax_scale is None else float(softmax_scale)
     key = (op, _sig(q_base), _sig(q_group), _sig(key_rows), _sig(value_rows), _sig(key_group_rows), _sig(tree.depth), _sig(tree.mask),
            _sig(lens), _sig(out), w_0, softmax_scale)
     plan = _LAYOUTS.get(key)

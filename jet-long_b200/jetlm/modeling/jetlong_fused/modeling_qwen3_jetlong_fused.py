@@ -716,6 +716,8 @@ class Qwen3JetLongFusedForCausalLM(Qwen3PreTrainedModel, GenerationMixin):
             for i, (tok, up) in enumerate(zip(drafted, links)):
                 if not -1 <= up < i:
                     raise ValueError(f"draft: the parent of token {i} must be -1 or an earlier token, got {up}")
+                if not 0 <= tok < self.vocab_size:
+                    raise ValueError(f"draft: token {i} must be in [0, {self.vocab_size}), got {tok}")
                 at = 0 if up < 0 else place[up]
                 if at is None or depth[at] + 1 > deepest or len(tokens) >= room:
                     place.append(None)

@@ -121,6 +121,9 @@ CASES = [
     (1, 256, 8, 1, [300], 0, 30, True, "chain"),           # 2048 query rows on one key head
     (5, 3, 14, 2, [1, 2, 64, 65, 2000], 0, 31, True, "absent"),
     (1, 9, 64, 8, [4099], 0, 2048, True, "tree"),
+    (1, 3, 128, 1, [200], 3, 64, True, "tree"),            # one node a row tile
+    (2, 40, 10, 2, [150, 300], 0, 90, True, "absent"),     # 25 nodes a row tile, three rows unused
+    (40, 2, 8, 8, list(range(0, 400, 10)), 0, 20, True, "tree"),   # more (sample, head) pairs than parts
 ]
 
 

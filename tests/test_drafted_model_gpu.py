@@ -86,6 +86,8 @@ def test_drafted_generation_inside_the_window_and_refusals(golden):
         model.generate_drafted(ids.repeat(2, 1), 4, lambda i: ([], []))
     with pytest.raises(ValueError, match="parent"):
         model.generate_drafted(ids, 4, lambda i: ([1, 2], [1, -1]))
+    with pytest.raises(ValueError, match="token 1 must be in"):
+        model.generate_drafted(ids, 4, lambda i: ([1, 128], [-1, 0]))
     small = BifocalKVCache(model.config, 32, device="cuda", dtype=torch.bfloat16)          # whole blocks of 128 rows
     with pytest.raises(RuntimeError, match="capacity"):
         model.generate_drafted(ids, 120, lambda i: ([], []), past_key_values=small)
