@@ -451,8 +451,40 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
           tc_fence_before();
           mbar_arrive(&sm.p_half[t][half]);
         };
+        if (!uniform) {
+          // what the row does not see in this class becomes -inf, in place
+#pragma unroll 1
+          for (int ch = 0; ch < 4; ++ch) {
+            const int a = max(c_lo - ch * 32, 0), z = min(c_hi - ch * 32, 32);
+            uint32_t keep = z > a ? (0xffffffffu >> (32 - (z - a))) << a : 0u;
+            const int u0 = tp0 + ch * 32 - len;        // first node of these columns (negative: columns before the nodes)
+            if (d >= 0 && u0 > -32 && u0 < p.nodes && (!far || p.nodes_far)) {
+              const uint32_t* words = reinterpret_cast<const uint32_t*>(p.mask + nrow * p.words);
+              const int i0 = u0 >> 5, sh = u0 & 31;
+              const uint32_t w0 = i0 >= 0 ? __ldg(words + i0) : 0u, w1 = i0 + 1 < 2 * p.words ? __ldg(words + i0 + 1) : 0u;
+              uint32_t bits = __funnelshift_r(w0, w1, sh);
+              const int left = p.nodes - u0;
+              if (left < 32) bits &= 0xffffffffu >> (32 - left);
+              if (p.nodes_far) {
+                for (uint32_t todo = bits; todo != 0u; todo &= todo - 1) {
+                  const int j = __ffs(todo) - 1;
+                  if ((d - p.depth[static_cast<int64_t>(seg.b) * p.nodes + u0 + j] > p.w_0) != far) bits &= ~(1u << j);
+                }
+              }
+              keep |= bits;
+            }
+            uint32_t s[32];
+            JL_TMEM_LD32(t_s + ch * 32, s, 0);
+            JL_TMEM_WAIT_LD32(s, 0);
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (!((keep >> i) & 1u)) s[i] = 0xff800000u;
+            JL_TMEM_ST32(t_s + ch * 32, s, 0);
+          }
+          tmem_wait_st();
+        }
         uint64_t acc2[4] = {0ull, 0ull, 0ull, 0ull};
-        if (uniform && p.unrolled) {
+        if (p.unrolled) {
           // all 128 scores in registers: half the loads, and P published 1300 clocks earlier than by the loop below
           uint32_t s[128];
           float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -489,29 +521,6 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
           uint32_t s[32];
           JL_TMEM_LD32(t_s + ch * 32, s, 0);
           JL_TMEM_WAIT_LD32(s, 0);
-          if (!uniform) {
-            const int a = max(c_lo - ch * 32, 0), z = min(c_hi - ch * 32, 32);
-            uint32_t keep = z > a ? (0xffffffffu >> (32 - (z - a))) << a : 0u;
-            const int u0 = tp0 + ch * 32 - len;        // first node of these columns (negative: columns before the nodes)
-            if (d >= 0 && u0 > -32 && u0 < p.nodes && (!far || p.nodes_far)) {
-              const uint32_t* words = reinterpret_cast<const uint32_t*>(p.mask + nrow * p.words);
-              const int i0 = u0 >> 5, sh = u0 & 31;
-              const uint32_t w0 = i0 >= 0 ? __ldg(words + i0) : 0u, w1 = i0 + 1 < 2 * p.words ? __ldg(words + i0 + 1) : 0u;
-              uint32_t bits = __funnelshift_r(w0, w1, sh);
-              const int left = p.nodes - u0;
-              if (left < 32) bits &= 0xffffffffu >> (32 - left);
-              if (p.nodes_far) {
-                for (uint32_t todo = bits; todo != 0u; todo &= todo - 1) {
-                  const int j = __ffs(todo) - 1;
-                  if ((d - p.depth[static_cast<int64_t>(seg.b) * p.nodes + u0 + j] > p.w_0) != far) bits &= ~(1u << j);
-                }
-              }
-              keep |= bits;
-            }
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (!((keep >> i) & 1u)) s[i] = 0xff800000u;        // -inf
-          }
           if (step32 < 4) {
             float m2[2] = {mx, -INFINITY};
 #pragma unroll

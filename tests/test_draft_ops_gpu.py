@@ -124,6 +124,11 @@ CASES = [
     (1, 3, 128, 1, [200], 3, 64, True, "tree"),            # one node a row tile
     (2, 40, 10, 2, [150, 300], 0, 90, True, "absent"),     # 25 nodes a row tile, three rows unused
     (40, 2, 8, 8, list(range(0, 400, 10)), 0, 20, True, "tree"),   # more (sample, head) pairs than parts
+    # caches so large that the walk counts as a long one, whatever they hold
+    (1, 12, 32, 8, [1030], 40000, 300, True, "absent"),
+    (1, 70, 32, 8, [700], 40000, 200, True, "forest"),
+    (2, 33, 16, 8, [0, 511], 20000, 5, True, "absent"),
+    (1, 64, 32, 8, [900], 40000, 64, False, "tree"),
 ]
 
 
