@@ -77,7 +77,8 @@ int jl_tree_append(const jl_tree_append_args* args, void* cuda_stream);
  * k_base.  q_group and k_group both NULL: one class, every pair is scored as q_base . k_base.
  * out (B, T, H, D) with strides, lse (B, H, T) fp32 contiguous or NULL.  A row that sees no key (an absent node of
  * an empty cache, a zero mask) is zero with lse = -inf; an absent node (depth < 0) sees nothing.
- * lens[b] is clamped to [0, rows - nodes]; no row past lens[b] + nodes is read into a result.  batch * kv_heads <= 65535.
+ * depth[b][t] < nodes.  A value row that an absent node would use may hold anything; the values of present nodes and of
+ * committed rows must be finite.  softmax_scale is positive and finite.  lens[b] is clamped to [0, rows - nodes]; no row past lens[b] + nodes is read into a result.  batch * kv_heads <= 65535.
  * workspace: jl_tree_attention_workspace_bytes, 16-byte aligned, not initialised by the caller and not kept between
  * calls; two calls that may overlap on the GPU need one each.
  * ------------------------------------------------------------------------------------------- */

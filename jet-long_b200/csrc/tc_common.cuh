@@ -209,6 +209,9 @@ __device__ __forceinline__ void commit_both(uint64_t* bar) {
 }  // namespace pair
 
 // Programmatic dependent launch: the kernel before lets its successor start early, the successor waits for its results.
+// Every kernel here lets its successor start only after its own wait.  So when a kernel starts, all kernels but the one before
+// it have ended, and it may read, ahead of its wait, what they wrote: the caller's tensors of a call whose earlier launch
+// has taken the wait.
 __device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_prerequisites() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 

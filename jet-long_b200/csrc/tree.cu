@@ -13,8 +13,8 @@ __global__ void __launch_bounds__(JL_TREE_MAX_NODES) tree_plan_kernel(const int3
   __shared__ int par[JL_TREE_MAX_NODES];
   const int b = blockIdx.x, t = threadIdx.x;
   const int64_t base = static_cast<int64_t>(b) * nodes;
-  tc::launch_dependents();
   tc::wait_prerequisites();
+  tc::launch_dependents();
   if (t < nodes) par[t] = parents[base + t];
   __syncthreads();
   if (t >= nodes) return;
@@ -51,8 +51,8 @@ struct AppendParams {
 
 // One warp per (node, head) row of 128 values: query heads, then key heads, then value heads of the node.
 __global__ void __launch_bounds__(128) tree_append_kernel(const AppendParams p) {
-  tc::launch_dependents();
   tc::wait_prerequisites();
+  tc::launch_dependents();
   const int lane = threadIdx.x & 31;
   const int per_node = p.heads + 2 * p.kv_heads;
   const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
@@ -144,6 +144,9 @@ int launch_tree_append(const jl_tree_append_args* a, cudaStream_t stream) {
                          reinterpret_cast<uintptr_t>(a->k_group_cache) | reinterpret_cast<uintptr_t>(a->q_weight) |
                          reinterpret_cast<uintptr_t>(a->k_weight);
   if (ptrs & 7) return fail(JL_ERR_BAD_ARG, "jl_tree_append: pointers must be 8-byte aligned");
+  const int64_t cache_size[] = {a->batch, a->cache_rows, a->kv_heads, a->batch, a->cache_rows, a->kv_heads};
+  for (int i = 0; i < 6; ++i)
+    if (cache_size[i] > 1 && st[9 + i] <= 0) return fail(JL_ERR_UNSUPPORTED, "jl_tree_append: a cache dimension larger than 1 needs a positive stride");
   if (a->batch == 0) return JL_OK;
   const int rc = check_device_arch();
   if (rc != JL_OK) return rc;
@@ -185,6 +188,8 @@ static int validate_tree_attention(const jl_tree_attention_args* a) {
   if (a->heads / a->kv_heads > 128) return fail(JL_ERR_UNSUPPORTED, "jl_tree_attention: at most 128 query heads per kv head");
   if (a->rows < a->nodes) return fail(JL_ERR_BAD_ARG, "jl_tree_attention: the cache (%d rows) does not hold the %d nodes", a->rows, a->nodes);
   if (a->w_0 < 0) return fail(JL_ERR_BAD_ARG, "jl_tree_attention: w_0 must be >= 0");
+  // the running maximum is taken of the unscaled scores
+  if (!(a->softmax_scale > 0.f) || isinf(a->softmax_scale)) return fail(JL_ERR_BAD_ARG, "jl_tree_attention: softmax_scale must be positive and finite");
   if ((a->q_group == nullptr) != (a->k_group == nullptr))
     return fail(JL_ERR_BAD_ARG, "jl_tree_attention: q_group and k_group come together or not at all");
   if (a->q_base == nullptr || a->k_base == nullptr || a->v == nullptr || a->out == nullptr || a->lens == nullptr || a->depth == nullptr ||

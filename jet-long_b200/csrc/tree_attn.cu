@@ -136,7 +136,6 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
   TreeSmem& sm = *reinterpret_cast<TreeSmem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int mb = static_cast<int>(blockIdx.x) % p.mbs, worker = static_cast<int>(blockIdx.x) / p.mbs;
-  launch_dependents();                           // the combine kernel may take its place and wait there for our end
   if (threadIdx.x >= 64 && threadIdx.x < 69) {   // the tensor maps: q[0], q[1], k[0], k[1], v
     const CUtensorMap* m = reinterpret_cast<const CUtensorMap*>(&maps) + (threadIdx.x - 64);
     asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
@@ -161,6 +160,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
   }
   wait_prerequisites();                          // nothing before this reads what an earlier kernel wrote
+  launch_dependents();                           // the combine kernel may take its place and wait there for our end
   if (warp == 0) {
     // ---- this CTA's part of the line of visits: total and start, 32 samples at a time ----
     int64_t total = 0;

@@ -439,8 +439,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) head_gemm_kernel(const __grid
   __syncthreads();
   if (kPair == 2) pair::cluster_sync();
   tc_fence_after();
-  launch_dependents();
   wait_prerequisites();                          // nothing before this reads what an earlier kernel wrote
+  launch_dependents();
   const uint32_t tmem = sm.tmem_base;
 
   PipeState st{0, 0, 0u};
@@ -496,8 +496,8 @@ __global__ void __launch_bounds__(256) scores_fold_kernel(const float2* part, co
   __shared__ int sa[8];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * (8 / kWarps) + warp / kWarps;
-  launch_dependents();
   wait_prerequisites();
+  launch_dependents();
   float m = -INFINITY, s = 0.f;
   int arg = 0x7fffffff;
   if (row < N) {

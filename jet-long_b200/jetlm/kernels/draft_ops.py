@@ -67,9 +67,14 @@ def _run(op: str, fn, args, index: int) -> None:
         N.check(op, status)
 
 
+def _no_broadcast(op: str, name: str, t: torch.Tensor) -> None:
+    if any(t.shape[i] > 1 and t.stride(i) <= 0 for i in range(3)):
+        raise ValueError(f"{op}: {name} must not be a broadcast view; call {name}.contiguous()")
+
+
 class DraftTree(NamedTuple):
-    """What the kernels need of a draft's parent links: `depth` (B, T) int32, -1 for an absent node, and `mask`
-    (B, T, (T + 63) // 64) int64 words whose bit u says that the node attends node u (itself and its ancestors)."""
+    """What the kernels need of a draft's parent links: `depth` (B, T) int32, -1 for an absent node and below T otherwise,
+    and `mask` (B, T, (T + 63) // 64) int64 words whose bit u says that the node attends node u (itself and its ancestors)."""
     depth: torch.Tensor
     mask: torch.Tensor
 
@@ -168,6 +173,8 @@ def _append_layout(op, q, k, v, q_weight, k_weight, inv_freq, key_rows, value_ro
         raise ValueError(f"{op}: expects q (B,T,H,D) and k, v (B,T,Hk,D)")
     if key_rows.shape[0] != B or key_rows.shape[2:] != (Hk, D) or value_rows.shape != key_rows.shape:
         raise ValueError(f"{op}: key_rows and value_rows must be (B, rows, Hk, D)")
+    for name, t in (("key_rows", key_rows), ("value_rows", value_rows)):
+        _no_broadcast(op, name, t)                    # two samples or heads would write the same rows
     _require_tree(op, tree, lens, B, T)
     for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
         if w.numel() != D or not w.is_contiguous() or w.dtype != q.dtype:
@@ -247,12 +254,13 @@ def _attention_layout(op, q_base, q_group, key_rows, value_rows, tree, lens, w_0
                                        or [_st(key_group_rows, i) for i in range(3)] != [_st(key_rows, i) for i in range(3)]):
         raise ValueError(f"{op}: key_group_rows must match key_rows in shape and strides")
     for name, t in tensors:
-        if any(t.shape[i] > 1 and t.stride(i) <= 0 for i in range(3)):
-            raise ValueError(f"{op}: {name} must not be a broadcast view; call {name}.contiguous()")
+        _no_broadcast(op, name, t)
     if Hk < 1 or H % Hk != 0:
         raise ValueError(f"{op}: query heads must be divisible by kv heads")
     if int(w_0) < 0:
         raise ValueError(f"{op}: w_0 must be >= 0")
+    if softmax_scale is not None and not 0.0 < softmax_scale < math.inf:
+        raise ValueError(f"{op}: softmax_scale must be positive and finite, got {softmax_scale}")
     _require_tree(op, tree, lens, B, T)
     if rows < T:
         raise ValueError(f"{op}: the cache ({rows} rows) does not hold the {T} nodes")
@@ -260,6 +268,7 @@ def _attention_layout(op, q_base, q_group, key_rows, value_rows, tree, lens, w_0
         if tuple(out.shape) != (B, T, H, D) or out.dtype != q_base.dtype:
             raise ValueError(f"{op}: out must be {q_base.dtype} with shape {(B, T, H, D)}")
         _check_view(op, "out", out)
+        _no_broadcast(op, "out", out)
     _require_arch(op, _require_cuda(op, *(t for _, t in tensors), tree.depth, tree.mask, lens, out))
     o_st = [_st(out, i) for i in range(3)] if out is not None else [T * H * D, H * D, D]
     ws_bytes = max(16, N.lib().jl_tree_attention_workspace_bytes(B, T, H, Hk, rows))

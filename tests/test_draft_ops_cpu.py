@@ -58,7 +58,7 @@ def test_c_entries_refuse_before_they_touch_a_device():
     def attention(**kw):
         a = n.TreeAttentionArgs()
         a.q_base = a.k_base = a.v = a.out = a.lens = a.depth = a.mask = 1024
-        a.batch, a.nodes, a.heads, a.kv_heads, a.head_dim, a.rows, a.w_0 = 1, 4, 4, 2, 128, 64, 16
+        a.batch, a.nodes, a.heads, a.kv_heads, a.head_dim, a.rows, a.w_0, a.softmax_scale = 1, 4, 4, 2, 128, 64, 16, 0.125
         for t in "qkvo":
             setattr(a, f"{t}_stride_s", 512)
             setattr(a, f"{t}_stride_h", 128)
@@ -70,7 +70,9 @@ def test_c_entries_refuse_before_they_touch_a_device():
     for want, kw in [(no, dict(head_dim=64)), (bad, dict(kv_heads=3)), (bad, dict(nodes=0)), (bad, dict(nodes=257)), (bad, dict(rows=3)),
                      (bad, dict(w_0=-1)), (bad, dict(q_group=1024)), (bad, dict(k_group=1024)), (bad, dict(v=None)), (bad, dict(mask=None)),
                      (bad, dict(q_base=1032)), (bad, dict(k_stride_s=129)), (bad, dict(o_stride_h=4)), (bad, dict(batch=-1)),
-                     (no, dict(heads=258, kv_heads=2)), (no, dict(k_stride_s=0)), (no, dict(q_stride_h=-128)), (no, dict(batch=2))]:
+                     (no, dict(heads=258, kv_heads=2)), (no, dict(k_stride_s=0)), (no, dict(q_stride_h=-128)), (no, dict(batch=2)),
+                     (bad, dict(softmax_scale=0.0)), (bad, dict(softmax_scale=-0.1)), (bad, dict(softmax_scale=float("nan"))),
+                     (bad, dict(softmax_scale=float("inf")))]:
         assert attention(**kw) == want, kw
     assert attention(batch=0) == n.JL_OK
 
@@ -79,12 +81,15 @@ def test_c_entries_refuse_before_they_touch_a_device():
         for f in ("q", "k", "v", "q_weight", "k_weight", "q_base", "k_cache", "v_cache", "inv_freq", "lens", "depth"):
             setattr(a, f, 1024)
         a.batch, a.nodes, a.heads, a.kv_heads, a.head_dim, a.cache_rows, a.group_size = 1, 4, 4, 2, 128, 64, 1
+        a.kc_stride_s = a.vc_stride_s = 256
+        a.kc_stride_h = a.vc_stride_h = 128
         for k, v in kw.items():
             setattr(a, k, v)
         return lib.jl_tree_append(C.byref(a), None)
 
     for want, kw in [(no, dict(head_dim=96)), (bad, dict(depth=None)), (bad, dict(nodes=0)), (bad, dict(q_group=1024, group_size=0)),
-                     (bad, dict(q=1028)), (bad, dict(kc_stride_s=2)), (bad, dict(cache_rows=-1))]:
+                     (bad, dict(q=1028)), (bad, dict(kc_stride_s=2)), (bad, dict(cache_rows=-1)),
+                     (no, dict(vc_stride_h=0)), (no, dict(batch=2))]:
         assert append(**kw) == want, kw
     assert append(batch=0) == n.JL_OK
 
@@ -140,7 +145,9 @@ def test_draft_ops_refuse():
                       ("w_0", dict(w_0=-1)), ("tree.depth", dict(tree=tree._replace(depth=tree.depth.long()))),
                       ("tree.mask", dict(tree=tree._replace(mask=torch.zeros(B, T, 2, dtype=torch.int64)))),
                       ("lens", dict(lens=torch.zeros(B, dtype=torch.int64))), ("does not hold", dict(key_rows=bf(B, 2, Hk, 128), value_rows=bf(B, 2, Hk, 128))),
-                      ("multiples of 8", dict(key_rows=torch.zeros(B, R, Hk, 132, dtype=torch.bfloat16)[..., :128]))]:
+                      ("multiples of 8", dict(key_rows=torch.zeros(B, R, Hk, 132, dtype=torch.bfloat16)[..., :128])),
+                      ("softmax_scale", dict(softmax_scale=0.0)), ("softmax_scale", dict(softmax_scale=float("nan"))),
+                      ("broadcast", dict(value_rows=bf(1, R, Hk, 128).expand(B, -1, -1, -1))), ("broadcast", dict(out=bf(B, 1, H, 128).expand(-1, T, -1, -1)))]:
         with pytest.raises(ValueError, match=match):
             d.tree_attention(**{**ok, **kw})
     w = bf(128)
@@ -148,7 +155,8 @@ def test_draft_ops_refuse():
               key_rows=bf(B, R, Hk, 128), value_rows=bf(B, R, Hk, 128), tree=tree, lens=lens, q_eps=1e-6, k_eps=1e-6)
     for match, kw in [("requires CUDA", {}), ("expects q", dict(v=bf(B, T, Hk + 1, 128))), ("key_rows and value_rows", dict(key_rows=bf(B, R, H, 128))),
                       ("q_weight", dict(q_weight=bf(64))), ("inv_freq", dict(inv_freq=torch.ones(8))), ("group_size", dict(group_size=0)),
-                      ("key_group_rows", dict(key_group_rows=bf(B, R, H, 128)))]:
+                      ("key_group_rows", dict(key_group_rows=bf(B, R, H, 128))), ("broadcast", dict(key_rows=bf(1, R, Hk, 128).expand(B, -1, -1, -1))),
+                      ("broadcast", dict(value_rows=bf(B, R, 1, 128).expand(-1, -1, Hk, -1)))]:
         with pytest.raises(ValueError, match=match):
             d.tree_append(**{**ok, **kw})
     with pytest.raises(ValueError, match="path"):

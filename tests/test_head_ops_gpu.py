@@ -244,3 +244,52 @@ def test_repeats_streams_and_graphs():
     for o in outs:
         assert all(torch.equal(a, b) for a, b in zip(o, want))
     assert not torch.equal(want[1], ref[1])
+
+
+def test_labels_straight_from_the_scores():
+    """The labels of one call are what the kernels of the call before it wrote, with nothing in between."""
+    from jetlm.kernels import head_ops
+    h, w, _ = make(700, 128, 20000)
+    want = head_ops.token_scores(h, w, top=True).top.clone()
+    ref = head_ops.linear_cross_entropy(h, w, want)
+    none = torch.full_like(want, -100)
+    for _ in range(20):
+        assert float(head_ops.linear_cross_entropy(h, w, none, reduction="sum")) == 0
+        assert torch.equal(head_ops.linear_cross_entropy(h, w, head_ops.token_scores(h, w, top=True).top), ref)
+
+
+def test_more_rows_than_one_launch_of_the_scores_takes():
+    """Rows are scored 16384 at a time; the last group here is one row, which alone would take the path of few rows."""
+    from jetlm.kernels import head_ops
+    h, w, y = make(2 * 16384 + 1, 64, 300)
+    lse, nll, dz, z = exact(h, w, y)
+    got = head_ops.token_scores(h, w, y, top=True)
+    tol = 2 * dz + 2.0 ** -20 * (1 + lse.abs())
+    assert ((got.lse.double() - lse).abs() <= tol).all() and ((got.nll.double() - nll).abs() <= 2 * tol).all()
+    assert (z.gather(1, got.top[:, None])[:, 0] >= z.amax(1) - 2 * dz).all()
+    n = int((y >= 0).sum())
+    loss = head_ops.linear_cross_entropy(h, w, y)
+    # 1024 threads add 33 values each, then 10 additions join them; one division
+    assert abs(float(loss) - float(nll.sum()) / n) <= float((2 * tol + 44 * F32 * nll.abs()).sum()) / n + 2 * F32 * float(nll.abs().sum()) / n
+
+
+@pytest.mark.parametrize("N, H, V", [(17000, 64, 9001), (120, 8, 1200001), (300, 136, 460000)])
+def test_gradients_over_several_pieces_of_the_vocabulary(N, H, V):
+    """More than 256 MB of d logits: the row gradients are added up over two pieces, of which the second is the shorter."""
+    from jetlm.kernels import head_ops
+    h, w, y = make(N, H, V)
+    h.requires_grad_(True)
+    w.requires_grad_(True)
+    dh, dw = torch.autograd.grad(head_ops.linear_cross_entropy(h, w, y, reduction="sum"), [h, w])
+    hd, wd = h.detach(), w.detach()
+    step = max(1, (1 << 24) // V)                                 # the oracle takes the rows in chunks: its matrices are (rows, V) in 64 bits
+    e_w, b_w = torch.zeros(V, H, dtype=torch.float64, device="cuda"), torch.zeros(V, H, dtype=torch.float64, device="cuda")
+    for lo in range(0, N, step):
+        sl = slice(lo, lo + step)
+        *_, eh, ew, bh, bw = exact(hd[sl], wd, y[sl], torch.ones(y[sl].shape, device="cuda"))
+        assert ((dh[sl].double() - eh).abs() <= bh).all(), lo
+        e_w += ew
+        b_w += bw
+    # A chunk's bound counts fp32 additions of its own rows only; over all N rows they may take N * F32 * sum |dz| |h|, and a
+    # chunk's bound holds HALF * sum |dz| |h| for the rounding of dz: a factor N * F32 / HALF of what is there.
+    assert ((dw.double() - e_w).abs() <= b_w * (1 + N * F32 / HALF)).all()
