@@ -106,6 +106,26 @@ typedef struct {
 size_t jl_tree_attention_workspace_bytes(int32_t batch, int32_t nodes, int32_t heads, int32_t kv_heads, int32_t rows);
 int jl_tree_attention(const jl_tree_attention_args* args, void* cuda_stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * jl_tree_keep — after a path has been chosen: cache row lens[b] + i becomes what row lens[b] + path[b][i] was, in place, in
+ * one launch.  path (batch, kept) int32 node indices, root first; a path ends at the first entry that is not larger than
+ * the one before it (-1 pads shorter ones) or whose row is outside the cache.  Rows past the path stay as they are.
+ * Node path[b][i] of a path has depth i, so positions do not change and rotated keys stay valid where they land.
+ * k_cache / v_cache: (B, rows, Hk, D) with strides; k_group_cache has the strides of k_cache.  Each may be NULL.
+ * ------------------------------------------------------------------------------------------- */
+typedef struct {
+  void* k_cache;
+  void* v_cache;
+  void* k_group_cache;
+  int64_t kc_stride_b, kc_stride_s, kc_stride_h, vc_stride_b, vc_stride_s, vc_stride_h;
+  int64_t cache_rows;
+  const int32_t* path;
+  const int32_t* lens;
+  int32_t batch, kept, kv_heads, head_dim;
+} jl_tree_keep_args;
+
+int jl_tree_keep(const jl_tree_keep_args* args, void* cuda_stream);
+
 /* Diagnostic (synchronises the device): non-zero if a bounded wait (1 s) inside jl_tree_attention has given up on the
  * current device since the last call; reading a raised status clears it.  The results since the last call are then invalid. */
 int jl_tree_status(void);

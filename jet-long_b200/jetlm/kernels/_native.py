@@ -195,11 +195,21 @@ class TreeAttentionArgs(C.Structure):
     ]
 
 
+class TreeKeepArgs(C.Structure):
+    _fields_ = [
+        ("k_cache", C.c_void_p), ("v_cache", C.c_void_p), ("k_group_cache", C.c_void_p),
+        *[(f"{t}_stride_{a}", C.c_int64) for t in ("kc", "vc") for a in "bsh"],
+        ("cache_rows", C.c_int64), ("path", C.c_void_p), ("lens", C.c_void_p),
+        ("batch", C.c_int32), ("kept", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32),
+    ]
+
+
 TREE_EXPORTS = [
     ("jl_tree_plan", C.c_int, [C.POINTER(TreePlanArgs), C.c_void_p]),
     ("jl_tree_append", C.c_int, [C.POINTER(TreeAppendArgs), C.c_void_p]),
     ("jl_tree_attention_workspace_bytes", C.c_size_t, [C.c_int32] * 5),
     ("jl_tree_attention", C.c_int, [C.POINTER(TreeAttentionArgs), C.c_void_p]),
+    ("jl_tree_keep", C.c_int, [C.POINTER(TreeKeepArgs), C.c_void_p]),
     ("jl_tree_status", C.c_int, []),
 ]
 

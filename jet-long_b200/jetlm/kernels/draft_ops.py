@@ -7,7 +7,7 @@ position lens[b] + depth; it attends the committed rows [0, lens[b]) and the nod
     tree = draft_tree(parents)                                                       # once per step
     q_base, q_group = tree_append(q, k, v, ..., key_rows, value_rows, tree, lens)    # per layer
     out, lse = tree_attention(q_base, q_group, key_rows, value_rows, tree, lens, w_0=..., key_group_rows=...)
-    keep_path(buffer, path, start)                                                   # after the path has been chosen
+    tree_keep(key_rows, value_rows, path, lens, key_group_rows=...)                  # per layer, after a path has been chosen
 
 The reference decodes one token per call (jetlm/kernels/cute_decode_sm90.py:2748-2799); these operators have no
 counterpart there.  Kernels run on the current torch CUDA stream; nothing here computes attention in PyTorch.
@@ -283,10 +283,47 @@ def _attention_layout(op, q_base, q_group, key_rows, value_rows, tree, lens, w_0
     return a, ws_bytes
 
 
-def keep_path(buffer: torch.Tensor, path: torch.Tensor, start: int) -> None:
-    """Move the rows of the accepted nodes together: buffer (B, rows, ...) gets rows start + path[i] in rows
-    start + i.  `path` (n,) int64 node indices on the device, root first.  Positions do not change (node path[i] has
-    depth i), so base-rotated and regrouped keys stay valid where they land."""
-    if path.dim() != 1 or path.dtype != torch.int64:
-        raise ValueError("keep_path: path must be int64 with shape (n,)")
-    buffer[:, start: start + path.numel()] = buffer.index_select(1, path + start)
+def tree_keep(key_rows: torch.Tensor, value_rows: torch.Tensor, path: torch.Tensor, lens: torch.Tensor, *,
+              key_group_rows: Optional[torch.Tensor] = None) -> None:
+    """Moves the rows of the accepted nodes together, in place (see jl_tree_keep): row lens[b] + i of key_rows, value_rows and
+    key_group_rows (B,rows,Hk,D views) becomes what row lens[b] + path[b, i] was.  path (B, n) int32 node indices on the
+    device, root first; a path ends at its first entry that is not larger than the one before (-1 pads).  Positions do not
+    change (node path[b, i] has depth i), so base-rotated and regrouped keys stay valid where they land."""
+    op = "tree_keep"
+    key = (op, _sig(key_rows), _sig(value_rows), _sig(path), _sig(lens), _sig(key_group_rows))
+    template = _LAYOUTS.get(key)
+    if template is None:
+        template = _keep_layout(key, _tree_keep_layout(op, key_rows, value_rows, path, lens, key_group_rows))
+    a = N.TreeKeepArgs.from_buffer_copy(template)
+    ptrs = dict(key_rows=key_rows.data_ptr(), value_rows=value_rows.data_ptr())
+    a.k_cache, a.v_cache = ptrs.values()
+    if key_group_rows is not None:
+        a.k_group_cache = ptrs["key_group_rows"] = key_group_rows.data_ptr()
+    _aligned(op, ptrs)
+    a.path, a.lens = path.data_ptr(), lens.data_ptr()
+    _run("jl_tree_keep", N.lib().jl_tree_keep, a, key_rows.device.index)
+
+
+def _tree_keep_layout(op, key_rows, value_rows, path, lens, key_group_rows):
+    caches = [("key_rows", key_rows), ("value_rows", value_rows)] + ([("key_group_rows", key_group_rows)] if key_group_rows is not None else [])
+    for name, t in caches:
+        _check_view(op, name, t)
+        _no_broadcast(op, name, t)
+        if t.dtype not in _SUPPORTED_DTYPES:
+            raise ValueError(f"{op}: {name} must be torch.bfloat16, got {t.dtype}")
+        if t.shape != key_rows.shape:
+            raise ValueError(f"{op}: key_rows, value_rows and key_group_rows must share their shape")
+    if key_group_rows is not None and [_st(key_group_rows, i) for i in range(3)] != [_st(key_rows, i) for i in range(3)]:
+        raise ValueError(f"{op}: key_group_rows must match key_rows in shape and strides")
+    B, rows, Hk, D = key_rows.shape
+    if path.dim() != 2 or path.shape[1] > N.JL_TREE_MAX_NODES:
+        raise ValueError(f"{op}: path must be (B, n) with at most {N.JL_TREE_MAX_NODES} nodes, got {tuple(path.shape)}")
+    _require_ints(op, "path", path, (B, path.shape[1]), torch.int32)
+    _require_ints(op, "lens", lens, (B,), torch.int32)
+    _require_arch(op, _require_cuda(op, *(t for _, t in caches), path, lens))
+    a = N.TreeKeepArgs()
+    for name, t in (("kc", key_rows), ("vc", value_rows)):
+        for i, axis in enumerate("bsh"):
+            setattr(a, f"{name}_stride_{axis}", _st(t, i))
+    a.cache_rows, a.batch, a.kept, a.kv_heads, a.head_dim = rows, B, path.shape[1], Hk, D
+    return a

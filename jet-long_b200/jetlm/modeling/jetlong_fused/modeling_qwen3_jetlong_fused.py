@@ -746,11 +746,9 @@ class Qwen3JetLongFusedForCausalLM(Qwen3PreTrainedModel, GenerationMixin):
                     break
                 path.append(nxt)
             if path != list(range(len(path))):
-                rows = torch.tensor(path, dtype=torch.long, device=dev)
+                rows = torch.tensor([path], dtype=torch.int32, device=dev)
                 for layer in cache.layers:
-                    for buf in (layer.keys, layer.values, layer.group_keys):
-                        if buf is not None:
-                            draft_ops.keep_path(buf, rows, seen)
+                    draft_ops.tree_keep(layer.keys, layer.values, rows, step.lens, key_group_rows=layer.group_keys)
             for layer in cache.layers:
                 layer.commit(len(path))
         self.drafted_steps = steps

@@ -18,7 +18,7 @@ def _n():
 
 @pytest.mark.parametrize("header, exports, structs", [
     ("jetlong_b200_tree.h", "TREE_EXPORTS", {"jl_tree_plan_args": "TreePlanArgs", "jl_tree_append_args": "TreeAppendArgs",
-                                             "jl_tree_attention_args": "TreeAttentionArgs"}),
+                                             "jl_tree_attention_args": "TreeAttentionArgs", "jl_tree_keep_args": "TreeKeepArgs"}),
     ("jetlong_b200_head.h", "HEAD_EXPORTS", {"jl_head_scores_args": "HeadScoresArgs", "jl_head_grads_args": "HeadGradsArgs"}),
 ])
 def test_header_matches_the_binding(tmp_path, header, exports, structs):
@@ -47,7 +47,7 @@ def test_header_matches_the_binding(tmp_path, header, exports, structs):
 def test_c_entries_refuse_before_they_touch_a_device():
     n = _n()
     lib = n.lib()
-    for fn in ("jl_tree_plan", "jl_tree_append", "jl_tree_attention", "jl_head_scores", "jl_head_grads"):
+    for fn in ("jl_tree_plan", "jl_tree_append", "jl_tree_attention", "jl_tree_keep", "jl_head_scores", "jl_head_grads"):
         assert getattr(lib, fn)(None, None) == n.JL_ERR_BAD_ARG
         assert b"NULL" in lib.jl_last_error()
     p = n.TreePlanArgs(1024, 1024, 1024, 1, 0)
@@ -92,6 +92,21 @@ def test_c_entries_refuse_before_they_touch_a_device():
                      (no, dict(vc_stride_h=0)), (no, dict(batch=2))]:
         assert append(**kw) == want, kw
     assert append(batch=0) == n.JL_OK
+
+    def keep(**kw):
+        a = n.TreeKeepArgs()
+        a.k_cache = a.v_cache = a.path = a.lens = 1024
+        a.batch, a.kept, a.kv_heads, a.head_dim, a.cache_rows = 1, 4, 2, 128, 64
+        a.kc_stride_s = a.vc_stride_s = 256
+        a.kc_stride_h = a.vc_stride_h = 128
+        for k, v in kw.items():
+            setattr(a, k, v)
+        return lib.jl_tree_keep(C.byref(a), None)
+
+    for want, kw in [(no, dict(head_dim=64)), (bad, dict(kept=257)), (bad, dict(kept=-1)), (bad, dict(path=None)), (bad, dict(lens=1026)),
+                     (bad, dict(v_cache=1032)), (bad, dict(kc_stride_s=132)), (no, dict(vc_stride_h=0)), (no, dict(batch=2)), (bad, dict(batch=65536))]:
+        assert keep(**kw) == want, kw
+    assert keep(batch=0) == keep(kept=0) == n.JL_OK
 
     def scores(**kw):
         a = n.HeadScoresArgs()
@@ -159,17 +174,14 @@ def test_draft_ops_refuse():
                       ("broadcast", dict(value_rows=bf(B, R, 1, 128).expand(-1, -1, Hk, -1)))]:
         with pytest.raises(ValueError, match=match):
             d.tree_append(**{**ok, **kw})
-    with pytest.raises(ValueError, match="path"):
-        d.keep_path(bf(1, 8, 2), torch.zeros(2, dtype=torch.int32), 0)
-
-
-def test_keep_path_moves_rows():
-    from jetlm.kernels import draft_ops as d
-    x = torch.arange(20.0).view(1, 10, 2).clone()
-    want = x.clone()
-    want[:, 4:7] = x[:, [4, 6, 9]]
-    d.keep_path(x, torch.tensor([0, 2, 5]), 4)
-    assert torch.equal(x, want)
+    path = torch.zeros(B, T, dtype=torch.int32)
+    ok = dict(key_rows=bf(B, R, Hk, 128), value_rows=bf(B, R, Hk, 128), path=path, lens=lens)
+    for match, kw in [("requires CUDA", {}), ("path", dict(path=path.long())), ("path", dict(path=path[0])), ("path", dict(path=path[:1])),
+                      ("at most 256", dict(path=torch.zeros(B, 257, dtype=torch.int32))), ("lens", dict(lens=lens.long())),
+                      ("share their shape", dict(value_rows=bf(B, R, 1, 128))), ("match key_rows", dict(key_group_rows=bf(B, Hk, R, 128).transpose(1, 2))),
+                      ("bfloat16", dict(value_rows=torch.zeros(B, R, Hk, 128))), ("broadcast", dict(value_rows=bf(1, R, Hk, 128).expand(B, -1, -1, -1)))]:
+        with pytest.raises(ValueError, match=match):
+            d.tree_keep(**{**ok, **kw})
 
 
 def test_head_ops_refuse():

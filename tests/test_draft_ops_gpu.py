@@ -331,3 +331,42 @@ def test_tree_append_writes_no_row_past_the_cache():
     whole_k.copy_(keep_k)
     d.tree_append(*args, torch.tensor([-3], dtype=torch.int32, device="cuda"), q_eps=1e-6, k_eps=1e-6)
     assert torch.equal(whole_k, keep_k)
+
+
+@pytest.mark.parametrize("B, Hk, n, group", [(1, 1, 1, False), (1, 8, 5, True), (3, 4, 9, True), (4, 9, 256, False), (2, 2, 37, True)])
+def test_tree_keep_moves_the_path_and_nothing_else(B, Hk, n, group):
+    from jetlm.kernels import draft_ops as d
+    g = torch.Generator().manual_seed(B * 1000 + n)
+    rows, T = 600, 256
+    bufs = [torch.randn(B, rows, Hk, 128, generator=g).cuda().bfloat16() for _ in range(2)]
+    bufs.insert(1, torch.randn(B, Hk, rows, 128, generator=g).cuda().bfloat16().transpose(1, 2))      # values head-major
+    lens = torch.tensor({1: [17], 2: [11, 300], 3: [5, 0, 344], 4: [1, 344, 77, 340]}[B], dtype=torch.int32)
+    path = torch.full((B, n), -1, dtype=torch.int32)
+    for b in range(B):
+        k = n if b == 0 else int(torch.randint(0, n + 1, (1,), generator=g))
+        path[b, :k] = torch.randperm(T, generator=g)[:k].sort().values.int()
+    want = [x.clone() for x in bufs]
+    for b in range(B):
+        keep = path[b][path[b] >= 0].long()
+        for w, x in zip(want, bufs):
+            w[b, int(lens[b]): int(lens[b]) + len(keep)] = x[b, (int(lens[b]) + keep).cuda()]
+    d.tree_keep(bufs[0], bufs[1], path.cuda(), lens.cuda(), key_group_rows=bufs[2] if group else None)
+    for i, (w, x) in enumerate(zip(want, bufs)):
+        if i < 2 or group:
+            assert torch.equal(x, w), i
+
+
+def test_tree_keep_stops_at_the_end_of_a_path_or_cache():
+    from jetlm.kernels import draft_ops as d
+    x = torch.randn(4, 64, 2, 128, generator=torch.Generator().manual_seed(3)).cuda().bfloat16()
+    y, before = x.clone(), x.clone()
+    path = torch.tensor([[1, 3, 3, 5], [2, 4, 1, 7], [0, 2, 1 << 30, 2000000000], [-5, 1, 2, 3]], dtype=torch.int32).cuda()
+    lens = torch.tensor([10, 20, 60, 5], dtype=torch.int32).cuda()
+    d.tree_keep(x, y, path, lens)                       # an entry that repeats, falls, leaves the cache, or is none
+    want = before.clone()
+    want[0, 10], want[0, 11] = before[0, 11], before[0, 13]
+    want[1, 20], want[1, 21] = before[1, 22], before[1, 24]
+    want[2, 60], want[2, 61] = before[2, 60], before[2, 62]
+    assert torch.equal(x, want) and torch.equal(y, want)
+    d.tree_keep(x, y, path, torch.tensor([-3, 64, 63, 1 << 30], dtype=torch.int32).cuda())       # lengths outside the cache
+    assert torch.equal(x, want) and torch.equal(y, want)
