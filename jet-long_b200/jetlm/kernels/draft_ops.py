@@ -25,7 +25,7 @@ from .jetlong_ops import _SUPPORTED_DTYPES, _check_view, _require_arch, _require
 
 # Checked call layouts: what a call's shapes, strides, types and devices were found to allow, with the argument structure
 # filled in except for its pointers.  A decode loop makes the same call for every layer and step, and the checks took longer
-# than the kernels (attention: 78 us a call, 34 with the layouts kept).
+# than the kernels (host time of an attention call: 78 us with them, 20 with the layouts kept).
 _LAYOUTS: dict = {}
 
 
@@ -37,28 +37,25 @@ def _keep_layout(key, value):
 
 
 def _sig(t: Optional[torch.Tensor]):
-    return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.get_device())
 
 
-def _aligned(op: str, pointers: dict, to: int = 16) -> None:
-    bits = 0
-    for p in pointers.values():
-        bits |= p
-    if bits % to:
-        raise ValueError(f"{op}: {next(n for n, p in pointers.items() if p % to)} must be {to}-byte aligned")
+def _misaligned(op: str, **tensors) -> ValueError:
+    return ValueError(f"{op}: {next(n for n, t in tensors.items() if t is not None and t.data_ptr() % 16)} must be 16-byte aligned")
 
 
 def _current_stream(index: int) -> int:
     return torch.cuda.current_stream(index).cuda_stream
 
 
-# the handle alone, without the Python object around it (0.2 us against 5)
+# the handle alone, without the Python object around it (0.2 us against 5), and the current device without the wrapper's checks
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _current_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def _run(op: str, fn, args, index: int) -> None:
     """One C call on the current stream of the tensors' device."""
-    if torch.cuda.current_device() == index:
+    if _current_device() == index:
         status = fn(C.byref(args), _raw_stream(index))
     else:
         with torch.cuda.device(index):
@@ -108,7 +105,7 @@ def draft_tree(parents: torch.Tensor) -> DraftTree:
     op = "draft_tree"
     if parents.dim() == 1:
         parents = parents.unsqueeze(0)
-    key = (op, parents.shape, parents.dtype, parents.device)
+    key = (op, parents.shape, parents.dtype, parents.get_device())
     if key not in _LAYOUTS:
         if parents.dim() != 2 or parents.dtype not in (torch.int32, torch.int64):
             raise ValueError(f"{op}: parents must be int32 or int64 with shape (B, T)")
@@ -120,7 +117,7 @@ def draft_tree(parents: torch.Tensor) -> DraftTree:
     dev = parents.device
     parents = parents.clamp(-2, T).to(torch.int32) if parents.dtype == torch.int64 else parents
     parents = parents.contiguous()
-    depth = torch.empty(B, T, dtype=torch.int32, device=dev)
+    depth = torch.empty_like(parents)
     mask = torch.empty(B, T, (T + 63) // 64, dtype=torch.int64, device=dev)
     if B > 0:
         _run("jl_tree_plan", N.lib().jl_tree_plan, N.TreePlanArgs(parents.data_ptr(), depth.data_ptr(), mask.data_ptr(), B, T), dev.index)
@@ -145,19 +142,21 @@ def tree_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_weight: tor
                                                     q_eps, k_eps, group_size, key_group_rows))
     if inv_freq.device != q.device or inv_freq.dtype != torch.float32 or not inv_freq.is_contiguous():
         inv_freq = inv_freq.to(device=q.device, dtype=torch.float32).contiguous()
-    q_base = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    q_group = torch.empty(q.shape, dtype=q.dtype, device=q.device) if group_size > 1 else None
+    q_base = torch.empty_like(q, memory_format=torch.contiguous_format)
+    q_group = torch.empty_like(q_base) if group_size > 1 else None
     a = N.TreeAppendArgs.from_buffer_copy(template)
-    ptrs = dict(q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), key_rows=key_rows.data_ptr(), value_rows=value_rows.data_ptr(),
-                q_weight=q_weight.data_ptr(), k_weight=k_weight.data_ptr())
-    a.q, a.k, a.v, a.k_cache, a.v_cache, a.q_weight, a.k_weight = ptrs.values()
+    a.q, a.k, a.v, a.q_weight, a.k_weight = ptrs = (q.data_ptr(), k.data_ptr(), v.data_ptr(), q_weight.data_ptr(), k_weight.data_ptr())
+    a.k_cache, a.v_cache = kc, vc = key_rows.data_ptr(), value_rows.data_ptr()
     a.q_base = q_base.data_ptr()
     if q_group is not None:
         a.q_group = q_group.data_ptr()
+    kg = 0
     if key_group_rows is not None:
-        a.k_group_cache = ptrs["key_group_rows"] = key_group_rows.data_ptr()
+        a.k_group_cache = kg = key_group_rows.data_ptr()
     a.inv_freq, a.lens, a.depth = inv_freq.data_ptr(), lens.data_ptr(), tree.depth.data_ptr()
-    _aligned(op, ptrs)
+    if (ptrs[0] | ptrs[1] | ptrs[2] | ptrs[3] | ptrs[4] | kc | vc | kg) & 15:
+        raise _misaligned(op, q=q, k=k, v=v, q_weight=q_weight, k_weight=k_weight, key_rows=key_rows, value_rows=value_rows,
+                          key_group_rows=key_group_rows)
     _run("jl_tree_append", N.lib().jl_tree_append, a, q.device.index)
     return q_base, (q_group if q_group is not None else q_base)
 
@@ -216,17 +215,17 @@ def tree_attention(q_base: torch.Tensor, q_group: torch.Tensor, key_rows: torch.
     template, ws_bytes = plan
     dev = q_base.device
     if out is None:
-        out = torch.empty(q_base.shape, dtype=q_base.dtype, device=dev)
+        out = torch.empty_like(q_base, memory_format=torch.contiguous_format)
     # split partials: this call's own memory from the stream-ordered allocator, so concurrent calls and captured graphs
     # never share it
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
     a = N.TreeAttentionArgs.from_buffer_copy(template)
-    ptrs = dict(q_base=q_base.data_ptr(), key_rows=key_rows.data_ptr(), value_rows=value_rows.data_ptr(), out=out.data_ptr())
-    a.q_base, a.k_base, a.v, a.out = ptrs.values()
+    a.q_base, a.k_base, a.v, a.out = ptrs = (q_base.data_ptr(), key_rows.data_ptr(), value_rows.data_ptr(), out.data_ptr())
+    qg = kg = 0
     if key_group_rows is not None:
-        a.q_group = ptrs["q_group"] = q_group.data_ptr()
-        a.k_group = ptrs["key_group_rows"] = key_group_rows.data_ptr()
-    _aligned(op, ptrs)
+        a.q_group, a.k_group = qg, kg = q_group.data_ptr(), key_group_rows.data_ptr()
+    if (ptrs[0] | ptrs[1] | ptrs[2] | ptrs[3] | qg | kg) & 15:
+        raise _misaligned(op, q_base=q_base, key_rows=key_rows, value_rows=value_rows, out=out, q_group=q_group, key_group_rows=key_group_rows)
     a.lens, a.depth, a.mask, a.workspace = lens.data_ptr(), tree.depth.data_ptr(), tree.mask.data_ptr(), ws.data_ptr()
     lse = None
     if return_lse:
@@ -295,11 +294,12 @@ def tree_keep(key_rows: torch.Tensor, value_rows: torch.Tensor, path: torch.Tens
     if template is None:
         template = _keep_layout(key, _tree_keep_layout(op, key_rows, value_rows, path, lens, key_group_rows))
     a = N.TreeKeepArgs.from_buffer_copy(template)
-    ptrs = dict(key_rows=key_rows.data_ptr(), value_rows=value_rows.data_ptr())
-    a.k_cache, a.v_cache = ptrs.values()
+    a.k_cache, a.v_cache = kc, vc = key_rows.data_ptr(), value_rows.data_ptr()
+    kg = 0
     if key_group_rows is not None:
-        a.k_group_cache = ptrs["key_group_rows"] = key_group_rows.data_ptr()
-    _aligned(op, ptrs)
+        a.k_group_cache = kg = key_group_rows.data_ptr()
+    if (kc | vc | kg) & 15:
+        raise _misaligned(op, key_rows=key_rows, value_rows=value_rows, key_group_rows=key_group_rows)
     a.path, a.lens = path.data_ptr(), lens.data_ptr()
     _run("jl_tree_keep", N.lib().jl_tree_keep, a, key_rows.device.index)
 

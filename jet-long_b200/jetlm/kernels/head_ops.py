@@ -28,18 +28,20 @@ class TokenScores(NamedTuple):
 
 def _rows(op: str, hidden: torch.Tensor, weight: torch.Tensor, labels: Optional[torch.Tensor]):
     """(hidden as (rows, H), labels as (rows,)) with the checks the kernels rely on; the layout checks are made once per layout."""
-    key = (op, _sig(hidden), _sig(weight), None if labels is None else (labels.shape, labels.dtype, labels.device))
+    key = (op, _sig(hidden), _sig(weight), None if labels is None else (labels.shape, labels.dtype, labels.get_device()))
     if key not in _LAYOUTS:
         _check_rows(op, hidden, weight, labels)
         _keep_layout(key, True)
     h = hidden if hidden.dim() == 2 else hidden.reshape(-1, hidden.shape[-1])          # a copy only where the leading dimensions do not collapse
-    for name, t in (("hidden", h), ("weight", weight)):
-        if t.shape[0] > 0 and (t.stride(1) != 1 or (t.shape[0] > 1 and (t.stride(0) % 8 or t.stride(0) < t.shape[1])) or t.data_ptr() % 16):
-            raise ValueError(f"{op}: {name} rows must be contiguous, 16-byte aligned and a multiple of 8 elements apart; "
-                             f"call {name}.contiguous()")
+    if (h.data_ptr() | weight.data_ptr()) & 15:
+        raise _bad_rows(op, "weight" if weight.data_ptr() & 15 else "hidden")
     if labels is not None and (labels.dim() != 1 or not labels.is_contiguous()):
         labels = labels.reshape(-1).contiguous()
     return h, labels
+
+
+def _bad_rows(op, name):
+    return ValueError(f"{op}: {name} rows must be contiguous, 16-byte aligned and a multiple of 8 elements apart; call {name}.contiguous()")
 
 
 def _check_rows(op, hidden, weight, labels):
@@ -53,11 +55,15 @@ def _check_rows(op, hidden, weight, labels):
         raise ValueError(f"{op}: the hidden size must be a multiple of 8 and the vocabulary not empty, got {tuple(weight.shape)}")
     if labels is not None and (labels.shape != hidden.shape[:-1] or labels.dtype != torch.int64 or labels.device != hidden.device):
         raise ValueError(f"{op}: labels must be int64 with shape {tuple(hidden.shape[:-1])} on {hidden.device}")
+    for name, t in (("hidden", hidden if hidden.dim() == 2 else hidden.reshape(-1, hidden.shape[-1])), ("weight", weight)):
+        if t.shape[0] > 0 and (t.stride(1) != 1 or (t.shape[0] > 1 and (t.stride(0) % 8 or t.stride(0) < t.shape[1]))):
+            raise _bad_rows(op, name)
     _require_arch(op, hidden.device)
 
 
 def _row_stride(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    rows, cols = t.shape
+    return t.stride(0) if rows > 1 else cols
 
 
 def _scores(h, w, labels, ignore_index, *, nll, top, reduction=None):
