@@ -32,11 +32,13 @@ constexpr int kEpiWarps = 8;                 // two per quarter of the accumulat
 constexpr int kGemmThreads = 128 + 32 * kEpiWarps;
 constexpr int kRegsLow = 72, kRegsHigh = 216;     // 128 x 72 + 256 x 216 = the launch total 384 x 168
 constexpr int kRingBytes = 196608;           // operand ring: as many stages of A and B rows, 64 deep, as fit
-constexpr int kMaxStages = 8;
+constexpr int kMaxStages = 10;
 constexpr int kStagingBytes = kEpiWarps * 4096;      // per epilogue warp a box of 32 rows x 128 bytes
 constexpr int kSms = 148;
 
-enum { kEpiScores = 0, kEpiDz = 1, kEpiF32 = 2, kEpiBf16 = 3 };
+constexpr int kFewRows = 32;                 // up to here the rows are the columns of the score product
+
+enum { kEpiScores = 0, kEpiDz = 1, kEpiF32 = 2, kEpiBf16 = 3, kEpiFew = 4 };
 
 struct GradScale {            // scalar factor of both gradients, applied to their fp32 sums
   const float *grad, *count;
@@ -54,10 +56,11 @@ struct GemmParams {
   int m_tiles, n_tiles, splits, k_blocks, kb_per_split, bn;
   int group_m;                // > 0: m fastest inside groups of this many m tiles; 0: n fastest
   int behind, alone_rounds;   // see TileWalk
-  int a_bytes, stage_bytes, stages;      // of the operand ring, per CTA
+  int m_step;                 // rows of A from one tile to the next
+  int a_bytes, tx_bytes, stage_bytes, stages;      // of the operand ring, per CTA: A's place, what a stage loads, a stage
   // scores
-  float2* part;               // [row][n tile][half] (maximum, sum of exponentials relative to it)
-  int* part_arg;              // [row][n tile][half] or NULL
+  float2* part;               // [row][n tile][half] (few rows: [row][m tile]) (maximum, sum of exponentials relative to it)
+  int* part_arg;              // the same or NULL
   float* picked;              // [row] logit of the label
   // dz
   const float* lse;
@@ -169,23 +172,24 @@ struct Product {
   // therefore take K in parts that are added in fp32 registers.  Error of the loss / time of 8191 rows x 4096 with parts of 256,
   // 512, 1024 and all of K: 2e-7 / 8.0 ms, 3.5e-7 / 7.5, 8e-7 / 7.25, 4e-6 / 7.1; a few rows are bound by the weight's bytes and
   // take the shortest parts at no cost.  Results that are rounded to bf16 need none of this.
-  static constexpr int kPart = kEpi_ != kEpiScores ? 1 << 30 : kPair_ == 1 ? 4 : 8;
+  static constexpr bool kParts = kEpi_ == kEpiScores || kEpi_ == kEpiFew;
+  static constexpr int kPart = !kParts ? 1 << 30 : kPair_ == 1 ? 4 : 8;
 };
 
 template <class P>
 __device__ __forceinline__ void produce(const GemmMaps& maps, const GemmParams& p, GemmSmem& sm, int rank, int worker, int workers, PipeState& st) {
   constexpr int kPair = P::kPair;
-  const int b_rows = p.bn / kPair, tx_bytes = p.a_bytes + b_rows * kBK * 2;
+  const int b_rows = p.bn / kPair;
   TileWalk walk(p, worker, workers);
   for (int t; walk.next(t);) {
     const TileCoord c = tile_coord(p, t);
-    const int m0 = (c.m * kPair + rank) * 128, n0 = c.n * p.bn + rank * b_rows;
+    const int m0 = (c.m * kPair + rank) * p.m_step, n0 = c.n * p.bn + rank * b_rows;
     const int kb0 = c.split * p.kb_per_split, kb1 = min(kb0 + p.kb_per_split, p.k_blocks);
     for (int kb = kb0; kb < kb1; ++kb, st.next(p.stages)) {
       const int s = st.slot;
       mbar_wait(&sm.empty[s], st.parity ^ 1u, sm);
       if (*reinterpret_cast<volatile int*>(&sm.failed)) return;
-      if (rank == 0) mbar_expect_tx(&sm.full[s], kPair * tx_bytes);
+      if (rank == 0) mbar_expect_tx(&sm.full[s], kPair * p.tx_bytes);
       const uint32_t bar = kPair == 2 ? pair::leader_addr(&sm.full[s]) : smem_u32(&sm.full[s]);
       uint8_t* sa = sm.ring + s * p.stage_bytes;
       uint8_t* sb = sa + p.a_bytes;
@@ -223,8 +227,8 @@ __device__ __forceinline__ void issue(const GemmParams& p, GemmSmem& sm, uint32_
     const int kb0 = c.split * p.kb_per_split, kb1 = min(kb0 + p.kb_per_split, p.k_blocks);
     uint32_t acc = 0;
     for (int kb = kb0; kb < kb1; ++kb, st.next(p.stages)) {
-      const bool first = kb == kb0 || (P::kEpi == kEpiScores && (kb - kb0) % P::kPart == 0);
-      const bool last = kb + 1 == kb1 || (P::kEpi == kEpiScores && (kb + 1 - kb0) % P::kPart == 0);
+      const bool first = kb == kb0 || (P::kParts && (kb - kb0) % P::kPart == 0);
+      const bool last = kb + 1 == kb1 || (P::kParts && (kb + 1 - kb0) % P::kPart == 0);
       if (first) {
         mbar_wait(&sm.acc_free[st.i & 1], ((st.i >> 1) & 1) ^ 1, sm);
         acc = tmem + (st.i & 1) * kAccCols;
@@ -297,7 +301,60 @@ __device__ __forceinline__ void finish(const GemmMaps& maps, const GemmParams& p
     const int64_t row_w = (static_cast<int64_t>(c.m) * kPair + rank) * 128 + quad * 32, row = row_w + lane;
     const int n0 = c.n * p.bn;
 
-    if constexpr (kEpi == kEpiScores) {
+    if constexpr (kEpi == kEpiFew) {
+      // The tile is m_step vocabulary entries by up to 32 rows.  Its logits are summed over the parts of K in registers (a thread has
+      // an entry and half of the rows) and go through shared memory to a warp per row.
+      float* const zs = reinterpret_cast<float*>(sm.ring + kRingBytes + kStagingBytes - p.N * 512);      // [row][128 entries], behind the ring
+      const int half_cols = p.bn / 2, c_lo = half * half_cols;
+      float z[kFewRows / 2];
+#pragma unroll
+      for (int j = 0; j < kFewRows / 2; ++j) z[j] = 0.f;
+      for (int part = 0; part * P::kPart < p.k_blocks; ++part) {
+        const uint32_t acc = tmem + (st.i & 1) * kAccCols + lane_base + c_lo;
+        mbar_wait(&sm.acc_full[st.i & 1], (st.i >> 1) & 1, sm);
+        tc_fence_after();
+#pragma unroll
+        for (int ch = 0; ch < kFewRows / 32; ++ch) {
+          if (ch * 16 < half_cols) {               // (the last chunk may read columns past this half, which are not used)
+            uint32_t x[16];
+            JL_TMEM_LD16(acc + ch * 16, x);
+            JL_TMEM_WAIT_LD16(x, 0);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) z[ch * 16 + j] += __uint_as_float(x[j]);
+          }
+        }
+        hand_back();
+      }
+      const int64_t v0 = static_cast<int64_t>(c.m) * p.m_step;
+      const int valid = static_cast<int>(p.M - v0 < p.m_step ? p.M - v0 : p.m_step);
+      asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpiWarps) : "memory");      // the tile before has been read
+#pragma unroll
+      for (int j = 0; j < kFewRows / 2; ++j)
+        if (j < half_cols && c_lo + j < p.N) zs[(c_lo + j) * 128 + quad * 32 + lane] = quad * 32 + lane < valid ? z[j] : -INFINITY;
+      asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpiWarps) : "memory");
+      for (int r = ew; r < p.N; r += kEpiWarps) {
+        const float4 x = *reinterpret_cast<const float4*>(zs + r * 128 + 4 * lane);
+        float m = fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w));
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+        const float m_use = m == -INFINITY ? 0.f : m;
+        float sum = (fast_exp2((x.x - m_use) * kLog2e) + fast_exp2((x.y - m_use) * kLog2e)) +
+                    (fast_exp2((x.z - m_use) * kLog2e) + fast_exp2((x.w - m_use) * kLog2e));
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+        const int64_t at = static_cast<int64_t>(r) * p.m_tiles + c.m;
+        if (p.part_arg != nullptr) {
+          const int first = x.x == m ? 0 : x.y == m ? 1 : x.z == m ? 2 : x.w == m ? 3 : 128;
+          const int arg = __reduce_min_sync(0xffffffffu, 4 * lane + first);
+          if (lane == 0) p.part_arg[at] = arg < valid ? static_cast<int>(v0) + arg : 0x7fffffff;
+        }
+        if (lane == 0) {
+          p.part[at] = make_float2(m, sum);
+          const int64_t y = p.labels != nullptr ? p.labels[r] - v0 : -1;
+          if (y >= 0 && y < valid) p.picked[r] = zs[r * 128 + y];
+        }
+      }
+    } else if constexpr (kEpi == kEpiScores) {
       // columns [c_lo, c_lo + width) of the tile, up to 128 of them in registers, summed over the parts of K
       const int c_lo = half == 0 ? 0 : (p.bn / 2 + 15) / 16 * 16, width = half == 0 ? (p.bn / 2 + 15) / 16 * 16 : p.bn - c_lo;
       float z[128];
@@ -659,17 +716,54 @@ int prepare(Gemm& g, const Matrix& A, const Matrix& B, const Result& out, const 
   int rc = bind_context();
   // a single CTA's one row tile may be short: only its rows are loaded (what the others hold reaches no result)
   const int a_rows = P::kAMn ? kBK : P::kPair == 1 && p.M < 128 ? static_cast<int>(cdiv(p.M, 8)) * 8 : 128;
+  p.m_step = 128;
   p.a_bytes = P::kAMn ? kABytes : a_rows * kBK * 2;
+  p.tx_bytes = p.a_bytes + plan.bn / P::kPair * kBK * 2;
   // pairs have one geometry, so that two products can share a launch; a single CTA's ring is as deep as its tiles allow (reads of
   // A rows past a short tile stay inside the ring and the staging behind it)
   p.stage_bytes = P::kPair == 2 ? kABytes + kMaxBN / 2 * kBK * 2 : p.a_bytes + plan.bn * kBK * 2;
-  p.stages = kRingBytes / p.stage_bytes < kMaxStages ? kRingBytes / p.stage_bytes : kMaxStages;
+  p.stages = kRingBytes / p.stage_bytes < 8 ? kRingBytes / p.stage_bytes : 8;
   if (rc == JL_OK) rc = A.ld == 0 ? make_map2(&g.maps.a, A.p, A.rows, 64, 64, 64, a_rows, false, cdiv(A.cols, 64), true)
                                   : make_map2(&g.maps.a, A.p, A.rows, A.cols, A.ld, kBK, a_rows, false, 1, false);
   if (rc == JL_OK) rc = make_map2(&g.maps.b, B.p, B.rows, B.cols, B.ld, kBK, P::kBMn ? kBK : plan.bn / P::kPair, false, 1, false);
   if (rc == JL_OK && out.p != nullptr)
     rc = out.ld == 0 ? make_map2(&g.maps.out, out.p, p.M, 64, 64, 64, 32, false, cdiv(p.N, 64), true)
                      : make_map2(&g.maps.out, out.p, p.M, p.N, out.ld, out.f32 ? 32 : 64, 32, out.f32, out.planes, true);
+  return rc;
+}
+
+// Scores of up to 32 rows: the weight's rows are the rows of the product and the hidden states its columns, so that a tile
+// multiplies 16 columns for one row instead of 128 rows, in equal shares for all SMs.  At the power cap the saved work is time:
+// 151936 x 4096, 1 row 240 us -> 193 in a loop and 202 -> 189 (6.6 TB/s) after a pause, 16 rows 243 -> 197 and 207 -> 194, 32 rows
+// 246 -> 213 and 208 -> 204.  With more rows the hidden states, loaded once for 115 weight rows instead of 208, cost what the MMAs
+// save: 48 rows 247 -> 236 and 210 -> 216.
+struct FewPlan { int step, tiles, bn; };
+FewPlan plan_few(int64_t rows, int64_t vocab) {
+  const int64_t rounds = cdiv(vocab, int64_t(128) * kSms);
+  int64_t step = cdiv(vocab, rounds * kSms);
+  if (step < 8) step = 8;
+  return FewPlan{static_cast<int>(step), static_cast<int>(cdiv(vocab, step)), static_cast<int>(cdiv(rows, 16)) * 16};
+}
+int prepare_few(Gemm& g, const Matrix& w, const Matrix& h, const FewPlan& f) {
+  GemmParams& p = g.p;
+  p.M = w.rows;
+  p.N = h.rows;
+  p.m_tiles = f.tiles;
+  p.n_tiles = p.splits = 1;
+  p.bn = f.bn;
+  p.m_step = f.step;
+  p.k_blocks = p.kb_per_split = static_cast<int>(cdiv(w.cols, kBK));
+  p.group_m = p.behind = p.alone_rounds = 0;
+  // Stages are packed: an MMA reads 128 rows of A and bn of B whatever is loaded, at the end of the ring into the staging behind it;
+  // what the rows past the loaded ones hold reaches no result.
+  p.a_bytes = static_cast<int>(cdiv(f.step * kBK * 2, 1024)) * 1024;
+  p.stage_bytes = p.a_bytes + static_cast<int>(cdiv(h.rows * kBK * 2, 1024)) * 1024;
+  p.tx_bytes = (f.step + static_cast<int>(h.rows)) * kBK * 2;
+  const int stages = (kRingBytes + kStagingBytes - static_cast<int>(h.rows) * 512) / p.stage_bytes;
+  p.stages = stages < kMaxStages ? stages : kMaxStages;
+  int rc = bind_context();
+  if (rc == JL_OK) rc = make_map2(&g.maps.a, w.p, w.rows, w.cols, w.ld, kBK, f.step, false, 1, false);
+  if (rc == JL_OK) rc = make_map2(&g.maps.b, h.p, h.rows, h.cols, h.ld, kBK, static_cast<int>(h.rows), false, 1, false);
   return rc;
 }
 
@@ -709,6 +803,7 @@ int launch(const Gemm& g0, const Gemm& g1, cudaStream_t stream) {
 template <class P>
 int launch_one(const Gemm& g, cudaStream_t stream) { return launch<P, void>(g, g, stream); }
 
+using ScoresFew = Product<1, false, false, kEpiFew>;
 using Scores1 = Product<1, false, false, kEpiScores>;
 using Scores2 = Product<2, false, false, kEpiScores>;
 using Dz1 = Product<1, false, false, kEpiDz>;
@@ -743,12 +838,14 @@ int group_of(int64_t K, int pair) {
 // The tiles' partials take 24 bytes per row and tile; rows beyond 16384 go through the same workspace in further launches
 // (each reads the weight once more, 0.2 ms beside 14 ms of products at a hidden size of 4096).
 constexpr int64_t kScoreRows = 16384;
-struct ScoresLayout { Plan plan; size_t part, arg, picked, nll, total; };
+struct ScoresLayout { Plan plan; FewPlan few; int tiles; size_t part, arg, picked, nll, total; };      // tiles: partials of a row
 ScoresLayout scores_layout(int64_t rows, int32_t vocab) {
   ScoresLayout l;
   const int64_t n = rows < 1 ? 1 : rows < kScoreRows ? rows : kScoreRows;
   l.plan = plan_tiles(n, vocab, pair_of(n), 16 * pair_of(n));
-  const size_t parts = static_cast<size_t>(n) * l.plan.n_tiles * 2;
+  l.few = plan_few(n <= kFewRows ? n : 1, vocab);
+  l.tiles = n <= kFewRows ? l.few.tiles : l.plan.n_tiles * 2;
+  const size_t parts = static_cast<size_t>(n) * l.tiles;
   l.part = 0;
   l.arg = up256(parts * sizeof(float2));
   l.picked = l.arg + up256(parts * sizeof(int));
@@ -815,7 +912,10 @@ int launch_scores(const jl_head_scores_args* a, cudaStream_t stream) {
     p.group_m = group_of(a->hidden_size, plan.pair);
     const Matrix h{static_cast<const __nv_bfloat16*>(a->hidden) + r0 * a->hidden_stride, n, a->hidden_size, a->hidden_stride};
     const Matrix w{a->weight, a->vocab, a->hidden_size, a->weight_stride};
-    if (plan.pair == 2) {
+    if (a->rows <= kFewRows) {
+      rc = prepare_few(g, w, h, l.few);
+      if (rc == JL_OK) rc = launch_one<ScoresFew>(g, stream);
+    } else if (plan.pair == 2) {
       rc = prepare<Scores2>(g, h, w, Result{}, plan, a->hidden_size, 1);
       if (rc == JL_OK) rc = launch_one<Scores2>(g, stream);
     } else {
@@ -825,7 +925,7 @@ int launch_scores(const jl_head_scores_args* a, cudaStream_t stream) {
     if (rc != JL_OK) return rc;
     const bool few = n < 4 * kSms;
     if (launch_dependent(few ? scores_fold_kernel<8> : scores_fold_kernel<1>, dim3(static_cast<unsigned>(few ? n : cdiv(n, 8))), dim3(256), 0, stream,
-                         static_cast<const float2*>(p.part), static_cast<const int*>(p.part_arg), static_cast<const float*>(p.picked), plan.n_tiles * 2, n,
+                         static_cast<const float2*>(p.part), static_cast<const int*>(p.part_arg), static_cast<const float*>(p.picked), l.tiles, n,
                          static_cast<int64_t>(a->vocab), p.labels, a->ignore_index, nll != nullptr ? nll + r0 : nullptr,
                          a->lse != nullptr ? a->lse + r0 : nullptr, a->top != nullptr ? a->top + r0 : nullptr) != cudaSuccess)
       return check_launch("jl_head_scores (fold)");
