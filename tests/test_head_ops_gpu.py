@@ -68,6 +68,29 @@ def test_token_scores(N, H, V):
     assert only.nll is None and only.top is None and torch.equal(only.lse, got.lse)
 
 
+@pytest.mark.parametrize("N, H, V", [(1, 520, 18945), (15, 72, 20000), (16, 2056, 9001), (17, 1032, 19000), (31, 64, 5), (32, 4096, 30011), (33, 256, 30011)])
+def test_token_scores_of_few_rows(N, H, V):
+    """Up to 32 rows the weight's rows are the rows of the product: one and several tiles a CTA, a last tile that is short or empty."""
+    test_token_scores(N, H, V)
+
+
+@pytest.mark.parametrize("N", [3, 32])
+def test_few_rows_in_masked_and_strided_places(N):
+    from jetlm.kernels import head_ops
+    h, w, y = make(N, 264, 5003, ignored=0)
+    big = torch.full((2 * N, 272), math.nan, device="cuda").bfloat16()       # rows and columns that do not belong to the operand
+    big[::2, :264] = h
+    wide = torch.full((5003, 280), math.inf, device="cuda").bfloat16()
+    wide[:, :264] = w
+    want = head_ops.token_scores(h, w, y, top=True)
+    got = head_ops.token_scores(big[::2, :264], wide[:, :264], y, top=True)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    h[1, 3] = math.nan
+    got = head_ops.token_scores(h, w, y, top=True)
+    keep = [i for i in range(N) if i != 1]
+    assert torch.equal(got.lse[keep], want.lse[keep]) and torch.equal(got.top[keep], want.top[keep]) and torch.isnan(got.lse[1])
+
+
 def test_equal_logits_give_the_lowest_index():
     from jetlm.kernels import head_ops
     h = torch.ones(5, 64, device="cuda").bfloat16()
