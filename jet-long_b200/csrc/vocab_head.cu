@@ -27,7 +27,7 @@ __device__ int g_head_status = 0;            // raised when a bounded wait gave 
 constexpr int kBK = 64;                      // K step: one 128-byte swizzle row of bf16
 constexpr int kMaxBN = 256;
 constexpr int kABytes = 128 * kBK * 2;       // a CTA's 128 rows of A
-constexpr int kAccCols = 256;                // tensor-memory columns of one accumulator; two of them alternate
+constexpr int kTmemCols = 512, kMaxAccs = 4;  // accumulators take turns
 constexpr int kEpiWarps = 8;                 // two per quarter of the accumulator's rows, each with half of the columns
 constexpr int kGemmThreads = 128 + 32 * kEpiWarps;
 constexpr int kRegsLow = 72, kRegsHigh = 216;     // 128 x 72 + 256 x 216 = the launch total 384 x 168
@@ -78,7 +78,7 @@ struct alignas(64) GemmMaps { CUtensorMap a, b, out; };
 struct GemmSmem {
   alignas(1024) uint8_t ring[kRingBytes];
   alignas(1024) uint8_t staging[kStagingBytes];
-  uint64_t full[kMaxStages], empty[kMaxStages], acc_full[2], acc_free[2];
+  uint64_t full[kMaxStages], empty[kMaxStages], acc_full[kMaxAccs], acc_free[kMaxAccs];
   uint32_t tmem_base;
   int failed;
 };
@@ -171,9 +171,11 @@ struct Product {
   // the 256 steps of K = 4096 a logit lost 2^-24 of its size 256 times, up to 1e-5 in all, and so did the losses.  Scores
   // therefore take K in parts that are added in fp32 registers.  Error of the loss / time of 8191 rows x 4096 with parts of 256,
   // 512, 1024 and all of K: 2e-7 / 8.0 ms, 3.5e-7 / 7.5, 8e-7 / 7.25, 4e-6 / 7.1; a few rows are bound by the weight's bytes and
-  // take the shortest parts at no cost.  Results that are rounded to bf16 need none of this.
+  // take parts of 256, up to 32 rows parts of 128 (error of one row's lse with 64, 128, 256: 0.7e-7, 1.4e-7, 2.6e-7; time of
+  // 151936 x 2048 in a loop 102.4, 102.3, 98.4 us).  Results that are rounded to bf16 need none of this.
+  static constexpr int kAccs = kEpi_ == kEpiFew ? 4 : 2, kAccCols = kTmemCols / kAccs;
   static constexpr bool kParts = kEpi_ == kEpiScores || kEpi_ == kEpiFew;
-  static constexpr int kPart = !kParts ? 1 << 30 : kPair_ == 1 ? 4 : 8;
+  static constexpr int kPart = !kParts ? 1 << 30 : kEpi_ == kEpiFew ? 2 : kPair_ == 1 ? 4 : 8;
 };
 
 template <class P>
@@ -230,8 +232,8 @@ __device__ __forceinline__ void issue(const GemmParams& p, GemmSmem& sm, uint32_
       const bool first = kb == kb0 || (P::kParts && (kb - kb0) % P::kPart == 0);
       const bool last = kb + 1 == kb1 || (P::kParts && (kb + 1 - kb0) % P::kPart == 0);
       if (first) {
-        mbar_wait(&sm.acc_free[st.i & 1], ((st.i >> 1) & 1) ^ 1, sm);
-        acc = tmem + (st.i & 1) * kAccCols;
+        mbar_wait(&sm.acc_free[st.i % P::kAccs], ((st.i / P::kAccs) & 1) ^ 1, sm);
+        acc = tmem + (st.i % P::kAccs) * P::kAccCols;
       }
       const int s = st.slot;
       mbar_wait(&sm.full[s], st.parity, sm);
@@ -252,8 +254,8 @@ __device__ __forceinline__ void issue(const GemmParams& p, GemmSmem& sm, uint32_
         if (kPair == 2) pair::commit_both(&sm.empty[s]);
         else mma_commit(&sm.empty[s]);
         if (last) {
-          if (kPair == 2) pair::commit_both(&sm.acc_full[st.i & 1]);
-          else mma_commit(&sm.acc_full[st.i & 1]);
+          if (kPair == 2) pair::commit_both(&sm.acc_full[st.i % P::kAccs]);
+          else mma_commit(&sm.acc_full[st.i % P::kAccs]);
         }
       }
       __syncwarp();
@@ -269,8 +271,7 @@ __device__ __forceinline__ void finish(const GemmMaps& maps, const GemmParams& p
   const int quad = ew & 3, half = ew >> 2;         // rows quad * 32 .. of the accumulator, first or second half of its columns
   const uint32_t lane_base = static_cast<uint32_t>(quad * 32) << 16;
   uint8_t* const stage = sm.staging + ew * 4096;
-  const uint32_t free_bar[2] = {kPair == 2 ? pair::leader_addr(&sm.acc_free[0]) : smem_u32(&sm.acc_free[0]),
-                                kPair == 2 ? pair::leader_addr(&sm.acc_free[1]) : smem_u32(&sm.acc_free[1])};
+  const uint32_t free_bar = kPair == 2 ? pair::leader_addr(&sm.acc_free[0]) : smem_u32(&sm.acc_free[0]);
   const float scale = kEpi == kEpiBf16 ? p.scale.get() : 1.f;
   // 32 rows x 128 bytes of results: 16-byte chunk `ch` of this thread's row
   auto chunk_ptr = [&](int ch) { return reinterpret_cast<uint4*>(stage + lane * 128 + ((ch ^ (lane & 7)) << 4)); };
@@ -292,7 +293,7 @@ __device__ __forceinline__ void finish(const GemmMaps& maps, const GemmParams& p
   auto hand_back = [&]() {                         // this warp has read the accumulator
     tc_fence_before();
     __syncwarp();
-    if (lane == 0) asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(free_bar[st.i & 1]) : "memory");
+    if (lane == 0) asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(free_bar + 8 * (st.i % P::kAccs)) : "memory");
     ++st.i;
   };
   TileWalk walk(p, worker, workers);
@@ -305,32 +306,27 @@ __device__ __forceinline__ void finish(const GemmMaps& maps, const GemmParams& p
       // The tile is m_step vocabulary entries by up to 32 rows.  Its logits are summed over the parts of K in registers (a thread has
       // an entry and half of the rows) and go through shared memory to a warp per row.
       float* const zs = reinterpret_cast<float*>(sm.ring + kRingBytes + kStagingBytes - p.N * 512);      // [row][128 entries], behind the ring
-      const int half_cols = p.bn / 2, c_lo = half * half_cols;
-      float z[kFewRows / 2];
+      const int c_lo = half * 16;
+      const bool mine = c_lo < p.bn;               // up to 16 rows the second half of the warps only reduces
+      float z[16];
 #pragma unroll
-      for (int j = 0; j < kFewRows / 2; ++j) z[j] = 0.f;
-      for (int part = 0; part * P::kPart < p.k_blocks; ++part) {
-        const uint32_t acc = tmem + (st.i & 1) * kAccCols + lane_base + c_lo;
-        mbar_wait(&sm.acc_full[st.i & 1], (st.i >> 1) & 1, sm);
+      for (int j = 0; j < 16; ++j) z[j] = 0.f;
+      for (int part = 0; mine && part * P::kPart < p.k_blocks; ++part) {
+        mbar_wait(&sm.acc_full[st.i % P::kAccs], (st.i / P::kAccs) & 1, sm);
         tc_fence_after();
+        uint32_t x[16];
+        JL_TMEM_LD16(tmem + (st.i % P::kAccs) * P::kAccCols + lane_base + c_lo, x);
+        JL_TMEM_WAIT_LD16(x, 0);
 #pragma unroll
-        for (int ch = 0; ch < kFewRows / 32; ++ch) {
-          if (ch * 16 < half_cols) {               // (the last chunk may read columns past this half, which are not used)
-            uint32_t x[16];
-            JL_TMEM_LD16(acc + ch * 16, x);
-            JL_TMEM_WAIT_LD16(x, 0);
-#pragma unroll
-            for (int j = 0; j < 16; ++j) z[ch * 16 + j] += __uint_as_float(x[j]);
-          }
-        }
+        for (int j = 0; j < 16; ++j) z[j] += __uint_as_float(x[j]);
         hand_back();
       }
       const int64_t v0 = static_cast<int64_t>(c.m) * p.m_step;
       const int valid = static_cast<int>(p.M - v0 < p.m_step ? p.M - v0 : p.m_step);
       asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpiWarps) : "memory");      // the tile before has been read
 #pragma unroll
-      for (int j = 0; j < kFewRows / 2; ++j)
-        if (j < half_cols && c_lo + j < p.N) zs[(c_lo + j) * 128 + quad * 32 + lane] = quad * 32 + lane < valid ? z[j] : -INFINITY;
+      for (int j = 0; j < 16; ++j)
+        if (mine && c_lo + j < p.N) zs[(c_lo + j) * 128 + quad * 32 + lane] = quad * 32 + lane < valid ? z[j] : -INFINITY;
       asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpiWarps) : "memory");
       for (int r = ew; r < p.N; r += kEpiWarps) {
         const float4 x = *reinterpret_cast<const float4*>(zs + r * 128 + 4 * lane);
@@ -361,8 +357,8 @@ __device__ __forceinline__ void finish(const GemmMaps& maps, const GemmParams& p
 #pragma unroll
       for (int j = 0; j < 128; ++j) z[j] = 0.f;
       for (int part = 0; part * P::kPart < p.k_blocks; ++part) {
-        const uint32_t acc = tmem + (st.i & 1) * kAccCols + lane_base + c_lo;
-        mbar_wait(&sm.acc_full[st.i & 1], (st.i >> 1) & 1, sm);
+        const uint32_t acc = tmem + (st.i % P::kAccs) * P::kAccCols + lane_base + c_lo;
+        mbar_wait(&sm.acc_full[st.i % P::kAccs], (st.i / P::kAccs) & 1, sm);
         tc_fence_after();
 #pragma unroll
         for (int ch = 0; ch < 8; ++ch) {
@@ -408,8 +404,8 @@ __device__ __forceinline__ void finish(const GemmMaps& maps, const GemmParams& p
         if (y >= 0) p.picked[row] = z_y;
       }
     } else {
-      const uint32_t acc = tmem + (st.i & 1) * kAccCols + lane_base;
-      mbar_wait(&sm.acc_full[st.i & 1], (st.i >> 1) & 1, sm);
+      const uint32_t acc = tmem + (st.i % P::kAccs) * P::kAccCols + lane_base;
+      mbar_wait(&sm.acc_full[st.i % P::kAccs], (st.i / P::kAccs) & 1, sm);
       tc_fence_after();
       float lse = 0.f, factor = 0.f;
       int y = -1;
@@ -480,7 +476,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) head_gemm_kernel(const __grid
   if (threadIdx.x == 0) {
     sm.failed = *reinterpret_cast<volatile int*>(&g_head_status) != 0 ? 1 : 0;
     for (int i = 0; i < kMaxStages; ++i) { mbar_init(&sm.full[i], 1); mbar_init(&sm.empty[i], 1); }
-    for (int i = 0; i < 2; ++i) { mbar_init(&sm.acc_full[i], 1); mbar_init(&sm.acc_free[i], kEpiWarps * kPair); }
+    for (int i = 0; i < kMaxAccs; ++i) { mbar_init(&sm.acc_full[i], 1); mbar_init(&sm.acc_free[i], P0::kEpi == kEpiFew && p0.bn <= 16 ? 4 : kEpiWarps * kPair); }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 2) {
@@ -734,8 +730,8 @@ int prepare(Gemm& g, const Matrix& A, const Matrix& B, const Result& out, const 
 
 // Scores of up to 32 rows: the weight's rows are the rows of the product and the hidden states its columns, so that a tile
 // multiplies 16 columns for one row instead of 128 rows, in equal shares for all SMs.  At the power cap the saved work is time:
-// 151936 x 4096, 1 row 240 us -> 193 in a loop and 202 -> 189 (6.6 TB/s) after a pause, 16 rows 243 -> 197 and 207 -> 194, 32 rows
-// 246 -> 213 and 208 -> 204.  With more rows the hidden states, loaded once for 115 weight rows instead of 208, cost what the MMAs
+// 151936 x 4096, 1 row 240 us -> 200 in a loop and 202 -> 189 (6.6 TB/s) after a pause, 16 rows 243 -> 203 and 207 -> 193, 32 rows
+// 246 -> 218 and 208 -> 198.  With more rows the hidden states, loaded once for 115 weight rows instead of 208, cost what the MMAs
 // save: 48 rows 247 -> 236 and 210 -> 216.
 struct FewPlan { int step, tiles, bn; };
 FewPlan plan_few(int64_t rows, int64_t vocab) {
