@@ -21,6 +21,8 @@ extern "C" {
  * contiguous, 16-byte aligned; hidden size a multiple of 8.  labels (rows,) int64, may be NULL with nll NULL.
  * nll, lse, top, loss_sum, loss_count, loss_mean may each be NULL.  loss_sum = sum of nll, loss_count = number of rows
  * whose label is not ignore_index, loss_mean = their quotient (fp32 scalars, summed in a fixed order).
+ * skip_ignored != 0: rows whose label is ignore_index need no lse (theirs is 0) and may be left out of the product; needs
+ * labels, top NULL.
  * workspace: jl_head_scores_workspace_bytes, 16-byte aligned, not initialised by the caller.
  * ------------------------------------------------------------------------------------------- */
 typedef struct {
@@ -37,11 +39,12 @@ typedef struct {
   float* loss_sum;
   float* loss_count;
   float* loss_mean;
+  int32_t skip_ignored, reserved;
   void* workspace;
   size_t workspace_bytes;
 } jl_head_scores_args;
 
-size_t jl_head_scores_workspace_bytes(int64_t rows, int32_t hidden_size, int32_t vocab);
+size_t jl_head_scores_workspace_bytes(int64_t rows, int32_t hidden_size, int32_t vocab, int32_t skip_ignored);
 int jl_head_scores(const jl_head_scores_args* args, void* cuda_stream);
 
 /* ---------------------------------------------------------------------------------------------

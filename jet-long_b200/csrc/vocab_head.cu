@@ -53,6 +53,9 @@ struct GradScale {            // scalar factor of both gradients, applied to the
 
 struct GemmParams {
   int64_t M, N;               // result extents (rows of A, rows of B)
+  // Of the rows of hidden states in the product only this many are in use, NULL: all.  They start at row0 of all rows in use.
+  const int32_t* rows_used;
+  int64_t row0;
   int m_tiles, n_tiles, splits, k_blocks, kb_per_split, bn;
   int group_m;                // > 0: m fastest inside groups of this many m tiles; 0: n fastest
   int behind, alone_rounds;   // see TileWalk
@@ -136,6 +139,22 @@ __device__ __forceinline__ TileCoord tile_coord(const GemmParams& p, int t) {
     c.n = r - c.m * p.n_tiles;
   }
   return c;
+}
+
+// Cost of a tile in K blocks: its own, and about three for a short tile's hand-over.
+__host__ __device__ inline int64_t tile_cost(const GemmParams& p) { return p.kb_per_split + 3; }
+__host__ __device__ inline int64_t tiles_of(const GemmParams& p) { return static_cast<int64_t>(p.m_tiles) * p.n_tiles * p.splits; }
+
+// Shares of the second product of a launch, so that the workers that carry one tile more of the first end with the others.
+__host__ __device__ inline void balance(const GemmParams& first, GemmParams& second) {
+  const int64_t W = kSms / 2, n0 = tiles_of(first), n1 = tiles_of(second), c0 = tile_cost(first), c1 = tile_cost(second);
+  const int64_t l = n0 / W, rem = n0 % W;
+  int64_t late = ((n0 * c0 + n1 * c1) / W - (l + 1) * c0) / c1;            // rounds of the workers with l + 1 tiles
+  if (late < 0) late = 0;
+  int64_t rounds = (n1 - rem * late + W - rem - 1) / (W - rem);
+  if (rounds < late) rounds = late = (n1 + W - 1) / W;
+  second.behind = static_cast<int>(rem);
+  second.alone_rounds = static_cast<int>(rounds - late);
 }
 
 // Persistent walk of a worker over the tiles of one product.  The first `behind` workers of a launch carry one tile more of the
@@ -457,6 +476,24 @@ __device__ __forceinline__ void finish(const GemmMaps& maps, const GemmParams& p
   }
 }
 
+// The product's extents for the rows in use.  One row is kept where a result is due whatever the number (it counts for nothing).
+template <class P>
+__device__ __forceinline__ GemmParams in_use(const GemmParams& p) {
+  GemmParams q = p;
+  if (P::kPair == 2 && p.rows_used != nullptr) {               // (single CTAs have one row tile at most)
+    int64_t n = *p.rows_used - p.row0;
+    if (n < (P::kParts ? 0 : 1)) n = P::kParts ? 0 : 1;
+    if (P::kAMn) {
+      const int kb = static_cast<int>((n + kBK - 1) / kBK);
+      q.k_blocks = q.kb_per_split = kb < p.k_blocks ? kb : p.k_blocks;
+    } else {
+      const int m = static_cast<int>((n + 128 * P::kPair - 1) / (128 * P::kPair));
+      q.m_tiles = m < p.m_tiles ? m : p.m_tiles;
+    }
+  }
+  return q;
+}
+
 // C tiles (128 * kPair rows x bn columns), fp32 accumulation in tensor memory, of one product or of two that need nothing of each
 // other, the second filling the SMs that the first leaves.  kPair = 2: a cluster of two CTAs works on one tile with cta_group::2
 // MMAs, each CTA loading its own 128 rows of A and half of the rows of B, so every byte of B in shared memory serves 256 rows.
@@ -497,24 +534,30 @@ __global__ void __launch_bounds__(kGemmThreads, 1) head_gemm_kernel(const __grid
   const uint32_t tmem = sm.tmem_base;
 
   PipeState st{0, 0, 0u};
+  const GemmParams q0 = in_use<P0>(p0);
+  GemmParams q1{};
+  if constexpr (kTwo) {
+    q1 = in_use<P1>(p1);
+    if (p0.rows_used != nullptr) balance(q0, q1);
+  }
   // the control warps give registers back, the epilogue warps (128 logits of a row each) take them
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsLow));
     if (warp == 0) {
       if (lane == 0) {
-        produce<P0>(maps0, p0, sm, rank, worker, workers, st);
-        if constexpr (kTwo) produce<P1>(maps1, p1, sm, rank, worker, workers, st);
+        produce<P0>(maps0, q0, sm, rank, worker, workers, st);
+        if constexpr (kTwo) produce<P1>(maps1, q1, sm, rank, worker, workers, st);
       }
     } else if (warp == 1 && rank == 0) {
       uint32_t leader;
       asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(leader));
-      issue<P0>(p0, sm, tmem, leader, worker, workers, st);
-      if constexpr (kTwo) issue<P1>(p1, sm, tmem, leader, worker, workers, st);
+      issue<P0>(q0, sm, tmem, leader, worker, workers, st);
+      if constexpr (kTwo) issue<P1>(q1, sm, tmem, leader, worker, workers, st);
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsHigh));
-    finish<P0>(maps0, p0, sm, tmem, warp - 4, lane, rank, worker, workers, st);
-    if constexpr (kTwo) finish<P1>(maps1, p1, sm, tmem, warp - 4, lane, rank, worker, workers, st);
+    finish<P0>(maps0, q0, sm, tmem, warp - 4, lane, rank, worker, workers, st);
+    if constexpr (kTwo) finish<P1>(maps1, q1, sm, tmem, warp - 4, lane, rank, worker, workers, st);
     if (lane == 0) bulk_wait_all();
   }
 
@@ -544,7 +587,8 @@ __device__ __forceinline__ void join_scores(float& m, float& s, int& arg, float 
 // one warp 14 us).  Every lane reads 4 partials at a time.
 template <int kWarps>
 __global__ void __launch_bounds__(256) scores_fold_kernel(const float2* part, const int* part_arg, const float* picked, int tiles, int64_t N, int64_t V,
-                                                          const int64_t* labels, int64_t ignore, float* nll, float* lse, int64_t* top) {
+                                                          const int64_t* labels, int64_t ignore, float* nll, float* lse, int64_t* top,
+                                                          const int32_t* rows_used, const int32_t* place, int64_t row0) {
   __shared__ float sm[8], ss[8];
   __shared__ int sa[8];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -553,6 +597,7 @@ __global__ void __launch_bounds__(256) scores_fold_kernel(const float2* part, co
   launch_dependents();
   float m = -INFINITY, s = 0.f;
   int arg = 0x7fffffff;
+  if (rows_used != nullptr && *rows_used - row0 < N) N = *rows_used - row0;
   if (row < N) {
     for (int i0 = (warp % kWarps) * 32 + lane; i0 < tiles; i0 += 4 * 32 * kWarps) {
       float2 p[4];
@@ -578,12 +623,13 @@ __global__ void __launch_bounds__(256) scores_fold_kernel(const float2* part, co
   }
   if (lane != 0 || row >= N) return;
   const float l = m + logf(s);
-  if (lse != nullptr) lse[row] = l;
+  const int64_t at = place != nullptr ? place[row0 + row] : row;
+  if (lse != nullptr) lse[at] = l;
   if (top != nullptr) top[row] = arg == 0x7fffffff ? 0 : arg;
   if (nll != nullptr) {
     const int64_t y = labels[row];
     // (m - z_y) + log s, not lse - z_y: a small loss keeps its digits
-    nll[row] = y == ignore ? 0.f : (y >= 0 && y < V ? (m - picked[row]) + logf(s) : __int_as_float(0x7fc00000));
+    nll[at] = y == ignore ? 0.f : (y >= 0 && y < V ? (m - picked[row]) + logf(s) : __int_as_float(0x7fc00000));
   }
 }
 
@@ -610,18 +656,109 @@ __global__ void __launch_bounds__(1024) loss_sum_kernel(const float* nll, const 
   if (mean != nullptr) *mean = s / c;
 }
 
-// d_hidden = scale * (sum of the K splits' fp32 results), rounded once; 4 values a thread
-__global__ void __launch_bounds__(256) grad_round_kernel(const float* x, int splits, int64_t n, __nv_bfloat16* out, GradScale g) {
+// d_hidden = scale * (sum of the K splits' fp32 results), rounded once; 4 values a thread.  place: where a row's results are (NULL:
+// at the row itself), -1: it has none.
+__global__ void __launch_bounds__(256) grad_round_kernel(const float* x, int splits, int64_t n, __nv_bfloat16* out, GradScale g, const int32_t* place,
+                                                         int row_len) {
   const int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 4;
   wait_prerequisites();
   if (i >= n) return;
-  float4 a = *reinterpret_cast<const float4*>(x + i);
+  int64_t from = i;
+  if (place != nullptr) {
+    const int64_t row = i / row_len;
+    const int32_t at = place[row];
+    if (at < 0) {
+      *reinterpret_cast<uint2*>(out + i) = make_uint2(0u, 0u);
+      return;
+    }
+    from += (at - row) * row_len;
+  }
+  float4 a = *reinterpret_cast<const float4*>(x + from);
   for (int s = 1; s < splits; ++s) {
-    const float4 b = *reinterpret_cast<const float4*>(x + s * n + i);
+    const float4 b = *reinterpret_cast<const float4*>(x + s * n + from);
     a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w;
   }
   const float c = g.get();
   *reinterpret_cast<uint2*>(out + i) = make_uint2(pack_bf16x2(a.x * c, a.y * c), pack_bf16x2(a.z * c, a.w * c));
+}
+
+// Rows that count: row_of[r] is the r-th row whose label is not `ignore`, place[i] the r of row i or -1, *used their number.
+// What does not count gets nll = lse = 0 (where asked for).  One block; 8192 rows a round.
+__global__ void __launch_bounds__(1024) rows_used_kernel(const int64_t* labels, int64_t ignore, int64_t N, int32_t* row_of, int32_t* place, int32_t* used,
+                                                         float* nll, float* lse) {
+  __shared__ int before[8 * 32];                   // counts of (chunk of 1024 rows, warp), then their prefix sums
+  __shared__ int base;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) base = 0;
+  wait_prerequisites();
+  launch_dependents();
+  for (int64_t i0 = 0; i0 < N; i0 += 8192) {
+    uint32_t votes[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int64_t i = i0 + j * 1024 + threadIdx.x;
+      votes[j] = __ballot_sync(0xffffffffu, i < N && labels[i] != ignore);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (lane == 0) before[j * 32 + warp] = __popc(votes[j]);
+    __syncthreads();
+    if (warp == 0) {
+      int c[8], sum = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) { c[j] = before[lane * 8 + j]; sum += c[j]; }
+      int incl = sum;
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const int o = __shfl_up_sync(0xffffffffu, incl, off);
+        if (lane >= off) incl += o;
+      }
+      int at = base + incl - sum;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) { before[lane * 8 + j] = at; at += c[j]; }
+      __syncwarp();
+      if (lane == 31) base = at;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int64_t i = i0 + j * 1024 + threadIdx.x;
+      const bool in = (votes[j] >> lane) & 1u;
+      const int r = before[j * 32 + warp] + __popc(votes[j] & ((1u << lane) - 1u));
+      if (i < N) {
+        place[i] = in ? r : -1;
+        if (in) {
+          row_of[r] = static_cast<int32_t>(i);
+        } else {
+          if (nll != nullptr) nll[i] = 0.f;
+          if (lse != nullptr) lse[i] = 0.f;
+        }
+      }
+    }
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) *used = base;
+}
+
+// Rows row0 .. row0 + gridDim.x of those in use, packed: hidden states, labels and, where given, lse and row gradients.  Up to the
+// next multiple of 64 (a K block of the weight's gradient) the rows after the last are zero; every label after it is `ignore`.
+__global__ void __launch_bounds__(128) rows_gather_kernel(const __nv_bfloat16* hidden, int64_t stride, int row_len, const int64_t* labels, int64_t ignore,
+                                                          const float* lse, const float* row_grad, const int32_t* row_of, const int32_t* used, int64_t row0,
+                                                          __nv_bfloat16* hidden_out, int64_t* labels_out, float* lse_out, float* row_grad_out) {
+  wait_prerequisites();
+  launch_dependents();
+  const int64_t r = row0 + blockIdx.x, n = *used;
+  const bool in = r < n;
+  const int64_t from = in ? row_of[r] : 0;
+  if (threadIdx.x == 0) {
+    labels_out[blockIdx.x] = in ? labels[from] : ignore;
+    if (lse != nullptr) lse_out[blockIdx.x] = in ? lse[from] : 0.f;
+    if (row_grad != nullptr) row_grad_out[blockIdx.x] = in ? row_grad[from] : 0.f;
+  }
+  if (r >= (n + kBK - 1) / kBK * kBK && r >= kBK) return;
+  const uint4* src = reinterpret_cast<const uint4*>(hidden + from * stride);
+  uint4* dst = reinterpret_cast<uint4*>(hidden_out + static_cast<int64_t>(blockIdx.x) * row_len);
+  for (int c = threadIdx.x; c < row_len / 8; c += 128) dst[c] = in ? src[c] : make_uint4(0u, 0u, 0u, 0u);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -763,8 +900,6 @@ int prepare_few(Gemm& g, const Matrix& w, const Matrix& h, const FewPlan& f) {
   return rc;
 }
 
-int64_t tiles_of(const GemmParams& p) { return static_cast<int64_t>(p.m_tiles) * p.n_tiles * p.splits; }
-
 template <class P0, class P1>
 int launch(const Gemm& g0, const Gemm& g1, cudaStream_t stream) {
   constexpr int kPair = P0::kPair;
@@ -808,21 +943,6 @@ using Dh1 = Product<1, false, true, kEpiF32>;
 using Dh2 = Product<2, false, true, kEpiF32>;
 using Dw2 = Product<2, true, true, kEpiBf16>;
 
-// Cost of a tile in K blocks: its own, and about three for a short tile's hand-over.
-int64_t tile_cost(const GemmParams& p) { return p.kb_per_split + 3; }
-
-// Shares of the second product of a launch, so that the workers that carry one tile more of the first end with the others.
-void balance(const Gemm& first, Gemm& second) {
-  const int64_t W = kSms / 2, n0 = tiles_of(first.p), n1 = tiles_of(second.p), c0 = tile_cost(first.p), c1 = tile_cost(second.p);
-  const int64_t l = n0 / W, rem = n0 % W;
-  int64_t late = ((n0 * c0 + n1 * c1) / W - (l + 1) * c0) / c1;            // rounds of the workers with l + 1 tiles
-  if (late < 0) late = 0;
-  int64_t rounds = cdiv(n1 - rem * late, W - rem);
-  if (rounds < late) rounds = late = cdiv(n1, W);
-  second.p.behind = static_cast<int>(rem);
-  second.p.alone_rounds = static_cast<int>(rounds - late);
-}
-
 int pair_of(int64_t rows) { return rows > 128 ? 2 : 1; }
 
 // Rows of m tiles whose A panel stays in L2 beside the streamed B: 40 MB of hidden states.
@@ -834,8 +954,24 @@ int group_of(int64_t K, int pair) {
 // The tiles' partials take 24 bytes per row and tile; rows beyond 16384 go through the same workspace in further launches
 // (each reads the weight once more, 0.2 ms beside 14 ms of products at a hidden size of 4096).
 constexpr int64_t kScoreRows = 16384;
-struct ScoresLayout { Plan plan; FewPlan few; int tiles; size_t part, arg, picked, nll, total; };      // tiles: partials of a row
-ScoresLayout scores_layout(int64_t rows, int32_t vocab) {
+// Rows whose label is ignored are left out of the products where there are more row tiles than one: the others are packed first
+// (1000 rows x 4096 x 151936, two in five ignored: loss and gradients 3.58 -> 2.69 ms after a pause, 4.10 -> 3.10 in a loop).
+constexpr int64_t kPackRows = 257;
+struct Packed { size_t hidden, labels, lse, row_grad, row_of, place, used; };      // offsets in the workspace
+Packed packed_layout(size_t& total, int64_t rows, int64_t chunk, int32_t hd) {
+  Packed k{};
+  auto take = [&](int64_t bytes) { const size_t at = total; total += up256(static_cast<size_t>(bytes)); return at; };
+  k.hidden = take(chunk * hd * 2);
+  k.labels = take(chunk * 8);
+  k.lse = take(chunk * 4);
+  k.row_grad = take(chunk * 4);
+  k.row_of = take(rows * 4);
+  k.place = take(rows * 4);
+  k.used = take(4);
+  return k;
+}
+struct ScoresLayout { Plan plan; FewPlan few; int tiles; size_t part, arg, picked, nll, total; bool pack; Packed packed; };      // tiles: partials of a row
+ScoresLayout scores_layout(int64_t rows, int32_t hd, int32_t vocab, bool skip_ignored) {
   ScoresLayout l;
   const int64_t n = rows < 1 ? 1 : rows < kScoreRows ? rows : kScoreRows;
   l.plan = plan_tiles(n, vocab, pair_of(n), 16 * pair_of(n));
@@ -847,12 +983,14 @@ ScoresLayout scores_layout(int64_t rows, int32_t vocab) {
   l.picked = l.arg + up256(parts * sizeof(int));
   l.nll = l.picked + up256(n * sizeof(float));
   l.total = l.nll + up256(static_cast<size_t>(rows) * sizeof(float));
+  l.pack = skip_ignored && rows >= kPackRows;
+  if (l.pack) l.packed = packed_layout(l.total, rows, n, hd);
   return l;
 }
 
 // Pieces of the vocabulary in the gradient pass: as large as 256 MB of dz allow (fewer, longer launches), balanced, a
 // multiple of 256.
-struct GradsLayout { int64_t piece; Plan dz, dh, dw; int splits; size_t dh32, total; };
+struct GradsLayout { int64_t piece; Plan dz, dh, dw; int splits; size_t dh32, total; bool pack; Packed packed; };
 GradsLayout grads_layout(int64_t rows, int32_t hd, int32_t vocab) {
   GradsLayout l;
   const int64_t n = rows > 0 ? rows : 1;
@@ -865,6 +1003,8 @@ GradsLayout grads_layout(int64_t rows, int32_t hd, int32_t vocab) {
   l.dh = plan_split(n, hd, pair_of(n), cdiv(l.piece, kBK), l.splits);
   l.dh32 = up256(static_cast<size_t>(n) * l.piece * 2);
   l.total = l.dh32 + up256(static_cast<size_t>(n) * hd * 4 * l.splits);
+  l.pack = rows >= kPackRows;
+  if (l.pack) l.packed = packed_layout(l.total, rows, rows, hd);
   return l;
 }
 
@@ -886,7 +1026,9 @@ int launch_scores(const jl_head_scores_args* a, cudaStream_t stream) {
   const bool want_loss = a->loss_sum != nullptr || a->loss_count != nullptr || a->loss_mean != nullptr;
   if (a->labels == nullptr && (a->nll != nullptr || want_loss))
     return fail(JL_ERR_BAD_ARG, "jl_head_scores: nll and the loss need labels");
-  const ScoresLayout l = scores_layout(a->rows, a->vocab);
+  if (a->skip_ignored && (a->labels == nullptr || a->top != nullptr))
+    return fail(JL_ERR_BAD_ARG, "jl_head_scores: skip_ignored needs labels and leaves no top");
+  const ScoresLayout l = scores_layout(a->rows, a->hidden_size, a->vocab, a->skip_ignored != 0);
   if (a->workspace == nullptr || a->workspace_bytes < l.total)
     return fail(JL_ERR_WORKSPACE, "jl_head_scores: workspace of %zu bytes needed, %zu given", l.total, a->workspace_bytes);
   if (reinterpret_cast<uintptr_t>(a->workspace) & 15) return fail(JL_ERR_BAD_ARG, "jl_head_scores: workspace not 16-byte aligned");
@@ -894,6 +1036,13 @@ int launch_scores(const jl_head_scores_args* a, cudaStream_t stream) {
   if (rc != JL_OK) return rc;
   uint8_t* ws = static_cast<uint8_t*>(a->workspace);
   float* nll = a->nll != nullptr || !want_loss ? a->nll : reinterpret_cast<float*>(ws + l.nll);
+  int32_t *const row_of = reinterpret_cast<int32_t*>(ws + l.packed.row_of), *const place = reinterpret_cast<int32_t*>(ws + l.packed.place),
+          *const used = reinterpret_cast<int32_t*>(ws + l.packed.used);
+  int64_t* const labels_packed = reinterpret_cast<int64_t*>(ws + l.packed.labels);
+  __nv_bfloat16* const hidden_packed = reinterpret_cast<__nv_bfloat16*>(ws + l.packed.hidden);
+  if (l.pack && launch_dependent(rows_used_kernel, dim3(1), dim3(1024), 0, stream, a->labels, a->ignore_index, a->rows, row_of, place, used, nll, a->lse) !=
+                    cudaSuccess)
+    return check_launch("jl_head_scores (rows in use)");
   for (int64_t r0 = 0; r0 < a->rows; r0 += kScoreRows) {
     const int64_t n = a->rows - r0 < kScoreRows ? a->rows - r0 : kScoreRows;
     Plan plan = l.plan;
@@ -903,10 +1052,18 @@ int launch_scores(const jl_head_scores_args* a, cudaStream_t stream) {
     p.part = reinterpret_cast<float2*>(ws + l.part);
     p.part_arg = a->top != nullptr ? reinterpret_cast<int*>(ws + l.arg) : nullptr;
     p.picked = reinterpret_cast<float*>(ws + l.picked);
-    p.labels = a->labels != nullptr ? a->labels + r0 : nullptr;
+    p.labels = l.pack ? labels_packed : a->labels != nullptr ? a->labels + r0 : nullptr;
     p.ignore = a->ignore_index; p.vocab = a->vocab;
     p.group_m = group_of(a->hidden_size, plan.pair);
-    const Matrix h{static_cast<const __nv_bfloat16*>(a->hidden) + r0 * a->hidden_stride, n, a->hidden_size, a->hidden_stride};
+    p.rows_used = l.pack ? used : nullptr;
+    p.row0 = r0;
+    if (l.pack && launch_dependent(rows_gather_kernel, dim3(static_cast<unsigned>(n)), dim3(128), 0, stream, static_cast<const __nv_bfloat16*>(a->hidden),
+                                   a->hidden_stride, a->hidden_size, a->labels, a->ignore_index, static_cast<const float*>(nullptr),
+                                   static_cast<const float*>(nullptr), static_cast<const int32_t*>(row_of), static_cast<const int32_t*>(used), r0, hidden_packed,
+                                   labels_packed, static_cast<float*>(nullptr), static_cast<float*>(nullptr)) != cudaSuccess)
+      return check_launch("jl_head_scores (packing)");
+    const Matrix h = l.pack ? Matrix{hidden_packed, n, a->hidden_size, a->hidden_size}
+                            : Matrix{static_cast<const __nv_bfloat16*>(a->hidden) + r0 * a->hidden_stride, n, a->hidden_size, a->hidden_stride};
     const Matrix w{a->weight, a->vocab, a->hidden_size, a->weight_stride};
     if (a->rows <= kFewRows) {
       rc = prepare_few(g, w, h, l.few);
@@ -922,8 +1079,9 @@ int launch_scores(const jl_head_scores_args* a, cudaStream_t stream) {
     const bool few = n < 4 * kSms;
     if (launch_dependent(few ? scores_fold_kernel<8> : scores_fold_kernel<1>, dim3(static_cast<unsigned>(few ? n : cdiv(n, 8))), dim3(256), 0, stream,
                          static_cast<const float2*>(p.part), static_cast<const int*>(p.part_arg), static_cast<const float*>(p.picked), l.tiles, n,
-                         static_cast<int64_t>(a->vocab), p.labels, a->ignore_index, nll != nullptr ? nll + r0 : nullptr,
-                         a->lse != nullptr ? a->lse + r0 : nullptr, a->top != nullptr ? a->top + r0 : nullptr) != cudaSuccess)
+                         static_cast<int64_t>(a->vocab), p.labels, a->ignore_index, nll != nullptr ? nll + (l.pack ? 0 : r0) : nullptr,
+                         a->lse != nullptr ? a->lse + (l.pack ? 0 : r0) : nullptr, a->top != nullptr ? a->top + r0 : nullptr, p.rows_used,
+                         l.pack ? static_cast<const int32_t*>(row_of) : nullptr, r0) != cudaSuccess)
       return check_launch("jl_head_scores (fold)");
   }
   if (want_loss && launch_dependent(loss_sum_kernel, dim3(1), dim3(1024), 0, stream, static_cast<const float*>(nll), a->labels, a->ignore_index, a->rows,
@@ -957,7 +1115,27 @@ int launch_grads(const jl_head_grads_args* a, cudaStream_t stream) {
   base.lse = a->lse;
   base.row_grad = a->grad_stride != 0 ? a->grad : nullptr;
   base.scale = GradScale{a->grad, a->grad_count, a->grad_stride != 0};
-  const Matrix h{a->hidden, N, H, a->hidden_stride};
+  Matrix h{a->hidden, N, H, a->hidden_stride};
+  const int32_t* place = nullptr;
+  if (l.pack) {
+    int32_t *const row_of = reinterpret_cast<int32_t*>(ws + l.packed.row_of), *const used = reinterpret_cast<int32_t*>(ws + l.packed.used);
+    int64_t* const labels = reinterpret_cast<int64_t*>(ws + l.packed.labels);
+    float *const lse = reinterpret_cast<float*>(ws + l.packed.lse), *const row_grad = reinterpret_cast<float*>(ws + l.packed.row_grad);
+    __nv_bfloat16* const hidden = reinterpret_cast<__nv_bfloat16*>(ws + l.packed.hidden);
+    place = reinterpret_cast<int32_t*>(ws + l.packed.place);
+    if (launch_dependent(rows_used_kernel, dim3(1), dim3(1024), 0, stream, a->labels, a->ignore_index, N, row_of, const_cast<int32_t*>(place), used,
+                         static_cast<float*>(nullptr), static_cast<float*>(nullptr)) != cudaSuccess)
+      return check_launch("jl_head_grads (rows in use)");
+    if (launch_dependent(rows_gather_kernel, dim3(static_cast<unsigned>(N)), dim3(128), 0, stream, static_cast<const __nv_bfloat16*>(a->hidden),
+                         a->hidden_stride, a->hidden_size, a->labels, a->ignore_index, a->lse, base.row_grad, static_cast<const int32_t*>(row_of),
+                         static_cast<const int32_t*>(used), int64_t(0), hidden, labels, lse, row_grad) != cudaSuccess)
+      return check_launch("jl_head_grads (packing)");
+    base.labels = labels;
+    base.lse = lse;
+    if (base.row_grad != nullptr) base.row_grad = row_grad;
+    base.rows_used = used;
+    h = Matrix{hidden, N, H, H};
+  }
   int splits = 1;
   for (int64_t v0 = 0; v0 < V; v0 += l.piece) {
     const int64_t piece = V - v0 < l.piece ? V - v0 : l.piece;
@@ -994,7 +1172,7 @@ int launch_grads(const jl_head_grads_args* a, cudaStream_t stream) {
     }
     if (rc == JL_OK && a->d_hidden != nullptr && a->d_weight != nullptr && l.dh.pair == 2) {
       // dh has few, long tiles (160 on 74 pairs for 4096 rows x 2560: 72 % of three rounds); dW's many short ones fill in
-      balance(dh, dw);
+      balance(dh.p, dw.p);
       rc = launch<Dh2, Dw2>(dh, dw, stream);
     } else {
       if (rc == JL_OK && a->d_hidden != nullptr) rc = l.dh.pair == 2 ? launch_one<Dh2>(dh, stream) : launch_one<Dh1>(dh, stream);
@@ -1004,7 +1182,7 @@ int launch_grads(const jl_head_grads_args* a, cudaStream_t stream) {
   }
   if (a->d_hidden != nullptr &&
       launch_dependent(grad_round_kernel, dim3(static_cast<unsigned>(cdiv(N * H, 1024))), dim3(256), 0, stream, static_cast<const float*>(dh32), splits, N * H,
-                       static_cast<__nv_bfloat16*>(a->d_hidden), base.scale) != cudaSuccess)
+                       static_cast<__nv_bfloat16*>(a->d_hidden), base.scale, place, a->hidden_size) != cudaSuccess)
     return check_launch("jl_head_grads (rounding)");
   return JL_OK;
 }
@@ -1015,8 +1193,8 @@ int launch_grads(const jl_head_grads_args* a, cudaStream_t stream) {
 
 extern "C" {
 
-size_t jl_head_scores_workspace_bytes(int64_t rows, int32_t hidden_size, int32_t vocab) {
-  return rows < 0 || hidden_size < 1 || vocab < 1 ? 0 : jl::scores_layout(rows, vocab).total + 256;
+size_t jl_head_scores_workspace_bytes(int64_t rows, int32_t hidden_size, int32_t vocab, int32_t skip_ignored) {
+  return rows < 0 || hidden_size < 1 || vocab < 1 ? 0 : jl::scores_layout(rows, hidden_size, vocab, skip_ignored != 0).total + 256;
 }
 
 int jl_head_scores(const jl_head_scores_args* args, void* cuda_stream) {

@@ -221,7 +221,7 @@ class HeadScoresArgs(C.Structure):
         ("hidden", C.c_void_p), ("weight", C.c_void_p), ("hidden_stride", C.c_int64), ("weight_stride", C.c_int64),
         ("labels", C.c_void_p), ("ignore_index", C.c_int64), ("rows", C.c_int64), ("hidden_size", C.c_int32), ("vocab", C.c_int32),
         ("nll", C.c_void_p), ("lse", C.c_void_p), ("top", C.c_void_p), ("loss_sum", C.c_void_p), ("loss_count", C.c_void_p),
-        ("loss_mean", C.c_void_p),
+        ("loss_mean", C.c_void_p), ("skip_ignored", C.c_int32), ("reserved", C.c_int32),
         ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
     ]
 
@@ -236,7 +236,7 @@ class HeadGradsArgs(C.Structure):
 
 
 HEAD_EXPORTS = [
-    ("jl_head_scores_workspace_bytes", C.c_size_t, [C.c_int64, C.c_int32, C.c_int32]),
+    ("jl_head_scores_workspace_bytes", C.c_size_t, [C.c_int64, C.c_int32, C.c_int32, C.c_int32]),
     ("jl_head_scores", C.c_int, [C.POINTER(HeadScoresArgs), C.c_void_p]),
     ("jl_head_grads_workspace_bytes", C.c_size_t, [C.c_int64, C.c_int32, C.c_int32]),
     ("jl_head_grads", C.c_int, [C.POINTER(HeadGradsArgs), C.c_void_p]),

@@ -66,19 +66,19 @@ def _row_stride(t: torch.Tensor) -> int:
     return t.stride(0) if rows > 1 else cols
 
 
-def _scores(h, w, labels, ignore_index, *, nll, top, reduction=None):
+def _scores(h, w, labels, ignore_index, *, nll, top, reduction=None, skip_ignored=0):
     """One jl_head_scores call on (rows, H) operands; returns (nll, lse, top, loss, loss_count), None where not asked for."""
     n, dev, a = h.shape[0], h.device, N.HeadScoresArgs()
     per_row = torch.empty(2 if nll else 1, n, dtype=torch.float32, device=dev)
     best = torch.empty(n, dtype=torch.int64, device=dev) if top else None
     scalars = torch.empty(2, dtype=torch.float32, device=dev) if reduction is not None else None
     lib = N.lib()
-    ws = torch.empty(lib.jl_head_scores_workspace_bytes(n, w.shape[1], w.shape[0]), dtype=torch.uint8, device=dev)
+    ws = torch.empty(lib.jl_head_scores_workspace_bytes(n, w.shape[1], w.shape[0], skip_ignored), dtype=torch.uint8, device=dev)
     a.weight, a.hidden_stride, a.weight_stride, a.ignore_index = w.data_ptr(), _row_stride(h), _row_stride(w), int(ignore_index)
     a.hidden, a.rows, a.hidden_size, a.vocab = h.data_ptr() or a.weight, n, w.shape[1], w.shape[0]
     if labels is not None:
         a.labels = labels.data_ptr() or a.weight                # no rows: never read
-    a.lse = per_row.data_ptr()
+    a.lse, a.skip_ignored = per_row.data_ptr(), skip_ignored
     if nll:
         a.nll = a.lse + 4 * n if n else a.weight
     if top:
@@ -113,7 +113,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
     def forward(ctx, hidden, weight, labels, ignore_index, reduction):
         h, lab = _rows("linear_cross_entropy", hidden, weight, labels)
         per_row = reduction == "none"
-        nll, lse, _, loss, count = _scores(h, weight, lab, ignore_index, nll=per_row, top=False, reduction=None if per_row else reduction)
+        nll, lse, _, loss, count = _scores(h, weight, lab, ignore_index, nll=per_row, top=False, reduction=None if per_row else reduction, skip_ignored=1)
         ctx.save_for_backward(h, weight, lab, lse, count if reduction == "mean" else None)
         ctx.ignore_index, ctx.per_row, ctx.shape = int(ignore_index), per_row, hidden.shape
         return nll.view(labels.shape) if per_row else loss
@@ -149,6 +149,7 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, labels: tor
     (V, H) bf16, labels (...) int64; reduction "mean" (over the labels that are not ignore_index; NaN if there is none, as
     in torch), "sum" or "none" (shape of labels).  The loss is fp32, the gradients are bf16.  The backward pass holds one
     piece of the vocabulary of d logits, in bf16; both gradients accumulate in fp32 and do not vary from run to run.
+    Rows whose label is ignore_index take no part: with more than 256 rows the others are packed and only they are multiplied.
     A label that is neither ignore_index nor in [0, V) makes the loss and the gradients NaN; nothing is read out of range.
     Both passes can be captured into a CUDA graph (with torch.autograd.grad, or .backward() while no eager graph of the
     same leaves is alive)."""

@@ -113,14 +113,15 @@ def test_c_entries_refuse_before_they_touch_a_device():
         a.hidden = a.weight = a.labels = a.nll = a.workspace = 1024
         a.hidden_stride = a.weight_stride = a.hidden_size = 64
         a.rows, a.vocab = 3, 100
-        a.workspace_bytes = lib.jl_head_scores_workspace_bytes(3, 64, 100)
+        a.workspace_bytes = lib.jl_head_scores_workspace_bytes(3, 64, 100, 0)
         for k, v in kw.items():
             setattr(a, k, v)
         return lib.jl_head_scores(C.byref(a), None)
 
     for want, kw in [(bad, dict(rows=-1)), (bad, dict(vocab=0)), (no, dict(hidden_size=60)), (bad, dict(hidden_stride=68)), (bad, dict(weight_stride=56)),
                      (bad, dict(labels=None)), (bad, dict(hidden=1032)), (n.JL_ERR_WORKSPACE, dict(workspace_bytes=16)),
-                     (n.JL_ERR_WORKSPACE, dict(workspace=None)), (no, dict(rows=(1 << 22) + 1))]:
+                     (n.JL_ERR_WORKSPACE, dict(workspace=None)), (no, dict(rows=(1 << 22) + 1)),
+                     (bad, dict(skip_ignored=1, top=1024)), (bad, dict(skip_ignored=1, labels=None, nll=None))]:
         assert scores(**kw) == want, kw
 
     def grads(**kw):

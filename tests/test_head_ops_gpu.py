@@ -125,6 +125,36 @@ def test_loss_and_gradients(N, H, V, reduction):
     assert (dh[y < 0] == 0).all()
 
 
+@pytest.mark.parametrize("counted", [0, 1, 63, 64, 65, 255, 256, 257, 511, 512, 513, 700])
+@pytest.mark.parametrize("ignore", [-100, 7])
+def test_rows_that_do_not_count_are_left_out(counted, ignore):
+    """700 rows, of which `counted` at random places count; the others hold NaN.  They have no loss and no gradient."""
+    from jetlm.kernels import head_ops
+    N, H, V = 700, 136, 3001
+    h, w, y = make(N, H, V, ignored=0)
+    y = torch.where(y == ignore, ignore + 1, y)
+    perm = torch.randperm(N, generator=torch.Generator().manual_seed(counted)).cuda()
+    used, rest = perm[:counted].sort().values, perm[counted:]
+    y[rest] = ignore
+    dirty = h.clone()
+    dirty[rest] = math.nan
+    dirty.requires_grad_(True)
+    w.requires_grad_(True)
+    nll = head_ops.linear_cross_entropy(dirty, w, y, ignore_index=ignore, reduction="none")
+    loss = head_ops.linear_cross_entropy(dirty, w, y, ignore_index=ignore, reduction="sum")
+    up = torch.randn(N, generator=torch.Generator().manual_seed(5)).cuda()
+    dh, dw = torch.autograd.grad(nll, [dirty, w], up)
+    _, _, dz, _, wdh, wdw, b_h, b_w = exact(h[used], w.detach(), y[used] if ignore < 0 else y[used].clone(), up[used])
+    lse, want, dz, _ = exact(h[used], w.detach(), y[used])
+    tol = 4 * dz + 2.0 ** -19 * (1 + lse.abs())
+    assert (nll[rest] == 0).all() and (dh[rest] == 0).all()
+    assert ((nll[used].double() - want).abs() <= tol).all()
+    assert abs(float(loss.detach()) - float(want.sum())) <= float(tol.sum()) + (N + 4) * F32 * float(want.abs().sum())
+    assert ((dh[used].double() - wdh).abs() <= b_h).all() and ((dw.double() - wdw).abs() <= b_w).all()
+    mean = head_ops.linear_cross_entropy(dirty, w, y, ignore_index=ignore)
+    assert torch.isnan(mean) if counted == 0 else abs(float(mean.detach()) * counted - float(loss.detach())) <= 4 * F32 * abs(float(loss.detach())) + 1e-30
+
+
 def test_gradient_agrees_with_differences():
     """d loss / d direction from the gradients against the loss itself moved by bf16-exact steps."""
     from jetlm.kernels import head_ops
