@@ -50,7 +50,7 @@ struct TreeParams {
   float scale_log2;
   const int32_t *lens, *depth;
   const uint64_t* mask;
-  float *part_o, *part_lse;    // [slot][state or tile] of [32 column groups][rpt rows][4] and [rpt rows]
+  float *part_o, *part_lse;    // [slot] (two row tiles: [slot][tile]) of [32 column groups][rpt rows][4] and [rpt rows]
   __nv_bfloat16* out;
   float* lse;
   int64_t os_b, os_s, os_h;
@@ -68,6 +68,7 @@ struct TreeSmem {
   uint64_t q_full[2], q_free[2], full[kStages], empty[kStages];
   uint64_t s_full[2], p_half[2][2], pv_done[2];
   alignas(16) int4 visit[kVisitRing];        // flags, sample, node index of the key tile's first row
+  float2 stats[2][128];                      // two states of one tile meet: reference maximum and sum of each row
   int64_t lo, hi;                            // this CTA's part of the line
   int start_b, start_kvh, start_v;
   uint32_t tmem_base;
@@ -133,7 +134,11 @@ struct RingPos {
 
 __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __grid_constant__ TreeMaps maps, const TreeParams p) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  TreeSmem& sm = *reinterpret_cast<TreeSmem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  TreeSmem& sm = *reinterpret_cast<TreeSmem*>(smem_raw);
+  if (smem_u32(smem_raw) & 1023) {               // not seen: the array's alignment is declared
+    if (threadIdx.x == 0) atomicExch(&g_tree_status, 1);
+    return;
+  }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int mb = static_cast<int>(blockIdx.x) % p.mbs, worker = static_cast<int>(blockIdx.x) / p.mbs;
   if (threadIdx.x >= 64 && threadIdx.x < 69) {   // the tensor maps: q[0], q[1], k[0], k[1], v
@@ -306,15 +311,24 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                                        *reinterpret_cast<volatile int*>(&sm.visit[g % kVisitRing].z), 0);
           if (__any_sync(0xffffffffu, visit.x & kTail)) {
             // value rows that belong to no node may hold anything, and 0 * NaN is NaN
-#pragma unroll 1
-            for (int r0 = 0; r0 < kTileN; r0 += 32) {
-              const int u = visit.z + r0 + lane;
-              const bool keep = u < 0 || (u < p.nodes && p.depth[static_cast<int64_t>(visit.y) * p.nodes + u] >= 0);
-              const uint32_t dead = __ballot_sync(0xffffffffu, !keep);
-              if (dead == 0u) continue;
+            int dep[kTileN / 32];                      // together: one latency instead of four
+#pragma unroll
+            for (int i = 0; i < kTileN / 32; ++i) {
+              const int u = visit.z + i * 32 + lane;
+              dep[i] = u < 0 ? 0 : u < p.nodes ? p.depth[static_cast<int64_t>(visit.y) * p.nodes + u] : -1;
+            }
+            uint32_t dead[kTileN / 32], any = 0u;
+#pragma unroll
+            for (int i = 0; i < kTileN / 32; ++i) any |= dead[i] = __ballot_sync(0xffffffffu, dep[i] < 0);
+            if (any != 0u) {
               uint8_t* const base = sm.kv[pos.slot] + ((lane >> 3) & 1) * kHalfBytes + (lane & 7) * 16;      // 16 lanes a row, two rows at a time
-              for (int r = lane >> 4; r < 32; r += 2)
-                if ((dead >> r) & 1u) *reinterpret_cast<uint4*>(base + (r0 + r) * 128) = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+              for (int i = 0; i < kTileN / 32; ++i)
+#pragma unroll 1
+                for (int r = lane >> 4; dead[i] >> r != 0u; r += 2) {
+                  if ((dead[i] >> r) & 1u) *reinterpret_cast<uint4*>(base + (i * 32 + r) * 128) = make_uint4(0u, 0u, 0u, 0u);
+                  if (r >= 30) break;
+                }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
@@ -356,29 +370,64 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
     const uint64_t scale2 = pack2(p.scale_log2, p.scale_log2);
     float m_ref = -INFINITY, l_sum = 0.f;
 
-    // the segment's partial: O / l in fp32 (zero where the row saw nothing) and the LSE in the log2 domain
-    auto leave_partial = [&](const Segment& s, int d, bool any) {
+    // The end of a segment.  Two states of one tile are joined, each warpgroup taking half of the columns (tensor memory is shared by
+    // the warps of a row quarter).  A segment that is all of its (sample, key head) leaves the result, another one a partial: O / l in
+    // fp32 (zero where the row saw nothing) and the LSE in the log2 domain.
+    auto leave = [&](const Segment& s, int d, bool any) {
+      float m = any && d >= 0 ? m_ref : -INFINITY, l = l_sum, mine = 1.f, other = 0.f;
+      if (!p.two_tiles) {
+        sm.stats[t][r] = make_float2(m, l);
+        tc_fence_before();
+        asm volatile("bar.sync 2, 256;" ::: "memory");
+        tc_fence_after();
+        const float2 o = sm.stats[t ^ 1][r];
+        const float top = fmaxf(m, o.x), ref = top == -INFINITY ? 0.f : top;
+        mine = m == -INFINITY ? 0.f : fast_exp2(m - ref);
+        other = o.x == -INFINITY ? 0.f : fast_exp2(o.x - ref);
+        l = (m == -INFINITY ? 0.f : l * mine) + (o.x == -INFINITY ? 0.f : o.y * other);
+        m = top;
+      }
+      const bool seen = m != -INFINITY, whole = s.v0 == 0 && s.v1 == s.vis.n;
+      const float inv = seen ? 1.f / l : 0.f;
+      mine = seen ? mine * inv : 0.f;
+      other *= inv;
       const int64_t slot = static_cast<int64_t>(mb) * (p.workers + p.batch * p.kv_heads) + worker + s.b * p.kv_heads + s.kvh;
-      const int64_t prow = (slot * 2 + t) * p.rpt;
-      const bool seen = any && d >= 0 && m_ref != -INFINITY;          // masked scores add ~1e-38 each to l_sum, never to m_ref
-      const float inv = seen ? 1.f / l_sum : 0.f;
+      const int64_t prow = (p.two_tiles ? slot * 2 + t : slot) * p.rpt;
+      const int ch0 = p.two_tiles ? 0 : 2 * t, ch1 = p.two_tiles ? 4 : 2 * t + 2, h = s.kvh * p.rep + r % p.rep;
 #pragma unroll 1
-      for (int ch = 0; ch < 4; ++ch) {
+      for (int ch = ch0; ch < ch1; ++ch) {
         uint32_t o[32];
-        if (any) {
-          JL_TMEM_LD32(t_o + ch * 32, o, 0);
-          JL_TMEM_WAIT_LD32(o, 0);
+        JL_TMEM_LD32(t_o + ch * 32, o, 0);
+        JL_TMEM_WAIT_LD32(o, 0);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) o[i] = mine != 0.f ? __float_as_uint(__uint_as_float(o[i]) * mine) : 0u;      // (nothing: stale, perhaps NaN)
+        if (!p.two_tiles) {
+          uint32_t x[32];
+          JL_TMEM_LD32(t_o + (1 - 2 * t) * 128 + ch * 32, x, 0);
+          JL_TMEM_WAIT_LD32(x, 0);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = other != 0.f ? __float_as_uint(fmaf(__uint_as_float(x[i]), other, __uint_as_float(o[i]))) : o[i];
         }
-        if (row_used) {        // [4 columns][row]: 32 rows of a warp are 512 contiguous bytes (a row at a time cost 7000 clocks)
+        if (row_used && whole) {
+          uint4* dst = reinterpret_cast<uint4*>(p.out + s.b * p.os_b + node * p.os_s + h * p.os_h + ch * 32);
+          auto pk = [&](int i) { return pack_bf16x2(__uint_as_float(o[i]), __uint_as_float(o[i + 1])); };
+#pragma unroll
+          for (int i = 0; i < 4; ++i) dst[i] = make_uint4(pk(8 * i), pk(8 * i + 2), pk(8 * i + 4), pk(8 * i + 6));
+        } else if (row_used) {               // [4 columns][row]: 32 rows of a warp are 512 contiguous bytes (a row at a time cost 7000 clocks)
           float4* dst = reinterpret_cast<float4*>(p.part_o + prow * kHeadDim) + r;
 #pragma unroll
           for (int i = 0; i < 8; ++i)
-            dst[(ch * 8 + i) * p.rpt] = seen ? make_float4(__uint_as_float(o[4 * i]) * inv, __uint_as_float(o[4 * i + 1]) * inv,
-                                                           __uint_as_float(o[4 * i + 2]) * inv, __uint_as_float(o[4 * i + 3]) * inv)
-                                             : make_float4(0.f, 0.f, 0.f, 0.f);
+            dst[(ch * 8 + i) * p.rpt] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]), __uint_as_float(o[4 * i + 2]),
+                                                    __uint_as_float(o[4 * i + 3]));
         }
       }
-      if (row_used) p.part_lse[prow + r] = seen ? m_ref + log2f(l_sum) : -INFINITY;
+      if (row_used && (p.two_tiles || t == 0)) {
+        const float lse = seen ? m + log2f(l) : -INFINITY;
+        if (!whole) p.part_lse[prow + r] = lse;
+        else if (p.lse != nullptr) p.lse[(static_cast<int64_t>(s.b) * p.kv_heads * p.rep + h) * p.nodes + node] = lse * kLn2;
+      }
+      tc_fence_before();                               // the next segment's P V follows our next P
+      if (!p.two_tiles) asm volatile("bar.sync 2, 256;" ::: "memory");      // and the other state's reading
     };
 
     Walk w(sm);
@@ -393,7 +442,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
       m_ref = -INFINITY;
       l_sum = 0.f;
       if (first >= seg.v1) {                           // this state has no visit in the segment
-        leave_partial(seg, -1, false);
+        leave(seg, -1, false);
         continue;
       }
       for (int v = first; v < seg.v1; v += step, ++n_done) {
@@ -409,6 +458,18 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
           const int64_t lo = (p.two_classes && !far ? edge : 0) - tp0, hi = (p.two_classes && far && edge < len ? edge : len) - tp0;
           c_lo = lo < 0 ? 0 : (lo > 128 ? 128 : static_cast<int>(lo));
           c_hi = d < 0 || hi < 0 ? 0 : (hi > 128 ? 128 : static_cast<int>(hi));
+        }
+        // the mask's bits of the tile's columns, fetched while the scores are formed: word i holds bits of columns 32 (i - 1) + shift ..
+        const int u_tile = tp0 - len;                  // node of the tile's first column (negative: columns before the nodes)
+        uint32_t words[kTileN / 32 + 1];
+        bool with_nodes = false;
+        if (!uniform) {
+          with_nodes = d >= 0 && u_tile > -kTileN && u_tile < p.nodes && (!far || p.nodes_far);
+#pragma unroll
+          for (int i = 0; i <= kTileN / 32; ++i) {
+            const int at = (u_tile >> 5) + i;
+            words[i] = with_nodes && at >= 0 && at < 2 * p.words ? __ldg(reinterpret_cast<const uint32_t*>(p.mask + nrow * p.words) + at) : 0u;
+          }
         }
         mbar_wait(&sm.s_full[t], n_done & 1, sm);
         tc_fence_after();
@@ -457,14 +518,13 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
           for (int ch = 0; ch < 4; ++ch) {
             const int a = max(c_lo - ch * 32, 0), z = min(c_hi - ch * 32, 32);
             uint32_t keep = z > a ? (0xffffffffu >> (32 - (z - a))) << a : 0u;
-            const int u0 = tp0 + ch * 32 - len;        // first node of these columns (negative: columns before the nodes)
-            if (d >= 0 && u0 > -32 && u0 < p.nodes && (!far || p.nodes_far)) {
-              const uint32_t* words = reinterpret_cast<const uint32_t*>(p.mask + nrow * p.words);
-              const int i0 = u0 >> 5, sh = u0 & 31;
-              const uint32_t w0 = i0 >= 0 ? __ldg(words + i0) : 0u, w1 = i0 + 1 < 2 * p.words ? __ldg(words + i0 + 1) : 0u;
-              uint32_t bits = __funnelshift_r(w0, w1, sh);
+            if (with_nodes) {
+              const int u0 = u_tile + ch * 32;         // first node of these columns
+              uint32_t bits = __funnelshift_r(words[0], words[1], u_tile & 31);
+#pragma unroll
+              for (int i = 0; i < kTileN / 32; ++i) words[i] = words[i + 1];
               const int left = p.nodes - u0;
-              if (left < 32) bits &= 0xffffffffu >> (32 - left);
+              if (left < 32) bits = left > 0 ? bits & (0xffffffffu >> (32 - left)) : 0u;
               if (p.nodes_far) {
                 for (uint32_t todo = bits; todo != 0u; todo &= todo - 1) {
                   const int j = __ffs(todo) - 1;
@@ -542,8 +602,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
       }
       mbar_wait(&sm.pv_done[t], (n_done - 1) & 1, sm);
       tc_fence_after();
-      leave_partial(seg, d, true);
-      tc_fence_before();                               // the next segment's P V follows our next P
+      leave(seg, d, true);
     }
   }
 
@@ -560,9 +619,9 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
   if (threadIdx.x == 0 && sm.failed) atomicExch(&g_tree_status, 1);
 }
 
-// Joins the partials of the segments that cover a (sample, key head).  One thread per (row, 4 columns), rows fastest, so that
-// partials are read as they were written.  grid x: blocks of 128 threads over a tile's 32 * rpt such items, y: row tile of the
-// (sample, key head), z: (sample, key head).
+// Joins the partials of the segments that cover a (sample, key head), where one segment did not have it all.  One thread per
+// (row, 4 columns), rows fastest, so that partials are read as they were written.  grid x: blocks of 128 threads over a tile's
+// 32 * rpt such items, y: row tile of the (sample, key head), z: (sample, key head).
 __global__ void __launch_bounds__(128) tree_combine_kernel(const TreeParams p) {
   const int lane = threadIdx.x & 31;
   const int heads = p.kv_heads * p.rep, b = static_cast<int>(blockIdx.z) / p.kv_heads, kvh = static_cast<int>(blockIdx.z) % p.kv_heads;
@@ -583,46 +642,51 @@ __global__ void __launch_bounds__(128) tree_combine_kernel(const TreeParams p) {
   const int64_t parts = parts_of(p, total);
   // the part that holds visit x of the line: the largest i with i * total / parts <= x
   const int i0 = static_cast<int>(((lo + 1) * parts + total - 1) / total) - 1, i1 = static_cast<int>(((hi + 1) * parts + total - 1) / total) - 1;
-  const int item = blockIdx.x * 128 + threadIdx.x, c = item / p.rpt, r = item - c * p.rpt;
+  if (i0 == i1) {                                          // one segment had it all: the result is there
+    if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0) wait_prerequisites();      // this kernel ends after the one before it
+    return;
+  }
   const int tile = blockIdx.y, mb = p.two_tiles ? tile >> 1 : 0;
-  const int nd = tile * p.npt + r / p.rep, h = kvh * p.rep + r % p.rep;
-  if (c >= 32 || nd >= p.nodes) return;
   const int64_t slot0 = static_cast<int64_t>(mb) * (p.workers + p.batch * p.kv_heads) + b * p.kv_heads + kvh + i0;
-  // two states per slot, or one of the slot's two tiles
-  const int n_parts = (i1 - i0 + 1) * (p.two_tiles ? 1 : 2), stride = p.two_tiles ? 2 : 1;
-  const int64_t first = slot0 * 2 + (p.two_tiles ? tile & 1 : 0);
-  const float* lse = p.part_lse + first * p.rpt + r;
-  const float4* o = reinterpret_cast<const float4*>(p.part_o) + first * p.rpt * 32 + item;
+  const int n_parts = i1 - i0 + 1, stride = p.two_tiles ? 2 : 1;
+  const int64_t first = p.two_tiles ? slot0 * 2 + (tile & 1) : slot0;
   const int64_t lse_step = static_cast<int64_t>(stride) * p.rpt, o_step = lse_step * 32;
   wait_prerequisites();
-  float m = -INFINITY, sum = 0.f;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int k0 = 0; k0 < n_parts; k0 += 8) {                // 8 partials in flight; the running maximum moves once a round
-    float l[8];
-    float4 x[8];
+  for (int item = blockIdx.x * 128 + threadIdx.x; item < 32 * p.rpt; item += gridDim.x * 128) {
+    const int c = item / p.rpt, r = item - c * p.rpt;
+    const int nd = tile * p.npt + r / p.rep, h = kvh * p.rep + r % p.rep;
+    if (nd >= p.nodes) continue;
+    const float* lse = p.part_lse + first * p.rpt + r;
+    const float4* o = reinterpret_cast<const float4*>(p.part_o) + first * p.rpt * 32 + item;
+    float m = -INFINITY, sum = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k0 = 0; k0 < n_parts; k0 += 8) {              // 8 partials in flight; the running maximum moves once a round
+      float l[8];
+      float4 x[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const bool in = k0 + j < n_parts;
-      l[j] = in ? lse[(k0 + j) * lse_step] : -INFINITY;
-      x[j] = in ? o[(k0 + j) * o_step] : make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int j = 0; j < 8; ++j) {
+        const bool in = k0 + j < n_parts;
+        l[j] = in ? lse[(k0 + j) * lse_step] : -INFINITY;
+        x[j] = in ? o[(k0 + j) * o_step] : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      float mn = m;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) mn = fmaxf(mn, l[j]);
+      const float ref = mn == -INFINITY ? 0.f : mn, f = fast_exp2(m - ref);
+      m = mn;
+      sum *= f; acc.x *= f; acc.y *= f; acc.z *= f; acc.w *= f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float w = fast_exp2(l[j] - ref);
+        sum += w;
+        acc.x = fmaf(w, x[j].x, acc.x); acc.y = fmaf(w, x[j].y, acc.y); acc.z = fmaf(w, x[j].z, acc.z); acc.w = fmaf(w, x[j].w, acc.w);
+      }
     }
-    float mn = m;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) mn = fmaxf(mn, l[j]);
-    const float ref = mn == -INFINITY ? 0.f : mn, f = fast_exp2(m - ref);
-    m = mn;
-    sum *= f; acc.x *= f; acc.y *= f; acc.z *= f; acc.w *= f;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float w = fast_exp2(l[j] - ref);
-      sum += w;
-      acc.x = fmaf(w, x[j].x, acc.x); acc.y = fmaf(w, x[j].y, acc.y); acc.z = fmaf(w, x[j].z, acc.z); acc.w = fmaf(w, x[j].w, acc.w);
-    }
+    const float inv = sum > 0.f ? 1.f / sum : 0.f;
+    *reinterpret_cast<uint2*>(p.out + b * p.os_b + nd * p.os_s + h * p.os_h + 4 * c) =
+        make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+    if (p.lse != nullptr && c == 0) p.lse[(static_cast<int64_t>(b) * heads + h) * p.nodes + nd] = sum > 0.f ? (m + log2f(sum)) * kLn2 : -INFINITY;
   }
-  const float inv = sum > 0.f ? 1.f / sum : 0.f;
-  *reinterpret_cast<uint2*>(p.out + b * p.os_b + nd * p.os_s + h * p.os_h + 4 * c) =
-      make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
-  if (p.lse != nullptr && c == 0) p.lse[(static_cast<int64_t>(b) * heads + h) * p.nodes + nd] = sum > 0.f ? (m + log2f(sum)) * kLn2 : -INFINITY;
 }
 
 struct Layout { int npt, rpt, two_tiles, mbs, workers; size_t lse, total; };
@@ -636,7 +700,7 @@ Layout layout_of(int32_t batch, int32_t nodes, int32_t heads, int32_t kv_heads) 
   l.rpt = (l.two_tiles ? l.npt : nodes) * rep;
   l.workers = kSms / l.mbs;
   if (l.workers < 1) l.workers = 1;
-  const size_t rows = static_cast<size_t>(l.mbs) * (l.workers + static_cast<size_t>(batch) * kv_heads) * 2 * l.rpt;
+  const size_t rows = static_cast<size_t>(l.mbs) * (l.workers + static_cast<size_t>(batch) * kv_heads) * (l.two_tiles ? 2 : 1) * l.rpt;
   l.lse = rows * kHeadDim * sizeof(float);
   l.total = l.lse + rows * sizeof(float);
   return l;
@@ -696,7 +760,8 @@ int launch_tree_attention(const jl_tree_attention_args* a, cudaStream_t stream) 
   }
   if (rc == JL_OK) rc = make_map4(&maps.v, a->v, a->batch, a->rows, a->kv_heads, a->v_stride_b, a->v_stride_s, a->v_stride_h, 1, kTileN);
   if (rc != JL_OK) return rc;
-  constexpr int kSmemBytes = sizeof(TreeSmem) + 1024;
+  constexpr int kSmemBytes = sizeof(TreeSmem);
+  static_assert(kSmemBytes <= 227 * 1024, "shared memory");
   static bool attr_set[64] = {false};
   int dev = -1;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return fail(JL_ERR_LAUNCH, "jl_tree_attention: no current CUDA device");
@@ -710,7 +775,11 @@ int launch_tree_attention(const jl_tree_attention_args* a, cudaStream_t stream) 
     return fail(JL_ERR_UNSUPPORTED, "jl_tree_attention: batch * kv_heads must be at most 65535");
   if (launch_dependent(tree_attention_kernel, dim3(p.mbs * p.workers), dim3(kThreads), kSmemBytes, stream, maps, p) != cudaSuccess)
     return check_launch("jl_tree_attention");
-  if (launch_dependent(tree_combine_kernel, dim3((32 * l.rpt + 127) / 128, row_tiles, a->batch * a->kv_heads), dim3(128), 0, stream, p) != cudaSuccess)
+  // enough blocks to fill the GPU, but no more: what most of them do for many samples is to see that nothing is left to do
+  const int64_t pairs = static_cast<int64_t>(a->batch) * a->kv_heads * row_tiles;
+  int64_t blocks = (int64_t(8) * kSms + pairs - 1) / pairs;
+  if (blocks > (32 * l.rpt + 127) / 128) blocks = (32 * l.rpt + 127) / 128;
+  if (launch_dependent(tree_combine_kernel, dim3(static_cast<unsigned>(blocks), row_tiles, a->batch * a->kv_heads), dim3(128), 0, stream, p) != cudaSuccess)
     return check_launch("jl_tree_attention (combine)");
   return JL_OK;
 }
