@@ -129,6 +129,11 @@ CASES = [
     (1, 70, 32, 8, [700], 40000, 200, True, "forest"),
     (2, 33, 16, 8, [0, 511], 20000, 5, True, "absent"),
     (1, 64, 32, 8, [900], 40000, 64, False, "tree"),
+    # so many pairs that most are one segment, which writes the result itself, and some are cut
+    (60, 9, 32, 8, list(range(1, 1200, 20)), 0, 200, True, "absent"),
+    (48, 40, 16, 4, list(range(0, 960, 20)), 3, 64, True, "absent"),     # two row tiles
+    (30, 100, 8, 2, list(range(0, 600, 20)), 0, 50, True, "forest"),     # four row tiles, two CTAs a part
+    (300, 1, 2, 1, list(range(300)), 0, 33, True, "absent"),
 ]
 
 
@@ -370,3 +375,16 @@ def test_tree_keep_stops_at_the_end_of_a_path_or_cache():
     assert torch.equal(x, want) and torch.equal(y, want)
     d.tree_keep(x, y, path, torch.tensor([-3, 64, 63, 1 << 30], dtype=torch.int32).cuda())       # lengths outside the cache
     assert torch.equal(x, want) and torch.equal(y, want)
+
+
+def test_tree_attention_whole_segments_into_strided_out():
+    """Results that a segment writes itself: into a view, without an LSE, and the same bits with one; what lies beside stays."""
+    case = (60, 9, 32, 8, list(range(1, 1200, 20)), 0, 200, True, "absent")
+    s = make(case)
+    ref, _ = call(s)
+    wide = torch.full((60, 9, 40, 136), 7.0, device="cuda").bfloat16()
+    out = wide[:, :, 4:36, :128]
+    assert call(s, out=out, return_lse=False) is out
+    assert torch.equal(out, ref)
+    wide[:, :, 4:36, :128] = 7.0
+    assert (wide == 7.0).all()

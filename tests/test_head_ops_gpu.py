@@ -346,3 +346,26 @@ def test_gradients_over_several_pieces_of_the_vocabulary(N, H, V):
     # A chunk's bound counts fp32 additions of its own rows only; over all N rows they may take N * F32 * sum |dz| |h|, and a
     # chunk's bound holds HALF * sum |dz| |h| for the rounding of dz: a factor N * F32 / HALF of what is there.
     assert ((dw.double() - e_w).abs() <= b_w * (1 + N * F32 / HALF)).all()
+
+
+def test_the_number_of_counted_rows_may_change_between_replays():
+    """A captured step takes the rows that count from the labels it meets, none or all of them too."""
+    from jetlm.kernels import head_ops
+    h, w, y = make(600, 136, 3001, ignored=0)
+    h.requires_grad_(True)
+    w.requires_grad_(True)
+
+    def step():
+        loss = head_ops.linear_cross_entropy(h, w, y, reduction="sum")
+        return (loss.detach(), *torch.autograd.grad(loss, [h, w]))
+
+    step()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step()
+    full = y.clone()
+    for keep in (600, 0, 1, 257, 599, 300):
+        y.copy_(full)
+        y[torch.randperm(600, generator=torch.Generator().manual_seed(keep)).cuda()[keep:]] = -100
+        g.replay()
+        assert all(torch.equal(a, b) for a, b in zip(out, step())), keep
