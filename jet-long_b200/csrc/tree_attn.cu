@@ -3,13 +3,14 @@
 // The rows of one product are the (node, query head) pairs that share a key head: row r of a 128-row tile is node
 // r / rep, head r % rep of the key head's group (rep = heads / kv_heads), so one pass over the cache serves every drafted
 // token.  A tree of up to 128 rows per key head takes ONE row tile, whose two softmax warpgroups work on alternate key
-// tiles of the same rows (two running states, joined at the end); a larger tree takes TWO row tiles per CTA, and further
-// CTAs that walk the same keys at the same time for its further rows.
+// tiles of the same rows (two running states, joined at the end of a segment); a larger tree takes TWO row tiles per CTA, and further
+// CTAs that walk the same keys at the same time for its further rows; the last tile of an odd number has CTAs of its own.
 //
 // Work is a line of VISITS: for every (sample, key head) the key tiles of the far class, then those of the near class (a
 // tile crossed by the boundary is visited in both with complementary masks).  The line is cut into equal parts, one per
 // SM, wherever that falls, so a batch of any lengths fills the GPU evenly; a part is made of SEGMENTS of one (sample, key
-// head) each, and every segment leaves one normalised fp32 partial (O, LSE) per row that tree_combine_kernel joins.
+// head) each.  A segment that is all of its (sample, key head) writes the result, every other one leaves one normalised fp32
+// partial (O, LSE) per row that tree_combine_kernel joins.
 // Nothing on the host depends on the lengths, which are read on the device.
 //
 //   warp 0      TMA producer of K and V tiles (one ring of 5, in the order of their use), running ahead over all borders; it
@@ -19,6 +20,11 @@
 //               the other (2000 clocks per 128 x 128 x 256 product pair instead of 1450)
 //   warp 3      TMA producer of the query tiles of the current class
 //   warps 4-11  softmax: one thread per row, P back to tensor memory over S
+//
+// The softmax is one pass over the keys: with the running maximum m (raised lazily, only when a score exceeds it by 2^8), O and l hold
+// sum e^(s - m) v and sum e^(s - m) in fp32; P is rounded to bf16 for the product, as the values are.  16 nodes x 4 heads over 131056
+// keys: 96 us for 537 MB of keys and values, the launch of the join included, bound by their stream (6.0 TB/s of 6.56 inside the
+// kernel).  64 nodes x 4 heads: 140 us, bound by the chain of a row tile's products and softmax (tensor pipe 58 %).
 #include "tc_common.cuh"
 #include "../../include/jetlong_b200_tree.h"
 
@@ -42,8 +48,8 @@ struct TreeParams {
   int batch, nodes, words, rep, kv_heads, rows;
   int npt;                     // nodes per row tile
   int rpt;                     // rows per row tile that can be in use
-  int two_tiles;               // two row tiles per CTA instead of two states of one
-  int mbs, workers;            // CTAs per part of the line, parts
+  int pairs, workers;          // CTAs of two row tiles per part of the line, parts
+  int workers_one;             // the last row tile of an odd number has CTAs of its own (two states of the one tile): parts, 0: none
   int unrolled;                // enough visits per part to pay for the unrolled softmax's instruction fetches
   int two_classes, nodes_far;  // nodes_far: w_0 is so small that drafted keys can be in the far class
   int64_t w_0;
@@ -93,8 +99,19 @@ __device__ __forceinline__ Visits visits_of(const TreeParams& p, int b) {
   return v;
 }
 
-// Parts that the line is cut into: one per worker, but none empty.
-__device__ __forceinline__ int64_t parts_of(const TreeParams& p, int64_t total) { return min(static_cast<int64_t>(p.workers), total); }
+// Row tiles 2 mb and 2 mb + 1 are worked on together, or tile 2 mb alone.
+__device__ __forceinline__ bool has_two(const TreeParams& p, int mb) { return mb < p.pairs; }
+
+// Parts that the line is cut into for these row tiles: one per worker, but none empty.
+__device__ __forceinline__ int64_t parts_of(const TreeParams& p, int mb, int64_t total) {
+  return min(static_cast<int64_t>(has_two(p, mb) ? p.workers : p.workers_one), total);
+}
+
+// Place of a partial: segment `i` (part + samples and key heads before it) of row tile 2 mb + t.
+__device__ __forceinline__ int64_t place_of(const TreeParams& p, int mb, int t, int64_t i) {
+  const int64_t per = p.workers + static_cast<int64_t>(p.batch) * p.kv_heads;
+  return has_two(p, mb) ? (mb * per + i) * 2 + t : p.pairs * per * 2 + i;
+}
 
 struct Segment {
   int b, kvh, v0, v1;          // visits [v0, v1)
@@ -140,12 +157,14 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
     return;
   }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int mb = static_cast<int>(blockIdx.x) % p.mbs, worker = static_cast<int>(blockIdx.x) / p.mbs;
+  const int alone = static_cast<int>(blockIdx.x) - p.pairs * p.workers;      // >= 0: on the one tile that is left
+  const bool two_tiles = alone < 0;
+  const int mb = two_tiles ? static_cast<int>(blockIdx.x) % p.pairs : p.pairs, worker = two_tiles ? static_cast<int>(blockIdx.x) / p.pairs : alone;
   if (threadIdx.x >= 64 && threadIdx.x < 69) {   // the tensor maps: q[0], q[1], k[0], k[1], v
     const CUtensorMap* m = reinterpret_cast<const CUtensorMap*>(&maps) + (threadIdx.x - 64);
     asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
   }
-  const int q_slots = p.two_tiles ? 1 : 2;
+  const int q_slots = two_tiles ? 1 : 2;
 
   if (threadIdx.x == 32) {
     sm.failed = *reinterpret_cast<volatile int*>(&g_tree_status) != 0 ? 1 : 0;
@@ -173,7 +192,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
     total *= p.kv_heads;
-    const int64_t parts = parts_of(p, total), lo = min(static_cast<int64_t>(worker), parts) * total / parts;
+    const int64_t parts = parts_of(p, mb, total), lo = min(static_cast<int64_t>(worker), parts) * total / parts;
     const int64_t hi = min(static_cast<int64_t>(worker) + 1, parts) * total / parts;
     int64_t base = 0;
     for (int b0 = 0; b0 < p.batch; b0 += 32) {
@@ -210,7 +229,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
         Segment seg;
         int g = 0;
         RingPos pos[2] = {RingPos(0), RingPos(1)};
-        const int step = p.two_tiles ? 1 : 2;
+        const int step = two_tiles ? 1 : 2;
         while (w.next(p, seg) && !*failed) {
           for (int v = seg.v0; v < seg.v1; ++v, ++g) {
             const int row = seg.key_tile(v) * kTileN;
@@ -244,8 +263,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
             const int slot = u % q_slots;
             mbar_wait(&sm.q_free[slot], ((u / q_slots) & 1) ^ 1, sm);
             if (*failed) break;
-            mbar_expect_tx(&sm.q_full[slot], (p.two_tiles ? 4 : 2) * half);
-            for (int t = 0; t < (p.two_tiles ? 2 : 1); ++t)
+            mbar_expect_tx(&sm.q_full[slot], (two_tiles ? 4 : 2) * half);
+            for (int t = 0; t < (two_tiles ? 2 : 1); ++t)
               for (int h = 0; h < 2; ++h)
                 tma_load_4d(sm.q[slot + t] + h * kHalfBytes, &maps.q[cls], &sm.q_full[slot], h * 64, seg.kvh * p.rep, (mb * 2 + t) * p.npt, seg.b);
             ++u;
@@ -257,7 +276,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
       // The whole warp walks the visits, so that ring indices, parities and descriptors are warp-uniform; one elected lane issues.
       uint32_t leader;
       asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(leader));
-      const int n = static_cast<int>(sm.hi - sm.lo), tiles = p.two_tiles ? 2 : 1;
+      const int n = static_cast<int>(sm.hi - sm.lo), tiles = two_tiles ? 2 : 1;
       RingPos pos(warp - 1);                           // K tiles are the ring's even tiles, V tiles the odd ones
       uint32_t parity = 0u;                            // bit t: parity of state t's next barrier phase
       if (warp == 1) {
@@ -269,22 +288,22 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
           const int flags = *reinterpret_cast<volatile int*>(&sm.visit[g % kVisitRing].x);
           if (__any_sync(0xffffffffu, flags & kQFirst)) {
             ++use;
-            mbar_wait(&sm.q_full[p.two_tiles ? 0 : use & 1], (p.two_tiles ? use : use >> 1) & 1, sm);
+            mbar_wait(&sm.q_full[two_tiles ? 0 : use & 1], (two_tiles ? use : use >> 1) & 1, sm);
           }
           if (*failed) break;
           const uint64_t kd = k_desc + static_cast<uint64_t>((pos.slot * kTileBytes) >> 4);
           for (int i = 0; i < tiles; ++i) {
-            const int t = p.two_tiles ? i : g & 1;
+            const int t = two_tiles ? i : g & 1;
             // The second tile starts when the first one's probabilities are out: half a visit apart, one tile's softmax runs under the
             // other's products, and they stay apart (64 nodes over 131072 keys: 142 -> 137 us).
-            if (p.two_tiles && g == 0 && i == 1) mbar_wait(&sm.p_half[0][1], 0u, sm);
+            if (two_tiles && g == 0 && i == 1) mbar_wait(&sm.p_half[0][1], 0u, sm);
             // the scores go where the probabilities of the state's previous item are: P V has to be done with them
-            if (g >= (p.two_tiles ? 1 : 2)) {
+            if (g >= (two_tiles ? 1 : 2)) {
               mbar_wait(&sm.pv_done[t], (parity >> t) & 1u, sm);
               parity ^= 1u << t;
             }
             tc_fence_after();
-            const uint64_t qd = q_desc + static_cast<uint64_t>(((p.two_tiles ? i : use & 1) * kTileBytes) >> 4);
+            const uint64_t qd = q_desc + static_cast<uint64_t>(((two_tiles ? i : use & 1) * kTileBytes) >> 4);
             if (leader) {
 #pragma unroll
               for (int kk = 0; kk < 8; ++kk) {
@@ -297,7 +316,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
           }
           if (leader) {
             mma_commit(&sm.empty[pos.slot]);
-            if (flags & kQLast) mma_commit(&sm.q_free[p.two_tiles ? 0 : use & 1]);
+            if (flags & kQLast) mma_commit(&sm.q_free[two_tiles ? 0 : use & 1]);
           }
           __syncwarp();
         }
@@ -335,7 +354,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
           }
           const uint64_t vd = v_desc + static_cast<uint64_t>((pos.slot * kTileBytes) >> 4);
           for (int i = 0; i < tiles; ++i) {
-            const int t = p.two_tiles ? i : g & 1;
+            const int t = two_tiles ? i : g & 1;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               mbar_wait(&sm.p_half[t][h], (parity >> t) & 1u, sm);
@@ -362,7 +381,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsHigh));
     const int t = (warp - 4) >> 2, quad = warp & 3;
     const int r = quad * 32 + lane;
-    const int node = p.two_tiles ? (mb * 2 + t) * p.npt + r / p.rep : r / p.rep;
+    const int node = (mb * 2 + (two_tiles ? t : 0)) * p.npt + r / p.rep;
     const bool row_used = r < p.npt * p.rep && node < p.nodes;
     const uint32_t lane_base = static_cast<uint32_t>(quad * 32) << 16;
     const uint32_t t_s = tmem + lane_base + t * 128;        // my row of scores; the bf16 P overlays its first 64 columns
@@ -375,7 +394,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
     // fp32 (zero where the row saw nothing) and the LSE in the log2 domain.
     auto leave = [&](const Segment& s, int d, bool any) {
       float m = any && d >= 0 ? m_ref : -INFINITY, l = l_sum, mine = 1.f, other = 0.f;
-      if (!p.two_tiles) {
+      if (!two_tiles) {
         sm.stats[t][r] = make_float2(m, l);
         tc_fence_before();
         asm volatile("bar.sync 2, 256;" ::: "memory");
@@ -391,9 +410,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
       const float inv = seen ? 1.f / l : 0.f;
       mine = seen ? mine * inv : 0.f;
       other *= inv;
-      const int64_t slot = static_cast<int64_t>(mb) * (p.workers + p.batch * p.kv_heads) + worker + s.b * p.kv_heads + s.kvh;
-      const int64_t prow = (p.two_tiles ? slot * 2 + t : slot) * p.rpt;
-      const int ch0 = p.two_tiles ? 0 : 2 * t, ch1 = p.two_tiles ? 4 : 2 * t + 2, h = s.kvh * p.rep + r % p.rep;
+      const int64_t prow = place_of(p, mb, t, worker + s.b * p.kv_heads + s.kvh) * p.rpt;
+      const int ch0 = two_tiles ? 0 : 2 * t, ch1 = two_tiles ? 4 : 2 * t + 2, h = s.kvh * p.rep + r % p.rep;
 #pragma unroll 1
       for (int ch = ch0; ch < ch1; ++ch) {
         uint32_t o[32];
@@ -401,7 +419,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
         JL_TMEM_WAIT_LD32(o, 0);
 #pragma unroll
         for (int i = 0; i < 32; ++i) o[i] = mine != 0.f ? __float_as_uint(__uint_as_float(o[i]) * mine) : 0u;      // (nothing: stale, perhaps NaN)
-        if (!p.two_tiles) {
+        if (!two_tiles) {
           uint32_t x[32];
           JL_TMEM_LD32(t_o + (1 - 2 * t) * 128 + ch * 32, x, 0);
           JL_TMEM_WAIT_LD32(x, 0);
@@ -421,20 +439,20 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
                                                     __uint_as_float(o[4 * i + 3]));
         }
       }
-      if (row_used && (p.two_tiles || t == 0)) {
+      if (row_used && (two_tiles || t == 0)) {
         const float lse = seen ? m + log2f(l) : -INFINITY;
         if (!whole) p.part_lse[prow + r] = lse;
         else if (p.lse != nullptr) p.lse[(static_cast<int64_t>(s.b) * p.kv_heads * p.rep + h) * p.nodes + node] = lse * kLn2;
       }
       tc_fence_before();                               // the next segment's P V follows our next P
-      if (!p.two_tiles) asm volatile("bar.sync 2, 256;" ::: "memory");      // and the other state's reading
+      if (!two_tiles) asm volatile("bar.sync 2, 256;" ::: "memory");      // and the other state's reading
     };
 
     Walk w(sm);
     Segment seg;
     int n_done = 0, g = 0;
     while (w.next(p, seg)) {
-      const int step = p.two_tiles ? 1 : 2, first = seg.v0 + (p.two_tiles ? 0 : (g ^ t) & 1);
+      const int step = two_tiles ? 1 : 2, first = seg.v0 + (two_tiles ? 0 : (g ^ t) & 1);
       g += seg.v1 - seg.v0;
       const int64_t nrow = static_cast<int64_t>(seg.b) * p.nodes + (row_used ? node : 0);
       const int d = row_used ? p.depth[nrow] : -1;
@@ -639,17 +657,16 @@ __global__ void __launch_bounds__(128) tree_combine_kernel(const TreeParams p) {
   total *= p.kv_heads;
   const int n_b = visits_of(p, b).n;
   const int64_t lo = before * p.kv_heads + static_cast<int64_t>(kvh) * n_b, hi = lo + n_b - 1;     // first and last visit
-  const int64_t parts = parts_of(p, total);
+  const int tile = blockIdx.y, mb = tile >> 1;
+  const int64_t parts = parts_of(p, mb, total);
   // the part that holds visit x of the line: the largest i with i * total / parts <= x
   const int i0 = static_cast<int>(((lo + 1) * parts + total - 1) / total) - 1, i1 = static_cast<int>(((hi + 1) * parts + total - 1) / total) - 1;
   if (i0 == i1) {                                          // one segment had it all: the result is there
     if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0) wait_prerequisites();      // this kernel ends after the one before it
     return;
   }
-  const int tile = blockIdx.y, mb = p.two_tiles ? tile >> 1 : 0;
-  const int64_t slot0 = static_cast<int64_t>(mb) * (p.workers + p.batch * p.kv_heads) + b * p.kv_heads + kvh + i0;
-  const int n_parts = i1 - i0 + 1, stride = p.two_tiles ? 2 : 1;
-  const int64_t first = p.two_tiles ? slot0 * 2 + (tile & 1) : slot0;
+  const int n_parts = i1 - i0 + 1, stride = has_two(p, mb) ? 2 : 1;
+  const int64_t first = place_of(p, mb, tile & 1, static_cast<int64_t>(b) * p.kv_heads + kvh + i0);
   const int64_t lse_step = static_cast<int64_t>(stride) * p.rpt, o_step = lse_step * 32;
   wait_prerequisites();
   for (int item = blockIdx.x * 128 + threadIdx.x; item < 32 * p.rpt; item += gridDim.x * 128) {
@@ -689,18 +706,22 @@ __global__ void __launch_bounds__(128) tree_combine_kernel(const TreeParams p) {
   }
 }
 
-struct Layout { int npt, rpt, two_tiles, mbs, workers; size_t lse, total; };
+struct Layout { int npt, rpt, pairs, workers, workers_one; size_t lse, total; };
 Layout layout_of(int32_t batch, int32_t nodes, int32_t heads, int32_t kv_heads) {
   Layout l;
   const int rep = heads / kv_heads;
   l.npt = 128 / rep;
   const int tiles = (nodes + l.npt - 1) / l.npt;
-  l.two_tiles = tiles > 1;
-  l.mbs = (tiles + 1) / 2;
-  l.rpt = (l.two_tiles ? l.npt : nodes) * rep;
-  l.workers = kSms / l.mbs;
-  if (l.workers < 1) l.workers = 1;
-  const size_t rows = static_cast<size_t>(l.mbs) * (l.workers + static_cast<size_t>(batch) * kv_heads) * (l.two_tiles ? 2 : 1) * l.rpt;
+  l.pairs = tiles / 2;
+  l.rpt = (tiles > 1 ? l.npt : nodes) * rep;
+  // SMs for pairs of row tiles and for the one that is left, by what a visit costs them, 36 : 17 (80 nodes over 131056 keys, three
+  // tiles: 217 us, with 36 : 13 250, 36 : 22 228; 259 with the last tile paired with an empty one)
+  const bool odd = tiles % 2 != 0;
+  l.workers = l.pairs == 0 ? 0 : odd ? kSms * 36 / (36 * l.pairs + 17) : kSms / l.pairs;
+  if (l.pairs > 0 && l.workers < 1) l.workers = 1;
+  l.workers_one = !odd ? 0 : kSms - l.pairs * l.workers < 1 ? 1 : kSms - l.pairs * l.workers;
+  const size_t bk = static_cast<size_t>(batch) * kv_heads;
+  const size_t rows = (l.pairs * (l.workers + bk) * 2 + (odd ? l.workers_one + bk : 0)) * l.rpt;
   l.lse = rows * kHeadDim * sizeof(float);
   l.total = l.lse + rows * sizeof(float);
   return l;
@@ -736,13 +757,13 @@ int launch_tree_attention(const jl_tree_attention_args* a, cudaStream_t stream) 
   if (reinterpret_cast<uintptr_t>(a->workspace) & 15) return fail(JL_ERR_BAD_ARG, "jl_tree_attention: workspace not 16-byte aligned");
   TreeParams p{};
   p.batch = a->batch; p.nodes = a->nodes; p.words = (a->nodes + 63) / 64; p.kv_heads = a->kv_heads; p.rep = a->heads / a->kv_heads; p.rows = a->rows;
-  p.npt = l.npt; p.rpt = l.rpt; p.two_tiles = l.two_tiles; p.mbs = l.mbs; p.workers = l.workers;
+  p.npt = l.npt; p.rpt = l.rpt; p.pairs = l.pairs; p.workers = l.workers; p.workers_one = l.workers_one;
   p.two_classes = a->q_group != nullptr;
   p.w_0 = a->w_0 < (int64_t(1) << 32) ? a->w_0 : (int64_t(1) << 32);           // no cache reaches further
   p.nodes_far = p.two_classes && p.w_0 < a->nodes - 1;
   // The unrolled softmax saves 1300 clocks a visit, and its instructions, cold, cost 8 us once: 16 nodes over 131072 keys 106.5 us
   // rolled and 102.8 unrolled, 64 nodes 171 and 142; the two are equal at 8 visits a part.
-  p.unrolled = static_cast<int64_t>(a->batch) * a->kv_heads * (a->rows / kTileN) >= 16ll * l.workers;
+  p.unrolled = static_cast<int64_t>(a->batch) * a->kv_heads * (a->rows / kTileN) >= 16ll * (l.pairs > 0 ? l.workers : l.workers_one);
   p.scale_log2 = a->softmax_scale * kLog2e;
   p.lens = a->lens; p.depth = a->depth; p.mask = a->mask;
   p.part_o = static_cast<float*>(a->workspace);
@@ -773,7 +794,7 @@ int launch_tree_attention(const jl_tree_attention_args* a, cudaStream_t stream) 
   const int row_tiles = (a->nodes + l.npt - 1) / l.npt;
   if (static_cast<int64_t>(a->batch) * a->kv_heads > 65535)
     return fail(JL_ERR_UNSUPPORTED, "jl_tree_attention: batch * kv_heads must be at most 65535");
-  if (launch_dependent(tree_attention_kernel, dim3(p.mbs * p.workers), dim3(kThreads), kSmemBytes, stream, maps, p) != cudaSuccess)
+  if (launch_dependent(tree_attention_kernel, dim3(p.pairs * p.workers + p.workers_one), dim3(kThreads), kSmemBytes, stream, maps, p) != cudaSuccess)
     return check_launch("jl_tree_attention");
   // enough blocks to fill the GPU, but no more: what most of them do for many samples is to see that nothing is left to do
   const int64_t pairs = static_cast<int64_t>(a->batch) * a->kv_heads * row_tiles;
