@@ -37,7 +37,10 @@ using namespace tc;
 __device__ int g_tree_status = 0;            // raised when a bounded wait gave up
 
 constexpr int kTileN = 128;                  // keys per visit
-constexpr int kStages = 5;                   // tiles in the ring: K of visit g is its tile 2 g, V is tile 2 g + 1
+// Tiles in the ring: K of visit g is its tile 2 g, V is tile 2 g + 1.  The number is odd, so a slot holds K and V in turn, and each
+// issuer waits for every second use of it only; the use between has landed by then: before Q K of visit g its issuer has waited for
+// P V of visit g - 3 (whose V was there), and before P V of visit g for scores of visit g - 1.
+constexpr int kStages = 5;
 constexpr int kTileBytes = 128 * 256;        // 128 rows x 128 bf16
 constexpr int kHalfBytes = 128 * 128;        // one 64-column half (a TMA box)
 constexpr int kThreads = 384;

@@ -3,13 +3,20 @@
 //
 //   z = h W^T,  lse = log sum exp z,  nll = lse - z_y,  dz = exp(z - lse) - onehot(y),  dh = g dz W,  dW = g dz^T h
 //
-// All three products run on one persistent tcgen05 kernel (head_gemm_kernel) whose epilogue is what differs:
+// All products run on one persistent tcgen05 kernel (head_gemm_kernel) whose epilogue is what differs:
 //   scores  z tile -> per row (maximum, sum of exponentials, argmax, logit of the label); a fold kernel joins the tiles
+//   few     the same with the weight's rows as the rows of the product, for up to 32 rows of hidden states
 //   dz      z tile -> exp(z - lse) - onehot in bf16, one piece of the vocabulary at a time
 //   dh      dz W accumulated in fp32 over the pieces (bulk reductions in L2), rounded once at the end
 //   dW      dz^T h, final for the piece
 // The score and dz products read hidden and weight along their rows (K-major); dh reads weight and dW reads dz and
-// hidden across them (MN-major), so nothing is transposed in memory.
+// hidden across them (MN-major), so nothing is transposed in memory.  Of a loss over more than 256 rows only those that count
+// are multiplied: they are packed first, and the products take their extents from the number on the device.
+//
+// Few rows are bound by the weight's bytes: 49 rows x 4096 x 151936 205 us after a pause (6.1 TB/s), in a loop 218 to 232, where the
+// power cap holds the clock at 1.30 GHz.  Many are bound by the tensor pipe at the capped clock: scores of 8191 rows x 4096
+// 7.2 ms in a loop (1412 TFLOP/s), 6.2 after a pause (1640); loss and gradients of 4096 rows x 2560 9.7 and 8.4 ms (1310 and 1515),
+// four products where three would do if the logits were kept.
 #include <cmath>
 #include <type_traits>
 
@@ -38,7 +45,7 @@ constexpr int kSms = 148;
 
 constexpr int kFewRows = 32;                 // up to here the rows are the columns of the score product
 
-enum { kEpiScores = 0, kEpiDz = 1, kEpiF32 = 2, kEpiBf16 = 3, kEpiFew = 4 };
+enum { kEpiScores = 0, kEpiDz = 1, kEpiF32 = 2, kEpiBf16 = 3, kEpiFew16 = 4, kEpiFew32 = 5 };
 
 struct GradScale {            // scalar factor of both gradients, applied to their fp32 sums
   const float *grad, *count;
@@ -190,11 +197,12 @@ struct Product {
   // the 256 steps of K = 4096 a logit lost 2^-24 of its size 256 times, up to 1e-5 in all, and so did the losses.  Scores
   // therefore take K in parts that are added in fp32 registers.  Error of the loss / time of 8191 rows x 4096 with parts of 256,
   // 512, 1024 and all of K: 2e-7 / 8.0 ms, 3.5e-7 / 7.5, 8e-7 / 7.25, 4e-6 / 7.1; a few rows are bound by the weight's bytes and
-  // take parts of 256, up to 32 rows parts of 128 (error of one row's lse with 64, 128, 256: 0.7e-7, 1.4e-7, 2.6e-7; time of
-  // 151936 x 2048 in a loop 102.4, 102.3, 98.4 us).  Results that are rounded to bf16 need none of this.
-  static constexpr int kAccs = kEpi_ == kEpiFew ? 4 : 2, kAccCols = kTmemCols / kAccs;
-  static constexpr bool kParts = kEpi_ == kEpiScores || kEpi_ == kEpiFew;
-  static constexpr int kPart = !kParts ? 1 << 30 : kEpi_ == kEpiFew ? 2 : kPair_ == 1 ? 4 : 8;
+  // take parts of 256, up to 32 rows parts of 128, up to 16 of 64 (error of one row's lse with 64, 128, 256: 0.7e-7, 1.4e-7, 2.6e-7;
+  // time of 151936 x 2048 in a loop 102.4, 102.3, 98.4 us, after a pause 98 with all; 32 rows x 4096: 225, 218, 207 us).
+  // Results that are rounded to bf16 need none of this.
+  static constexpr int kAccs = kEpi_ >= kEpiFew16 ? 4 : 2, kAccCols = kTmemCols / kAccs;
+  static constexpr bool kFew = kEpi_ == kEpiFew16 || kEpi_ == kEpiFew32, kParts = kEpi_ == kEpiScores || kFew;
+  static constexpr int kPart = !kParts ? 1 << 30 : kEpi_ == kEpiFew16 ? 1 : kEpi_ == kEpiFew32 ? 2 : kPair_ == 1 ? 4 : 8;
 };
 
 template <class P>
@@ -321,16 +329,16 @@ __device__ __forceinline__ void finish(const GemmMaps& maps, const GemmParams& p
     const int64_t row_w = (static_cast<int64_t>(c.m) * kPair + rank) * 128 + quad * 32, row = row_w + lane;
     const int n0 = c.n * p.bn;
 
-    if constexpr (kEpi == kEpiFew) {
+    if constexpr (P::kFew) {
       // The tile is m_step vocabulary entries by up to 32 rows.  Its logits are summed over the parts of K in registers (a thread has
       // an entry and half of the rows) and go through shared memory to a warp per row.
       float* const zs = reinterpret_cast<float*>(sm.ring + kRingBytes + kStagingBytes - p.N * 512);      // [row][128 entries], behind the ring
       const int c_lo = half * 16;
-      const bool mine = c_lo < p.bn;               // up to 16 rows the second half of the warps only reduces
+      const bool mine = half == 0 || kEpi == kEpiFew32;      // up to 16 rows the second half of the warps only reduces
       float z[16];
 #pragma unroll
       for (int j = 0; j < 16; ++j) z[j] = 0.f;
-      for (int part = 0; mine && part * P::kPart < p.k_blocks; ++part) {
+      for (int kb = 0; mine && kb < p.k_blocks; kb += P::kPart) {
         mbar_wait(&sm.acc_full[st.i % P::kAccs], (st.i / P::kAccs) & 1, sm);
         tc_fence_after();
         uint32_t x[16];
@@ -513,7 +521,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) head_gemm_kernel(const __grid
   if (threadIdx.x == 0) {
     sm.failed = *reinterpret_cast<volatile int*>(&g_head_status) != 0 ? 1 : 0;
     for (int i = 0; i < kMaxStages; ++i) { mbar_init(&sm.full[i], 1); mbar_init(&sm.empty[i], 1); }
-    for (int i = 0; i < kMaxAccs; ++i) { mbar_init(&sm.acc_full[i], 1); mbar_init(&sm.acc_free[i], P0::kEpi == kEpiFew && p0.bn <= 16 ? 4 : kEpiWarps * kPair); }
+    for (int i = 0; i < kMaxAccs; ++i) { mbar_init(&sm.acc_full[i], 1); mbar_init(&sm.acc_free[i], P0::kEpi == kEpiFew16 ? 4 : kEpiWarps * kPair); }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 2) {
@@ -936,7 +944,8 @@ int launch(const Gemm& g0, const Gemm& g1, cudaStream_t stream) {
 template <class P>
 int launch_one(const Gemm& g, cudaStream_t stream) { return launch<P, void>(g, g, stream); }
 
-using ScoresFew = Product<1, false, false, kEpiFew>;
+using ScoresFew16 = Product<1, false, false, kEpiFew16>;
+using ScoresFew32 = Product<1, false, false, kEpiFew32>;
 using Scores1 = Product<1, false, false, kEpiScores>;
 using Scores2 = Product<2, false, false, kEpiScores>;
 using Dz1 = Product<1, false, false, kEpiDz>;
@@ -1069,7 +1078,7 @@ int launch_scores(const jl_head_scores_args* a, cudaStream_t stream) {
     const Matrix w{a->weight, a->vocab, a->hidden_size, a->weight_stride};
     if (a->rows <= kFewRows) {
       rc = prepare_few(g, w, h, l.few);
-      if (rc == JL_OK) rc = launch_one<ScoresFew>(g, stream);
+      if (rc == JL_OK) rc = a->rows <= 16 ? launch_one<ScoresFew16>(g, stream) : launch_one<ScoresFew32>(g, stream);
     } else if (plan.pair == 2) {
       rc = prepare<Scores2>(g, h, w, Result{}, plan, a->hidden_size, 1);
       if (rc == JL_OK) rc = launch_one<Scores2>(g, stream);

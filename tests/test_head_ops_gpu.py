@@ -369,3 +369,21 @@ def test_the_number_of_counted_rows_may_change_between_replays():
         y[torch.randperm(600, generator=torch.Generator().manual_seed(keep)).cuda()[keep:]] = -100
         g.replay()
         assert all(torch.equal(a, b) for a, b in zip(out, step())), keep
+
+
+def test_one_gradient_of_many_rows_and_calls_without_any():
+    from jetlm.kernels import head_ops
+    h, w, y = make(900, 136, 5003)
+    h.requires_grad_(True)
+    w.requires_grad_(True)
+    loss = head_ops.linear_cross_entropy(h, w, y)
+    dh, dw = torch.autograd.grad(loss, [h, w])
+    assert torch.equal(torch.autograd.grad(head_ops.linear_cross_entropy(h, w.detach(), y), h)[0], dh)
+    assert torch.equal(torch.autograd.grad(head_ops.linear_cross_entropy(h.detach(), w, y), w)[0], dw)
+    with torch.no_grad():
+        quiet = head_ops.linear_cross_entropy(h, w, y)
+    assert torch.equal(quiet, loss.detach()) and not quiet.requires_grad
+    with torch.inference_mode():
+        assert torch.equal(head_ops.linear_cross_entropy(h, w, y), loss.detach())
+    kept = [t.clone() for t in (h.detach(), w.detach(), y)]
+    assert all(torch.equal(a, b) for a, b in zip(kept, (h.detach(), w.detach(), y)))
