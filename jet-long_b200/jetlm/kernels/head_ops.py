@@ -69,29 +69,29 @@ def _row_stride(t: torch.Tensor) -> int:
 def _scores(h, w, labels, ignore_index, *, nll, top, reduction=None, skip_ignored=0):
     """One jl_head_scores call on (rows, H) operands; returns (nll, lse, top, loss, loss_count), None where not asked for."""
     n, dev, a = h.shape[0], h.device, N.HeadScoresArgs()
-    per_row = torch.empty(2 if nll else 1, n, dtype=torch.float32, device=dev)
-    best = torch.empty(n, dtype=torch.int64, device=dev) if top else None
-    scalars = torch.empty(2, dtype=torch.float32, device=dev) if reduction is not None else None
+    lse = torch.empty(n, dtype=torch.float32, device=dev)
+    per_row = torch.empty_like(lse) if nll else None
+    best = torch.empty_like(lse, dtype=torch.int64) if top else None
+    loss = torch.empty((), dtype=torch.float32, device=dev) if reduction is not None else None
+    count = torch.empty_like(loss) if reduction == "mean" else None
     lib = N.lib()
     ws = torch.empty(lib.jl_head_scores_workspace_bytes(n, w.shape[1], w.shape[0], skip_ignored), dtype=torch.uint8, device=dev)
     a.weight, a.hidden_stride, a.weight_stride, a.ignore_index = w.data_ptr(), _row_stride(h), _row_stride(w), int(ignore_index)
     a.hidden, a.rows, a.hidden_size, a.vocab = h.data_ptr() or a.weight, n, w.shape[1], w.shape[0]
     if labels is not None:
         a.labels = labels.data_ptr() or a.weight                # no rows: never read
-    a.lse, a.skip_ignored = per_row.data_ptr(), skip_ignored
+    a.lse, a.skip_ignored = lse.data_ptr(), skip_ignored
     if nll:
-        a.nll = a.lse + 4 * n if n else a.weight
+        a.nll = per_row.data_ptr() or a.weight
     if top:
         a.top = best.data_ptr()
-    if reduction is not None:
-        a.loss_count = scalars.data_ptr() + 4
-        if reduction == "mean":
-            a.loss_mean = scalars.data_ptr()
-        else:
-            a.loss_sum = scalars.data_ptr()
+    if count is not None:
+        a.loss_mean, a.loss_count = loss.data_ptr(), count.data_ptr()
+    elif loss is not None:
+        a.loss_sum = loss.data_ptr()
     a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
     _run("jl_head_scores", lib.jl_head_scores, a, dev.index)
-    return (per_row[1] if nll else None, per_row[0], best, *((scalars[0], scalars[1]) if scalars is not None else (None, None)))
+    return per_row, lse, best, loss, count
 
 
 def token_scores(hidden: torch.Tensor, weight: torch.Tensor, labels: Optional[torch.Tensor] = None, *, ignore_index: int = -100,
