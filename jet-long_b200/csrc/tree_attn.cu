@@ -711,7 +711,7 @@ __global__ void __launch_bounds__(128) tree_combine_kernel(const TreeParams p) {
 
 struct Layout { int npt, rpt, pairs, workers, workers_one; size_t lse, total; };
 Layout layout_of(int32_t batch, int32_t nodes, int32_t heads, int32_t kv_heads) {
-  Layout l;
+  Layout l{};
   const int rep = heads / kv_heads;
   l.npt = 128 / rep;
   const int tiles = (nodes + l.npt - 1) / l.npt;

@@ -331,7 +331,7 @@ __device__ __forceinline__ void finish(const GemmMaps& maps, const GemmParams& p
 
     if constexpr (P::kFew) {
       // The tile is m_step vocabulary entries by up to 32 rows.  Its logits are summed over the parts of K in registers (a thread has
-      // an entry and half of the rows) and go through shared memory to a warp per row.
+      // an entry and 16 of the rows) and go through shared memory to a warp per row.
       float* const zs = reinterpret_cast<float*>(sm.ring + kRingBytes + kStagingBytes - p.N * 512);      // [row][128 entries], behind the ring
       const int c_lo = half * 16;
       const bool mine = half == 0 || kEpi == kEpiFew32;      // up to 16 rows the second half of the warps only reduces
@@ -983,7 +983,7 @@ Packed packed_layout(size_t& total, int64_t rows, int64_t chunk, int32_t hd) {
 }
 struct ScoresLayout { Plan plan; FewPlan few; int tiles; size_t part, arg, picked, nll, total; bool pack; Packed packed; };      // tiles: partials of a row
 ScoresLayout scores_layout(int64_t rows, int32_t hd, int32_t vocab, bool skip_ignored) {
-  ScoresLayout l;
+  ScoresLayout l{};
   const int64_t n = rows < 1 ? 1 : rows < kScoreRows ? rows : kScoreRows;
   l.plan = plan_tiles(n, vocab, pair_of(n), 16 * pair_of(n));
   l.few = plan_few(n <= kFewRows ? n : 1, vocab);
@@ -1003,7 +1003,7 @@ ScoresLayout scores_layout(int64_t rows, int32_t hd, int32_t vocab, bool skip_ig
 // multiple of 256.
 struct GradsLayout { int64_t piece; Plan dz, dh, dw; int splits; size_t dh32, total; bool pack; Packed packed; };
 GradsLayout grads_layout(int64_t rows, int32_t hd, int32_t vocab) {
-  GradsLayout l;
+  GradsLayout l{};
   const int64_t n = rows > 0 ? rows : 1;
   int64_t most = (int64_t(256) << 20) / (n * 2) / 256 * 256;
   if (most < 2048) most = 2048;
@@ -1087,7 +1087,7 @@ int launch_scores(const jl_head_scores_args* a, cudaStream_t stream) {
       if (rc == JL_OK) rc = launch_one<Scores1>(g, stream);
     }
     if (rc != JL_OK) return rc;
-    const bool few = n < 4 * kSms;
+    const bool few = n < 16 * kSms;          // (1000 rows of 1188 partials: 25 us with a warp each, 12 with eight)
     if (launch_dependent(few ? scores_fold_kernel<8> : scores_fold_kernel<1>, dim3(static_cast<unsigned>(few ? n : cdiv(n, 8))), dim3(256), 0, stream,
                          static_cast<const float2*>(p.part), static_cast<const int*>(p.part_arg), static_cast<const float*>(p.picked), l.tiles, n,
                          static_cast<int64_t>(a->vocab), p.labels, a->ignore_index, nll != nullptr ? nll + (l.pack ? 0 : r0) : nullptr,
