@@ -69,7 +69,7 @@ struct GemmParams {
   int m_step;                 // rows of A from one tile to the next
   int a_bytes, tx_bytes, stage_bytes, stages;      // of the operand ring, per CTA: A's place, what a stage loads, a stage
   // scores
-  float2* part;               // [row][n tile][half] (few rows: [row][m tile]) (maximum, sum of exponentials relative to it)
+  float2* part;               // [row][n tile][half] (few rows: [row][m tile]) (maximum, sum of exponentials relative to it, less 1)
   int* part_arg;              // the same or NULL
   float* picked;              // [row] logit of the label
   // dz
@@ -361,10 +361,17 @@ __device__ __forceinline__ void finish(const GemmMaps& maps, const GemmParams& p
 #pragma unroll
         for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
         const float m_use = m == -INFINITY ? 0.f : m;
-        float sum = (fast_exp2((x.x - m_use) * kLog2e) + fast_exp2((x.y - m_use) * kLog2e)) +
-                    (fast_exp2((x.z - m_use) * kLog2e) + fast_exp2((x.w - m_use) * kLog2e));
+        const float e[4] = {fast_exp2((x.x - m_use) * kLog2e), fast_exp2((x.y - m_use) * kLog2e), fast_exp2((x.z - m_use) * kLog2e),
+                            fast_exp2((x.w - m_use) * kLog2e)};
+        float less = 0.f;
+        int ones = 0;
 #pragma unroll
-        for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+        for (int j = 0; j < 4; ++j) {
+          ones += __popc(__ballot_sync(0xffffffffu, e[j] == 1.f));
+          less += e[j] == 1.f ? 0.f : e[j];
+        }
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) less += __shfl_xor_sync(0xffffffffu, less, off);
         const int64_t at = static_cast<int64_t>(r) * p.m_tiles + c.m;
         if (p.part_arg != nullptr) {
           const int first = x.x == m ? 0 : x.y == m ? 1 : x.z == m ? 2 : x.w == m ? 3 : 128;
@@ -372,7 +379,7 @@ __device__ __forceinline__ void finish(const GemmMaps& maps, const GemmParams& p
           if (lane == 0) p.part_arg[at] = arg < valid ? static_cast<int>(v0) + arg : 0x7fffffff;
         }
         if (lane == 0) {
-          p.part[at] = make_float2(m, sum);
+          p.part[at] = make_float2(m, less + static_cast<float>(ones - 1));
           const int64_t y = p.labels != nullptr ? p.labels[r] - v0 : -1;
           if (y >= 0 && y < valid) p.picked[r] = zs[r * 128 + y];
         }
@@ -422,11 +429,16 @@ __device__ __forceinline__ void finish(const GemmMaps& maps, const GemmParams& p
         for (int j = 127; j >= 0; --j) arg = z[j] == m && j < valid ? j : arg;
       }
       // (z - m) first: exact for the logits that count, whatever their size
+      int ones = 0;
 #pragma unroll
-      for (int j = 0; j < 128; ++j) s4[j & 3] += fast_exp2((z[j] - m_use) * kLog2e);
+      for (int j = 0; j < 128; ++j) {
+        const float e = fast_exp2((z[j] - m_use) * kLog2e);
+        ones += e == 1.f ? 1 : 0;
+        s4[j & 3] += e == 1.f ? 0.f : e;
+      }
       if (row < p.M) {
         const int64_t at = (row * p.n_tiles + c.n) * 2 + half;
-        p.part[at] = make_float2(m, (s4[0] + s4[1]) + (s4[2] + s4[3]));
+        p.part[at] = make_float2(m, (s4[0] + s4[1]) + (s4[2] + s4[3]) + static_cast<float>(ones - 1));
         if (p.part_arg != nullptr) p.part_arg[at] = arg == 0x7fffffff ? arg : n0 + c_lo + arg;
         if (y >= 0) p.picked[row] = z_y;
       }
@@ -583,12 +595,15 @@ __global__ void __launch_bounds__(kGemmThreads, 1) head_gemm_kernel(const __grid
   if (threadIdx.x == 0 && sm.failed) atomicExch(&g_head_status, 1);
 }
 
-// (maximum, sum of exponentials relative to it, lowest index of the maximum) of two disjoint sets of logits
-__device__ __forceinline__ void join_scores(float& m, float& s, int& arg, float om, float os, int oa) {
+// (maximum, r, lowest index of the maximum) of two disjoint sets of logits, where 1 + r is the sum of exponentials relative to the
+// maximum: the 1 is the maximum's own.  Kept apart, it does not round away what the others add up to, and log1p(r) is the loss of a
+// row that is sure of its label: with one sum, a loss of 1e-6 was off by up to a quarter.  No logits: (-inf, -1).
+__device__ __forceinline__ void join_scores(float& m, float& r, int& arg, float om, float orest, int oa) {
   if (om > m || (om == m && oa < arg)) arg = oa;
-  const float mn = fmaxf(m, om), ref = mn == -INFINITY ? 0.f : mn;
-  s = s * fast_exp2((m - ref) * kLog2e) + os * fast_exp2((om - ref) * kLog2e);
-  m = mn;
+  const bool other = om > m;
+  const float hi = other ? om : m, lo = other ? m : om, ref = hi == -INFINITY ? 0.f : hi;
+  r = (other ? orest : r) + (1.f + (other ? r : orest)) * fast_exp2((lo - ref) * kLog2e);
+  m = hi;
 }
 
 // Folds the tiles' partials of a row; kWarps warps share a row (8 when there are few rows: 731 partials of one row took
@@ -597,13 +612,13 @@ template <int kWarps>
 __global__ void __launch_bounds__(256) scores_fold_kernel(const float2* part, const int* part_arg, const float* picked, int tiles, int64_t N, int64_t V,
                                                           const int64_t* labels, int64_t ignore, float* nll, float* lse, int64_t* top,
                                                           const int32_t* rows_used, const int32_t* place, int64_t row0) {
-  __shared__ float sm[8], ss[8];
+  __shared__ float sm[8], sr[8];
   __shared__ int sa[8];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * (8 / kWarps) + warp / kWarps;
   wait_prerequisites();
   launch_dependents();
-  float m = -INFINITY, s = 0.f;
+  float m = -INFINITY, r = -1.f;
   int arg = 0x7fffffff;
   if (rows_used != nullptr && *rows_used - row0 < N) N = *rows_used - row0;
   if (row < N) {
@@ -613,31 +628,31 @@ __global__ void __launch_bounds__(256) scores_fold_kernel(const float2* part, co
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int i = i0 + j * 32 * kWarps;
-        p[j] = i < tiles ? part[row * tiles + i] : make_float2(-INFINITY, 0.f);
+        p[j] = i < tiles ? part[row * tiles + i] : make_float2(-INFINITY, -1.f);
         a[j] = i < tiles && part_arg != nullptr ? part_arg[row * tiles + i] : 0x7fffffff;
       }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) join_scores(m, s, arg, p[j].x, p[j].y, a[j]);
+      for (int j = 0; j < 4; ++j) join_scores(m, r, arg, p[j].x, p[j].y, a[j]);
     }
   }
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1)
-    join_scores(m, s, arg, __shfl_xor_sync(0xffffffffu, m, off), __shfl_xor_sync(0xffffffffu, s, off), __shfl_xor_sync(0xffffffffu, arg, off));
+    join_scores(m, r, arg, __shfl_xor_sync(0xffffffffu, m, off), __shfl_xor_sync(0xffffffffu, r, off), __shfl_xor_sync(0xffffffffu, arg, off));
   if (kWarps > 1) {
-    if (lane == 0) { sm[warp] = m; ss[warp] = s; sa[warp] = arg; }
+    if (lane == 0) { sm[warp] = m; sr[warp] = r; sa[warp] = arg; }
     __syncthreads();
     if (warp != 0) return;
-    for (int i = 1; i < kWarps; ++i) join_scores(m, s, arg, sm[i], ss[i], sa[i]);
+    for (int i = 1; i < kWarps; ++i) join_scores(m, r, arg, sm[i], sr[i], sa[i]);
   }
   if (lane != 0 || row >= N) return;
-  const float l = m + logf(s);
+  const float log_s = log1pf(r), l = m + log_s;
   const int64_t at = place != nullptr ? place[row0 + row] : row;
   if (lse != nullptr) lse[at] = l;
   if (top != nullptr) top[row] = arg == 0x7fffffff ? 0 : arg;
   if (nll != nullptr) {
     const int64_t y = labels[row];
     // (m - z_y) + log s, not lse - z_y: a small loss keeps its digits
-    nll[at] = y == ignore ? 0.f : (y >= 0 && y < V ? (m - picked[row]) + logf(s) : __int_as_float(0x7fc00000));
+    nll[at] = y == ignore ? 0.f : (y >= 0 && y < V ? (m - picked[row]) + log_s : __int_as_float(0x7fc00000));
   }
 }
 
