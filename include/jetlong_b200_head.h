@@ -48,12 +48,12 @@ size_t jl_head_scores_workspace_bytes(int64_t rows, int32_t hidden_size, int32_t
 int jl_head_scores(const jl_head_scores_args* args, void* cuda_stream);
 
 /* ---------------------------------------------------------------------------------------------
- * jl_head_grads — gradients of sum_i g_i nll_i, from the lse that jl_head_scores returned:
+ * jl_head_grads — gradients of sum_i g_i nll_i, from the lse and nll that jl_head_scores returned for the same operands:
  *   dz_iv = g_i (e^{z_iv - lse_i} - [v == label_i])  (0 where label_i == ignore_index),
  *   d_hidden = dz weight,  d_weight = dz^T hidden;
  *   g_i = grad[i] (grad_stride 1) or *grad / (*grad_count if grad_count != NULL; 0 for a count of 0) for every row.
  * z is formed again piece by piece of the vocabulary; a piece of dz is held in bf16 in the workspace, both products
- * accumulate in fp32.  d_hidden (rows, hidden) and d_weight (vocab, hidden) bf16 contiguous; either may be NULL.
+ * accumulate in fp32.  At the label dz_i is g_i (e^{-nll_i} - 1), which does not cancel where the label is all but certain.  d_hidden (rows, hidden) and d_weight (vocab, hidden) bf16 contiguous; either may be NULL.
  * Results do not depend on the timing of anything (no atomics).
  * ------------------------------------------------------------------------------------------- */
 typedef struct {
@@ -65,6 +65,7 @@ typedef struct {
   int64_t rows;
   int32_t hidden_size, vocab;
   const float* lse;
+  const float* nll;
   const float* grad;
   int64_t grad_stride;      /* 0: one scalar for every row, 1: one value per row */
   const float* grad_count;  /* may be NULL; only with grad_stride 0 */

@@ -6,7 +6,7 @@
 // All products run on one persistent tcgen05 kernel (head_gemm_kernel) whose epilogue is what differs:
 //   scores  z tile -> per row (maximum, sum of exponentials, argmax, logit of the label); a fold kernel joins the tiles
 //   few     the same with the weight's rows as the rows of the product, for up to 32 rows of hidden states
-//   dz      z tile -> exp(z - lse) - onehot in bf16, one piece of the vocabulary at a time
+//   dz      z tile -> exp(z - lse) - onehot in bf16, one piece of the vocabulary at a time; at the label exp(-nll) - 1
 //   dh      dz W accumulated in fp32 over the pieces (bulk reductions in L2), rounded once at the end
 //   dW      dz^T h, final for the piece
 // The score and dz products read hidden and weight along their rows (K-major); dh reads weight and dW reads dz and
@@ -73,7 +73,7 @@ struct GemmParams {
   int* part_arg;              // the same or NULL
   float* picked;              // [row] logit of the label
   // dz
-  const float* lse;
+  const float *lse, *nll;
   const float* row_grad;      // NULL or one factor per row
   // both
   const int64_t* labels;      // may be NULL for scores
@@ -199,7 +199,8 @@ struct Product {
   // 512, 1024 and all of K: 2e-7 / 8.0 ms, 3.5e-7 / 7.5, 8e-7 / 7.25, 4e-6 / 7.1; a few rows are bound by the weight's bytes and
   // take parts of 256, up to 32 rows parts of 128, up to 16 of 64 (error of one row's lse with 64, 128, 256: 0.7e-7, 1.4e-7, 2.6e-7;
   // time of 151936 x 2048 in a loop 102.4, 102.3, 98.4 us, after a pause 98 with all; 32 rows x 4096: 225, 218, 207 us).
-  // Results that are rounded to bf16 need none of this.
+  // Results that are rounded to bf16 need none of this: in dz a probability may be off by 1e-4 of itself, and the label's p - 1, where
+  // that would be all there is, is taken from the loss.
   static constexpr int kAccs = kEpi_ >= kEpiFew16 ? 4 : 2, kAccCols = kTmemCols / kAccs;
   static constexpr bool kFew = kEpi_ == kEpiFew16 || kEpi_ == kEpiFew32, kParts = kEpi_ == kEpiScores || kFew;
   static constexpr int kPart = !kParts ? 1 << 30 : kEpi_ == kEpiFew16 ? 1 : kEpi_ == kEpiFew32 ? 2 : kPair_ == 1 ? 4 : 8;
@@ -446,7 +447,7 @@ __device__ __forceinline__ void finish(const GemmMaps& maps, const GemmParams& p
       const uint32_t acc = tmem + (st.i % P::kAccs) * P::kAccCols + lane_base;
       mbar_wait(&sm.acc_full[st.i % P::kAccs], (st.i / P::kAccs) & 1, sm);
       tc_fence_after();
-      float lse = 0.f, factor = 0.f;
+      float lse = 0.f, factor = 0.f, dz_y = 0.f;
       int y = -1;
       if constexpr (kEpi == kEpiDz) {
         if (row < p.M) {
@@ -457,6 +458,9 @@ __device__ __forceinline__ void finish(const GemmMaps& maps, const GemmParams& p
             if (label < 0 || label >= p.vocab) factor = __int_as_float(0x7fc00000);
             const int64_t rel = label - p.v0 - n0;
             y = rel >= 0 && rel < p.bn ? static_cast<int>(rel) : -1;
+            // p - 1 = e^-nll - 1.  exp(z - lse) - 1 would cancel: this z is cut off over all of K, and a row with 1 - p = 1e-6 got
+            // a hundred times its gradient.
+            if (y >= 0) dz_y = expm1f(-p.nll[row]);
           }
         }
       }
@@ -472,7 +476,7 @@ __device__ __forceinline__ void finish(const GemmMaps& maps, const GemmParams& p
           if constexpr (kEpi == kEpiDz) {
 #pragma unroll
             for (int j = 0; j < 32; ++j) {
-              const float pr = fast_exp2((__uint_as_float(z[j]) - lse) * kLog2e) - (y == cc + j ? 1.f : 0.f);
+              const float pr = y == cc + j ? dz_y : fast_exp2((__uint_as_float(z[j]) - lse) * kLog2e);
               z[j] = used ? __float_as_uint(pr * factor) : 0u;      // a row that does not count is zero whatever it holds
             }
             if (n0 + cc + 32 > p.N) {                              // the piece's last block of 64 columns is stored whole
@@ -765,11 +769,12 @@ __global__ void __launch_bounds__(1024) rows_used_kernel(const int64_t* labels, 
   if (threadIdx.x == 0) *used = base;
 }
 
-// Rows row0 .. row0 + gridDim.x of those in use, packed: hidden states, labels and, where given, lse and row gradients.  Up to the
+// Rows row0 .. row0 + gridDim.x of those in use, packed: hidden states, labels and, where given, lse with nll and row gradients.  Up to the
 // next multiple of 64 (a K block of the weight's gradient) the rows after the last are zero; every label after it is `ignore`.
 __global__ void __launch_bounds__(128) rows_gather_kernel(const __nv_bfloat16* hidden, int64_t stride, int row_len, const int64_t* labels, int64_t ignore,
-                                                          const float* lse, const float* row_grad, const int32_t* row_of, const int32_t* used, int64_t row0,
-                                                          __nv_bfloat16* hidden_out, int64_t* labels_out, float* lse_out, float* row_grad_out) {
+                                                          const float* lse, const float* nll, const float* row_grad, const int32_t* row_of, const int32_t* used,
+                                                          int64_t row0, __nv_bfloat16* hidden_out, int64_t* labels_out, float* lse_out, float* nll_out,
+                                                          float* row_grad_out) {
   wait_prerequisites();
   launch_dependents();
   const int64_t r = row0 + blockIdx.x, n = *used;
@@ -777,7 +782,10 @@ __global__ void __launch_bounds__(128) rows_gather_kernel(const __nv_bfloat16* h
   const int64_t from = in ? row_of[r] : 0;
   if (threadIdx.x == 0) {
     labels_out[blockIdx.x] = in ? labels[from] : ignore;
-    if (lse != nullptr) lse_out[blockIdx.x] = in ? lse[from] : 0.f;
+    if (lse != nullptr) {
+      lse_out[blockIdx.x] = in ? lse[from] : 0.f;
+      nll_out[blockIdx.x] = in ? nll[from] : 0.f;
+    }
     if (row_grad != nullptr) row_grad_out[blockIdx.x] = in ? row_grad[from] : 0.f;
   }
   if (r >= (n + kBK - 1) / kBK * kBK && r >= kBK) return;
@@ -983,13 +991,14 @@ constexpr int64_t kScoreRows = 16384;
 // Rows whose label is ignored are left out of the products where there are more row tiles than one: the others are packed first
 // (1000 rows x 4096 x 151936, two in five ignored: loss and gradients 3.58 -> 2.69 ms after a pause, 4.10 -> 3.10 in a loop).
 constexpr int64_t kPackRows = 257;
-struct Packed { size_t hidden, labels, lse, row_grad, row_of, place, used; };      // offsets in the workspace
+struct Packed { size_t hidden, labels, lse, nll, row_grad, row_of, place, used; };      // offsets in the workspace
 Packed packed_layout(size_t& total, int64_t rows, int64_t chunk, int32_t hd) {
   Packed k{};
   auto take = [&](int64_t bytes) { const size_t at = total; total += up256(static_cast<size_t>(bytes)); return at; };
   k.hidden = take(chunk * hd * 2);
   k.labels = take(chunk * 8);
   k.lse = take(chunk * 4);
+  k.nll = take(chunk * 4);
   k.row_grad = take(chunk * 4);
   k.row_of = take(rows * 4);
   k.place = take(rows * 4);
@@ -1085,8 +1094,9 @@ int launch_scores(const jl_head_scores_args* a, cudaStream_t stream) {
     p.row0 = r0;
     if (l.pack && launch_dependent(rows_gather_kernel, dim3(static_cast<unsigned>(n)), dim3(128), 0, stream, static_cast<const __nv_bfloat16*>(a->hidden),
                                    a->hidden_stride, a->hidden_size, a->labels, a->ignore_index, static_cast<const float*>(nullptr),
-                                   static_cast<const float*>(nullptr), static_cast<const int32_t*>(row_of), static_cast<const int32_t*>(used), r0, hidden_packed,
-                                   labels_packed, static_cast<float*>(nullptr), static_cast<float*>(nullptr)) != cudaSuccess)
+                                   static_cast<const float*>(nullptr), static_cast<const float*>(nullptr), static_cast<const int32_t*>(row_of),
+                                   static_cast<const int32_t*>(used), r0, hidden_packed, labels_packed, static_cast<float*>(nullptr), static_cast<float*>(nullptr),
+                                   static_cast<float*>(nullptr)) != cudaSuccess)
       return check_launch("jl_head_scores (packing)");
     const Matrix h = l.pack ? Matrix{hidden_packed, n, a->hidden_size, a->hidden_size}
                             : Matrix{static_cast<const __nv_bfloat16*>(a->hidden) + r0 * a->hidden_stride, n, a->hidden_size, a->hidden_stride};
@@ -1127,6 +1137,7 @@ int launch_grads(const jl_head_grads_args* a, cudaStream_t stream) {
   if (a->workspace == nullptr || a->workspace_bytes < l.total)
     return fail(JL_ERR_WORKSPACE, "jl_head_grads: workspace of %zu bytes needed, %zu given", l.total, a->workspace_bytes);
   if (reinterpret_cast<uintptr_t>(a->workspace) & 15) return fail(JL_ERR_BAD_ARG, "jl_head_grads: workspace not 16-byte aligned");
+  if (a->nll == nullptr) return fail(JL_ERR_BAD_ARG, "jl_head_grads: nll is NULL");
   rc = check_device_arch();
   if (rc != JL_OK) return rc;
   const int64_t N = a->rows, H = a->hidden_size, V = a->vocab;
@@ -1139,6 +1150,7 @@ int launch_grads(const jl_head_grads_args* a, cudaStream_t stream) {
   GemmParams base{};
   base.labels = a->labels; base.ignore = a->ignore_index; base.vocab = V;
   base.lse = a->lse;
+  base.nll = a->nll;
   base.row_grad = a->grad_stride != 0 ? a->grad : nullptr;
   base.scale = GradScale{a->grad, a->grad_count, a->grad_stride != 0};
   Matrix h{a->hidden, N, H, a->hidden_stride};
@@ -1146,18 +1158,20 @@ int launch_grads(const jl_head_grads_args* a, cudaStream_t stream) {
   if (l.pack) {
     int32_t *const row_of = reinterpret_cast<int32_t*>(ws + l.packed.row_of), *const used = reinterpret_cast<int32_t*>(ws + l.packed.used);
     int64_t* const labels = reinterpret_cast<int64_t*>(ws + l.packed.labels);
-    float *const lse = reinterpret_cast<float*>(ws + l.packed.lse), *const row_grad = reinterpret_cast<float*>(ws + l.packed.row_grad);
+    float *const lse = reinterpret_cast<float*>(ws + l.packed.lse), *const nll = reinterpret_cast<float*>(ws + l.packed.nll),
+          *const row_grad = reinterpret_cast<float*>(ws + l.packed.row_grad);
     __nv_bfloat16* const hidden = reinterpret_cast<__nv_bfloat16*>(ws + l.packed.hidden);
     place = reinterpret_cast<int32_t*>(ws + l.packed.place);
     if (launch_dependent(rows_used_kernel, dim3(1), dim3(1024), 0, stream, a->labels, a->ignore_index, N, row_of, const_cast<int32_t*>(place), used,
                          static_cast<float*>(nullptr), static_cast<float*>(nullptr)) != cudaSuccess)
       return check_launch("jl_head_grads (rows in use)");
     if (launch_dependent(rows_gather_kernel, dim3(static_cast<unsigned>(N)), dim3(128), 0, stream, static_cast<const __nv_bfloat16*>(a->hidden),
-                         a->hidden_stride, a->hidden_size, a->labels, a->ignore_index, a->lse, base.row_grad, static_cast<const int32_t*>(row_of),
-                         static_cast<const int32_t*>(used), int64_t(0), hidden, labels, lse, row_grad) != cudaSuccess)
+                         a->hidden_stride, a->hidden_size, a->labels, a->ignore_index, a->lse, a->nll, base.row_grad, static_cast<const int32_t*>(row_of),
+                         static_cast<const int32_t*>(used), int64_t(0), hidden, labels, lse, nll, row_grad) != cudaSuccess)
       return check_launch("jl_head_grads (packing)");
     base.labels = labels;
     base.lse = lse;
+    base.nll = nll;
     if (base.row_grad != nullptr) base.row_grad = row_grad;
     base.rows_used = used;
     h = Matrix{hidden, N, H, H};

@@ -230,7 +230,7 @@ class HeadGradsArgs(C.Structure):
     _fields_ = [
         ("hidden", C.c_void_p), ("weight", C.c_void_p), ("hidden_stride", C.c_int64), ("weight_stride", C.c_int64),
         ("labels", C.c_void_p), ("ignore_index", C.c_int64), ("rows", C.c_int64), ("hidden_size", C.c_int32), ("vocab", C.c_int32),
-        ("lse", C.c_void_p), ("grad", C.c_void_p), ("grad_stride", C.c_int64), ("grad_count", C.c_void_p),
+        ("lse", C.c_void_p), ("nll", C.c_void_p), ("grad", C.c_void_p), ("grad_stride", C.c_int64), ("grad_count", C.c_void_p),
         ("d_hidden", C.c_void_p), ("d_weight", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
     ]
 

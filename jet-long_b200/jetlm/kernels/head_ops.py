@@ -112,16 +112,21 @@ class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, labels, ignore_index, reduction):
         h, lab = _rows("linear_cross_entropy", hidden, weight, labels)
-        per_row = reduction == "none"
-        nll, lse, _, loss, count = _scores(h, weight, lab, ignore_index, nll=per_row, top=False, reduction=None if per_row else reduction, skip_ignored=1)
-        ctx.save_for_backward(h, weight, lab, lse, count if reduction == "mean" else None)
+        per_row, grads = reduction == "none", any(ctx.needs_input_grad)
+        nll, lse, _, loss, count = _scores(h, weight, lab, ignore_index, nll=per_row or grads, top=False, reduction=None if per_row else reduction,
+                                           skip_ignored=1)
+        if grads:
+            ctx.save_for_backward(h, weight, lab, lse, nll, count if reduction == "mean" else None)
         ctx.ignore_index, ctx.per_row, ctx.shape = int(ignore_index), per_row, hidden.shape
-        return nll.view(labels.shape) if per_row else loss
+        if not per_row:
+            return loss
+        # a copy of its own for the caller, who may write into it before the backward pass reads the losses
+        return nll.view(labels.shape).clone() if grads else nll.view(labels.shape)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        h, w, lab, lse, count = ctx.saved_tensors
+        h, w, lab, lse, nll, count = ctx.saved_tensors
         n, dev, a, lib = h.shape[0], h.device, N.HeadGradsArgs(), N.lib()
         d_h = torch.empty(h.shape, dtype=h.dtype, device=dev) if ctx.needs_input_grad[0] else None
         d_w = torch.empty(w.shape, dtype=w.dtype, device=dev) if ctx.needs_input_grad[1] else None
@@ -129,7 +134,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
             grad = grad.to(torch.float32).reshape(-1).contiguous()
         ws = torch.empty(lib.jl_head_grads_workspace_bytes(n, w.shape[1], w.shape[0]), dtype=torch.uint8, device=dev)
         a.weight, a.hidden_stride, a.weight_stride, a.ignore_index = w.data_ptr(), _row_stride(h), _row_stride(w), ctx.ignore_index
-        a.hidden, a.labels, a.lse, a.grad = (t.data_ptr() or a.weight for t in (h, lab, lse, grad))      # no rows: never read
+        a.hidden, a.labels, a.lse, a.nll, a.grad = (t.data_ptr() or a.weight for t in (h, lab, lse, nll, grad))      # no rows: never read
         a.rows, a.hidden_size, a.vocab, a.grad_stride = n, w.shape[1], w.shape[0], 1 if ctx.per_row else 0
         if count is not None:
             a.grad_count = count.data_ptr()

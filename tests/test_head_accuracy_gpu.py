@@ -69,3 +69,43 @@ def test_scores_of_sure_rows_keep_their_digits(N, H):
     assert (rel <= 2.0 ** -11).all(), (rel.max(), want[rel.argmax()])
     plain = head_ops.linear_cross_entropy(h, w, y, reduction="none")
     assert ((plain.double() - want).abs() <= 2.0 ** -11 * want).all()
+
+
+@pytest.mark.parametrize("reduction", ["sum", "none", "mean"])
+@pytest.mark.parametrize("N, H", [(1, 4096), (17, 2048), (49, 4096), (128, 2048), (200, 4096), (300, 2048), (300, 4096)])
+def test_gradient_of_sure_rows(N, H, reduction):
+    """1 - p from 1e-2 down to 1e-6: every row's gradient is right relative to the row itself, not to gradients of size one."""
+    from jetlm.kernels import head_ops
+    h, w, y = sure_rows(N, H, 1e-6, 1e-2, seed=5)
+    if N > 256:                                       # rows that do not count in between: the others are packed
+        y[3::7] = -100
+    used = y >= 0
+    hu, yu = h[used], y[used]
+    _, _, q, dz = exact(hu, w, yu)
+    n = len(yu)
+    up = torch.linspace(0.5, 2.0, N, device="cuda") if reduction == "none" else torch.tensor(1.5, device="cuda")
+    c = (up[used] if reduction == "none" else (up / n if reduction == "mean" else up).expand(n)).double()[:, None]
+    hg, wg = h.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    dh, dw = torch.autograd.grad(head_ops.linear_cross_entropy(hg, wg, y, reduction=reduction), [hg, wg], up)
+    dz = dz * c
+    want_h, want_w = dz @ w.double(), dz.T @ hu.double()
+    # d logits are rounded once (HALF of each), probabilities are off by less than 2^-11 (z cut off 256 times at 2^-23 of up to 8, lse,
+    # exponential) and fp32 sums over V / 16 steps lose less than 2^-12; the result is rounded once
+    each = HALF + 2.0 ** -10
+    bound = each * (dz.abs() @ w.double().norm(dim=1)) + HALF * (1 + HALF) * want_h.norm(dim=1)
+    err = (dh[used].double() - want_h).norm(dim=1)
+    assert (err <= bound).all(), ((err / bound).max(), (q / (1 + q))[(err / bound).argmax()])
+    assert (dh[~used] == 0).all()
+    bound_w = each * (dz.abs().T @ hu.double().abs()) + HALF * (1 + HALF) * want_w.abs() + 1e-30
+    assert ((dw.double() - want_w).abs() <= bound_w).all()
+
+
+def test_losses_may_be_overwritten_before_the_backward_pass():
+    from jetlm.kernels import head_ops
+    h, w, y = sure_rows(40, 256, 1e-3, 1e-1)
+    h.requires_grad_(True)
+    m = torch.linspace(0, 1, 40, device="cuda")
+    want, = torch.autograd.grad((head_ops.linear_cross_entropy(h, w, y, reduction="none") * m).sum(), h)
+    loss = head_ops.linear_cross_entropy(h, w, y, reduction="none")
+    loss *= m
+    assert torch.equal(torch.autograd.grad(loss.sum(), h)[0], want)
