@@ -78,7 +78,9 @@ int jl_tree_append(const jl_tree_append_args* args, void* cuda_stream);
  * out (B, T, H, D) with strides, lse (B, H, T) fp32 contiguous or NULL.  A row that sees no key (an absent node of
  * an empty cache, a zero mask) is zero with lse = -inf; an absent node (depth < 0) sees nothing.
  * depth[b][t] < nodes.  A value row that an absent node would use may hold anything; the values of present nodes and of
- * committed rows must be finite.  softmax_scale is positive and finite.  lens[b] is clamped to [0, rows - nodes]; no row past lens[b] + nodes is read into a result.  batch * kv_heads <= 65535.
+ * committed rows must be finite.  softmax_scale is positive and finite.  batch * kv_heads <= 65535.
+ * 0 <= lens[b] <= rows.  Places of the tree that reach past the last row (lens[b] + t >= rows) are absent nodes, whatever depth and mask
+ * say of them; a negative length counts as 0, one above rows as rows - nodes.  No row past lens[b] + nodes is read into a result.
  * workspace: jl_tree_attention_workspace_bytes, 16-byte aligned, not initialised by the caller and not kept between
  * calls; two calls that may overlap on the GPU need one each.
  * ------------------------------------------------------------------------------------------- */

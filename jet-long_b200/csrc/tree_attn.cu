@@ -85,14 +85,18 @@ struct TreeSmem {
 };
 
 // The visits of one (sample, key head): far key tiles [0, far), then near key tiles near0 ..
-struct Visits { int len, far, near0, n; };
+// `nodes`: the places of the tree that the cache has rows for.  A node behind them is an absent one, as tree_append stored no key of it.
+// A length that is none of this cache counts as the nearest one that leaves a row to every place.
+struct Visits { int len, nodes, far, near0, n; };
 __device__ __forceinline__ Visits visits_of(const TreeParams& p, int b) {
   Visits v;
-  v.len = min(max(p.lens[b], 0), p.rows - p.nodes);
-  const int64_t end = v.len + p.nodes;
+  v.len = max(p.lens[b], 0);
+  if (v.len > p.rows) v.len = p.rows - p.nodes;
+  v.nodes = min(p.nodes, p.rows - v.len);
+  const int64_t end = static_cast<int64_t>(v.len) + v.nodes;
   v.far = v.near0 = 0;
   if (p.two_classes) {
-    int64_t hi = p.nodes_far ? end : v.len + p.nodes - 1 - p.w_0;              // keys below this can be far for some node
+    int64_t hi = p.nodes_far ? end : static_cast<int64_t>(v.len) + p.nodes - 1 - p.w_0;      // keys below this can be far for some node
     hi = hi < 0 ? 0 : (hi > end ? end : hi);
     v.far = static_cast<int>((hi + kTileN - 1) / kTileN);
     const int64_t lo = v.len - p.w_0;                                          // keys from this on can be near
@@ -458,7 +462,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
       const int step = two_tiles ? 1 : 2, first = seg.v0 + (two_tiles ? 0 : (g ^ t) & 1);
       g += seg.v1 - seg.v0;
       const int64_t nrow = static_cast<int64_t>(seg.b) * p.nodes + (row_used ? node : 0);
-      const int d = row_used ? p.depth[nrow] : -1;
+      const int d = row_used && node < seg.vis.nodes ? p.depth[nrow] : -1;
       const int len = seg.vis.len;
       m_ref = -INFINITY;
       l_sum = 0.f;
@@ -485,7 +489,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
         uint32_t words[kTileN / 32 + 1];
         bool with_nodes = false;
         if (!uniform) {
-          with_nodes = d >= 0 && u_tile > -kTileN && u_tile < p.nodes && (!far || p.nodes_far);
+          with_nodes = d >= 0 && u_tile > -kTileN && u_tile < seg.vis.nodes && (!far || p.nodes_far);
 #pragma unroll
           for (int i = 0; i <= kTileN / 32; ++i) {
             const int at = (u_tile >> 5) + i;
@@ -544,7 +548,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
               uint32_t bits = __funnelshift_r(words[0], words[1], u_tile & 31);
 #pragma unroll
               for (int i = 0; i < kTileN / 32; ++i) words[i] = words[i + 1];
-              const int left = p.nodes - u0;
+              const int left = seg.vis.nodes - u0;
               if (left < 32) bits = left > 0 ? bits & (0xffffffffu >> (32 - left)) : 0u;
               if (p.nodes_far) {
                 for (uint32_t todo = bits; todo != 0u; todo &= todo - 1) {

@@ -200,8 +200,8 @@ def tree_attention(q_base: torch.Tensor, q_group: torch.Tensor, key_rows: torch.
                    softmax_scale: Optional[float] = None, out: Optional[torch.Tensor] = None, return_lse: bool = True):
     """Bifocal attention of a drafted tree over the cache (see jl_tree_attention).  q_base / q_group (B,T,H,D) views
     sharing strides; key_rows / key_group_rows / value_rows (B,rows,Hk,D) views of this layer's whole cache buffers, the
-    nodes' rows included; lens (B,) int32 committed tokens per sample, on the device, lens[b] + T <= rows.  Pairs more
-    than w_0 positions apart are scored q_group . key_group_rows, the others q_base . key_rows; without key_group_rows
+    nodes' rows included; lens (B,) int32 committed tokens per sample, on the device.  A node whose row lens[b] + t is past
+    the cache is an absent one (places of a padded batch may reach there, nodes should not).  Pairs more than w_0 positions apart are scored q_group . key_group_rows, the others q_base . key_rows; without key_group_rows
     (group size 1) every pair is scored q_base . key_rows.  Nothing depends on lens on the host, so the launches can sit
     in a CUDA graph.  Returns (out (B,T,H,D), lse (B,H,T) fp32) or out; a row that sees no key is zero with lse -inf."""
     op = "tree_attention"

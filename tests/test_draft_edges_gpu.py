@@ -1,0 +1,65 @@
+"""Tree-of-drafts operators at the edges: at the end of a cache."""
+import math
+
+import pytest
+import torch
+
+from test_draft_ops_gpu import D, HALF, attend_64, call, check_attention, inv_freq, make, paths_of
+
+pytestmark = pytest.mark.gpu
+
+
+def full_cache(rows, T, H, Hk, present, w_0, two, seed, spare):
+    """Sample b has present[b] nodes of T places and a cache that they fill to the last row (to `spare` rows from it for the last sample)."""
+    B = len(present)
+    s = make((B, T, H, Hk, [rows - T] * B, 0, w_0, two, "tree"), seed=seed, poison=False)
+    assert s["k"].shape[1] == rows
+    for b, n in enumerate(present):
+        s["par"][b, n:] = -2
+    s["paths"] = paths_of(s["par"])
+    s["lens"] = [rows - n for n in present]
+    s["lens"][-1] -= spare
+    for b, n in enumerate(present):                   # rows that hold nothing
+        for t in (s["k"], s["kg"], s["v"]):
+            if t is not None:
+                t[b, s["lens"][b] + n:] = math.nan
+    return s
+
+
+@pytest.mark.parametrize("w_0", [0, 5, 100, 5000])
+@pytest.mark.parametrize("rows, T, H, Hk, present, two", [
+    (300, 40, 16, 8, [40, 10, 1, 0, 7], True), (256, 16, 32, 8, [16, 3, 0, 5], True), (384, 130, 8, 8, [130, 64, 2, 1], True),
+    (129, 9, 8, 2, [1, 0, 9, 2], False), (64, 64, 12, 4, [0, 64, 1, 30], True), (1300, 70, 32, 8, [5, 70, 33, 3], True)])
+def test_nodes_that_reach_the_last_row_of_the_cache(rows, T, H, Hk, present, two, w_0):
+    """A padded batch whose places do not all fit, but whose nodes do: every sample is attended where its nodes are."""
+    s = full_cache(rows, T, H, Hk, present, w_0, two, seed=rows + w_0, spare=2 if rows > T else 0)
+    want, want_lse, absv = attend_64(s["qb"], s["qg"], s["k"], s["kg"], s["v"], s["paths"], s["lens"], w_0, D ** -0.5)
+    out, lse = call(s)
+    check_attention(out, lse, want, absv, want_lse)
+
+
+def test_append_and_attention_agree_on_a_full_cache():
+    """Nodes written by tree_append into the last rows are attended where they were written."""
+    from jetlm.kernels import draft_ops as d
+    g = torch.Generator(device="cuda").manual_seed(1)
+    rn = lambda *s: torch.randn(*s, generator=g, device="cuda").bfloat16()        # noqa: E731
+    par = torch.full((2, 12), -2, dtype=torch.int32)
+    par[0, :3], par[1, :12] = torch.tensor([-1, 0, 0]), torch.arange(-1, 11)
+    lens = [97, 60]
+    kc, vc, kg = rn(2, 100, 4, D), rn(2, 100, 4, D), rn(2, 100, 4, D)
+    tree, dl = d.draft_tree(par.cuda()), torch.tensor(lens, dtype=torch.int32, device="cuda")
+    qb, qg = d.tree_append(rn(2, 12, 8, D), rn(2, 12, 4, D), rn(2, 12, 4, D), rn(D), rn(D), inv_freq(), kc, vc, tree, dl, q_eps=1e-6, k_eps=1e-6,
+                           group_size=3, key_group_rows=kg)
+    want, want_lse, absv = attend_64(qb, qg, kc, kg, vc, paths_of(par), lens, 20, D ** -0.5)
+    out, lse = d.tree_attention(qb, qg, kc, vc, tree, dl, w_0=20, key_group_rows=kg)
+    check_attention(out, lse, want, absv, want_lse)
+
+
+def test_a_node_whose_row_is_past_the_cache_is_an_absent_one():
+    """Its key has no place: it sees nothing (zero, lse -inf), nobody sees it, and the nodes before it are as they are without it."""
+    s = make((2, 6, 8, 4, [94, 94], 0, 30, True, "chain"), seed=4, poison=False)      # 100 rows
+    s["lens"] = [97, 100]
+    s["paths"] = [[p if t < 3 else [] for t, p in enumerate(s["paths"][0])], [[] for _ in s["paths"][1]]]
+    want, want_lse, absv = attend_64(s["qb"], s["qg"], s["k"], s["kg"], s["v"], s["paths"], s["lens"], 30, D ** -0.5)
+    out, lse = call(s)
+    check_attention(out, lse, want, absv, want_lse)
