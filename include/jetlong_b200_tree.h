@@ -77,6 +77,7 @@ int jl_tree_append(const jl_tree_append_args* args, void* cuda_stream);
  * k_base.  q_group and k_group both NULL: one class, every pair is scored as q_base . k_base.
  * out (B, T, H, D) with strides, lse (B, H, T) fp32 contiguous or NULL.  A row that sees no key (an absent node of
  * an empty cache, a zero mask) is zero with lse = -inf; an absent node (depth < 0) sees nothing.
+ * A row with a score of NaN (a query of NaN, say) is NaN, and so is its lse; no other row is.
  * depth[b][t] < nodes.  A value row that an absent node would use may hold anything; the values of present nodes and of
  * committed rows must be finite.  softmax_scale is positive and finite.  batch * kv_heads <= 65535.
  * 0 <= lens[b] <= rows.  Places of the tree that reach past the last row (lens[b] + t >= rows) are absent nodes, whatever depth and mask

@@ -398,9 +398,10 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
 
     // The end of a segment.  Two states of one tile are joined, each warpgroup taking half of the columns (tensor memory is shared by
     // the warps of a row quarter).  A segment that is all of its (sample, key head) leaves the result, another one a partial: O / l in
-    // fp32 (zero where the row saw nothing) and the LSE in the log2 domain.
+    // fp32 (zero where the row saw nothing) and the LSE in the log2 domain.  A row has seen something when its sum is not 0: scores of
+    // NaN leave the maximum at -inf, their sum is NaN, and so is then all that the row leaves.
     auto leave = [&](const Segment& s, int d, bool any) {
-      float m = any && d >= 0 ? m_ref : -INFINITY, l = l_sum, mine = 1.f, other = 0.f;
+      float m = any && d >= 0 ? m_ref : -INFINITY, l = any && d >= 0 ? l_sum : 0.f, mine = 1.f, other = 0.f;
       if (!two_tiles) {
         sm.stats[t][r] = make_float2(m, l);
         tc_fence_before();
@@ -410,10 +411,10 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
         const float top = fmaxf(m, o.x), ref = top == -INFINITY ? 0.f : top;
         mine = m == -INFINITY ? 0.f : fast_exp2(m - ref);
         other = o.x == -INFINITY ? 0.f : fast_exp2(o.x - ref);
-        l = (m == -INFINITY ? 0.f : l * mine) + (o.x == -INFINITY ? 0.f : o.y * other);
+        l = l * mine + o.y * other;
         m = top;
       }
-      const bool seen = m != -INFINITY, whole = s.v0 == 0 && s.v1 == s.vis.n;
+      const bool seen = l != 0.f, whole = s.v0 == 0 && s.v1 == s.vis.n;
       const float inv = seen ? 1.f / l : 0.f;
       mine = seen ? mine * inv : 0.f;
       other *= inv;
@@ -706,10 +707,10 @@ __global__ void __launch_bounds__(128) tree_combine_kernel(const TreeParams p) {
         acc.x = fmaf(w, x[j].x, acc.x); acc.y = fmaf(w, x[j].y, acc.y); acc.z = fmaf(w, x[j].z, acc.z); acc.w = fmaf(w, x[j].w, acc.w);
       }
     }
-    const float inv = sum > 0.f ? 1.f / sum : 0.f;
+    const float inv = sum != 0.f ? 1.f / sum : 0.f;            // NaN where a partial is
     *reinterpret_cast<uint2*>(p.out + b * p.os_b + nd * p.os_s + h * p.os_h + 4 * c) =
         make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
-    if (p.lse != nullptr && c == 0) p.lse[(static_cast<int64_t>(b) * heads + h) * p.nodes + nd] = sum > 0.f ? (m + log2f(sum)) * kLn2 : -INFINITY;
+    if (p.lse != nullptr && c == 0) p.lse[(static_cast<int64_t>(b) * heads + h) * p.nodes + nd] = sum != 0.f ? (m + log2f(sum)) * kLn2 : -INFINITY;
   }
 }
 

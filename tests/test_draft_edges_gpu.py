@@ -1,4 +1,4 @@
-"""Tree-of-drafts operators at the edges: at the end of a cache."""
+"""Tree-of-drafts operators at the edges: at the end of a cache, with NaN in the queries."""
 import math
 
 import pytest
@@ -63,3 +63,31 @@ def test_a_node_whose_row_is_past_the_cache_is_an_absent_one():
     want, want_lse, absv = attend_64(s["qb"], s["qg"], s["k"], s["kg"], s["v"], s["paths"], s["lens"], 30, D ** -0.5)
     out, lse = call(s)
     check_attention(out, lse, want, absv, want_lse)
+
+
+@pytest.mark.parametrize("case", [
+    (1, 5, 16, 8, [200], 0, 60, True, "chain"), (1, 12, 32, 8, [9000], 3, 3000, True, "chain"), (1, 64, 32, 8, [20000], 0, 700, True, "forest"),
+    (40, 4, 8, 8, list(range(10, 410, 10)), 0, 33, True, "chain"), (1, 16, 32, 8, [3000], 60000, 900, True, "tree"), (2, 80, 32, 8, [5000, 77], 0, 50, False, "tree")],
+    ids=["whole", "split", "two_tiles", "many", "long_form", "three_tiles"])
+def test_a_query_of_nan_gives_nan(case):
+    """As in the plain form; no other row notices."""
+    s = make(case, seed=9)
+    ref, ref_lse = call(s)
+    b, t, h = case[0] - 1, 2, 1
+    s["qb"][b, t, h], s["qg"][b, t, h] = math.nan, math.nan
+    out, lse = call(s)
+    assert torch.isnan(out[b, t, h]).all() and torch.isnan(lse[b, h, t])
+    out[b, t, h], lse[b, h, t] = ref[b, t, h], ref_lse[b, h, t]
+    assert torch.equal(out, ref) and torch.equal(lse, ref_lse)
+
+
+def test_a_score_of_nan_in_one_class_only():
+    """NaN in the far query alone: rows with far keys are NaN, the others are not."""
+    s = make((1, 3, 8, 8, [50], 0, 30, True, "chain"), seed=3, poison=False)
+    ref, ref_lse = call(s)
+    s["qg"][0, 1] = math.nan
+    out, lse = call(s)
+    assert torch.isnan(out[0, 1]).all() and torch.isnan(lse[0, :, 1]).all()
+    assert torch.equal(out[0, [0, 2]], ref[0, [0, 2]]) and torch.equal(lse[0, :, [0, 2]], ref_lse[0, :, [0, 2]])
+    s["w_0"] = 1000
+    assert torch.isfinite(call(s)[0]).all()
