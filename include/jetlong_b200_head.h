@@ -49,7 +49,7 @@ int jl_head_scores(const jl_head_scores_args* args, void* cuda_stream);
 
 /* ---------------------------------------------------------------------------------------------
  * jl_head_grads — gradients of sum_i g_i nll_i, from the lse and nll that jl_head_scores returned for the same operands:
- *   dz_iv = g_i (e^{z_iv - lse_i} - [v == label_i])  (0 where label_i == ignore_index),
+ *   dz_iv = g_i (e^{z_iv - lse_i} - [v == label_i])  (0 where label_i == ignore_index, whatever row i holds),
  *   d_hidden = dz weight,  d_weight = dz^T hidden;
  *   g_i = grad[i] (grad_stride 1) or *grad / (*grad_count if grad_count != NULL; 0 for a count of 0) for every row.
  * z is formed again piece by piece of the vocabulary; a piece of dz is held in bf16 in the workspace, both products

@@ -75,6 +75,10 @@ struct GemmParams {
   // dz
   const float *lse, *nll;
   const float* row_grad;      // NULL or one factor per row
+  const __nv_bfloat16* hidden;      // copy_counted()'s operands
+  __nv_bfloat16* counted;     // NULL: no copy
+  int64_t hidden_stride;
+  int row_len;
   // both
   const int64_t* labels;      // may be NULL for scores
   int64_t ignore, vocab, v0;  // column 0 of the product is vocabulary entry v0
@@ -500,6 +504,17 @@ __device__ __forceinline__ void finish(const GemmMaps& maps, const GemmParams& p
   }
 }
 
+// The rows of hidden states with zeros for those that do not count, one warp of every CTA a row at a time: d logits of such a row are
+// zero, and 0 * NaN in the weight's gradient is not.  Warp 3 does it while the dz product runs, where it has nothing else to do.
+__device__ __forceinline__ void copy_counted(const GemmParams& p, int lane) {
+  for (int64_t row = blockIdx.x; row < p.M; row += gridDim.x) {
+    const bool counts = p.labels[row] != p.ignore;
+    const uint4* src = reinterpret_cast<const uint4*>(p.hidden + row * p.hidden_stride);
+    uint4* dst = reinterpret_cast<uint4*>(p.counted + row * p.row_len);
+    for (int c = lane; c < p.row_len / 8; c += 32) dst[c] = counts ? src[c] : make_uint4(0u, 0u, 0u, 0u);
+  }
+}
+
 // The product's extents for the rows in use.  One row is kept where a result is due whatever the number (it counts for nothing).
 template <class P>
 __device__ __forceinline__ GemmParams in_use(const GemmParams& p) {
@@ -577,6 +592,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) head_gemm_kernel(const __grid
       asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(leader));
       issue<P0>(q0, sm, tmem, leader, worker, workers, st);
       if constexpr (kTwo) issue<P1>(q1, sm, tmem, leader, worker, workers, st);
+    } else if (P0::kEpi == kEpiDz && warp == 3 && p0.counted != nullptr) {
+      copy_counted(p0, lane);
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsHigh));
@@ -1025,7 +1042,7 @@ ScoresLayout scores_layout(int64_t rows, int32_t hd, int32_t vocab, bool skip_ig
 
 // Pieces of the vocabulary in the gradient pass: as large as 256 MB of dz allow (fewer, longer launches), balanced, a
 // multiple of 256.
-struct GradsLayout { int64_t piece; Plan dz, dh, dw; int splits; size_t dh32, total; bool pack; Packed packed; };
+struct GradsLayout { int64_t piece; Plan dz, dh, dw; int splits; size_t dh32, counted, total; bool pack; Packed packed; };
 GradsLayout grads_layout(int64_t rows, int32_t hd, int32_t vocab) {
   GradsLayout l{};
   const int64_t n = rows > 0 ? rows : 1;
@@ -1039,7 +1056,9 @@ GradsLayout grads_layout(int64_t rows, int32_t hd, int32_t vocab) {
   l.dh32 = up256(static_cast<size_t>(n) * l.piece * 2);
   l.total = l.dh32 + up256(static_cast<size_t>(n) * hd * 4 * l.splits);
   l.pack = rows >= kPackRows;
+  l.counted = l.total;
   if (l.pack) l.packed = packed_layout(l.total, rows, rows, hd);
+  else l.total += up256(static_cast<size_t>(n) * hd * 2);
   return l;
 }
 
@@ -1176,6 +1195,9 @@ int launch_grads(const jl_head_grads_args* a, cudaStream_t stream) {
     base.rows_used = used;
     h = Matrix{hidden, N, H, H};
   }
+  // the weight's gradient multiplies every row, if by zero: it takes rows that do not count as zero (packed rows are that already)
+  __nv_bfloat16* const counted = l.pack || a->d_weight == nullptr ? nullptr : reinterpret_cast<__nv_bfloat16*>(ws + l.counted);
+  const Matrix hw = counted != nullptr ? Matrix{counted, N, H, H} : h;
   int splits = 1;
   bool rounded = false;
   auto round_rows = [&]() -> int {
@@ -1190,6 +1212,12 @@ int launch_grads(const jl_head_grads_args* a, cudaStream_t stream) {
     const Matrix dz{ws, N, piece, 0};
     Gemm z{GemmMaps{}, base}, dh{GemmMaps{}, base}, dw{GemmMaps{}, base};
     z.p.v0 = v0;
+    if (v0 == 0) {
+      z.p.hidden = static_cast<const __nv_bfloat16*>(a->hidden);
+      z.p.counted = counted;
+      z.p.hidden_stride = a->hidden_stride;
+      z.p.row_len = a->hidden_size;
+    }
     z.p.group_m = group_of(H, l.dz.pair);
     Plan plan = l.dz;
     plan.n_tiles = static_cast<int>(cdiv(piece, plan.bn));
@@ -1215,7 +1243,7 @@ int launch_grads(const jl_head_grads_args* a, cudaStream_t stream) {
       plan = l.dw;
       plan.m_tiles = static_cast<int>(cdiv(piece, 256));
       dw.p.group_m = 0;
-      rc = prepare<Dw2>(dw, dz, h, Result{static_cast<__nv_bfloat16*>(a->d_weight) + v0 * H, H, false, 1}, plan, N, 1);
+      rc = prepare<Dw2>(dw, dz, hw, Result{static_cast<__nv_bfloat16*>(a->d_weight) + v0 * H, H, false, 1}, plan, N, 1);
     }
     if (rc == JL_OK && a->d_hidden != nullptr && a->d_weight != nullptr && l.dh.pair == 2) {
       // dh has few, long tiles (160 on 74 pairs for 4096 rows x 2560: 72 % of three rounds); dW's many short ones fill in

@@ -154,7 +154,8 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, labels: tor
     (V, H) bf16, labels (...) int64; reduction "mean" (over the labels that are not ignore_index; NaN if there is none, as
     in torch), "sum" or "none" (shape of labels).  The loss is fp32, the gradients are bf16.  The backward pass holds one
     piece of the vocabulary of d logits, in bf16; both gradients accumulate in fp32 and do not vary from run to run.
-    Rows whose label is ignore_index take no part: with more than 256 rows the others are packed and only they are multiplied.
+    Rows whose label is ignore_index take no part, whatever they hold: with more than 256 rows the others are packed and only
+    they are multiplied.
     A label that is neither ignore_index nor in [0, V) makes the loss and the gradients NaN; nothing is read out of range.
     Both passes can be captured into a CUDA graph (with torch.autograd.grad, or .backward() while no eager graph of the
     same leaves is alive)."""
