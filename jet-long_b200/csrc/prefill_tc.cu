@@ -1128,6 +1128,7 @@ int prefill_tc_status() {
   int* w = status_word();
   int v = 0;
   if (w != nullptr) {
+    if (cudaDeviceSynchronize() != cudaSuccess) return -1;      // the copy alone waits for the legacy stream and what blocks on it
     if (cudaMemcpy(&v, w, sizeof(int), cudaMemcpyDeviceToHost) != cudaSuccess) return -1;
     if (v != 0) cudaMemset(w, 0, sizeof(int));      // reading a raised status clears it, so later launches run again
   }

@@ -815,6 +815,7 @@ int launch_tree_attention(const jl_tree_attention_args* a, cudaStream_t stream) 
 
 int tree_status() {
   int v = 0;
+  if (cudaDeviceSynchronize() != cudaSuccess) return -1;      // the copy alone waits for the legacy stream and what blocks on it
   if (cudaMemcpyFromSymbol(&v, g_tree_status, sizeof(int)) != cudaSuccess) return -1;
   const int zero = 0;
   if (v != 0) cudaMemcpyToSymbol(g_tree_status, &zero, sizeof(int));

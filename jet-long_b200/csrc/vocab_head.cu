@@ -1287,6 +1287,7 @@ int jl_head_grads(const jl_head_grads_args* args, void* cuda_stream) {
 
 int jl_head_status(void) {
   int v = 0;
+  if (cudaDeviceSynchronize() != cudaSuccess) return -1;      // the copy alone waits for the legacy stream and what blocks on it
   if (cudaMemcpyFromSymbol(&v, jl::g_head_status, sizeof(int)) != cudaSuccess) return -1;
   const int zero = 0;
   if (v != 0) cudaMemcpyToSymbol(jl::g_head_status, &zero, sizeof(int));
