@@ -518,9 +518,9 @@ class Qwen3JetLongFusedModel(Qwen3PreTrainedModel):
                                        past_key_values=past_key_values if use_cache else None)
 
     def _check_kernel_status(self, extended: bool) -> None:
-        """With `model.check_kernel_status = True` (or JETLONG_CHECK_STATUS=1) every extended forward ends by
-        reading the status words of the kernels' bounded waits and raises if one gave up.  Off by default: the
-        read synchronises the device."""
+        """With `model.check_kernel_status = True` (or JETLONG_CHECK_STATUS=1) every extended forward, and every step that
+        takes scores or a loss from the head's kernels, ends by reading the status words of the kernels' bounded waits and
+        raises if one gave up.  Off by default: the read synchronises the device."""
         import os
         if extended and (getattr(self, "check_kernel_status", False) or os.environ.get("JETLONG_CHECK_STATUS") == "1"):
             from jetlm.kernels import jetlong_ops as ops
@@ -550,7 +550,9 @@ class Qwen3JetLongFusedModel(Qwen3PreTrainedModel):
         for layer in self.layers[: self.config.num_hidden_layers]:
             hidden = layer(hidden, attention_mask=None, position_embeddings=position_embeddings,
                            position_ids=None, past_key_values=cache, use_cache=True)
-        return self.norm(hidden)
+        hidden = self.norm(hidden)
+        self._check_kernel_status(True)
+        return hidden
 
     def _forward_token_sharded(self, input_ids, past_key_values, use_cache, shard, **kwargs) -> BaseModelOutputWithPast:
         """Sequence-parallel forward; `input_ids` is the whole (B, S) call on every rank.
@@ -633,9 +635,10 @@ class Qwen3JetLongFusedForCausalLM(Qwen3PreTrainedModel, GenerationMixin):
         hidden = outputs.last_hidden_state
         keep = slice(-logits_to_keep, None) if isinstance(logits_to_keep, int) else logits_to_keep
         if labels is not None and self.fused_loss:
-            return CausalLMOutputWithPast(loss=self._fused_loss(hidden[:, keep, :], labels, **kwargs), logits=None,
-                                          past_key_values=outputs.past_key_values, hidden_states=outputs.hidden_states,
-                                          attentions=outputs.attentions)
+            loss = self._fused_loss(hidden[:, keep, :], labels, **kwargs)
+            self.model._check_kernel_status(True)
+            return CausalLMOutputWithPast(loss=loss, logits=None, past_key_values=outputs.past_key_values,
+                                          hidden_states=outputs.hidden_states, attentions=outputs.attentions)
         logits = self.lm_head(hidden[:, keep, :])
         loss = None
         if labels is not None:
@@ -671,6 +674,7 @@ class Qwen3JetLongFusedForCausalLM(Qwen3PreTrainedModel, GenerationMixin):
             hi = min(lo + chunk_tokens, n - 1)                    # the last token predicts nothing
             hidden = self.model(input_ids=input_ids[:, lo:hi], past_key_values=past_key_values, use_cache=True).last_hidden_state
             out[:, lo:hi] = head_ops.token_scores(hidden, self.lm_head.weight, input_ids[:, lo + 1: hi + 1]).nll
+        self.model._check_kernel_status(True)
         return out
 
     @torch.no_grad()
@@ -701,7 +705,13 @@ class Qwen3JetLongFusedForCausalLM(Qwen3PreTrainedModel, GenerationMixin):
         for lo in range(0, n_prompt, chunk_tokens):
             hidden = self.model(input_ids=input_ids[:, lo: lo + chunk_tokens], past_key_values=cache, use_cache=True).last_hidden_state
         weight = self.lm_head.weight
-        out = [int(head_ops.token_scores(hidden[:, -1], weight, top=True).top)]
+
+        def best_of(rows):
+            top = head_ops.token_scores(rows, weight, top=True).top
+            self.model._check_kernel_status(True)
+            return top.tolist()
+
+        out = best_of(hidden[:, -1])
         ids, inv_freq, regrouped, steps = input_ids[0].tolist(), self.model.rotary_emb.inv_freq, None, 0
         while len(out) < max_new_tokens:
             seen = cache.get_seq_length()
@@ -736,7 +746,7 @@ class Qwen3JetLongFusedForCausalLM(Qwen3PreTrainedModel, GenerationMixin):
             step = TreeStep(draft_ops.draft_tree(torch.tensor([parents], dtype=torch.int32, device=dev)),
                             torch.tensor([seen], dtype=torch.int32, device=dev), far_rows)
             hidden = self.model.tree_step(torch.tensor([tokens], dtype=torch.long, device=dev), cache, step, group)
-            best = head_ops.token_scores(hidden[0], weight, top=True).top.tolist()
+            best = best_of(hidden[0])
             steps += 1
             path = [0]
             while True:
