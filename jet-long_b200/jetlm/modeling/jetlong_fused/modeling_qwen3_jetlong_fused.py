@@ -697,6 +697,10 @@ class Qwen3JetLongFusedForCausalLM(Qwen3PreTrainedModel, GenerationMixin):
             raise ValueError("generate_drafted takes one prompt at a time")
         dev, n_prompt = input_ids.device, input_ids.shape[1]
         cache = past_key_values
+        if cache is not None and not isinstance(cache, BifocalKVCache):
+            raise TypeError(f"generate_drafted needs a BifocalKVCache, got {type(cache).__name__}")
+        if cache is not None and cache.shard is not None and cache.shard.world > 1:
+            raise ValueError("generate_drafted runs on one GPU: its cache must not be sharded")      # row i is taken as position i
         if cache is None:
             cache = BifocalKVCache(self.config, n_prompt + max_new_tokens + 256, batch=1, device=dev, dtype=self.lm_head.weight.dtype,
                                    regrouped_far_keys=True)
