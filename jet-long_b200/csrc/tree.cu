@@ -195,10 +195,10 @@ int launch_tree_keep(const jl_tree_keep_args* a, cudaStream_t stream) {
 int launch_tree_plan(const jl_tree_plan_args* a, cudaStream_t stream) {
   if (a->batch < 0 || a->nodes < 1 || a->nodes > JL_TREE_MAX_NODES)
     return fail(JL_ERR_BAD_ARG, "jl_tree_plan: need batch >= 0 and 1 <= nodes <= %d, got %d and %d", JL_TREE_MAX_NODES, a->batch, a->nodes);
+  if (a->batch == 0) return JL_OK;                      // empty arrays may be NULL
   if (a->parents == nullptr || a->depth == nullptr || a->mask == nullptr) return fail(JL_ERR_BAD_ARG, "jl_tree_plan: NULL pointer");
   if ((reinterpret_cast<uintptr_t>(a->parents) | reinterpret_cast<uintptr_t>(a->depth)) & 3 || reinterpret_cast<uintptr_t>(a->mask) & 7)
     return fail(JL_ERR_BAD_ARG, "jl_tree_plan: misaligned pointer");
-  if (a->batch == 0) return JL_OK;
   const int rc = check_device_arch();
   if (rc != JL_OK) return rc;
   if (launch_dependent(tree_plan_kernel, dim3(a->batch), dim3((a->nodes + 31) / 32 * 32), 0, stream, a->parents, a->depth, a->mask, a->nodes) != cudaSuccess)
@@ -208,11 +208,12 @@ int launch_tree_plan(const jl_tree_plan_args* a, cudaStream_t stream) {
 
 int launch_tree_append(const jl_tree_append_args* a, cudaStream_t stream) {
   if (a->head_dim != kHeadDim) return fail(JL_ERR_UNSUPPORTED, "jl_tree_append: head_dim must be 128, got %d", a->head_dim);
+  if (a->batch < 0 || a->nodes < 1 || a->nodes > JL_TREE_MAX_NODES || a->heads < 1 || a->kv_heads < 1 || a->cache_rows < 0)
+    return fail(JL_ERR_BAD_ARG, "jl_tree_append: sizes out of range");
+  if (a->batch == 0) return JL_OK;                      // empty arrays may be NULL
   if (a->q == nullptr || a->k == nullptr || a->v == nullptr || a->q_weight == nullptr || a->k_weight == nullptr || a->q_base == nullptr ||
       a->k_cache == nullptr || a->v_cache == nullptr || a->inv_freq == nullptr || a->lens == nullptr || a->depth == nullptr)
     return fail(JL_ERR_BAD_ARG, "jl_tree_append: NULL pointer");
-  if (a->batch < 0 || a->nodes < 1 || a->nodes > JL_TREE_MAX_NODES || a->heads < 1 || a->kv_heads < 1 || a->cache_rows < 0)
-    return fail(JL_ERR_BAD_ARG, "jl_tree_append: sizes out of range");
   if ((a->q_group != nullptr || a->k_group_cache != nullptr) && a->group_size < 1)
     return fail(JL_ERR_BAD_ARG, "jl_tree_append: group_size must be >= 1");
   const int64_t st[] = {a->q_stride_b, a->q_stride_s, a->q_stride_h, a->k_stride_b, a->k_stride_s, a->k_stride_h,
@@ -229,7 +230,6 @@ int launch_tree_append(const jl_tree_append_args* a, cudaStream_t stream) {
   const int64_t cache_size[] = {a->batch, a->cache_rows, a->kv_heads, a->batch, a->cache_rows, a->kv_heads};
   for (int i = 0; i < 6; ++i)
     if (cache_size[i] > 1 && st[9 + i] <= 0) return fail(JL_ERR_UNSUPPORTED, "jl_tree_append: a cache dimension larger than 1 needs a positive stride");
-  if (a->batch == 0) return JL_OK;
   const int rc = check_device_arch();
   if (rc != JL_OK) return rc;
   AppendParams p{};
@@ -274,6 +274,7 @@ static int validate_tree_attention(const jl_tree_attention_args* a) {
   if (!(a->softmax_scale > 0.f) || isinf(a->softmax_scale)) return fail(JL_ERR_BAD_ARG, "jl_tree_attention: softmax_scale must be positive and finite");
   if ((a->q_group == nullptr) != (a->k_group == nullptr))
     return fail(JL_ERR_BAD_ARG, "jl_tree_attention: q_group and k_group come together or not at all");
+  if (a->batch == 0) return JL_OK;                      // empty arrays may be NULL
   if (a->q_base == nullptr || a->k_base == nullptr || a->v == nullptr || a->out == nullptr || a->lens == nullptr || a->depth == nullptr ||
       a->mask == nullptr)
     return fail(JL_ERR_BAD_ARG, "jl_tree_attention: NULL pointer");

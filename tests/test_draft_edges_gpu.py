@@ -1,4 +1,4 @@
-"""Tree-of-drafts operators at the edges: at the end of a cache, with NaN in the queries."""
+"""Tree-of-drafts operators at the edges: at the end of a cache, with NaN in the queries, without samples."""
 import math
 
 import pytest
@@ -91,3 +91,17 @@ def test_a_score_of_nan_in_one_class_only():
     assert torch.equal(out[0, [0, 2]], ref[0, [0, 2]]) and torch.equal(lse[0, :, [0, 2]], ref_lse[0, :, [0, 2]])
     s["w_0"] = 1000
     assert torch.isfinite(call(s)[0]).all()
+
+
+def test_no_samples():
+    from jetlm.kernels import draft_ops as d
+    z = lambda *s: torch.empty(*s, device="cuda", dtype=torch.bfloat16)        # noqa: E731
+    lens = torch.empty(0, dtype=torch.int32, device="cuda")
+    tree = d.draft_tree(torch.empty(0, 3, dtype=torch.int32, device="cuda"))
+    k, v = z(0, 20, 2, D), z(0, 20, 2, D)
+    qb, qg = d.tree_append(z(0, 3, 4, D), z(0, 3, 2, D), z(0, 3, 2, D), torch.ones(D, device="cuda").bfloat16(), torch.ones(D, device="cuda").bfloat16(),
+                           inv_freq(), k, v, tree, lens, q_eps=1e-6, k_eps=1e-6, group_size=2)
+    assert qb.shape == qg.shape == (0, 3, 4, D)
+    out, lse = d.tree_attention(qb, qg, k, v, tree, lens, w_0=4)
+    assert out.shape == (0, 3, 4, D) and lse.shape == (0, 4, 3)
+    d.tree_keep(k, v, torch.empty(0, 3, dtype=torch.int32, device="cuda"), lens)
