@@ -19,6 +19,10 @@ int fail(int status, const char* fmt, ...);
 int check_launch(const char* what);
 int check_device_arch();
 
+// Whether any of these addresses is not a multiple of `bytes` (NULL is one).
+template <class... P>
+bool misaligned(uintptr_t bytes, const P*... p) { return ((reinterpret_cast<uintptr_t>(p) | ... | uintptr_t(0)) & (bytes - 1)) != 0; }
+
 // ---------------------------------------------------------------------------------------------
 // Small device helpers
 // ---------------------------------------------------------------------------------------------

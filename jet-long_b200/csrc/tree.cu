@@ -227,6 +227,7 @@ int launch_tree_append(const jl_tree_append_args* a, cudaStream_t stream) {
                          reinterpret_cast<uintptr_t>(a->k_group_cache) | reinterpret_cast<uintptr_t>(a->q_weight) |
                          reinterpret_cast<uintptr_t>(a->k_weight);
   if (ptrs & 7) return fail(JL_ERR_BAD_ARG, "jl_tree_append: pointers must be 8-byte aligned");
+  if (misaligned(4, a->inv_freq, a->lens, a->depth)) return fail(JL_ERR_BAD_ARG, "jl_tree_append: inv_freq, lens and depth must be 4-byte aligned");
   const int64_t cache_size[] = {a->batch, a->cache_rows, a->kv_heads, a->batch, a->cache_rows, a->kv_heads};
   for (int i = 0; i < 6; ++i)
     if (cache_size[i] > 1 && st[9 + i] <= 0) return fail(JL_ERR_UNSUPPORTED, "jl_tree_append: a cache dimension larger than 1 needs a positive stride");
@@ -282,6 +283,8 @@ static int validate_tree_attention(const jl_tree_attention_args* a) {
                          reinterpret_cast<uintptr_t>(a->k_base) | reinterpret_cast<uintptr_t>(a->k_group) |
                          reinterpret_cast<uintptr_t>(a->v) | reinterpret_cast<uintptr_t>(a->out);
   if (ptrs & 15) return fail(JL_ERR_BAD_ARG, "jl_tree_attention: pointers must be 16-byte aligned");
+  if (misaligned(4, a->lens, a->depth, a->lse) || misaligned(8, a->mask))
+    return fail(JL_ERR_BAD_ARG, "jl_tree_attention: lens, depth and lse must be 4-byte aligned, mask 8-byte");
   const int64_t st[] = {a->q_stride_b, a->q_stride_s, a->q_stride_h, a->k_stride_b, a->k_stride_s, a->k_stride_h,
                         a->v_stride_b, a->v_stride_s, a->v_stride_h, a->o_stride_b, a->o_stride_s, a->o_stride_h};
   for (int64_t x : st)

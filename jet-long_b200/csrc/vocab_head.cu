@@ -1082,6 +1082,8 @@ int launch_scores(const jl_head_scores_args* a, cudaStream_t stream) {
     return fail(JL_ERR_BAD_ARG, "jl_head_scores: nll and the loss need labels");
   if (a->skip_ignored && (a->labels == nullptr || a->top != nullptr))
     return fail(JL_ERR_BAD_ARG, "jl_head_scores: skip_ignored needs labels and leaves no top");
+  if (misaligned(8, a->labels, a->top) || misaligned(4, a->nll, a->lse, a->loss_sum, a->loss_count, a->loss_mean))
+    return fail(JL_ERR_BAD_ARG, "jl_head_scores: labels and top must be 8-byte aligned, the fp32 results 4-byte");
   const ScoresLayout l = scores_layout(a->rows, a->hidden_size, a->vocab, a->skip_ignored != 0);
   if (a->workspace == nullptr || a->workspace_bytes < l.total)
     return fail(JL_ERR_WORKSPACE, "jl_head_scores: workspace of %zu bytes needed, %zu given", l.total, a->workspace_bytes);
@@ -1157,6 +1159,8 @@ int launch_grads(const jl_head_grads_args* a, cudaStream_t stream) {
     return fail(JL_ERR_WORKSPACE, "jl_head_grads: workspace of %zu bytes needed, %zu given", l.total, a->workspace_bytes);
   if (reinterpret_cast<uintptr_t>(a->workspace) & 15) return fail(JL_ERR_BAD_ARG, "jl_head_grads: workspace not 16-byte aligned");
   if (a->nll == nullptr) return fail(JL_ERR_BAD_ARG, "jl_head_grads: nll is NULL");
+  if (misaligned(8, a->labels) || misaligned(4, a->lse, a->nll, a->grad, a->grad_count))
+    return fail(JL_ERR_BAD_ARG, "jl_head_grads: labels must be 8-byte aligned, the fp32 operands 4-byte");
   rc = check_device_arch();
   if (rc != JL_OK) return rc;
   const int64_t N = a->rows, H = a->hidden_size, V = a->vocab;

@@ -1,6 +1,8 @@
 """Arguments of the drafted-token and vocabulary-head C entries that are refused, or need nothing, before a device is touched."""
 import ctypes as C
 
+import pytest
+
 
 def _n():
     from jetlm.kernels import _native
@@ -66,3 +68,25 @@ def test_no_samples_need_no_arrays():
     # sizes that are out of range stay so
     assert plan(batch=0, nodes=0) == append(batch=0, nodes=300) == attention(batch=0, kv_heads=3) == n.JL_ERR_BAD_ARG
     assert append(batch=0, head_dim=64) == n.JL_ERR_UNSUPPORTED
+
+
+def scores(**kw):
+    n = _n()
+    a = n.HeadScoresArgs()
+    a.hidden = a.weight = a.labels = a.nll = a.workspace = 1024
+    a.hidden_stride = a.weight_stride = a.hidden_size = 64
+    a.rows, a.vocab = 3, 100
+    a.workspace_bytes = n.lib().jl_head_scores_workspace_bytes(3, 64, 100, 0)
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return n.lib().jl_head_scores(C.byref(a), None)
+
+
+@pytest.mark.parametrize("call, field, address", [
+    *[(append, f, 1026) for f in ("inv_freq", "lens", "depth")], *[(attention, f, 1026) for f in ("lens", "depth", "lse")], (attention, "mask", 1028),
+    (scores, "labels", 1028), (scores, "top", 1028), *[(scores, f, 1026) for f in ("nll", "lse", "loss_sum", "loss_count", "loss_mean")],
+    (grads, "labels", 1028), *[(grads, f, 1026) for f in ("lse", "nll", "grad", "grad_count")]])
+def test_misaligned_arrays_are_refused(call, field, address):
+    """The kernels load whole words; nothing of such a call may reach the device (there is none here, and one is asked for last)."""
+    n = _n()
+    assert call(**{field: address}) == n.JL_ERR_BAD_ARG and b"aligned" in n.lib().jl_last_error()
