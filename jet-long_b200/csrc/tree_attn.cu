@@ -59,7 +59,7 @@ struct TreeParams {
   float scale_log2;
   const int32_t *lens, *depth;
   const uint64_t* mask;
-  float *part_o, *part_lse;    // [slot] (two row tiles: [slot][tile]) of [32 column groups][rpt rows][4] and [rpt rows]
+  float *part_o, *part_lse;    // [place] (two row tiles: [place][tile]) of [32 column groups][rpt rows][4] and [rpt rows]
   __nv_bfloat16* out;
   float* lse;
   int64_t os_b, os_s, os_h;
@@ -114,9 +114,10 @@ __device__ __forceinline__ int64_t parts_of(const TreeParams& p, int mb, int64_t
   return min(static_cast<int64_t>(has_two(p, mb) ? p.workers : p.workers_one), total);
 }
 
-// Place of a partial: segment `i` (part + samples and key heads before it) of row tile 2 mb + t.
+// Place of a partial of row tile 2 mb + t.  Only a part's first and last segment can be less than their (sample, key head): `i` is
+// twice the part for the first, one more for the last.
 __device__ __forceinline__ int64_t place_of(const TreeParams& p, int mb, int t, int64_t i) {
-  const int64_t per = p.workers + static_cast<int64_t>(p.batch) * p.kv_heads;
+  const int64_t per = 2 * static_cast<int64_t>(p.workers);
   return has_two(p, mb) ? (mb * per + i) * 2 + t : p.pairs * per * 2 + i;
 }
 
@@ -400,7 +401,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
     // the warps of a row quarter).  A segment that is all of its (sample, key head) leaves the result, another one a partial: O / l in
     // fp32 (zero where the row saw nothing) and the LSE in the log2 domain.  A row has seen something when its sum is not 0: scores of
     // NaN leave the maximum at -inf, their sum is NaN, and so is then all that the row leaves.
-    auto leave = [&](const Segment& s, int d, bool any) {
+    auto leave = [&](const Segment& s, bool leads, int d, bool any) {      // leads: the part's first segment
       float m = any && d >= 0 ? m_ref : -INFINITY, l = any && d >= 0 ? l_sum : 0.f, mine = 1.f, other = 0.f;
       if (!two_tiles) {
         sm.stats[t][r] = make_float2(m, l);
@@ -418,7 +419,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
       const float inv = seen ? 1.f / l : 0.f;
       mine = seen ? mine * inv : 0.f;
       other *= inv;
-      const int64_t prow = place_of(p, mb, t, worker + s.b * p.kv_heads + s.kvh) * p.rpt;
+      const int64_t prow = place_of(p, mb, t, 2 * worker + (leads ? 0 : 1)) * p.rpt;
       const int ch0 = two_tiles ? 0 : 2 * t, ch1 = two_tiles ? 4 : 2 * t + 2, h = s.kvh * p.rep + r % p.rep;
 #pragma unroll 1
       for (int ch = ch0; ch < ch1; ++ch) {
@@ -460,6 +461,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
     Segment seg;
     int n_done = 0, g = 0;
     while (w.next(p, seg)) {
+      const bool leads = g == 0;
       const int step = two_tiles ? 1 : 2, first = seg.v0 + (two_tiles ? 0 : (g ^ t) & 1);
       g += seg.v1 - seg.v0;
       const int64_t nrow = static_cast<int64_t>(seg.b) * p.nodes + (row_used ? node : 0);
@@ -468,7 +470,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
       m_ref = -INFINITY;
       l_sum = 0.f;
       if (first >= seg.v1) {                           // this state has no visit in the segment
-        leave(seg, -1, false);
+        leave(seg, leads, -1, false);
         continue;
       }
       for (int v = first; v < seg.v1; v += step, ++n_done) {
@@ -628,7 +630,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
       }
       mbar_wait(&sm.pv_done[t], (n_done - 1) & 1, sm);
       tc_fence_after();
-      leave(seg, d, true);
+      leave(seg, leads, d, true);
     }
   }
 
@@ -674,8 +676,10 @@ __global__ void __launch_bounds__(128) tree_combine_kernel(const TreeParams p) {
     return;
   }
   const int n_parts = i1 - i0 + 1, stride = has_two(p, mb) ? 2 : 1;
-  const int64_t first = place_of(p, mb, tile & 1, static_cast<int64_t>(b) * p.kv_heads + kvh + i0);
-  const int64_t lse_step = static_cast<int64_t>(stride) * p.rpt, o_step = lse_step * 32;
+  // in part i0 it is the first segment if it starts there, else the last; in every later part the first
+  const int64_t first = place_of(p, mb, tile & 1, 2 * static_cast<int64_t>(i0));
+  const int64_t skip = static_cast<int64_t>(i0) * total / parts < lo ? stride * p.rpt : 0;
+  const int64_t lse_step = 2 * static_cast<int64_t>(stride) * p.rpt, o_step = lse_step * 32;
   wait_prerequisites();
   for (int item = blockIdx.x * 128 + threadIdx.x; item < 32 * p.rpt; item += gridDim.x * 128) {
     const int c = item / p.rpt, r = item - c * p.rpt;
@@ -691,8 +695,9 @@ __global__ void __launch_bounds__(128) tree_combine_kernel(const TreeParams p) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const bool in = k0 + j < n_parts;
-        l[j] = in ? lse[(k0 + j) * lse_step] : -INFINITY;
-        x[j] = in ? o[(k0 + j) * o_step] : make_float4(0.f, 0.f, 0.f, 0.f);
+        const int64_t late = k0 + j == 0 ? skip : 0;
+        l[j] = in ? lse[(k0 + j) * lse_step + late] : -INFINITY;
+        x[j] = in ? o[(k0 + j) * o_step + late * 32] : make_float4(0.f, 0.f, 0.f, 0.f);
       }
       float mn = m;
 #pragma unroll
@@ -715,7 +720,7 @@ __global__ void __launch_bounds__(128) tree_combine_kernel(const TreeParams p) {
 }
 
 struct Layout { int npt, rpt, pairs, workers, workers_one; size_t lse, total; };
-Layout layout_of(int32_t batch, int32_t nodes, int32_t heads, int32_t kv_heads) {
+Layout layout_of(int32_t nodes, int32_t heads, int32_t kv_heads) {
   Layout l{};
   const int rep = heads / kv_heads;
   l.npt = 128 / rep;
@@ -728,8 +733,7 @@ Layout layout_of(int32_t batch, int32_t nodes, int32_t heads, int32_t kv_heads) 
   l.workers = l.pairs == 0 ? 0 : odd ? kSms * 36 / (36 * l.pairs + 17) : kSms / l.pairs;
   if (l.pairs > 0 && l.workers < 1) l.workers = 1;
   l.workers_one = !odd ? 0 : kSms - l.pairs * l.workers < 1 ? 1 : kSms - l.pairs * l.workers;
-  const size_t bk = static_cast<size_t>(batch) * kv_heads;
-  const size_t rows = (l.pairs * (l.workers + bk) * 2 + (odd ? l.workers_one + bk : 0)) * l.rpt;
+  const size_t rows = static_cast<size_t>(l.pairs * l.workers * 2 + l.workers_one) * 2 * l.rpt;      // two places a part
   l.lse = rows * kHeadDim * sizeof(float);
   l.total = l.lse + rows * sizeof(float);
   return l;
@@ -755,11 +759,11 @@ int make_map4(CUtensorMap* m, const void* base, int batch, int seq, int heads, i
 
 size_t tree_attention_workspace_bytes(int32_t batch, int32_t nodes, int32_t heads, int32_t kv_heads, int32_t) {
   if (batch < 1 || nodes < 1 || kv_heads < 1 || heads < kv_heads || heads / kv_heads > 128) return 0;
-  return layout_of(batch, nodes, heads, kv_heads).total;
+  return layout_of(nodes, heads, kv_heads).total;
 }
 
 int launch_tree_attention(const jl_tree_attention_args* a, cudaStream_t stream) {
-  const Layout l = layout_of(a->batch, a->nodes, a->heads, a->kv_heads);
+  const Layout l = layout_of(a->nodes, a->heads, a->kv_heads);
   if (a->workspace == nullptr || a->workspace_bytes < l.total)
     return fail(JL_ERR_WORKSPACE, "jl_tree_attention: workspace of %zu bytes needed, %zu given", l.total, a->workspace_bytes);
   if (reinterpret_cast<uintptr_t>(a->workspace) & 15) return fail(JL_ERR_BAD_ARG, "jl_tree_attention: workspace not 16-byte aligned");

@@ -90,3 +90,13 @@ def test_misaligned_arrays_are_refused(call, field, address):
     """The kernels load whole words; nothing of such a call may reach the device (there is none here, and one is asked for last)."""
     n = _n()
     assert call(**{field: address}) == n.JL_ERR_BAD_ARG and b"aligned" in n.lib().jl_last_error()
+
+
+def test_the_attention_workspace_does_not_grow_with_the_batch():
+    """A part of the line of visits leaves two partial results at most: 148 parts, two row tiles of 128 rows, 512 bytes of O and 4 of lse."""
+    n = _n()
+    size = n.lib().jl_tree_attention_workspace_bytes
+    for nodes, heads, kv in [(1, 8, 8), (16, 32, 8), (64, 32, 8), (80, 32, 8), (256, 8, 1), (256, 128, 1), (255, 64, 1)]:
+        one = size(1, nodes, heads, kv, 4096)
+        assert 0 < one <= 2 * (148 * 2 + 1) * 128 * 516
+        assert size(65535 // kv, nodes, heads, kv, 4096) == one
