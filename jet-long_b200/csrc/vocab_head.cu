@@ -394,7 +394,7 @@ __device__ __forceinline__ void finish(const GemmMaps& maps, const GemmParams& p
       const int c_lo = half == 0 ? 0 : (p.bn / 2 + 15) / 16 * 16, width = half == 0 ? (p.bn / 2 + 15) / 16 * 16 : p.bn - c_lo;
       float z[128];
 #pragma unroll
-      for (int j = 0; j < 128; ++j) z[j] = 0.f;
+      for (int j = 0; j < 128; ++j) z[j] = (j & ~15) < width ? 0.f : -INFINITY;      // blocks of 16 past the half are not read
       for (int part = 0; part * P::kPart < p.k_blocks; ++part) {
         const uint32_t acc = tmem + (st.i % P::kAccs) * P::kAccCols + lane_base + c_lo;
         mbar_wait(&sm.acc_full[st.i % P::kAccs], (st.i / P::kAccs) & 1, sm);
@@ -413,12 +413,14 @@ __device__ __forceinline__ void finish(const GemmMaps& maps, const GemmParams& p
       }
       const int64_t rest = p.N - n0 - c_lo;
       const int valid = static_cast<int>(rest < 0 ? 0 : rest < width ? rest : width);
+      if (valid < width) {                             // the vocabulary ends in here
+#pragma unroll
+        for (int j = 0; j < 128; ++j)
+          if (j >= valid) z[j] = -INFINITY;
+      }
       float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int j = 0; j < 128; ++j) {
-        if (j >= valid) z[j] = -INFINITY;
-        m4[j & 3] = fmaxf(m4[j & 3], z[j]);
-      }
+      for (int j = 0; j < 64; ++j) m4[j & 3] = max3(m4[j & 3], z[2 * j], z[2 * j + 1]);
       const float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
       const float m_use = m == -INFINITY ? 0.f : m;
       const int64_t y64 = p.labels != nullptr && row < p.M ? p.labels[row] - p.v0 - n0 - c_lo : -1;

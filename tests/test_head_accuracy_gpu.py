@@ -71,12 +71,14 @@ def test_scores_of_sure_rows_keep_their_digits(N, H):
     assert ((plain.double() - want).abs() <= 2.0 ** -11 * want).all()
 
 
+@pytest.mark.parametrize("lo, hi", [(1e-6, 1e-2), (0.05, 0.95)])
 @pytest.mark.parametrize("reduction", ["sum", "none", "mean"])
 @pytest.mark.parametrize("N, H", [(1, 4096), (17, 2048), (49, 4096), (128, 2048), (200, 4096), (300, 2048), (300, 4096)])
-def test_gradient_of_sure_rows(N, H, reduction):
-    """1 - p from 1e-2 down to 1e-6: every row's gradient is right relative to the row itself, not to gradients of size one."""
+def test_gradient_of_sure_rows(N, H, reduction, lo, hi):
+    """1 - p from 1e-2 down to 1e-6, and of usual rows: every row's gradient is right relative to the row itself, not to gradients of
+    size one."""
     from jetlm.kernels import head_ops
-    h, w, y = sure_rows(N, H, 1e-6, 1e-2, seed=5)
+    h, w, y = sure_rows(N, H, lo, hi, seed=5)
     if N > 256:                                       # rows that do not count in between: the others are packed
         y[3::7] = -100
     used = y >= 0
