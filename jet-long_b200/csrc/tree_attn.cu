@@ -22,9 +22,10 @@
 //   warps 4-11  softmax: one thread per row, P back to tensor memory over S
 //
 // The softmax is one pass over the keys: with the running maximum m (raised lazily, only when a score exceeds it by 2^8), O and l hold
-// sum e^(s - m) v and sum e^(s - m) in fp32; P is rounded to bf16 for the product, as the values are.  16 nodes x 4 heads over 131056
-// keys: 96 us for 537 MB of keys and values, the launch of the join included, bound by their stream (6.0 TB/s of 6.56 inside the
-// kernel).  64 nodes x 4 heads: 140 us, bound by the chain of a row tile's products and softmax (tensor pipe 58 %).
+// sum e^(s - m) v and sum e^(s - m) in fp32; P is rounded to bf16 for the product, as the values are.  Times of a replayed graph of the
+// call, the join included, after a pause and (in brackets) in a loop at the power cap.  16 nodes x 4 heads over 131056 keys: 96 us
+// [107] for 537 MB of keys and values, bound by their stream (6.0 TB/s of 6.56 inside the kernel).  64 nodes x 4 heads: 143 us [170],
+// bound by the chain of a row tile's products and softmax (tensor pipe 58 %).
 #include "tc_common.cuh"
 #include "../../include/jetlong_b200_tree.h"
 
@@ -728,7 +729,8 @@ Layout layout_of(int32_t nodes, int32_t heads, int32_t kv_heads) {
   l.pairs = tiles / 2;
   l.rpt = (tiles > 1 ? l.npt : nodes) * rep;
   // SMs for pairs of row tiles and for the one that is left, by what a visit costs them, 36 : 17 (80 nodes over 131056 keys, three
-  // tiles: 217 us, with 36 : 13 250, 36 : 22 228; 259 with the last tile paired with an empty one)
+  // tiles: 217 us, with 36 : 13 250, 36 : 22 228; 259 with the last tile paired with an empty one).  The ratio was varied at that size
+  // alone; with it, 40 nodes x 8 heads over 74631 keys took 129 us instead of 160, 8 samples of 78 nodes 158 instead of 184.
   const bool odd = tiles % 2 != 0;
   l.workers = l.pairs == 0 ? 0 : odd ? kSms * 36 / (36 * l.pairs + 17) : kSms / l.pairs;
   if (l.pairs > 0 && l.workers < 1) l.workers = 1;
@@ -774,7 +776,8 @@ int launch_tree_attention(const jl_tree_attention_args* a, cudaStream_t stream) 
   p.w_0 = a->w_0 < (int64_t(1) << 32) ? a->w_0 : (int64_t(1) << 32);           // no cache reaches further
   p.nodes_far = p.two_classes && p.w_0 < a->nodes - 1;
   // The unrolled softmax saves 1300 clocks a visit, and its instructions, cold, cost 8 us once: 16 nodes over 131072 keys 106.5 us
-  // rolled and 102.8 unrolled, 64 nodes 171 and 142; the two are equal at 8 visits a part.
+  // rolled and 102.8 unrolled, 64 nodes 171 and 142; the two are equal at 8 visits a part.  The choice goes by the rows that the
+  // cache has, since its lengths are on the device: 4 nodes over 1037 keys in a cache of 131072 rows take 18.4 us, in one of 1044 16.4.
   p.unrolled = static_cast<int64_t>(a->batch) * a->kv_heads * (a->rows / kTileN) >= 16ll * (l.pairs > 0 ? l.workers : l.workers_one);
   p.scale_log2 = a->softmax_scale * kLog2e;
   p.lens = a->lens; p.depth = a->depth; p.mask = a->mask;

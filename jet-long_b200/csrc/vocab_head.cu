@@ -13,9 +13,9 @@
 // hidden across them (MN-major), so nothing is transposed in memory.  Of a loss over more than 256 rows only those that count
 // are multiplied: they are packed first, and the products take their extents from the number on the device.
 //
-// Few rows are bound by the weight's bytes: 49 rows x 4096 x 151936 205 us after a pause (6.1 TB/s), in a loop 218 to 232, where the
+// Few rows are bound by the weight's bytes: 49 rows x 4096 x 151936 205 us after a pause (6.1 TB/s), in a loop 218 to 241, where the
 // power cap holds the clock at 1.30 GHz.  Many are bound by the tensor pipe at the capped clock: scores of 8191 rows x 4096
-// 7.2 ms in a loop (1412 TFLOP/s), 6.2 after a pause (1640); loss and gradients of 4096 rows x 2560 9.7 and 8.4 ms (1310 and 1515),
+// 7.2 ms in a loop (1416 TFLOP/s), 6.3 after a pause (1620); loss and gradients of 4096 rows x 2560 9.7 and 8.4 ms (1310 and 1515),
 // four products where three would do if the logits were kept.
 #include <cmath>
 #include <type_traits>
